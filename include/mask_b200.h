@@ -400,6 +400,51 @@ int mask_spmm_srbcrs_static_scratch(const mask_plan* plan, const int32_t* d_val_
                                     int32_t M, int32_t K, int32_t N, const float* d_B, int64_t ldb,
                                     float* d_C, int64_t ldc, int epilogue, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Classifier head: softmax cross entropy of hidden * weight over the labelled rows, with its
+ * gradients, without the logits in memory.  What follows the last sparse product of a graph network
+ * in training and evaluation (the reference's GCN driver takes it from its tensor library,
+ * end2end/gcn/eva_gcn_sparsene.py:599-781).
+ *
+ * A row is labelled if 0 <= label < classes; every other label leaves the row out: its loss and its
+ * row of dhidden are 0, and what its row of hidden holds (infinities and NaN too) reaches nothing.
+ *   logit[r,v] = sum_d hidden[r,d] weight[d,v],  loss[r] = log sum_v exp logit[r,v] - logit[r,label[r]]
+ *   mean: loss[0] = their mean over the labelled rows, sum: their sum (both 0 if no row is labelled);
+ *   none: loss[r] for every row, gradients those of the sum.  Gradients are multiplied by grad_scale.
+ * float32 operands are multiplied as three products of bfloat16 parts (relative error of a product
+ * below 2^-16), 16-bit ones exactly; sums are float32.  The gradient of the logits is held in the
+ * parts' type between its products; infinite or NaN logits of a labelled row make its loss and the
+ * gradients NaN.  Results do not depend on the order of anything: the same call gives the same bits.
+ *
+ * Scratch: mask_linear_xent_scratch_bytes(head) bytes, 256-byte aligned, one call at a time (two captured graphs
+ * that may run at once need two).  Asynchronous on `stream`.  Should a kernel give up on one of its bounded
+ * waits, every loss is NaN.
+ * ------------------------------------------------------------------------------------------ */
+typedef enum mask_dtype { MASK_F32 = 0, MASK_BF16 = 1, MASK_F16 = 2 } mask_dtype;
+typedef enum mask_reduction { MASK_REDUCE_NONE = 0, MASK_REDUCE_MEAN = 1, MASK_REDUCE_SUM = 2 } mask_reduction;
+
+typedef struct mask_head {
+    int32_t dtype;              /* mask_dtype of hidden, weight and their gradients */
+    int32_t reduction;          /* mask_reduction */
+    int64_t rows;               /* < 2^31 - 256 */
+    int32_t dim, classes;       /* 1 or more, < 2^31 - 256 */
+    const void* d_hidden;       /* [rows, dim], rows hidden_stride elements apart */
+    int64_t hidden_stride;
+    const void* d_weight;       /* element (d, v) at d * weight_dim_stride + v * weight_class_stride */
+    int64_t weight_dim_stride, weight_class_stride;
+    const int64_t* d_labels;    /* [rows] */
+    float* d_loss;              /* [1], or [rows] for MASK_REDUCE_NONE */
+    float grad_scale;
+    int32_t reserved;
+    void* d_dhidden;            /* like hidden, or NULL */
+    int64_t dhidden_stride;
+    void* d_dweight;            /* like weight, or NULL; its elements must not overlap */
+    int64_t dweight_dim_stride, dweight_class_stride;
+} mask_head;
+
+size_t mask_linear_xent_scratch_bytes(const mask_head* head);   /* 0 for arguments that mask_linear_xent refuses */
+int mask_linear_xent(const mask_head* head, void* d_scratch, size_t scratch_bytes, void* stream);
+
 /* Development knobs for kernel variants, process-wide: "sweep" (1 = persistent tcgen05 kernel except
  * where the warp-level one measures faster (by N and the plan), 2 = always, 0 = warp-level kernels only),
  * "nslab" (tcgen05 kernel: 128-column slabs per sweep, 1 / 2 / 4; 0 = the plan table's choice),

@@ -59,6 +59,8 @@ SIGNATURES = {
     "mask_spmm": (C.c_int, [vp, vp, i32, vp, i64, vp, i64, vp, vp, sz, C.c_int, vp]),
     "mask_static_scratch_capacity": (sz, []),
     "mask_spmm_srbcrs_static_scratch": (C.c_int, [vp, vp, vp, vp, i32, i32, i32, vp, i64, vp, i64, C.c_int, vp]),
+    "mask_linear_xent_scratch_bytes": (sz, [vp]),
+    "mask_linear_xent": (C.c_int, [vp, vp, sz, vp]),
     "mask_tune": (C.c_int, [C.c_char_p, C.c_int]),
     "mask_spmm_kernel_name": (C.c_int, [vp, C.c_int, i32, C.c_int, C.c_char_p, sz]),
     "mask_spmm_warp_shape": (C.c_int, [vp, C.c_int, i32, C.c_int, C.POINTER(i32), C.POINTER(i32)]),
@@ -72,12 +74,21 @@ SIGNATURES = {
 }
 
 REORDER = {"none": 0, "row_rcm": 1, "first_col_sort": 2, "jaccard_greedy": 3}
+REDUCTION = {"none": 0, "mean": 1, "sum": 2}
 POLICY = {"auto": 0, "row": 1, "strict_lb": 2, "multi_bind": 3, "ref_auto": 4}
 
 
 class Matrix(C.Structure):
     """mask_matrix"""
     _fields_ = [("format", i32), ("M", i32), ("K", i32), ("reserved", i32), ("val_sidx", vp), ("offsets", vp), ("index", vp), ("values", vp)]
+
+
+class Head(C.Structure):
+    """mask_head"""
+    _fields_ = [("dtype", i32), ("reduction", i32), ("rows", i64), ("dim", i32), ("classes", i32), ("hidden", vp), ("hidden_stride", i64),
+                ("weight", vp), ("weight_dim_stride", i64), ("weight_class_stride", i64), ("labels", vp), ("loss", vp),
+                ("grad_scale", C.c_float), ("reserved", i32), ("dhidden", vp), ("dhidden_stride", i64), ("dweight", vp),
+                ("dweight_dim_stride", i64), ("dweight_class_stride", i64)]
 
 
 class Features(C.Structure):

@@ -28,11 +28,10 @@
 // copy is multicast.  Every wait is bounded; an expired wait raises the block's abort flag and the
 // plan's status word, every role leaves its loops, the block waits out its copies in flight and
 // the tensor core's work, frees its tensor memory and returns.
-#include <cuda.h>
-
 #include <mutex>
 
 #include "spmm_common.cuh"
+#include "tensor_map.h"
 #include "umma_ptx.cuh"
 
 namespace mask {
@@ -347,12 +346,7 @@ __global__ void __launch_bounds__(kTmaThreads, 2) spmm_tma_kernel(const SpmmArgs
     if (tid == 0 && *abort_flag) atomicExch(status, 1);
 }
 
-// cuTensorMapEncodeTiled through the runtime's driver entry point lookup (the library does not link libcuda).
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_tiled_fn() {
+EncodeTiledFn encode_tiled_fn() {
     static EncodeTiledFn fn = nullptr;
     static std::once_flag once;
     std::call_once(once, [] {

@@ -1,0 +1,606 @@
+// Classifier head: softmax cross entropy of hidden * weight over the labelled rows and its gradients, without the
+// logits in memory (mask_linear_xent).
+//
+// With L the labelled rows, l = H W, s_r = log sum_v exp l_rv and G_rv = exp(l_rv - s_r) - [v = y_r]:
+//     loss_r = s_r - l_{r,y_r},   dH = scale G W^T,   dW = scale H^T G.
+// Steps (matrix products in xent_gemm.cuh):
+//   1. the labelled rows are numbered (their order kept) and packed, with the weight, into zero-padded 16-bit planes that
+//      TMA can fetch: every later step costs what the labelled rows cost, and nothing an unlabelled row holds goes on;
+//   2. logits tile by tile, each row's running maximum and sum kept; parts of the classes are joined in a fixed order;
+//   3. for a piece of the classes at a time: the logits' tiles again, now turned into G (in 16-bit planes, in scratch), then
+//      dH += G W and that piece of dW = G^T H.
+// Up to 256 classes fit one tile, and steps 2 and 3 share one product.  Contractions that leave SMs idle are split and
+// their parts summed in a fixed order.
+#include <algorithm>
+
+#include "common.cuh"
+#include "tensor_map.h"
+#include "xent_gemm.cuh"
+
+namespace mask {
+
+constexpr int kXentCountThreads = 1024;
+constexpr size_t kXentPieceBytes = (size_t)512 << 20;   // what a piece of G may take
+
+// ---- numbering of the labelled rows ------------------------------------------------------------------
+__device__ __forceinline__ bool labelled(int64_t y, int32_t classes) { return y >= 0 && y < classes; }
+
+// One block per chunk of rows: how many of them are labelled.
+__global__ void __launch_bounds__(kXentCountThreads) xent_count_kernel(const int64_t* __restrict__ labels, int64_t rows, int32_t classes, int64_t chunk,
+                                                                       int32_t* __restrict__ counts) {
+    __shared__ int sums[32];
+    const int64_t r0 = blockIdx.x * chunk, r1 = min(rows, r0 + chunk);
+    int n = 0;
+    for (int64_t r = r0 + threadIdx.x; r < r1; r += kXentCountThreads) n += labelled(labels[r], classes);
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = n;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        n = __reduce_add_sync(0xffffffffu, sums[threadIdx.x]);
+        if (threadIdx.x == 0) counts[blockIdx.x] = n;
+    }
+}
+
+// Writes row_of and label of the chunk's labelled rows behind those of the chunks before it; the last block leaves the
+// total.  Losses of rows without a label are set to 0 here.
+__global__ void __launch_bounds__(kXentCountThreads) xent_number_kernel(const int64_t* __restrict__ labels, int64_t rows, int32_t classes, int64_t chunk,
+                                                                        const int32_t* __restrict__ counts, int32_t* __restrict__ row_of,
+                                                                        int32_t* __restrict__ label, int32_t* __restrict__ total,
+                                                                        int32_t* __restrict__ status, float* __restrict__ row_loss) {
+    __shared__ int sums[32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int at = 0;
+    for (int b = threadIdx.x; b < (int)blockIdx.x; b += kXentCountThreads) at += counts[b];
+    at = __reduce_add_sync(0xffffffffu, at);
+    if (lane == 0) sums[warp] = at;
+    __syncthreads();
+    at = __reduce_add_sync(0xffffffffu, sums[lane]);
+    const int64_t r0 = blockIdx.x * chunk, r1 = min(rows, r0 + chunk);
+    for (int64_t rb = r0; rb < r1; rb += kXentCountThreads) {
+        const int64_t r = rb + threadIdx.x;
+        const int64_t y = r < r1 ? labels[r] : -1;
+        const bool mine = labelled(y, classes);
+        const unsigned ballot = __ballot_sync(0xffffffffu, mine);
+        __syncthreads();
+        if (lane == 0) sums[warp] = __popc(ballot);
+        __syncthreads();
+        const int in_warp = sums[lane];
+        const int before = __reduce_add_sync(0xffffffffu, lane < warp ? in_warp : 0);
+        if (mine) {
+            const int to = at + before + __popc(ballot & ((1u << lane) - 1));
+            row_of[to] = (int32_t)r;
+            label[to] = (int32_t)y;
+        } else if (r < r1 && row_loss) {
+            row_loss[r] = 0.f;
+        }
+        at += __reduce_add_sync(0xffffffffu, in_warp);
+    }
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
+        *total = at;
+        *status = 0;
+    }
+}
+
+// ---- planes ----------------------------------------------------------------------------------------------
+struct XentPackArgs {
+    int32_t dtype, dim, dim_pad, classes;
+    int64_t rows;
+    const int32_t* count;
+    const int32_t* row_of;
+    const int64_t* labels;
+    const void* hidden;
+    int64_t hidden_stride;
+    uint16_t* h_planes;        // [P][rows_pad][dim_pad]
+    int64_t h_plane;
+    const void* weight;        // NULL: the weight is used where it lies
+    int64_t w_dim_stride, w_class_stride;
+    uint16_t* w_planes;        // [P][classes][dim_pad]
+    int64_t w_plane;
+    void* dhidden;             // rows without a label are set to 0
+    int64_t dhidden_stride;
+};
+
+// hi and lo of a float; an infinite or NaN hi has no lo
+__device__ __forceinline__ void split_bf16(float x, uint32_t& hi, uint32_t& lo) {
+    const __nv_bfloat16 h = __float2bfloat16_rn(x);
+    const float hf = __bfloat162float(h);
+    const __nv_bfloat16 l = __float2bfloat16_rn(isfinite(hf) ? x - hf : 0.f);
+    hi = __bfloat16_as_ushort(h);
+    lo = __bfloat16_as_ushort(l);
+}
+
+// One row of `dim` elements `stride` apart to the planes, by a warp; `src` NULL writes zeros.
+template <bool kFloat>
+__device__ __forceinline__ void pack_row(const void* src, int64_t stride, int dim, int dim_pad, uint16_t* to, int64_t plane, int lane) {
+    const bool vec = stride == 1 && (reinterpret_cast<uintptr_t>(src) & (kFloat ? 15 : 7)) == 0;
+    for (int d = 4 * lane; d < dim_pad; d += 128) {
+        if constexpr (kFloat) {
+            float x[4] = {0.f, 0.f, 0.f, 0.f};
+            const float* f = static_cast<const float*>(src);
+            if (src && vec && d + 4 <= dim) {
+                const float4 v = __ldg(reinterpret_cast<const float4*>(f + d));
+                x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+            } else if (src) {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (d + j < dim) x[j] = __ldg(f + (d + j) * stride);
+            }
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) split_bf16(x[j], h[j], l[j]);
+            *reinterpret_cast<uint2*>(to + d) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+            *reinterpret_cast<uint2*>(to + plane + d) = make_uint2(l[0] | l[1] << 16, l[2] | l[3] << 16);
+        } else {
+            uint2 v = make_uint2(0u, 0u);
+            const uint16_t* f = static_cast<const uint16_t*>(src);
+            if (src && vec && d + 4 <= dim) {
+                v = __ldg(reinterpret_cast<const uint2*>(f + d));
+            } else if (src) {
+                uint32_t x[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (d + j < dim) x[j] = __ldg(f + (d + j) * stride);
+                v = make_uint2(x[0] | x[1] << 16, x[2] | x[3] << 16);
+            }
+            *reinterpret_cast<uint2*>(to + d) = v;
+        }
+    }
+}
+
+constexpr int kXentPackThreads = 256;
+
+template <bool kFloat>
+__global__ void __launch_bounds__(kXentPackThreads) xent_pack_kernel(const XentPackArgs p) {
+    constexpr int kBytes = kFloat ? 4 : 2;
+    const int lane = threadIdx.x & 31;
+    const int64_t warps = (int64_t)gridDim.x * (kXentPackThreads / 32), w0 = grid_warp();
+    const int count = *p.count;
+    // labelled rows, and zeros up to a whole tile
+    const int64_t end = ((int64_t)count + kXentTileM - 1) / kXentTileM * kXentTileM;
+    for (int64_t i = w0; i < end; i += warps) {
+        const void* src = i < count ? static_cast<const char*>(p.hidden) + (int64_t)p.row_of[i] * p.hidden_stride * kBytes : nullptr;
+        pack_row<kFloat>(src, 1, p.dim, p.dim_pad, p.h_planes + i * p.dim_pad, p.h_plane, lane);
+    }
+    if (p.dhidden && count < p.rows) {
+        for (int64_t r = w0; r < p.rows; r += warps) {
+            if (labelled(p.labels[r], p.classes)) continue;
+            char* to = static_cast<char*>(p.dhidden) + r * p.dhidden_stride * kBytes;
+            for (int d = lane; d < p.dim; d += 32) {
+                if constexpr (kFloat) reinterpret_cast<float*>(to)[d] = 0.f;
+                else reinterpret_cast<uint16_t*>(to)[d] = 0;
+            }
+        }
+    }
+    if (!p.weight) return;
+    if (p.w_dim_stride == 1 || p.w_class_stride != 1) {
+        for (int64_t v = w0; v < p.classes; v += warps)
+            pack_row<kFloat>(static_cast<const char*>(p.weight) + v * p.w_class_stride * kBytes, p.w_dim_stride, p.dim, p.dim_pad,
+                             p.w_planes + v * p.dim_pad, p.w_plane, lane);
+        return;
+    }
+    // classes are contiguous: tiles of 32 x 32 turned over in shared memory
+    __shared__ uint32_t tile[kXentPackThreads / 32][32][33];
+    uint32_t(*t)[33] = tile[threadIdx.x >> 5];
+    const int64_t vt = (p.classes + 31) / 32, dt = (p.dim_pad + 31) / 32;
+    for (int64_t i = w0; i < vt * dt; i += warps) {
+        const int64_t v0 = i % vt * 32, d0 = i / vt * 32;
+        for (int j = 0; j < 32; j++) {
+            uint32_t x = 0;
+            if (d0 + j < p.dim && v0 + lane < p.classes) {
+                const int64_t at = (d0 + j) * p.w_dim_stride + v0 + lane;
+                if constexpr (kFloat) x = __ldg(static_cast<const uint32_t*>(p.weight) + at);
+                else x = __ldg(static_cast<const uint16_t*>(p.weight) + at);
+            }
+            t[j][lane] = x;
+        }
+        __syncwarp();
+        for (int j = 0; j < 32; j++) {
+            if (v0 + j < p.classes && d0 + lane < p.dim_pad) {
+                uint16_t* to = p.w_planes + (v0 + j) * p.dim_pad + d0 + lane;
+                const uint32_t x = t[lane][j];
+                if constexpr (kFloat) {
+                    uint32_t h, l;
+                    split_bf16(__uint_as_float(x), h, l);
+                    to[0] = (uint16_t)h;
+                    to[p.w_plane] = (uint16_t)l;
+                } else {
+                    to[0] = (uint16_t)x;
+                }
+            }
+        }
+        __syncwarp();
+    }
+}
+
+// ---- joining -----------------------------------------------------------------------------------------------
+// Log sums and losses of the rows from the parts of the classes, in the parts' order.
+__global__ void __launch_bounds__(256) xent_join_kernel(const XentArgs p) {
+    const int count = *p.count, lane = threadIdx.x & 31;
+    const int64_t end = ((int64_t)count + 31) / 32 * 32;
+    for (int64_t r = grid_thread(); r < end; r += (int64_t)gridDim.x * blockDim.x) {
+        float loss = 0.f;
+        if (r < count) {
+            float top = -INFINITY, sum = 0.f;
+            for (int i = 0; i < 2 * p.splits; i++) top = fmaxf(top, p.stats[(int64_t)i * p.rows_pad + r].x);
+            const float base = top == -INFINITY ? 0.f : top * kLog2e;
+            for (int i = 0; i < 2 * p.splits; i++) {
+                const float2 s = p.stats[(int64_t)i * p.rows_pad + r];
+                sum += s.y * fast_exp2(s.x * kLog2e - base);
+            }
+            const float lse2 = base + log2f(sum);
+            p.lse2[r] = lse2;
+            loss = fmaf(lse2, kLn2, -p.label_logit[r]);
+            if (p.row_loss) p.row_loss[p.row_of[r]] = loss;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+        if (lane == 0) p.warp_loss[r >> 5] = loss;
+    }
+}
+
+// Parts of a product summed in their order, scaled and written where the caller wants them: 4 values a thread, neighbouring
+// threads along the axis that is contiguous in the output.
+struct XentReduceArgs {
+    const float* part;
+    int64_t part_rows;
+    int32_t part_ld, splits;
+    int32_t m, n;
+    const int32_t* count;      // labelled rows (for the scale)
+    int32_t m_is_count;        // as many rows as are labelled, each to row_of[m]
+    const int32_t* row_of;
+    void* out;
+    int64_t out_m, out_n, m0;
+    int32_t out_type;
+    float scale;
+    int32_t mean;
+};
+
+__global__ void __launch_bounds__(256) xent_reduce_kernel(const XentReduceArgs p) {
+    const int count = *p.count;
+    const int64_t m_end = p.m_is_count ? count : p.m, n_vec = (p.n + 3) / 4;
+    const float scale = p.mean ? (count > 0 ? p.scale / (float)count : 0.f) : p.scale;
+    const bool m_fast = p.out_m == 1 && p.out_n != 1;
+    for (int64_t i = grid_thread(); i < m_end * n_vec; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t m = m_fast ? i % m_end : i / n_vec, n = 4 * (m_fast ? i / m_end : i % n_vec);
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < p.splits; s++) {
+            const float4 v = *reinterpret_cast<const float4*>(p.part + (s * p.part_rows + m) * p.part_ld + n);
+            a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+        }
+        const float v[4] = {scale * a.x, scale * a.y, scale * a.z, scale * a.w};
+        const int64_t at = (p.m_is_count ? (int64_t)p.row_of[m] : p.m0 + m) * p.out_m + n * p.out_n;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (n + j >= p.n) break;
+            if (p.out_type == MASK_F32) static_cast<float*>(p.out)[at + j * p.out_n] = v[j];
+            else if (p.out_type == MASK_F16) static_cast<__half*>(p.out)[at + j * p.out_n] = __float2half_rn(v[j]);
+            else static_cast<__nv_bfloat16*>(p.out)[at + j * p.out_n] = __float2bfloat16_rn(v[j]);
+        }
+    }
+}
+
+// The loss of all rows, in a fixed order and 64 bits; NaN where a kernel gave up on a wait.
+__global__ void __launch_bounds__(1024) xent_loss_kernel(const int32_t* count_, const float* __restrict__ warp_loss, const int32_t* status, float* loss,
+                                                         int64_t rows, int reduction) {
+    const int count = *count_;
+    if (*status) {
+        const int64_t n = reduction == MASK_REDUCE_NONE ? rows : 1;
+        for (int64_t r = threadIdx.x; r < n; r += 1024) loss[r] = NAN;
+        return;
+    }
+    if (reduction == MASK_REDUCE_NONE) return;
+    __shared__ double sums[32];
+    double sum = 0.0;
+    for (int64_t i = threadIdx.x; i < ((int64_t)count + 31) / 32; i += 1024) sum += warp_loss[i];
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        sum = sums[threadIdx.x];
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (threadIdx.x == 0) *loss = count == 0 ? 0.f : (float)(reduction == MASK_REDUCE_MEAN ? sum / count : sum);
+    }
+}
+
+// ---- plan of a call ---------------------------------------------------------------------------------------
+static int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+
+struct XentPlan {
+    int planes, dim_pad;
+    int64_t rows_pad, chunk;
+    int n_chunks;
+    bool grads, one_pass, pack_weight;
+    int bn_logits, bn_dim;
+    int stats_splits;
+    int piece, n_pieces;                 // classes of a piece (a multiple of 256 unless one tile holds all), pieces
+    int g_ld;
+    int dh_splits, dw_splits;
+    bool dh_parts, dw_parts;
+    int64_t part_dh_rows, part_dw_rows;
+    int part_ld;
+    // byte offsets into the scratch
+    size_t counts, row_of, label, total, stats, label_logit, lse2, warp_loss, h_planes, w_planes, g, part_dh, part_dw, bytes;
+};
+
+// Parts to cut `units` of work per tile into, so that `tiles` tiles fill the SMs: the fewest rounds of the longest part.
+// A part costs two units beside its own (the accumulator's way out).
+static int best_splits(int64_t tiles, int64_t units, int64_t sms) {
+    int64_t best = 1, best_cost = INT64_MAX;
+    const int64_t most = std::min<int64_t>(units, std::max<int64_t>(1, 4 * sms / std::max<int64_t>(tiles, 1)));
+    for (int64_t s = 1; s <= most; s++) {
+        const int64_t cost = (tiles * s + sms - 1) / sms * ((units + s - 1) / s + 2);
+        if (cost < best_cost) { best_cost = cost; best = s; }
+    }
+    return (int)best;
+}
+
+static int tile_width(int n) {
+    if (n <= 64) return 64;
+    return n <= 128 || round_up(n, 128) < round_up(n, 256) ? 128 : 256;
+}
+
+static XentPlan plan_xent(const mask_head& h) {
+    XentPlan p = {};
+    const int64_t sms = sm_count();
+    p.planes = h.dtype == MASK_F32 ? 2 : 1;
+    p.dim_pad = (int)round_up(h.dim, 8);
+    p.rows_pad = round_up(std::max<int64_t>(h.rows, 1), kXentTileM);
+    p.chunk = std::max<int64_t>(kXentCountThreads, round_up((h.rows + 2047) / 2048, kXentCountThreads));
+    p.n_chunks = (int)std::max<int64_t>(1, (h.rows + p.chunk - 1) / p.chunk);
+    p.grads = h.d_dhidden || h.d_dweight;
+    p.pack_weight = p.planes == 2 || h.weight_dim_stride != 1 || h.weight_class_stride % 8 || h.weight_class_stride < h.dim ||
+                    (reinterpret_cast<uintptr_t>(h.d_weight) & 15);
+    p.bn_logits = h.classes <= 64 ? 64 : (h.classes <= 128 ? 128 : 256);
+    p.bn_dim = tile_width(h.dim);
+    p.one_pass = p.grads && h.classes <= 256;
+    const int64_t m_tiles = p.rows_pad / kXentTileM;
+    p.stats_splits = p.one_pass ? 1 : best_splits(m_tiles, (h.classes + p.bn_logits - 1) / p.bn_logits, sms);
+    if (p.grads) {
+        if (p.one_pass) {
+            p.piece = h.classes;
+            p.g_ld = (int)round_up(p.bn_logits, 128);
+        } else {
+            const int64_t fit = (int64_t)(kXentPieceBytes / (size_t)(2 * p.planes * p.rows_pad)) / 256 * 256;
+            p.piece = p.g_ld = (int)std::min<int64_t>(round_up(h.classes, 256), std::max<int64_t>(fit, 256));
+        }
+        p.n_pieces = (int)((h.classes + (int64_t)p.piece - 1) / p.piece);
+        const int64_t n_tiles = (h.dim + p.bn_dim - 1) / p.bn_dim;
+        p.part_ld = (int)(n_tiles * p.bn_dim);
+        if (h.d_dhidden) {
+            p.dh_splits = best_splits(m_tiles * n_tiles, (p.piece + kXentTileK - 1) / kXentTileK, sms);
+            p.dh_parts = p.dh_splits > 1 || p.n_pieces > 1;
+            p.part_dh_rows = p.rows_pad;
+        }
+        if (h.d_dweight) {
+            p.dw_splits = best_splits((p.piece + kXentTileM - 1) / kXentTileM * n_tiles, (p.rows_pad + kXentTileK - 1) / kXentTileK, sms);
+            p.dw_parts = p.dw_splits > 1;
+            p.part_dw_rows = round_up(p.piece, kXentTileM);
+        }
+    }
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const size_t rp = (size_t)p.rows_pad;
+    p.total = take(256);
+    p.counts = take(4 * (size_t)p.n_chunks);
+    p.row_of = take(4 * rp);
+    p.label = take(4 * rp);
+    p.stats = p.one_pass ? 0 : take(16 * rp * p.stats_splits);
+    p.label_logit = take(4 * rp);
+    p.lse2 = take(4 * rp);
+    p.warp_loss = take(rp / 8);
+    p.h_planes = take(2 * (size_t)p.planes * rp * p.dim_pad);
+    p.w_planes = p.pack_weight ? take(2 * (size_t)p.planes * h.classes * p.dim_pad) : 0;
+    if (p.grads) {
+        p.g = take(2 * (size_t)p.planes * rp * p.g_ld);
+        if (p.dh_parts) p.part_dh = take(4 * (size_t)p.dh_splits * p.part_dh_rows * p.part_ld);
+        if (p.dw_parts) p.part_dw = take(4 * (size_t)p.dw_splits * p.part_dw_rows * p.part_ld);
+    }
+    p.bytes = at;
+    return p;
+}
+
+// Planes of 16-bit values as a tensor [planes][rows][columns], `ld` elements from row to row.
+static int plane_map(CUtensorMap* map, const void* data, int64_t cols, int64_t rows, int planes, int64_t ld, int64_t plane, int box_cols, int box_rows) {
+    EncodeTiledFn enc = encode_tiled_fn();
+    if (!enc) return fail(MASK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)planes};
+    const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)plane * 2};
+    const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(data), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        set_error("cuTensorMapEncodeTiled failed with code %d (%lld x %lld, pitch %lld)", (int)r, (long long)rows, (long long)cols, (long long)ld);
+        return MASK_ERR_CUDA;
+    }
+    return MASK_OK;
+}
+
+template <int BN, int P, int MODE>
+static int launch_xent_gemm_as(const XentArgs& a, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mg, int64_t items, cudaStream_t st) {
+    using L = XentLayout<BN, P, MODE>;
+    static std::atomic<uint64_t> done{0};
+    const int rc = opt_in_shared_memory(reinterpret_cast<const void*>(xent_gemm_kernel<BN, P, MODE>), L::kDynamicBytes, done);
+    if (rc != MASK_OK) return rc;
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(items, sm_count()));
+    xent_gemm_kernel<BN, P, MODE><<<grid, kXentThreads, L::kDynamicBytes, st>>>(a, ma, mb, mg);
+    MASK_CUDA_TRY(cudaGetLastError());
+    return MASK_OK;
+}
+
+template <int MODE>
+static int launch_xent_gemm(int bn, int planes, const XentArgs& a, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mg, int64_t items,
+                            cudaStream_t st) {
+    if (planes == 1) {
+        if (bn == 64) return launch_xent_gemm_as<64, 1, MODE>(a, ma, mb, mg, items, st);
+        if (bn == 128) return launch_xent_gemm_as<128, 1, MODE>(a, ma, mb, mg, items, st);
+        return launch_xent_gemm_as<256, 1, MODE>(a, ma, mb, mg, items, st);
+    }
+    if (bn == 64) return launch_xent_gemm_as<64, 2, MODE>(a, ma, mb, mg, items, st);
+    if (bn == 128) return launch_xent_gemm_as<128, 2, MODE>(a, ma, mb, mg, items, st);
+    return launch_xent_gemm_as<256, 2, MODE>(a, ma, mb, mg, items, st);
+}
+
+static const char* refuse_head(const mask_head* h) {
+    if (!h) return "head is NULL";
+    if (h->dtype < MASK_F32 || h->dtype > MASK_F16) return "dtype must be MASK_F32, MASK_BF16 or MASK_F16";
+    if (h->reduction < MASK_REDUCE_NONE || h->reduction > MASK_REDUCE_SUM) return "reduction must be MASK_REDUCE_NONE, _MEAN or _SUM";
+    constexpr int64_t most = ((int64_t)1 << 31) - 256;
+    if (h->rows < 0 || h->rows >= most) return "rows out of range";
+    if (h->dim < 1 || h->dim >= most || h->classes < 1 || h->classes >= most) return "dim and classes must be at least 1 and below 2^31 - 256";
+    if (h->hidden_stride < 0 || h->weight_dim_stride < 0 || h->weight_class_stride < 0 || h->dhidden_stride < 0 || h->dweight_dim_stride < 0 ||
+        h->dweight_class_stride < 0)
+        return "strides must not be negative";
+    if (!h->d_weight || (h->rows > 0 && (!h->d_hidden || !h->d_labels))) return "an operand is NULL";
+    if (!h->d_loss && (h->reduction != MASK_REDUCE_NONE || h->rows > 0)) return "loss is NULL";
+    const uintptr_t element = h->dtype == MASK_F32 ? 3 : 1;
+    if ((reinterpret_cast<uintptr_t>(h->d_hidden) | reinterpret_cast<uintptr_t>(h->d_weight) | reinterpret_cast<uintptr_t>(h->d_dhidden) |
+         reinterpret_cast<uintptr_t>(h->d_dweight)) & element)
+        return "an operand is not aligned to its type";
+    if ((reinterpret_cast<uintptr_t>(h->d_loss) & 3) || (reinterpret_cast<uintptr_t>(h->d_labels) & 7)) return "loss or labels are not aligned to their type";
+    if (h->d_dhidden && h->rows > 1 && h->dhidden_stride < h->dim) return "rows of dhidden overlap";
+    return nullptr;
+}
+
+static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cudaStream_t st) {
+    auto at = [&](size_t offset) { return scratch + offset; };
+    int32_t* total = reinterpret_cast<int32_t*>(at(plan.total));
+    int32_t* row_of = reinterpret_cast<int32_t*>(at(plan.row_of));
+    int32_t* label = reinterpret_cast<int32_t*>(at(plan.label));
+    int32_t* counts = reinterpret_cast<int32_t*>(at(plan.counts));
+    float* row_loss = h.reduction == MASK_REDUCE_NONE ? h.d_loss : nullptr;
+    const int P = plan.planes;
+    const int64_t rp = plan.rows_pad, m_tiles = rp / kXentTileM;
+
+    if (plan.n_chunks > 1) xent_count_kernel<<<plan.n_chunks, kXentCountThreads, 0, st>>>(h.d_labels, h.rows, h.classes, plan.chunk, counts);
+    xent_number_kernel<<<plan.n_chunks, kXentCountThreads, 0, st>>>(h.d_labels, h.rows, h.classes, plan.chunk, counts, row_of, label, total, total + 1, row_loss);
+    MASK_CUDA_TRY(cudaGetLastError());
+
+    XentPackArgs pk = {};
+    pk.dtype = h.dtype; pk.dim = h.dim; pk.dim_pad = plan.dim_pad; pk.classes = h.classes; pk.rows = h.rows;
+    pk.count = total; pk.row_of = row_of; pk.labels = h.d_labels;
+    pk.hidden = h.d_hidden; pk.hidden_stride = h.hidden_stride;
+    pk.h_planes = reinterpret_cast<uint16_t*>(at(plan.h_planes)); pk.h_plane = rp * plan.dim_pad;
+    pk.dhidden = h.d_dhidden; pk.dhidden_stride = h.dhidden_stride;
+    if (plan.pack_weight) {
+        pk.weight = h.d_weight; pk.w_dim_stride = h.weight_dim_stride; pk.w_class_stride = h.weight_class_stride;
+        pk.w_planes = reinterpret_cast<uint16_t*>(at(plan.w_planes)); pk.w_plane = (int64_t)h.classes * plan.dim_pad;
+    }
+    const int64_t pack_rows = rp + (plan.pack_weight ? h.classes : 0);
+    const unsigned pack_grid = (unsigned)std::min<int64_t>((pack_rows + 7) / 8, 8 * (int64_t)sm_count());
+    if (h.dtype == MASK_F32) xent_pack_kernel<true><<<pack_grid, kXentPackThreads, 0, st>>>(pk);
+    else xent_pack_kernel<false><<<pack_grid, kXentPackThreads, 0, st>>>(pk);
+    MASK_CUDA_TRY(cudaGetLastError());
+
+    const void* w_data = plan.pack_weight ? (const void*)pk.w_planes : h.d_weight;
+    const int64_t w_ld = plan.pack_weight ? plan.dim_pad : h.weight_class_stride, w_plane = plan.pack_weight ? pk.w_plane : w_ld * h.classes;
+    const int w_cols = plan.pack_weight ? plan.dim_pad : h.dim;
+    int rc;
+    CUtensorMap h_k, w_k, none = {};     // K-major, contracted over dim
+    if ((rc = plane_map(&h_k, pk.h_planes, plan.dim_pad, rp, P, plan.dim_pad, pk.h_plane, 64, kXentTileM))) return rc;
+    if ((rc = plane_map(&w_k, w_data, w_cols, h.classes, P, w_ld, w_plane, 64, plan.bn_logits))) return rc;
+
+    XentArgs a = {};
+    a.count = total; a.status = total + 1;
+    a.classes = h.classes; a.dim = h.dim; a.v0 = 0; a.vc = h.classes;
+    a.rows_pad = (int32_t)rp; a.half_type = h.dtype == MASK_F16;
+    a.label = label; a.row_of = row_of; a.row_loss = row_loss;
+    a.stats = reinterpret_cast<float2*>(at(plan.stats));
+    a.label_logit = reinterpret_cast<float*>(at(plan.label_logit));
+    a.lse2 = reinterpret_cast<float*>(at(plan.lse2));
+    a.warp_loss = reinterpret_cast<float*>(at(plan.warp_loss));
+    a.scale = h.grad_scale; a.mean = h.reduction == MASK_REDUCE_MEAN;
+    a.out_type = h.dtype;
+
+    if (!plan.one_pass) {
+        a.splits = plan.stats_splits;
+        if ((rc = launch_xent_gemm<kXentStats>(plan.bn_logits, P, a, h_k, w_k, none, m_tiles * a.splits, st))) return rc;
+        xent_join_kernel<<<(unsigned)std::min<int64_t>((rp + 255) / 256, 4 * (int64_t)sm_count()), 256, 0, st>>>(a);
+        MASK_CUDA_TRY(cudaGetLastError());
+    }
+    if (plan.grads) {
+        char* g = at(plan.g);
+        const int64_t g_plane = rp * plan.g_ld;
+        CUtensorMap g_st, g_k, g_mn, w_mn, h_mn;
+        if ((rc = plane_map(&g_st, g, plan.g_ld, rp, P, plan.g_ld, g_plane, 32, 32))) return rc;
+        if ((rc = plane_map(&g_k, g, plan.g_ld, rp, P, plan.g_ld, g_plane, 64, kXentTileM))) return rc;
+        if ((rc = plane_map(&g_mn, g, plan.g_ld, rp, P, plan.g_ld, g_plane, 64, 64))) return rc;
+        if ((rc = plane_map(&w_mn, w_data, w_cols, h.classes, P, w_ld, w_plane, 64, 64))) return rc;
+        if ((rc = plane_map(&h_mn, pk.h_planes, plan.dim_pad, rp, P, plan.dim_pad, pk.h_plane, 64, 64))) return rc;
+        const int64_t n_tiles = plan.part_ld / plan.bn_dim;
+        const unsigned most_blocks = (unsigned)(8 * sm_count());
+        XentReduceArgs r = {};
+        r.part_ld = plan.part_ld; r.n = h.dim; r.count = total; r.row_of = row_of; r.out_type = h.dtype; r.scale = a.scale; r.mean = a.mean;
+        const uintptr_t vec = h.dtype == MASK_F32 ? 4 : 8;      // elements of 16 bytes
+        for (int piece = 0; piece < plan.n_pieces; piece++) {
+            a.v0 = piece * plan.piece;
+            a.vc = std::min(plan.piece, h.classes - a.v0);
+            const int64_t v_tiles = (a.vc + plan.bn_logits - 1) / plan.bn_logits;
+            if (plan.one_pass) rc = launch_xent_gemm<kXentGradOne>(plan.bn_logits, P, a, h_k, w_k, g_st, m_tiles, st);
+            else rc = launch_xent_gemm<kXentGrad>(plan.bn_logits, P, a, h_k, w_k, g_st, m_tiles * v_tiles, st);
+            if (rc) return rc;
+            if (h.d_dhidden) {
+                XentArgs b = a;
+                b.splits = plan.dh_splits;
+                b.store = !plan.dh_parts ? kXentFinal : (piece == 0 ? kXentPartial : kXentAccumulate);
+                b.part = reinterpret_cast<float*>(at(plan.part_dh)); b.part_rows = plan.part_dh_rows; b.part_ld = plan.part_ld;
+                b.out = h.d_dhidden; b.out_m = h.dhidden_stride; b.out_n = 1;
+                b.out_vec = h.dhidden_stride % (int64_t)vec == 0 && (reinterpret_cast<uintptr_t>(h.d_dhidden) & 15) == 0;
+                if ((rc = launch_xent_gemm<kXentDHidden>(plan.bn_dim, P, b, g_k, w_mn, none, m_tiles * n_tiles * b.splits, st))) return rc;
+            }
+            if (h.d_dweight) {
+                XentArgs b = a;
+                b.splits = plan.dw_splits;
+                b.store = plan.dw_parts ? kXentPartial : kXentFinal;
+                b.part = reinterpret_cast<float*>(at(plan.part_dw)); b.part_rows = plan.part_dw_rows; b.part_ld = plan.part_ld;
+                b.out = h.d_dweight; b.out_m = h.dweight_class_stride; b.out_n = h.dweight_dim_stride;
+                b.out_vec = b.out_n == 1 && b.out_m % (int64_t)vec == 0 && (reinterpret_cast<uintptr_t>(h.d_dweight) & 15) == 0;
+                const int64_t wm_tiles = (a.vc + kXentTileM - 1) / kXentTileM;
+                if ((rc = launch_xent_gemm<kXentDWeight>(plan.bn_dim, P, b, g_mn, h_mn, none, wm_tiles * n_tiles * b.splits, st))) return rc;
+                if (plan.dw_parts) {
+                    XentReduceArgs w = r;
+                    w.part = b.part; w.part_rows = b.part_rows; w.splits = b.splits; w.m = a.vc; w.m0 = a.v0;
+                    w.out = b.out; w.out_m = b.out_m; w.out_n = b.out_n;
+                    const int64_t n = (int64_t)w.m * ((w.n + 3) / 4);
+                    xent_reduce_kernel<<<std::min(blocks_for(n, 256), most_blocks), 256, 0, st>>>(w);
+                    MASK_CUDA_TRY(cudaGetLastError());
+                }
+            }
+        }
+        if (h.d_dhidden && plan.dh_parts) {
+            r.part = reinterpret_cast<float*>(at(plan.part_dh)); r.part_rows = plan.part_dh_rows; r.splits = plan.dh_splits;
+            r.m_is_count = 1;
+            r.out = h.d_dhidden; r.out_m = h.dhidden_stride; r.out_n = 1;
+            const int64_t n = rp * ((r.n + 3) / 4);
+            xent_reduce_kernel<<<(unsigned)std::min<int64_t>((n + 255) / 256, most_blocks), 256, 0, st>>>(r);
+            MASK_CUDA_TRY(cudaGetLastError());
+        }
+    }
+    xent_loss_kernel<<<1, 1024, 0, st>>>(total, a.warp_loss, total + 1, h.d_loss, h.rows, h.reduction);
+    MASK_CUDA_TRY(cudaGetLastError());
+    return MASK_OK;
+}
+
+}  // namespace mask
+
+extern "C" size_t mask_linear_xent_scratch_bytes(const mask_head* head) {
+    if (const char* why = mask::refuse_head(head)) {
+        mask::set_error("%s", why);
+        return 0;
+    }
+    return mask::plan_xent(*head).bytes;
+}
+
+extern "C" int mask_linear_xent(const mask_head* head, void* d_scratch, size_t scratch_bytes, void* stream) {
+    using namespace mask;
+    if (const char* why = refuse_head(head)) return fail(MASK_ERR_INVALID_ARGUMENT, why);
+    const XentPlan plan = plan_xent(*head);
+    MASK_REQUIRE(d_scratch != nullptr && (reinterpret_cast<uintptr_t>(d_scratch) & 255) == 0, "scratch must be 256-byte aligned");
+    if (scratch_bytes < plan.bytes) return fail(MASK_ERR_SCRATCH_TOO_SMALL, "scratch is smaller than mask_linear_xent_scratch_bytes");
+    return run_xent(*head, plan, static_cast<char*>(d_scratch), static_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,563 @@
+// The matrix products of the classifier head (xent.cu) on the tensor cores: logits = H W with the statistics of the
+// softmax or its gradient as epilogue, and the two products of that gradient G with W and with H.
+//
+// One persistent block per SM: a producer thread feeds a ring of stages by TMA, one thread issues the MMAs into two
+// accumulators of tensor memory, eight warps take the finished accumulator apart while the next one is computed.
+// Operands are 16-bit "planes": one for bf16 and fp16 input; FP32 input is split into two bf16 planes, x = hi + lo + e with
+// |e| <= 2^-18 |x|, and a product is hi hi + hi lo + lo hi (the dropped lo lo is 2^-18 of it at most).  All three
+// products have the layouts TMA and the MMA take as they are, whichever axis is contracted:
+//     logits[r,v] = sum_d H[r,d] W[v,d]     both operands K-major
+//     dH[r,d]     = sum_v G[r,v] W[v,d]     G K-major, W MN-major
+//     dW[v,d]     = sum_r G[r,v] H[r,d]     both MN-major
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "launch.cuh"
+#include "umma_ptx.cuh"
+
+namespace mask {
+
+constexpr int kXentTileM = 128, kXentTileK = 64;
+constexpr int kXentWarps = 8;                       // epilogue warps: 4 quarters of 32 rows x 2 halves of the columns
+constexpr int kXentThreads = 32 * (kXentWarps + 2);   // + producer + MMA issuer
+
+enum XentMode {
+    kXentStats,      // logits -> running maximum and sum of each row over a range of classes
+    kXentGrad,       // logits -> G of a piece of the classes, with the rows' log sums known
+    kXentGradOne,    // the same where one tile holds all classes: log sum, loss and G in one pass
+    kXentDHidden,    // G W
+    kXentDWeight     // G^T H
+};
+
+enum XentStore { kXentFinal, kXentPartial, kXentAccumulate };
+
+struct XentArgs {
+    const int32_t* count;      // labelled rows (device)
+    int32_t classes, dim;
+    int32_t v0, vc;            // piece of the classes
+    int32_t splits;            // stats: parts of the classes' tiles; products: parts of the contraction
+    int32_t rows_pad;
+    int32_t half_type;         // planes hold fp16 instead of bf16
+    const int32_t* label;      // [labelled row]
+    const int32_t* row_of;     // [labelled row] -> row of the caller's arrays
+    float2* stats;             // [2 * splits][rows_pad]: maximum, sum of exp(logit - maximum)
+    float* label_logit;        // [labelled row]
+    float* lse2;               // [labelled row]: log2 of the row's sum of exponentials
+    float* row_loss;           // caller's, or NULL
+    float* warp_loss;          // [rows_pad / 32]: sums of 32 rows' losses
+    float* part;               // [splits][m_pad][n_pad]
+    int64_t part_rows;         // m_pad
+    int32_t part_ld;           // n_pad
+    int32_t store;             // XentStore
+    void* out;                 // final store: element (m, n) at m * out_m + n * out_n
+    int64_t out_m, out_n;
+    int32_t out_type;          // MASK_F32 / MASK_BF16 / MASK_F16
+    int32_t out_vec;           // rows of 32 values may be written as 16-byte vectors
+    float scale;
+    int32_t mean;              // scale / count
+    int32_t* status;
+};
+
+__device__ __forceinline__ float xent_scale(const XentArgs& p, int count) { return p.mean ? (count > 0 ? p.scale / (float)count : 0.f) : p.scale; }
+
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+template <int BN, int P, int MODE>
+struct XentLayout {
+    static constexpr bool kWritesG = MODE == kXentGrad || MODE == kXentGradOne;
+    static constexpr int kTileA = kXentTileM * kXentTileK * 2, kTileB = BN * kXentTileK * 2;
+    static constexpr int kStage = P * (kTileA + kTileB);
+    static constexpr int kStaging = kWritesG ? kXentWarps * 4096 : 0;      // 32 rows x 32 columns x 2 planes or buffers a warp
+    static constexpr int kMost = 227 * 1024 - 1024 - 256 - kStaging;
+    static constexpr int S = kMost / kStage < 8 ? kMost / kStage : 8;
+    static constexpr int kTmemCols = 2 * BN;
+    static constexpr int kStagingAt = S * kStage;
+    static constexpr int kBars = kStagingAt + kStaging;
+    static constexpr int kNumBars = 2 * S + 4 + 1;
+    static constexpr int kTmemSlot = kBars + kNumBars * 8;
+    static constexpr int kAbort = kTmemSlot + 8;
+    static constexpr int kBytes = kAbort + 8;
+    static constexpr int kDynamicBytes = kBytes + 1024;                    // room to align the base
+    static_assert(S >= 2 && kDynamicBytes <= 227 * 1024 && kTmemCols <= 512, "tile does not fit");
+};
+
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]),
+          "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]),
+          "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(taddr)
+        : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+}
+__device__ __forceinline__ void xent_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b, bool half_type) {
+    if (half_type) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Adds 32 logits of a row to its running maximum and sum.
+__device__ __forceinline__ void online_softmax(const float (&v)[32], float& top, float& sum) {
+    float t[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int i = 4; i < 32; i++) t[i & 3] = fmaxf(t[i & 3], v[i]);
+    const float now = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+    const float base = now == -INFINITY ? 0.f : now * kLog2e;    // a row that has seen only -inf
+    float s[4] = {sum * fast_exp2(top * kLog2e - base), 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 32; i++) s[i & 3] += fast_exp2(fmaf(v[i], kLog2e, -base));
+    sum = (s[0] + s[1]) + (s[2] + s[3]);
+    top = now;
+}
+
+template <int BN, int P, int MODE>
+__global__ void __launch_bounds__(kXentThreads, 1)
+xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                 const __grid_constant__ CUtensorMap map_g) {
+    using L = XentLayout<BN, P, MODE>;
+    constexpr int S = L::S;
+    constexpr bool kLogits = MODE == kXentStats || MODE == kXentGrad || MODE == kXentGradOne;
+    constexpr bool kAmn = MODE == kXentDWeight, kBmn = !kLogits;
+    extern __shared__ unsigned char xent_smem_raw[];
+    const uint32_t raw = (uint32_t)__cvta_generic_to_shared(xent_smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    unsigned char* gbase = xent_smem_raw + (base - raw);
+    const uint32_t bars = base + L::kBars;
+    auto full_bar = [&](int s) { return bars + 8u * s; };
+    auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
+    auto accf_bar = [&](int b) { return bars + 8u * (2 * S + b); };
+    auto acce_bar = [&](int b) { return bars + 8u * (2 * S + 2 + b); };
+    const uint32_t drain_bar = bars + 8u * (2 * S + 4);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kAbort);
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + L::kTmemSlot);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < S; s++) {
+            mbar_init(full_bar(s), 1);
+            mbar_init(empty_bar(s), 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(accf_bar(b), 1);
+            mbar_init(acce_bar(b), MODE == kXentGradOne ? kXentWarps / 2 : kXentWarps);
+        }
+        mbar_init(drain_bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kXentWarps + 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kTmemSlot), "r"(L::kTmemCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *tmem_slot;
+
+    // ---- work: an item is a tile of rows with a range of column tiles and a range of blocks of the contraction ----------
+    const int count = *p.count;
+    const int m_extent = MODE == kXentDWeight ? p.vc : count;
+    const int n_extent = kLogits ? p.vc : p.dim;
+    const int k_extent = kLogits ? p.dim : (MODE == kXentDHidden ? p.vc : count);
+    const int m_tiles = (m_extent + kXentTileM - 1) / kXentTileM, n_tiles = (n_extent + BN - 1) / BN;
+    const int k_blocks = (k_extent + kXentTileK - 1) / kXentTileK;
+    // stats: parts of the column tiles; G: every tile an item; products: every tile once for each part of the contraction
+    const int64_t items = (int64_t)m_tiles * (MODE == kXentStats ? p.splits : (kLogits ? n_tiles : n_tiles * p.splits));
+    struct Item { int m, split, n0, n1, k0, k1; };
+    auto item_of = [&](int64_t i) {
+        Item t;
+        if constexpr (kLogits) {          // row tiles fastest: blocks that run together read the same tile of W
+            const int q = (int)(i / m_tiles);
+            t.m = (int)(i - (int64_t)q * m_tiles);
+            t.split = MODE == kXentStats ? q : 0;
+            t.n0 = MODE == kXentStats ? (int)((int64_t)n_tiles * q / p.splits) : q;
+            t.n1 = MODE == kXentStats ? (int)((int64_t)n_tiles * (q + 1) / p.splits) : q + 1;
+            t.k0 = 0;
+            t.k1 = k_blocks;
+        } else {                          // column tiles fastest: they share the tile of G
+            const int64_t q = i / n_tiles;
+            t.n0 = (int)(i - q * n_tiles);
+            t.n1 = t.n0 + 1;
+            t.split = (int)(q / m_tiles);
+            t.m = (int)(q - (int64_t)t.split * m_tiles);
+            t.k0 = (int)((int64_t)k_blocks * t.split / p.splits);
+            t.k1 = (int)((int64_t)k_blocks * (t.split + 1) / p.splits);
+        }
+        return t;
+    };
+
+    if (warp == kXentWarps) {
+        // ------------------------------ producer -----------------------------------------------------------------------
+        if (lane == 0) {
+            int s = 0;
+            uint32_t round = 0;
+            bool ok = true;
+            for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+                const Item t = item_of(i);
+                for (int n = t.n0; n < t.n1 && ok; n++) {
+                    for (int k = t.k0; k < t.k1; k++) {
+                        if (round > 0 && !mbar_wait(empty_bar(s), (round - 1) & 1, abort_flag)) { ok = false; break; }
+                        const uint32_t bar = full_bar(s), at = base + s * L::kStage;
+                        xent_expect_tx(bar, L::kStage);
+#pragma unroll
+                        for (int z = 0; z < P; z++) {
+                            const uint32_t a = at + z * L::kTileA, b = at + P * L::kTileA + z * L::kTileB;
+                            if constexpr (kAmn) {
+#pragma unroll
+                                for (int j = 0; j < kXentTileM / 64; j++)
+                                    tma_load_3d(a + j * 8192, &map_a, bar, t.m * kXentTileM + j * 64, k * kXentTileK, z);
+                            } else {
+                                tma_load_3d(a, &map_a, bar, k * kXentTileK, t.m * kXentTileM, z);
+                            }
+                            if constexpr (kBmn) {
+#pragma unroll
+                                for (int j = 0; j < BN / 64; j++)
+                                    tma_load_3d(b + j * 8192, &map_b, bar, n * BN + j * 64, (MODE == kXentDHidden ? p.v0 : 0) + k * kXentTileK, z);
+                            } else {
+                                tma_load_3d(b, &map_b, bar, k * kXentTileK, p.v0 + n * BN, z);
+                            }
+                        }
+                        if (++s == S) { s = 0; round++; }
+                    }
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == kXentWarps + 1) {
+        // ------------------------------ MMA issuer ---------------------------------------------------------------------
+        if (lane == 0) {
+            const uint32_t fmt = p.half_type ? 0u : 1u;
+            // instruction descriptor: D = F32, A and B bf16 or fp16, M = 128
+            const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) |
+                                   ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kXentTileM >> 4) << 24);
+            // 128-byte swizzle; K-major: groups of 8 rows 1024 bytes apart; MN-major: 64-wide atoms 8192 bytes apart, groups of 8 k 1024
+            const uint64_t a0 = umma_smem_desc(base, kAmn ? 512 : 1, 64, 2);
+            const uint64_t b0 = umma_smem_desc(base + P * L::kTileA, kBmn ? 512 : 1, 64, 2);
+            constexpr uint32_t kStepA = kAmn ? 128 : 2, kStepB = kBmn ? 128 : 2;   // 16 of the contraction, in 16 bytes
+            int s = 0;
+            uint32_t round = 0, acc_it = 0;
+            bool ok = true;
+            for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+                const Item t = item_of(i);
+                if (t.k0 >= t.k1) continue;
+                for (int n = t.n0; n < t.n1 && ok; n++) {
+                    const uint32_t buf = acc_it & 1, acc = tmem_base + buf * BN;
+                    if (acc_it >= 2 && !mbar_wait(acce_bar(buf), ((acc_it >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    uint32_t open = 0;
+                    for (int k = t.k0; k < t.k1; k++) {
+                        if (!mbar_wait_spin(full_bar(s), round & 1, abort_flag)) { ok = false; break; }
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint64_t a = a0 + (uint64_t)(s * L::kStage >> 4), b = b0 + (uint64_t)(s * L::kStage >> 4);
+#pragma unroll
+                        for (int c = 0; c < (P == 2 ? 3 : 1); c++) {     // hi hi, hi lo, lo hi
+                            const uint64_t ac = a + (c == 2 ? L::kTileA >> 4 : 0), bc = b + (c == 1 ? L::kTileB >> 4 : 0);
+#pragma unroll
+                            for (int j = 0; j < kXentTileK / 16; j++) {
+                                umma_f16(acc, ac + j * kStepA, bc + j * kStepB, idesc, open);
+                                open = 1;
+                            }
+                        }
+                        umma_commit(empty_bar(s));
+                        if (++s == S) { s = 0; round++; }
+                    }
+                    if (!ok) break;
+                    umma_commit(accf_bar(buf));
+                    acc_it++;
+                }
+            }
+            umma_commit(drain_bar);
+            const long long start = clock64();
+            while (!mbar_test(drain_bar, 0)) {
+                if (clock64() - start > kUmmaWaitCycles) { *abort_flag = 1; break; }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ------------------------------ epilogue -----------------------------------------------------------------------
+        constexpr int kHalf = BN / 2;
+        const int quarter = warp & 3, half = warp >> 2;
+        uint32_t acc_it = 0;
+        bool ok = true;
+        const bool half_type = p.half_type != 0;
+        [[maybe_unused]] const uint32_t staging = base + L::kStagingAt + warp * 4096;
+        [[maybe_unused]] uint32_t stage_it = 0;
+        // waits for the next accumulator; its address for this warp
+        auto acquire = [&]() -> uint32_t {
+            const uint32_t buf = acc_it & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(accf_bar(buf), (acc_it >> 1) & 1, abort_flag))) ok = false;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            return tmem_base + ((uint32_t)(32 * quarter) << 16) + buf * BN + half * kHalf;
+        };
+        auto release = [&]() {
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acce_bar(acc_it & 1));
+            acc_it++;
+        };
+        // G of 32 columns to global memory through this warp's staging buffer
+        [[maybe_unused]] auto write_g = [&](const float (&g)[32], int m, int col) {
+            if constexpr (L::kWritesG) {
+                // P == 1: two buffers in turn, so the older copy may still be read; P == 2: both planes at once
+                if (lane == 0) {
+                    if constexpr (P == 1) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                    else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                }
+                __syncwarp();
+                const uint32_t row = staging + lane * 64, x = (lane >> 1) & 3;
+                const uint32_t first = P == 1 ? (stage_it & 1) * 2048 : 0;
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float u = g[8 * c + 2 * j], w = g[8 * c + 2 * j + 1];
+                        h[j] = pack_half2(u, w, P == 1 && half_type);
+                        if constexpr (P == 2) {
+                            const float uh = __uint_as_float(h[j] << 16), wh = __uint_as_float(h[j] & 0xffff0000u);
+                            l[j] = pack_half2(u - uh, w - wh, false);
+                        }
+                    }
+                    st_shared_v4(row + first + ((c ^ x) << 4), h[0], h[1], h[2], h[3]);
+                    if constexpr (P == 2) st_shared_v4(row + 2048 + ((c ^ x) << 4), l[0], l[1], l[2], l[3]);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+#pragma unroll
+                    for (int z = 0; z < P; z++) tma_store_3d(&map_g, staging + first + z * 2048, col, m * kXentTileM + 32 * quarter, z);
+                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                }
+                stage_it++;
+            }
+        };
+
+        for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+            const Item t = item_of(i);
+            const int r = t.m * kXentTileM + 32 * quarter + lane;     // row of the tile that this thread holds
+            if constexpr (MODE == kXentStats) {
+                const int y = r < count ? p.label[r] : -1;
+                float top = -INFINITY, sum = 0.f, picked = 0.f;
+                bool have = false;
+                for (int n = t.n0; n < t.n1; n++) {
+                    const uint32_t acc = acquire();
+                    if (!ok) break;
+#pragma unroll 1
+                    for (int c = 0; c < kHalf; c += 32) {
+                        const int col = n * BN + half * kHalf + c;
+                        if (col >= p.classes) break;
+                        uint32_t u[32];
+                        tmem_ld32(acc + c, u);
+                        float v[32];
+#pragma unroll
+                        for (int j = 0; j < 32; j++) v[j] = __uint_as_float(u[j]);
+                        if (col + 32 > p.classes) {
+#pragma unroll
+                            for (int j = 0; j < 32; j++)
+                                if (col + j >= p.classes) v[j] = -INFINITY;
+                        }
+                        online_softmax(v, top, sum);
+                        if (__any_sync(0xffffffffu, (uint32_t)(y - col) < 32u)) {
+#pragma unroll
+                            for (int j = 0; j < 32; j++)
+                                if (y - col == j) { picked = v[j]; have = true; }
+                        }
+                    }
+                    release();
+                }
+                if (ok && r < count) {
+                    p.stats[(int64_t)(2 * t.split + half) * p.rows_pad + r] = make_float2(top, sum);
+                    if (have) p.label_logit[r] = picked;
+                }
+            } else if constexpr (MODE == kXentGrad) {
+                const bool live = r < count;
+                const int y = live ? p.label[r] - p.v0 : -1;
+                const float lse2 = live ? p.lse2[r] : 0.f;
+                const uint32_t acc = acquire();
+                if (!ok) break;
+#pragma unroll 1
+                for (int c = 0; c < kHalf; c += 32) {
+                    const int col = t.n0 * BN + half * kHalf + c;     // within the piece
+                    uint32_t u[32];
+                    tmem_ld32(acc + c, u);
+                    float g[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const float e = fast_exp2(fmaf(__uint_as_float(u[j]), kLog2e, -lse2));
+                        g[j] = !live || col + j >= p.vc ? 0.f : (y == col + j ? e - 1.f : e);
+                    }
+                    write_g(g, t.m, col);
+                }
+                release();
+            } else if constexpr (MODE == kXentGradOne) {
+                // every other tile is this warp's, with all its columns: a row's statistics stay in one thread
+                if ((int)(acc_it & 1) != half) { acc_it++; continue; }
+                const bool live = r < count;
+                const int y = live ? p.label[r] : -1;
+                const uint32_t acc = acquire() - half * kHalf;
+                if (!ok) break;
+                float top = -INFINITY, sum = 0.f, picked = 0.f;
+#pragma unroll 1
+                for (int col = 0; col < BN; col += 32) {
+                    if (col >= p.classes) break;
+                    uint32_t u[32];
+                    tmem_ld32(acc + col, u);
+                    float v[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j++) v[j] = col + j < p.classes ? __uint_as_float(u[j]) : -INFINITY;
+                    online_softmax(v, top, sum);
+#pragma unroll
+                    for (int j = 0; j < 32; j++)
+                        if (y - col == j) picked = v[j];
+                }
+                const float lse2 = fmaf(top, kLog2e, log2f(sum));
+                const float loss = live ? fmaf(lse2, kLn2, -picked) : 0.f;
+                if (live && p.row_loss) p.row_loss[p.row_of[r]] = loss;
+                float w = loss;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+                if (lane == 0) p.warp_loss[t.m * (kXentTileM / 32) + quarter] = w;
+#pragma unroll 1
+                for (int col = 0; col < BN; col += 32) {
+                    uint32_t u[32];
+                    tmem_ld32(acc + col, u);
+                    float g[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const float e = fast_exp2(fmaf(__uint_as_float(u[j]), kLog2e, -lse2));
+                        g[j] = !live || col + j >= p.classes ? 0.f : (y == col + j ? e - 1.f : e);
+                    }
+                    write_g(g, t.m, col);
+                }
+                release();
+            } else {
+                const bool empty = t.k0 >= t.k1;      // nothing to contract: the sum is zero
+                uint32_t acc = 0;
+                if (!empty) {
+                    acc = acquire();
+                    if (!ok) break;
+                }
+                const float scale = xent_scale(p, count);
+                const bool live = r < m_extent;
+#pragma unroll 1
+                for (int c = 0; c < kHalf; c += 32) {
+                    const int col = t.n0 * BN + half * kHalf + c;
+                    if (col >= n_extent) break;
+                    __syncwarp();
+                    uint32_t u[32];
+                    if (!empty) {
+                        tmem_ld32(acc + c, u);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; j++) u[j] = 0u;
+                    }
+                    if (!live) continue;
+                    if (p.store != kXentFinal) {
+                        float4* to = reinterpret_cast<float4*>(p.part + ((int64_t)t.split * p.part_rows + r) * p.part_ld + col);
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            float4 v = make_float4(__uint_as_float(u[4 * j]), __uint_as_float(u[4 * j + 1]), __uint_as_float(u[4 * j + 2]), __uint_as_float(u[4 * j + 3]));
+                            if (p.store == kXentAccumulate) {
+                                const float4 w = to[j];
+                                v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+                            }
+                            to[j] = v;
+                        }
+                        continue;
+                    }
+                    const int64_t row = MODE == kXentDHidden ? (int64_t)p.row_of[r] : (int64_t)p.v0 + r;
+                    const int64_t at = row * p.out_m + (int64_t)col * p.out_n;
+                    if (p.out_vec && col + 32 <= n_extent) {
+                        if (p.out_type == MASK_F32) {
+                            float4* to = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+#pragma unroll
+                            for (int j = 0; j < 8; j++)
+                                to[j] = make_float4(scale * __uint_as_float(u[4 * j]), scale * __uint_as_float(u[4 * j + 1]),
+                                                    scale * __uint_as_float(u[4 * j + 2]), scale * __uint_as_float(u[4 * j + 3]));
+                        } else {
+                            uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
+#pragma unroll
+                            for (int j = 0; j < 4; j++) {
+                                uint32_t h[4];
+#pragma unroll
+                                for (int q = 0; q < 4; q++)
+                                    h[q] = pack_half2(scale * __uint_as_float(u[8 * j + 2 * q]), scale * __uint_as_float(u[8 * j + 2 * q + 1]), p.out_type == MASK_F16);
+                                to[j] = make_uint4(h[0], h[1], h[2], h[3]);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; j++) {
+                            if (col + j >= n_extent) continue;
+                            const float v = scale * __uint_as_float(u[j]);
+                            if (p.out_type == MASK_F32) static_cast<float*>(p.out)[at + j * p.out_n] = v;
+                            else if (p.out_type == MASK_F16) static_cast<__half*>(p.out)[at + j * p.out_n] = __float2half_rn(v);
+                            else static_cast<__nv_bfloat16*>(p.out)[at + j * p.out_n] = __float2bfloat16_rn(v);
+                        }
+                    }
+                }
+                if (!empty) release();
+            }
+        }
+        if constexpr (L::kWritesG) {
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+            __syncwarp();
+        }
+    }
+
+    // ---- teardown: everybody gets here, aborting or not ---------------------------------------------------------------
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (*abort_flag) {
+        // copies that were issued but never consumed may still be landing in this block's shared memory
+        const long long start = clock64();
+        while (clock64() - start < 2000000LL) {
+        }
+        __syncthreads();
+    }
+    if (warp == kXentWarps + 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(L::kTmemCols) : "memory");
+    }
+    if (tid == 0 && *abort_flag) atomicExch(p.status, 1);
+}
+
+}  // namespace mask

@@ -331,6 +331,24 @@ def _product(packed, dense, out, policy, relu, plan, tf32x3, whole_vectors):
     return got
 
 
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, reduction: str = "mean", grads: bool = False,
+                         grad_scale: float = 1.0):
+    """Softmax cross entropy of ``hidden[rows, dim] @ weight[dim, classes]`` against int64 ``labels[rows]`` on the current
+    stream, without the logits in memory; float32, bfloat16 or float16.  Rows whose label is not one of the classes (-1, say)
+    are left out: no loss, no gradient, whatever they hold.  ``reduction``: "mean" over the labelled rows or "sum" (0 without
+    any), "none" for a loss per row.  The loss is float32.
+
+    With ``grads`` returns (loss, dhidden, dweight): the gradients of the loss (of its sum for "none") times ``grad_scale``,
+    in the operands' dtype, dweight contiguous along the axis along which ``weight`` is.  ``weight`` may have any strides
+    (pass a table of one embedding per class as ``table.t()``), ``hidden`` any distance between its rows."""
+    if reduction not in _lib.REDUCTION:
+        raise RuntimeError(f"reduction must be one of {', '.join(_lib.REDUCTION)}")
+    got = (_lib._binding or _lib.binding()).linear_xent(hidden, weight, labels, _lib.REDUCTION[reduction], grad_scale, grads)
+    if type(got) is int:
+        check(got, "mask_linear_xent")
+    return got
+
+
 def kernel_signature(packed, N: int, plan: Plan, tf32x3: bool = False) -> tuple[str, int]:
     """(name of the kernel ``spmm`` launches for this matrix, plan and N; the library's kernel revision)."""
     fmt = 2 if isinstance(packed, PackedMCO) else (1 if isinstance(packed, PackedMETCF) else 0)
