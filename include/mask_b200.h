@@ -411,9 +411,10 @@ int mask_spmm_srbcrs_static_scratch(const mask_plan* plan, const int32_t* d_val_
  *   logit[r,v] = sum_d hidden[r,d] weight[d,v],  loss[r] = log sum_v exp logit[r,v] - logit[r,label[r]]
  *   mean: loss[0] = their mean over the labelled rows, sum: their sum (both 0 if no row is labelled);
  *   none: loss[r] for every row, gradients those of the sum.  Gradients are multiplied by grad_scale.
- * float32 operands are multiplied as three products of bfloat16 parts (relative error of a product
- * below 2^-16), 16-bit ones exactly; sums are float32.  The gradient of the logits is held in the
- * parts' type between its products; infinite or NaN logits of a labelled row make its loss and the
+ * float32 operands are multiplied as three products of float16 parts of 22 bits together (relative error of a
+ * product at most 2^-20; values below 2^-18 of the largest finite magnitude of their operand, labelled rows
+ * only, are exact to 2^-40 of that), 16-bit ones exactly; sums are float32.  The gradient of the logits is
+ * held in the same parts, or in the operands' 16-bit type, between its products; infinite or NaN logits of a labelled row make its loss and the
  * gradients NaN.  Results do not depend on the order of anything: the same call gives the same bits.
  *
  * Scratch: mask_linear_xent_scratch_bytes(head) bytes, 256-byte aligned, one call at a time (two captured graphs

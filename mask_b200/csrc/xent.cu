@@ -9,7 +9,7 @@
 //   2. logits tile by tile, each row's running maximum and sum kept; parts of the classes are joined in a fixed order;
 //   3. for a piece of the classes at a time: the logits' tiles again, now turned into G (in 16-bit planes, in scratch), then
 //      dH += G W and that piece of dW = G^T H.
-// Up to 256 classes fit one tile, and steps 2 and 3 share one product.  Contractions that leave SMs idle are split and
+// Few classes (up to 256, FP32 128) fit one tile, and steps 2 and 3 share one product.  Contractions that leave SMs idle are split and
 // their parts summed in a fixed order.
 #include <algorithm>
 
@@ -46,7 +46,8 @@ __global__ void __launch_bounds__(kXentCountThreads) xent_count_kernel(const int
 __global__ void __launch_bounds__(kXentCountThreads) xent_number_kernel(const int64_t* __restrict__ labels, int64_t rows, int32_t classes, int64_t chunk,
                                                                         const int32_t* __restrict__ counts, int32_t* __restrict__ row_of,
                                                                         int32_t* __restrict__ label, int32_t* __restrict__ total,
-                                                                        int32_t* __restrict__ status, float* __restrict__ row_loss) {
+                                                                        int32_t* __restrict__ status, uint32_t* __restrict__ range,
+                                                                        float* __restrict__ row_loss) {
     __shared__ int sums[32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int at = 0;
@@ -78,6 +79,7 @@ __global__ void __launch_bounds__(kXentCountThreads) xent_number_kernel(const in
     if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
         *total = at;
         *status = 0;
+        range[0] = range[1] = 0;
     }
 }
 
@@ -98,20 +100,62 @@ struct XentPackArgs {
     int64_t w_plane;
     void* dhidden;             // rows without a label are set to 0
     int64_t dhidden_stride;
+    uint32_t* range;           // FP32: bits of the largest finite magnitude of the labelled rows of hidden, and of weight
 };
 
-// hi and lo of a float; an infinite or NaN hi has no lo
-__device__ __forceinline__ void split_bf16(float x, uint32_t& hi, uint32_t& lo) {
-    const __nv_bfloat16 h = __float2bfloat16_rn(x);
-    const float hf = __bfloat162float(h);
-    const __nv_bfloat16 l = __float2bfloat16_rn(isfinite(hf) ? x - hf : 0.f);
-    hi = __bfloat16_as_ushort(h);
-    lo = __bfloat16_as_ushort(l);
+__device__ __forceinline__ uint32_t finite_magnitude(float x) {
+    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+}
+
+// The largest finite magnitudes of both operands (FP32 input).  A maximum does not depend on the order.
+__global__ void __launch_bounds__(256) xent_range_kernel(const XentPackArgs p) {
+    const int lane = threadIdx.x & 31;
+    const int64_t warps = (int64_t)gridDim.x * 8, w0 = grid_warp();
+    const float* hidden = static_cast<const float*>(p.hidden);
+    const float* weight = static_cast<const float*>(p.weight);
+    uint32_t most[2] = {0, 0};
+    auto scan = [&](const float* row, int64_t n, int64_t stride, uint32_t& m) {
+        if (stride == 1 && (reinterpret_cast<uintptr_t>(row) & 15) == 0) {
+            int64_t d = 4 * lane;
+            for (; d + 4 <= n; d += 128) {
+                const float4 v = __ldg(reinterpret_cast<const float4*>(row + d));
+                m = max(m, max(max(finite_magnitude(v.x), finite_magnitude(v.y)), max(finite_magnitude(v.z), finite_magnitude(v.w))));
+            }
+            for (; d < n; d++) m = max(m, finite_magnitude(__ldg(row + d)));
+        } else {
+            for (int64_t d = lane; d < n; d += 32) m = max(m, finite_magnitude(__ldg(row + d * stride)));
+        }
+    };
+    const int count = *p.count;
+    for (int64_t i = w0; i < count; i += warps) scan(hidden + p.row_of[i] * p.hidden_stride, p.dim, 1, most[0]);
+    if (p.w_class_stride == 1) {       // in stretches of at most 4096 along the axis that is contiguous
+        const int64_t parts = (p.classes + 4095) / 4096;
+        for (int64_t i = w0; i < p.dim * parts; i += warps) {
+            const int64_t v = i % parts * 4096;
+            scan(weight + i / parts * p.w_dim_stride + v, min((int64_t)4096, p.classes - v), 1, most[1]);
+        }
+    } else {
+        for (int64_t v = w0; v < p.classes; v += warps) scan(weight + v * p.w_class_stride, p.dim, p.w_dim_stride, most[1]);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, most[k]);
+        if (lane == 0 && m) atomicMax(p.range + k, m);
+    }
+}
+
+// hi and lo of a scaled float; an infinite or NaN hi has no lo
+__device__ __forceinline__ void split_half(float x, uint32_t& hi, uint32_t& lo) {
+    const __half h = __float2half_rn(x);
+    const float hf = __half2float(h);
+    hi = __half_as_ushort(h);
+    lo = __half_as_ushort(__float2half_rn(isfinite(hf) ? x - hf : 0.f));
 }
 
 // One row of `dim` elements `stride` apart to the planes, by a warp; `src` NULL writes zeros.
 template <bool kFloat>
-__device__ __forceinline__ void pack_row(const void* src, int64_t stride, int dim, int dim_pad, uint16_t* to, int64_t plane, int lane) {
+__device__ __forceinline__ void pack_row(const void* src, int64_t stride, int dim, int dim_pad, uint16_t* to, int64_t plane, float scale, int lane) {
     const bool vec = stride == 1 && (reinterpret_cast<uintptr_t>(src) & (kFloat ? 15 : 7)) == 0;
     for (int d = 4 * lane; d < dim_pad; d += 128) {
         if constexpr (kFloat) {
@@ -127,7 +171,7 @@ __device__ __forceinline__ void pack_row(const void* src, int64_t stride, int di
             }
             uint32_t h[4], l[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) split_bf16(x[j], h[j], l[j]);
+            for (int j = 0; j < 4; j++) split_half(scale * x[j], h[j], l[j]);
             *reinterpret_cast<uint2*>(to + d) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
             *reinterpret_cast<uint2*>(to + plane + d) = make_uint2(l[0] | l[1] << 16, l[2] | l[3] << 16);
         } else {
@@ -155,11 +199,12 @@ __global__ void __launch_bounds__(kXentPackThreads) xent_pack_kernel(const XentP
     const int lane = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * (kXentPackThreads / 32), w0 = grid_warp();
     const int count = *p.count;
+    const float h_scale = kFloat ? exp2f((float)(14 - plane_exponent(p.range[0]))) : 1.f, w_scale = kFloat ? exp2f((float)(14 - plane_exponent(p.range[1]))) : 1.f;
     // labelled rows, and zeros up to a whole tile
     const int64_t end = ((int64_t)count + kXentTileM - 1) / kXentTileM * kXentTileM;
     for (int64_t i = w0; i < end; i += warps) {
         const void* src = i < count ? static_cast<const char*>(p.hidden) + (int64_t)p.row_of[i] * p.hidden_stride * kBytes : nullptr;
-        pack_row<kFloat>(src, 1, p.dim, p.dim_pad, p.h_planes + i * p.dim_pad, p.h_plane, lane);
+        pack_row<kFloat>(src, 1, p.dim, p.dim_pad, p.h_planes + i * p.dim_pad, p.h_plane, h_scale, lane);
     }
     if (p.dhidden && count < p.rows) {
         for (int64_t r = w0; r < p.rows; r += warps) {
@@ -175,7 +220,7 @@ __global__ void __launch_bounds__(kXentPackThreads) xent_pack_kernel(const XentP
     if (p.w_dim_stride == 1 || p.w_class_stride != 1) {
         for (int64_t v = w0; v < p.classes; v += warps)
             pack_row<kFloat>(static_cast<const char*>(p.weight) + v * p.w_class_stride * kBytes, p.w_dim_stride, p.dim, p.dim_pad,
-                             p.w_planes + v * p.dim_pad, p.w_plane, lane);
+                             p.w_planes + v * p.dim_pad, p.w_plane, w_scale, lane);
         return;
     }
     // classes are contiguous: tiles of 32 x 32 turned over in shared memory
@@ -200,7 +245,7 @@ __global__ void __launch_bounds__(kXentPackThreads) xent_pack_kernel(const XentP
                 const uint32_t x = t[lane][j];
                 if constexpr (kFloat) {
                     uint32_t h, l;
-                    split_bf16(__uint_as_float(x), h, l);
+                    split_half(w_scale * __uint_as_float(x), h, l);
                     to[0] = (uint16_t)h;
                     to[p.w_plane] = (uint16_t)l;
                 } else {
@@ -217,19 +262,20 @@ __global__ void __launch_bounds__(kXentPackThreads) xent_pack_kernel(const XentP
 __global__ void __launch_bounds__(256) xent_join_kernel(const XentArgs p) {
     const int count = *p.count, lane = threadIdx.x & 31;
     const int64_t end = ((int64_t)count + 31) / 32 * 32;
+    const float f = logit_factor(p.range);
     for (int64_t r = grid_thread(); r < end; r += (int64_t)gridDim.x * blockDim.x) {
         float loss = 0.f;
         if (r < count) {
             float top = -INFINITY, sum = 0.f;
             for (int i = 0; i < 2 * p.splits; i++) top = fmaxf(top, p.stats[(int64_t)i * p.rows_pad + r].x);
-            const float base = top == -INFINITY ? 0.f : top * kLog2e;
+            const float base = top == -INFINITY ? 0.f : top * f;
             for (int i = 0; i < 2 * p.splits; i++) {
                 const float2 s = p.stats[(int64_t)i * p.rows_pad + r];
-                sum += s.y * fast_exp2(s.x * kLog2e - base);
+                sum += s.y * fast_exp2(fmaf(s.x, f, -base));
             }
             const float lse2 = base + log2f(sum);
             p.lse2[r] = lse2;
-            loss = fmaf(lse2, kLn2, -p.label_logit[r]);
+            loss = kLn2 * fmaf(-p.label_logit[r], f, lse2);
             if (p.row_loss) p.row_loss[p.row_of[r]] = loss;
         }
 #pragma unroll
@@ -252,13 +298,14 @@ struct XentReduceArgs {
     int64_t out_m, out_n, m0;
     int32_t out_type;
     float scale;
-    int32_t mean;
+    int32_t mean, operand;
+    const uint32_t* range;
 };
 
 __global__ void __launch_bounds__(256) xent_reduce_kernel(const XentReduceArgs p) {
     const int count = *p.count;
     const int64_t m_end = p.m_is_count ? count : p.m, n_vec = (p.n + 3) / 4;
-    const float scale = p.mean ? (count > 0 ? p.scale / (float)count : 0.f) : p.scale;
+    const ProductScale scale = product_scale(p.scale, p.mean, count, p.range, p.operand);
     const bool m_fast = p.out_m == 1 && p.out_n != 1;
     for (int64_t i = grid_thread(); i < m_end * n_vec; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t m = m_fast ? i % m_end : i / n_vec, n = 4 * (m_fast ? i / m_end : i % n_vec);
@@ -267,7 +314,7 @@ __global__ void __launch_bounds__(256) xent_reduce_kernel(const XentReduceArgs p
             const float4 v = *reinterpret_cast<const float4*>(p.part + (s * p.part_rows + m) * p.part_ld + n);
             a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
         }
-        const float v[4] = {scale * a.x, scale * a.y, scale * a.z, scale * a.w};
+        const float v[4] = {scale(a.x), scale(a.y), scale(a.z), scale(a.w)};
         const int64_t at = (p.m_is_count ? (int64_t)p.row_of[m] : p.m0 + m) * p.out_m + n * p.out_n;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -352,7 +399,8 @@ static XentPlan plan_xent(const mask_head& h) {
                     (reinterpret_cast<uintptr_t>(h.d_weight) & 15);
     p.bn_logits = h.classes <= 64 ? 64 : (h.classes <= 128 ? 128 : 256);
     p.bn_dim = tile_width(h.dim);
-    p.one_pass = p.grads && h.classes <= 256;
+    // one tile of all classes: 256 columns, with two planes of G in shared memory 128
+    p.one_pass = p.grads && h.classes <= (p.planes == 2 ? 128 : 256);
     const int64_t m_tiles = p.rows_pad / kXentTileM;
     p.stats_splits = p.one_pass ? 1 : best_splits(m_tiles, (h.classes + p.bn_logits - 1) / p.bn_logits, sms);
     if (p.grads) {
@@ -428,7 +476,7 @@ static int launch_xent_gemm_as(const XentArgs& a, const CUtensorMap& ma, const C
     const int rc = opt_in_shared_memory(reinterpret_cast<const void*>(xent_gemm_kernel<BN, P, MODE>), L::kDynamicBytes, done);
     if (rc != MASK_OK) return rc;
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(items, sm_count()));
-    xent_gemm_kernel<BN, P, MODE><<<grid, kXentThreads, L::kDynamicBytes, st>>>(a, ma, mb, mg);
+    xent_gemm_kernel<BN, P, MODE><<<grid, xent_threads(P), L::kDynamicBytes, st>>>(a, ma, mb, mg);
     MASK_CUDA_TRY(cudaGetLastError());
     return MASK_OK;
 }
@@ -443,7 +491,8 @@ static int launch_xent_gemm(int bn, int planes, const XentArgs& a, const CUtenso
     }
     if (bn == 64) return launch_xent_gemm_as<64, 2, MODE>(a, ma, mb, mg, items, st);
     if (bn == 128) return launch_xent_gemm_as<128, 2, MODE>(a, ma, mb, mg, items, st);
-    return launch_xent_gemm_as<256, 2, MODE>(a, ma, mb, mg, items, st);
+    if constexpr (MODE == kXentGradOne) return fail(MASK_ERR_INVALID_ARGUMENT, "no such kernel");
+    else return launch_xent_gemm_as<256, 2, MODE>(a, ma, mb, mg, items, st);
 }
 
 static const char* refuse_head(const mask_head* h) {
@@ -473,12 +522,13 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
     int32_t* row_of = reinterpret_cast<int32_t*>(at(plan.row_of));
     int32_t* label = reinterpret_cast<int32_t*>(at(plan.label));
     int32_t* counts = reinterpret_cast<int32_t*>(at(plan.counts));
+    uint32_t* range = reinterpret_cast<uint32_t*>(total + 2);
     float* row_loss = h.reduction == MASK_REDUCE_NONE ? h.d_loss : nullptr;
     const int P = plan.planes;
     const int64_t rp = plan.rows_pad, m_tiles = rp / kXentTileM;
 
     if (plan.n_chunks > 1) xent_count_kernel<<<plan.n_chunks, kXentCountThreads, 0, st>>>(h.d_labels, h.rows, h.classes, plan.chunk, counts);
-    xent_number_kernel<<<plan.n_chunks, kXentCountThreads, 0, st>>>(h.d_labels, h.rows, h.classes, plan.chunk, counts, row_of, label, total, total + 1, row_loss);
+    xent_number_kernel<<<plan.n_chunks, kXentCountThreads, 0, st>>>(h.d_labels, h.rows, h.classes, plan.chunk, counts, row_of, label, total, total + 1, range, row_loss);
     MASK_CUDA_TRY(cudaGetLastError());
 
     XentPackArgs pk = {};
@@ -491,10 +541,15 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
         pk.weight = h.d_weight; pk.w_dim_stride = h.weight_dim_stride; pk.w_class_stride = h.weight_class_stride;
         pk.w_planes = reinterpret_cast<uint16_t*>(at(plan.w_planes)); pk.w_plane = (int64_t)h.classes * plan.dim_pad;
     }
+    pk.range = range;
     const int64_t pack_rows = rp + (plan.pack_weight ? h.classes : 0);
     const unsigned pack_grid = (unsigned)std::min<int64_t>((pack_rows + 7) / 8, 8 * (int64_t)sm_count());
-    if (h.dtype == MASK_F32) xent_pack_kernel<true><<<pack_grid, kXentPackThreads, 0, st>>>(pk);
-    else xent_pack_kernel<false><<<pack_grid, kXentPackThreads, 0, st>>>(pk);
+    if (h.dtype == MASK_F32) {
+        xent_range_kernel<<<pack_grid, 256, 0, st>>>(pk);
+        xent_pack_kernel<true><<<pack_grid, kXentPackThreads, 0, st>>>(pk);
+    } else {
+        xent_pack_kernel<false><<<pack_grid, kXentPackThreads, 0, st>>>(pk);
+    }
     MASK_CUDA_TRY(cudaGetLastError());
 
     const void* w_data = plan.pack_weight ? (const void*)pk.w_planes : h.d_weight;
@@ -508,7 +563,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
     XentArgs a = {};
     a.count = total; a.status = total + 1;
     a.classes = h.classes; a.dim = h.dim; a.v0 = 0; a.vc = h.classes;
-    a.rows_pad = (int32_t)rp; a.half_type = h.dtype == MASK_F16;
+    a.rows_pad = (int32_t)rp; a.half_type = h.dtype != MASK_BF16; a.range = P == 2 ? range : nullptr;
     a.label = label; a.row_of = row_of; a.row_loss = row_loss;
     a.stats = reinterpret_cast<float2*>(at(plan.stats));
     a.label_logit = reinterpret_cast<float*>(at(plan.label_logit));
@@ -535,7 +590,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
         const int64_t n_tiles = plan.part_ld / plan.bn_dim;
         const unsigned most_blocks = (unsigned)(8 * sm_count());
         XentReduceArgs r = {};
-        r.part_ld = plan.part_ld; r.n = h.dim; r.count = total; r.row_of = row_of; r.out_type = h.dtype; r.scale = a.scale; r.mean = a.mean;
+        r.part_ld = plan.part_ld; r.n = h.dim; r.count = total; r.row_of = row_of; r.out_type = h.dtype; r.scale = a.scale; r.mean = a.mean; r.range = a.range;
         const uintptr_t vec = h.dtype == MASK_F32 ? 4 : 8;      // elements of 16 bytes
         for (int piece = 0; piece < plan.n_pieces; piece++) {
             a.v0 = piece * plan.piece;
@@ -574,7 +629,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
         }
         if (h.d_dhidden && plan.dh_parts) {
             r.part = reinterpret_cast<float*>(at(plan.part_dh)); r.part_rows = plan.part_dh_rows; r.splits = plan.dh_splits;
-            r.m_is_count = 1;
+            r.m_is_count = 1; r.operand = 1;
             r.out = h.d_dhidden; r.out_m = h.dhidden_stride; r.out_n = 1;
             const int64_t n = rp * ((r.n + 3) / 4);
             xent_reduce_kernel<<<(unsigned)std::min<int64_t>((n + 255) / 256, most_blocks), 256, 0, st>>>(r);

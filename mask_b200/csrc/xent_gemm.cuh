@@ -3,9 +3,13 @@
 //
 // One persistent block per SM: a producer thread feeds a ring of stages by TMA, one thread issues the MMAs into two
 // accumulators of tensor memory, eight warps take the finished accumulator apart while the next one is computed.
-// Operands are 16-bit "planes": one for bf16 and fp16 input; FP32 input is split into two bf16 planes, x = hi + lo + e with
-// |e| <= 2^-18 |x|, and a product is hi hi + hi lo + lo hi (the dropped lo lo is 2^-18 of it at most).  All three
-// products have the layouts TMA and the MMA take as they are, whichever axis is contracted:
+// Operands are 16-bit "planes": one for bf16 and fp16 input.  FP32 input is scaled by a power of two that brings the
+// operand's largest magnitude to 2^14..2^15 and split into two fp16 planes, x = hi + lo + e with |e| <= 2^-22 |x|, or 2^-40
+// of the largest where that is more; a product is hi hi + hi lo + lo hi (the dropped lo lo is 2^-22 of it at most).
+// The MMA cuts its sum off to 32 bits toward zero after every 16 products (2730 such steps in a row left 2e-5 of the
+// result); for FP32 input an accumulator therefore takes kXentSegment blocks of the contraction, and the segments are added
+// in registers, rounded to nearest.  For 16-bit input what is cut off is far below the result's own rounding.
+// All three products have the layouts TMA and the MMA take as they are, whichever axis is contracted:
 //     logits[r,v] = sum_d H[r,d] W[v,d]     both operands K-major
 //     dH[r,d]     = sum_v G[r,v] W[v,d]     G K-major, W MN-major
 //     dW[v,d]     = sum_r G[r,v] H[r,d]     both MN-major
@@ -21,8 +25,11 @@
 namespace mask {
 
 constexpr int kXentTileM = 128, kXentTileK = 64;
+constexpr int kXentSegment = 4;                     // blocks of the contraction that an accumulator takes (FP32 input)
 constexpr int kXentWarps = 8;                       // epilogue warps: 4 quarters of 32 rows x 2 halves of the columns
-constexpr int kXentThreads = 32 * (kXentWarps + 2);   // + producer + MMA issuer
+// + producer + MMA issuer; with segments summed in registers (P == 2) two warps more make three whole warpgroups, whose
+// 168 registers a thread are dealt again: 216 to the two that take accumulators apart, 72 to the third (3 x 168 in all).
+constexpr int xent_threads(int planes) { return 32 * (kXentWarps + (planes == 2 ? 4 : 2)); }
 
 enum XentMode {
     kXentStats,      // logits -> running maximum and sum of each row over a range of classes
@@ -40,7 +47,7 @@ struct XentArgs {
     int32_t v0, vc;            // piece of the classes
     int32_t splits;            // stats: parts of the classes' tiles; products: parts of the contraction
     int32_t rows_pad;
-    int32_t half_type;         // planes hold fp16 instead of bf16
+    int32_t half_type;         // planes hold fp16, not bf16
     const int32_t* label;      // [labelled row]
     const int32_t* row_of;     // [labelled row] -> row of the caller's arrays
     float2* stats;             // [2 * splits][rows_pad]: maximum, sum of exp(logit - maximum)
@@ -58,10 +65,27 @@ struct XentArgs {
     int32_t out_vec;           // rows of 32 values may be written as 16-byte vectors
     float scale;
     int32_t mean;              // scale / count
+    const uint32_t* range;     // bits of the largest finite magnitudes of hidden and weight, or NULL: planes are the operands themselves
     int32_t* status;
 };
 
-__device__ __forceinline__ float xent_scale(const XentArgs& p, int count) { return p.mean ? (count > 0 ? p.scale / (float)count : 0.f) : p.scale; }
+// Power of two of an operand's planes: planes = 2^(14 - e) operand.  Below 2^-100 everything is scaled alike.
+__device__ __forceinline__ int plane_exponent(uint32_t largest) { return max((int)(largest >> 23) - 127, -100); }
+constexpr int kGradExponent = 15;      // planes of G hold 2^15 G for FP32 input
+
+__device__ __forceinline__ float xent_scale(float scale, bool mean, int count) { return mean ? (count > 0 ? scale / (float)count : 0.f) : scale; }
+// The same for a product of G's planes with those of an operand: two factors, since the power of two alone may be too small
+// for a float.
+struct ProductScale {
+    float a, b;
+    __device__ __forceinline__ float operator()(float x) const { return a * x * b; }
+};
+__device__ __forceinline__ ProductScale product_scale(float scale, bool mean, int count, const uint32_t* range, int operand) {
+    scale = xent_scale(scale, mean, count);
+    if (!range) return {scale, 1.f};
+    const int e = plane_exponent(range[operand]) - 14 - kGradExponent;
+    return {ldexpf(scale, e / 2), ldexpf(1.f, e - e / 2)};
+}
 
 __device__ __forceinline__ float fast_exp2(float x) {
     float y;
@@ -69,6 +93,10 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return y;
 }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// What a product of the planes of hidden and weight is multiplied with to become a logit in units of log 2.
+__device__ __forceinline__ float logit_factor(const uint32_t* range) {
+    return range ? ldexpf(kLog2e, min(plane_exponent(range[0]) + plane_exponent(range[1]) - 28, 126)) : kLog2e;   // finite: 0 stays 0
+}
 
 template <int BN, int P, int MODE>
 struct XentLayout {
@@ -76,12 +104,14 @@ struct XentLayout {
     static constexpr int kTileA = kXentTileM * kXentTileK * 2, kTileB = BN * kXentTileK * 2;
     static constexpr int kStage = P * (kTileA + kTileB);
     static constexpr int kStaging = kWritesG ? kXentWarps * 4096 : 0;      // 32 rows x 32 columns x 2 planes or buffers a warp
-    static constexpr int kMost = 227 * 1024 - 1024 - 256 - kStaging;
+    static constexpr int kMost = 227 * 1024 - 1024 - 256 - kStaging - (MODE == kXentGradOne ? 2 * 2 * 128 * 12 : 0);
     static constexpr int S = kMost / kStage < 8 ? kMost / kStage : 8;
     static constexpr int kTmemCols = 2 * BN;
     static constexpr int kStagingAt = S * kStage;
-    static constexpr int kBars = kStagingAt + kStaging;
-    static constexpr int kNumBars = 2 * S + 4 + 1;
+    static constexpr int kExchange = kStagingAt + kStaging;                // one-pass mode: [2 turns][2 halves][128 rows] x 12 bytes
+    static constexpr int kExchangeBytes = MODE == kXentGradOne ? 2 * 2 * 128 * 12 : 0;
+    static constexpr int kBars = kExchange + kExchangeBytes;
+    static constexpr int kNumBars = 2 * S + 4 + 1 + 4;
     static constexpr int kTmemSlot = kBars + kNumBars * 8;
     static constexpr int kAbort = kTmemSlot + 8;
     static constexpr int kBytes = kAbort + 8;
@@ -134,22 +164,22 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b, bool half_type)
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Adds 32 logits of a row to its running maximum and sum.
-__device__ __forceinline__ void online_softmax(const float (&v)[32], float& top, float& sum) {
+// Adds 32 logits of a row, in units of 1 / f bits, to its running maximum and sum.
+__device__ __forceinline__ void online_softmax(const float (&v)[32], float f, float& top, float& sum) {
     float t[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
     for (int i = 4; i < 32; i++) t[i & 3] = fmaxf(t[i & 3], v[i]);
     const float now = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
-    const float base = now == -INFINITY ? 0.f : now * kLog2e;    // a row that has seen only -inf
-    float s[4] = {sum * fast_exp2(top * kLog2e - base), 0.f, 0.f, 0.f};
+    const float base = now == -INFINITY ? 0.f : now * f;         // a row that has seen only -inf
+    float s[4] = {sum * fast_exp2(fmaf(top, f, -base)), 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 32; i++) s[i & 3] += fast_exp2(fmaf(v[i], kLog2e, -base));
+    for (int i = 0; i < 32; i++) s[i & 3] += fast_exp2(fmaf(v[i], f, -base));
     sum = (s[0] + s[1]) + (s[2] + s[3]);
     top = now;
 }
 
 template <int BN, int P, int MODE>
-__global__ void __launch_bounds__(kXentThreads, 1)
+__global__ void __launch_bounds__(xent_threads(P), 1)
 xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const __grid_constant__ CUtensorMap map_g) {
     using L = XentLayout<BN, P, MODE>;
@@ -166,6 +196,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
     auto accf_bar = [&](int b) { return bars + 8u * (2 * S + b); };
     auto acce_bar = [&](int b) { return bars + 8u * (2 * S + 2 + b); };
     const uint32_t drain_bar = bars + 8u * (2 * S + 4);
+    auto exchange_bar = [&](int q) { return bars + 8u * (2 * S + 5 + q); };
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kAbort);
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + L::kTmemSlot);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -178,8 +209,9 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(accf_bar(b), 1);
-            mbar_init(acce_bar(b), MODE == kXentGradOne ? kXentWarps / 2 : kXentWarps);
+            mbar_init(acce_bar(b), kXentWarps);
         }
+        for (int q = 0; q < 4; q++) mbar_init(exchange_bar(q), 2);
         mbar_init(drain_bar, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -224,114 +256,160 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
         return t;
     };
 
-    if (warp == kXentWarps) {
-        // ------------------------------ producer -----------------------------------------------------------------------
-        if (lane == 0) {
-            int s = 0;
-            uint32_t round = 0;
-            bool ok = true;
-            for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
-                const Item t = item_of(i);
-                for (int n = t.n0; n < t.n1 && ok; n++) {
-                    for (int k = t.k0; k < t.k1; k++) {
-                        if (round > 0 && !mbar_wait(empty_bar(s), (round - 1) & 1, abort_flag)) { ok = false; break; }
-                        const uint32_t bar = full_bar(s), at = base + s * L::kStage;
-                        xent_expect_tx(bar, L::kStage);
-#pragma unroll
-                        for (int z = 0; z < P; z++) {
-                            const uint32_t a = at + z * L::kTileA, b = at + P * L::kTileA + z * L::kTileB;
-                            if constexpr (kAmn) {
-#pragma unroll
-                                for (int j = 0; j < kXentTileM / 64; j++)
-                                    tma_load_3d(a + j * 8192, &map_a, bar, t.m * kXentTileM + j * 64, k * kXentTileK, z);
-                            } else {
-                                tma_load_3d(a, &map_a, bar, k * kXentTileK, t.m * kXentTileM, z);
+    if (warp >= kXentWarps) {
+        if constexpr (P == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == kXentWarps) {
+            // ------------------------------ producer -----------------------------------------------------------------------
+            if (lane == 0) {
+                int s = 0;
+                uint32_t round = 0;
+                bool ok = true;
+                for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+                    const Item t = item_of(i);
+                    for (int n = t.n0; n < t.n1 && ok; n++) {
+                        for (int k = t.k0; k < t.k1; k++) {
+                            if (round > 0 && !mbar_wait(empty_bar(s), (round - 1) & 1, abort_flag)) { ok = false; break; }
+                            const uint32_t bar = full_bar(s), at = base + s * L::kStage;
+                            xent_expect_tx(bar, L::kStage);
+    #pragma unroll
+                            for (int z = 0; z < P; z++) {
+                                const uint32_t a = at + z * L::kTileA, b = at + P * L::kTileA + z * L::kTileB;
+                                if constexpr (kAmn) {
+    #pragma unroll
+                                    for (int j = 0; j < kXentTileM / 64; j++)
+                                        tma_load_3d(a + j * 8192, &map_a, bar, t.m * kXentTileM + j * 64, k * kXentTileK, z);
+                                } else {
+                                    tma_load_3d(a, &map_a, bar, k * kXentTileK, t.m * kXentTileM, z);
+                                }
+                                if constexpr (kBmn) {
+    #pragma unroll
+                                    for (int j = 0; j < BN / 64; j++)
+                                        tma_load_3d(b + j * 8192, &map_b, bar, n * BN + j * 64, (MODE == kXentDHidden ? p.v0 : 0) + k * kXentTileK, z);
+                                } else {
+                                    tma_load_3d(b, &map_b, bar, k * kXentTileK, p.v0 + n * BN, z);
+                                }
                             }
-                            if constexpr (kBmn) {
-#pragma unroll
-                                for (int j = 0; j < BN / 64; j++)
-                                    tma_load_3d(b + j * 8192, &map_b, bar, n * BN + j * 64, (MODE == kXentDHidden ? p.v0 : 0) + k * kXentTileK, z);
-                            } else {
-                                tma_load_3d(b, &map_b, bar, k * kXentTileK, p.v0 + n * BN, z);
-                            }
+                            if (++s == S) { s = 0; round++; }
                         }
-                        if (++s == S) { s = 0; round++; }
                     }
                 }
             }
-        }
-        __syncwarp();
-    } else if (warp == kXentWarps + 1) {
-        // ------------------------------ MMA issuer ---------------------------------------------------------------------
-        if (lane == 0) {
-            const uint32_t fmt = p.half_type ? 0u : 1u;
-            // instruction descriptor: D = F32, A and B bf16 or fp16, M = 128
-            const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) |
-                                   ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kXentTileM >> 4) << 24);
-            // 128-byte swizzle; K-major: groups of 8 rows 1024 bytes apart; MN-major: 64-wide atoms 8192 bytes apart, groups of 8 k 1024
-            const uint64_t a0 = umma_smem_desc(base, kAmn ? 512 : 1, 64, 2);
-            const uint64_t b0 = umma_smem_desc(base + P * L::kTileA, kBmn ? 512 : 1, 64, 2);
-            constexpr uint32_t kStepA = kAmn ? 128 : 2, kStepB = kBmn ? 128 : 2;   // 16 of the contraction, in 16 bytes
-            int s = 0;
-            uint32_t round = 0, acc_it = 0;
-            bool ok = true;
-            for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
-                const Item t = item_of(i);
-                if (t.k0 >= t.k1) continue;
-                for (int n = t.n0; n < t.n1 && ok; n++) {
-                    const uint32_t buf = acc_it & 1, acc = tmem_base + buf * BN;
-                    if (acc_it >= 2 && !mbar_wait(acce_bar(buf), ((acc_it >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    uint32_t open = 0;
-                    for (int k = t.k0; k < t.k1; k++) {
-                        if (!mbar_wait_spin(full_bar(s), round & 1, abort_flag)) { ok = false; break; }
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint64_t a = a0 + (uint64_t)(s * L::kStage >> 4), b = b0 + (uint64_t)(s * L::kStage >> 4);
-#pragma unroll
-                        for (int c = 0; c < (P == 2 ? 3 : 1); c++) {     // hi hi, hi lo, lo hi
-                            const uint64_t ac = a + (c == 2 ? L::kTileA >> 4 : 0), bc = b + (c == 1 ? L::kTileB >> 4 : 0);
-#pragma unroll
-                            for (int j = 0; j < kXentTileK / 16; j++) {
-                                umma_f16(acc, ac + j * kStepA, bc + j * kStepB, idesc, open);
-                                open = 1;
+            __syncwarp();
+        } else if (warp == kXentWarps + 1) {
+            // ------------------------------ MMA issuer ---------------------------------------------------------------------
+            if (lane == 0) {
+                const uint32_t fmt = p.half_type ? 0u : 1u;
+                // instruction descriptor: D = F32, A and B bf16 or fp16, M = 128
+                const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) |
+                                       ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kXentTileM >> 4) << 24);
+                // 128-byte swizzle; K-major: groups of 8 rows 1024 bytes apart; MN-major: 64-wide atoms 8192 bytes apart, groups of 8 k 1024
+                const uint64_t a0 = umma_smem_desc(base, kAmn ? 512 : 1, 64, 2);
+                const uint64_t b0 = umma_smem_desc(base + P * L::kTileA, kBmn ? 512 : 1, 64, 2);
+                constexpr uint32_t kStepA = kAmn ? 128 : 2, kStepB = kBmn ? 128 : 2;   // 16 of the contraction, in 16 bytes
+                int s = 0;
+                uint32_t round = 0, acc_it = 0;
+                bool ok = true;
+                for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+                    const Item t = item_of(i);
+                    if (t.k0 >= t.k1) continue;
+                    for (int n = t.n0; n < t.n1 && ok; n++) {
+                        uint32_t buf = 0, acc = 0, open = 0;
+                        for (int k = t.k0; k < t.k1; k++) {
+                            if (!open) {
+                                buf = acc_it & 1;
+                                acc = tmem_base + buf * BN;
+                                if (acc_it >= 2 && !mbar_wait(acce_bar(buf), ((acc_it >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
+                                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                            }
+                            if (!mbar_wait_spin(full_bar(s), round & 1, abort_flag)) { ok = false; break; }
+                            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                            const uint64_t a = a0 + (uint64_t)(s * L::kStage >> 4), b = b0 + (uint64_t)(s * L::kStage >> 4);
+    #pragma unroll
+                            for (int c = 0; c < (P == 2 ? 3 : 1); c++) {     // hi hi, hi lo, lo hi
+                                const uint64_t ac = a + (c == 2 ? L::kTileA >> 4 : 0), bc = b + (c == 1 ? L::kTileB >> 4 : 0);
+    #pragma unroll
+                                for (int j = 0; j < kXentTileK / 16; j++) {
+                                    umma_f16(acc, ac + j * kStepA, bc + j * kStepB, idesc, open);
+                                    open = 1;
+                                }
+                            }
+                            umma_commit(empty_bar(s));
+                            if (++s == S) { s = 0; round++; }
+                            if (k + 1 == t.k1 || (P == 2 && (k + 1 - t.k0) % kXentSegment == 0)) {
+                                umma_commit(accf_bar(buf));
+                                acc_it++;
+                                open = 0;
                             }
                         }
-                        umma_commit(empty_bar(s));
-                        if (++s == S) { s = 0; round++; }
+                        if (!ok) break;
                     }
-                    if (!ok) break;
-                    umma_commit(accf_bar(buf));
-                    acc_it++;
+                }
+                umma_commit(drain_bar);
+                const long long start = clock64();
+                while (!mbar_test(drain_bar, 0)) {
+                    if (clock64() - start > kUmmaWaitCycles) { *abort_flag = 1; break; }
                 }
             }
-            umma_commit(drain_bar);
-            const long long start = clock64();
-            while (!mbar_test(drain_bar, 0)) {
-                if (clock64() - start > kUmmaWaitCycles) { *abort_flag = 1; break; }
-            }
+            __syncwarp();
         }
-        __syncwarp();
     } else {
         // ------------------------------ epilogue -----------------------------------------------------------------------
+        if constexpr (P == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         constexpr int kHalf = BN / 2;
+        constexpr int kChunks = kHalf / 32, kUnroll = P == 2 ? kChunks : 1;
         const int quarter = warp & 3, half = warp >> 2;
         uint32_t acc_it = 0;
         bool ok = true;
         const bool half_type = p.half_type != 0;
         [[maybe_unused]] const uint32_t staging = base + L::kStagingAt + warp * 4096;
         [[maybe_unused]] uint32_t stage_it = 0;
-        // waits for the next accumulator; its address for this warp
-        auto acquire = [&]() -> uint32_t {
-            const uint32_t buf = acc_it & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait(accf_bar(buf), (acc_it >> 1) & 1, abort_flag))) ok = false;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            return tmem_base + ((uint32_t)(32 * quarter) << 16) + buf * BN + half * kHalf;
-        };
+        uint32_t acc = 0;                                // the tile's accumulator in tensor memory (P == 1)
+        [[maybe_unused]] float total[P == 2 ? kHalf : 1];   // or its sum so far
         auto release = [&]() {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(acce_bar(acc_it & 1));
             acc_it++;
+        };
+        auto next_accumulator = [&]() -> bool {
+            const uint32_t buf = acc_it & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(accf_bar(buf), (acc_it >> 1) & 1, abort_flag))) return false;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            acc = tmem_base + ((uint32_t)(32 * quarter) << 16) + buf * BN + half * kHalf;
+            return true;
+        };
+        // The tile's columns of this warp: left in tensor memory, or summed up from its segments.
+        auto acquire = [&](int k0, int k1) -> bool {
+            if constexpr (P == 1) return next_accumulator();
+            for (int k = k0; k < k1; k += kXentSegment) {
+                if (!next_accumulator()) return false;
+#pragma unroll
+                for (int c = 0; c < kChunks; c++) {
+                    uint32_t u[32];
+                    tmem_ld32(acc + 32 * c, u);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        const float x = __uint_as_float(u[j]);
+                        total[P == 2 ? 32 * c + j : 0] = k == k0 ? x : total[P == 2 ? 32 * c + j : 0] + x;
+                    }
+                }
+                release();
+            }
+            return true;
+        };
+        auto done = [&]() {
+            if constexpr (P == 1) release();
+        };
+        auto values = [&](int c, float (&v)[32]) {
+            if constexpr (P == 1) {
+                uint32_t u[32];
+                tmem_ld32(acc + 32 * c, u);
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] = __uint_as_float(u[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] = total[32 * c + j];
+            }
         };
         // G of 32 columns to global memory through this warp's staging buffer
         [[maybe_unused]] auto write_g = [&](const float (&g)[32], int m, int col) {
@@ -350,10 +428,10 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const float u = g[8 * c + 2 * j], w = g[8 * c + 2 * j + 1];
-                        h[j] = pack_half2(u, w, P == 1 && half_type);
+                        h[j] = pack_half2(u, w, half_type);
                         if constexpr (P == 2) {
-                            const float uh = __uint_as_float(h[j] << 16), wh = __uint_as_float(h[j] & 0xffff0000u);
-                            l[j] = pack_half2(u - uh, w - wh, false);
+                            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+                            l[j] = pack_half2(u - f.x, w - f.y, true);
                         }
                     }
                     st_shared_v4(row + first + ((c ^ x) << 4), h[0], h[1], h[2], h[3]);
@@ -370,6 +448,60 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             }
         };
 
+        [[maybe_unused]] uint32_t turn = 0;
+        // 32 values of row r of a product, from column col, to the parts or to the caller
+        [[maybe_unused]] auto write_out = [&](const float (&v)[32], const ProductScale& scale, int split, int r, int col) {
+            if (p.store != kXentFinal) {
+                float4* to = reinterpret_cast<float4*>(p.part + ((int64_t)split * p.part_rows + r) * p.part_ld + col);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    float4 x = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                    if (p.store == kXentAccumulate) {
+                        const float4 w = to[j];
+                        x.x += w.x; x.y += w.y; x.z += w.z; x.w += w.w;
+                    }
+                    to[j] = x;
+                }
+                return;
+            }
+            const int64_t row = MODE == kXentDHidden ? (int64_t)p.row_of[r] : (int64_t)p.v0 + r;
+            const int64_t at = row * p.out_m + (int64_t)col * p.out_n;
+            if (p.out_vec && col + 32 <= n_extent) {
+                if (p.out_type == MASK_F32) {
+                    float4* to = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) to[j] = make_float4(scale(v[4 * j]), scale(v[4 * j + 1]), scale(v[4 * j + 2]), scale(v[4 * j + 3]));
+                } else {
+                    uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        uint32_t h[4];
+#pragma unroll
+                        for (int q = 0; q < 4; q++) h[q] = pack_half2(scale(v[8 * j + 2 * q]), scale(v[8 * j + 2 * q + 1]), p.out_type == MASK_F16);
+                        to[j] = make_uint4(h[0], h[1], h[2], h[3]);
+                    }
+                }
+                return;
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                if (col + j >= n_extent) continue;
+                const float x = scale(v[j]);
+                if (p.out_type == MASK_F32) static_cast<float*>(p.out)[at + j * p.out_n] = x;
+                else if (p.out_type == MASK_F16) static_cast<__half*>(p.out)[at + j * p.out_n] = __float2half_rn(x);
+                else static_cast<__nv_bfloat16*>(p.out)[at + j * p.out_n] = __float2bfloat16_rn(x);
+            }
+        };
+        const float f = kLogits ? logit_factor(p.range) : 0.f;
+        [[maybe_unused]] const float unit = P == 2 ? (float)(1 << kGradExponent) : 1.f;
+        // exp(logit) over the row's sum, less 1 at its label; 0 outside the rows and classes
+        [[maybe_unused]] auto gradient = [&](float (&v)[32], int col, int classes, bool live, int y, float lse2) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                const float e = fast_exp2(fmaf(v[j], f, -lse2));
+                v[j] = !live || col + j >= classes ? 0.f : unit * (y == col + j ? e - 1.f : e);
+            }
+        };
         for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
             const Item t = item_of(i);
             const int r = t.m * kXentTileM + 32 * quarter + lane;     // row of the tile that this thread holds
@@ -378,30 +510,26 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 float top = -INFINITY, sum = 0.f, picked = 0.f;
                 bool have = false;
                 for (int n = t.n0; n < t.n1; n++) {
-                    const uint32_t acc = acquire();
-                    if (!ok) break;
-#pragma unroll 1
-                    for (int c = 0; c < kHalf; c += 32) {
-                        const int col = n * BN + half * kHalf + c;
+                    if (!acquire(t.k0, t.k1)) { ok = false; break; }
+#pragma unroll(kUnroll)
+                    for (int c = 0; c < kChunks; c++) {
+                        const int col = n * BN + half * kHalf + 32 * c;
                         if (col >= p.classes) break;
-                        uint32_t u[32];
-                        tmem_ld32(acc + c, u);
                         float v[32];
-#pragma unroll
-                        for (int j = 0; j < 32; j++) v[j] = __uint_as_float(u[j]);
+                        values(c, v);
                         if (col + 32 > p.classes) {
 #pragma unroll
                             for (int j = 0; j < 32; j++)
                                 if (col + j >= p.classes) v[j] = -INFINITY;
                         }
-                        online_softmax(v, top, sum);
+                        online_softmax(v, f, top, sum);
                         if (__any_sync(0xffffffffu, (uint32_t)(y - col) < 32u)) {
 #pragma unroll
                             for (int j = 0; j < 32; j++)
                                 if (y - col == j) { picked = v[j]; have = true; }
                         }
                     }
-                    release();
+                    done();
                 }
                 if (ok && r < count) {
                     p.stats[(int64_t)(2 * t.split + half) * p.rows_pad + r] = make_float2(top, sum);
@@ -411,130 +539,89 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 const bool live = r < count;
                 const int y = live ? p.label[r] - p.v0 : -1;
                 const float lse2 = live ? p.lse2[r] : 0.f;
-                const uint32_t acc = acquire();
-                if (!ok) break;
-#pragma unroll 1
-                for (int c = 0; c < kHalf; c += 32) {
-                    const int col = t.n0 * BN + half * kHalf + c;     // within the piece
-                    uint32_t u[32];
-                    tmem_ld32(acc + c, u);
-                    float g[32];
-#pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const float e = fast_exp2(fmaf(__uint_as_float(u[j]), kLog2e, -lse2));
-                        g[j] = !live || col + j >= p.vc ? 0.f : (y == col + j ? e - 1.f : e);
-                    }
-                    write_g(g, t.m, col);
+                if (!acquire(t.k0, t.k1)) { ok = false; break; }
+#pragma unroll(kUnroll)
+                for (int c = 0; c < kChunks; c++) {
+                    const int col = t.n0 * BN + half * kHalf + 32 * c;     // within the piece
+                    float v[32];
+                    values(c, v);
+                    gradient(v, col, p.vc, live, y, lse2);
+                    write_g(v, t.m, col);
                 }
-                release();
+                done();
             } else if constexpr (MODE == kXentGradOne) {
-                // every other tile is this warp's, with all its columns: a row's statistics stay in one thread
-                if ((int)(acc_it & 1) != half) { acc_it++; continue; }
                 const bool live = r < count;
                 const int y = live ? p.label[r] : -1;
-                const uint32_t acc = acquire() - half * kHalf;
-                if (!ok) break;
+                if (!acquire(t.k0, t.k1)) { ok = false; break; }
                 float top = -INFINITY, sum = 0.f, picked = 0.f;
-#pragma unroll 1
-                for (int col = 0; col < BN; col += 32) {
+#pragma unroll(kUnroll)
+                for (int c = 0; c < kChunks; c++) {
+                    const int col = half * kHalf + 32 * c;
                     if (col >= p.classes) break;
-                    uint32_t u[32];
-                    tmem_ld32(acc + col, u);
                     float v[32];
+                    values(c, v);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) v[j] = col + j < p.classes ? __uint_as_float(u[j]) : -INFINITY;
-                    online_softmax(v, top, sum);
+                    for (int j = 0; j < 32; j++)
+                        if (col + j >= p.classes) v[j] = -INFINITY;
+                    online_softmax(v, f, top, sum);
 #pragma unroll
                     for (int j = 0; j < 32; j++)
                         if (y - col == j) picked = v[j];
                 }
-                const float lse2 = fmaf(top, kLog2e, log2f(sum));
-                const float loss = live ? fmaf(lse2, kLn2, -picked) : 0.f;
-                if (live && p.row_loss) p.row_loss[p.row_of[r]] = loss;
-                float w = loss;
+                // The two warps that hold halves of the same rows tell each other.  Two turns' worth of room: a warp writes
+                // turn i + 2 after the other has arrived at turn i + 1, hence read turn i.
+                float* ex = reinterpret_cast<float*>(gbase + L::kExchange) + (turn & 1) * 2 * 128 * 3;
+                float* mine = ex + (half * 128 + 32 * quarter + lane) * 3;
+                mine[0] = top;
+                mine[1] = sum;
+                mine[2] = picked;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(exchange_bar(quarter));
+                if (!__all_sync(0xffffffffu, mbar_wait(exchange_bar(quarter), turn & 1, abort_flag))) { ok = false; break; }
+                turn++;
+                // both halves in the same order on both sides, so that both get the same bits
+                const float* a = ex + (32 * quarter + lane) * 3;
+                const float* b = a + 128 * 3;
+                const float most = fmaxf(a[0], b[0]);
+                const float bs = most == -INFINITY ? 0.f : most * f;
+                const float lse2 = bs + log2f(a[1] * fast_exp2(fmaf(a[0], f, -bs)) + b[1] * fast_exp2(fmaf(b[0], f, -bs)));
+                if (half == 0) {
+                    const float loss = live ? kLn2 * fmaf(-(a[2] + b[2]), f, lse2) : 0.f;
+                    if (live && p.row_loss) p.row_loss[p.row_of[r]] = loss;
+                    float w = loss;
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-                if (lane == 0) p.warp_loss[t.m * (kXentTileM / 32) + quarter] = w;
-#pragma unroll 1
-                for (int col = 0; col < BN; col += 32) {
-                    uint32_t u[32];
-                    tmem_ld32(acc + col, u);
-                    float g[32];
-#pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const float e = fast_exp2(fmaf(__uint_as_float(u[j]), kLog2e, -lse2));
-                        g[j] = !live || col + j >= p.classes ? 0.f : (y == col + j ? e - 1.f : e);
-                    }
-                    write_g(g, t.m, col);
+                    for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+                    if (lane == 0) p.warp_loss[t.m * (kXentTileM / 32) + quarter] = w;
                 }
-                release();
+#pragma unroll(kUnroll)
+                for (int c = 0; c < kChunks; c++) {
+                    const int col = half * kHalf + 32 * c;
+                    float v[32];
+                    values(c, v);
+                    gradient(v, col, p.classes, live, y, lse2);
+                    write_g(v, t.m, col);
+                }
+                done();
             } else {
                 const bool empty = t.k0 >= t.k1;      // nothing to contract: the sum is zero
-                uint32_t acc = 0;
-                if (!empty) {
-                    acc = acquire();
-                    if (!ok) break;
-                }
-                const float scale = xent_scale(p, count);
+                if (!empty && !acquire(t.k0, t.k1)) { ok = false; break; }
+                const ProductScale scale = product_scale(p.scale, p.mean, count, p.range, MODE == kXentDHidden ? 1 : 0);
                 const bool live = r < m_extent;
-#pragma unroll 1
-                for (int c = 0; c < kHalf; c += 32) {
-                    const int col = t.n0 * BN + half * kHalf + c;
+#pragma unroll(kUnroll)
+                for (int c = 0; c < kChunks; c++) {
+                    const int col = t.n0 * BN + half * kHalf + 32 * c;
                     if (col >= n_extent) break;
-                    __syncwarp();
-                    uint32_t u[32];
+                    float v[32];
                     if (!empty) {
-                        tmem_ld32(acc + c, u);
+                        __syncwarp();
+                        values(c, v);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 32; j++) u[j] = 0u;
+                        for (int j = 0; j < 32; j++) v[j] = 0.f;
                     }
-                    if (!live) continue;
-                    if (p.store != kXentFinal) {
-                        float4* to = reinterpret_cast<float4*>(p.part + ((int64_t)t.split * p.part_rows + r) * p.part_ld + col);
-#pragma unroll
-                        for (int j = 0; j < 8; j++) {
-                            float4 v = make_float4(__uint_as_float(u[4 * j]), __uint_as_float(u[4 * j + 1]), __uint_as_float(u[4 * j + 2]), __uint_as_float(u[4 * j + 3]));
-                            if (p.store == kXentAccumulate) {
-                                const float4 w = to[j];
-                                v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
-                            }
-                            to[j] = v;
-                        }
-                        continue;
-                    }
-                    const int64_t row = MODE == kXentDHidden ? (int64_t)p.row_of[r] : (int64_t)p.v0 + r;
-                    const int64_t at = row * p.out_m + (int64_t)col * p.out_n;
-                    if (p.out_vec && col + 32 <= n_extent) {
-                        if (p.out_type == MASK_F32) {
-                            float4* to = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
-#pragma unroll
-                            for (int j = 0; j < 8; j++)
-                                to[j] = make_float4(scale * __uint_as_float(u[4 * j]), scale * __uint_as_float(u[4 * j + 1]),
-                                                    scale * __uint_as_float(u[4 * j + 2]), scale * __uint_as_float(u[4 * j + 3]));
-                        } else {
-                            uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
-#pragma unroll
-                            for (int j = 0; j < 4; j++) {
-                                uint32_t h[4];
-#pragma unroll
-                                for (int q = 0; q < 4; q++)
-                                    h[q] = pack_half2(scale * __uint_as_float(u[8 * j + 2 * q]), scale * __uint_as_float(u[8 * j + 2 * q + 1]), p.out_type == MASK_F16);
-                                to[j] = make_uint4(h[0], h[1], h[2], h[3]);
-                            }
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; j++) {
-                            if (col + j >= n_extent) continue;
-                            const float v = scale * __uint_as_float(u[j]);
-                            if (p.out_type == MASK_F32) static_cast<float*>(p.out)[at + j * p.out_n] = v;
-                            else if (p.out_type == MASK_F16) static_cast<__half*>(p.out)[at + j * p.out_n] = __float2half_rn(v);
-                            else static_cast<__nv_bfloat16*>(p.out)[at + j * p.out_n] = __float2bfloat16_rn(v);
-                        }
-                    }
+                    if (live) write_out(v, scale, t.split, r, col);
                 }
-                if (!empty) release();
+                if (!empty) done();
             }
         }
         if constexpr (L::kWritesG) {

@@ -1,14 +1,14 @@
 """The classifier head (``engine.linear_cross_entropy``) against its definition in 64 bits.
 
-Tolerances are sums of what each step may be off by (``u`` = half a step of a type, relative):
-  * a product of two float32 values is taken as hi hi + hi lo + lo hi of bfloat16 parts: x = hi + lo + e with
-    |e| <= 2^-8 2^-8 |x| / 2 for each operand and the dropped lo lo <= 2^-16 |x y|: 2^-15 |x y| in all at worst; of 16-bit
-    values exactly;
-  * float32 sums: at most one unit in the last place (2^-23 of what has been summed) for each step of 16 products, three
-    times as many steps for float32 operands, and one for each of at most 600 parts;
+Tolerances are sums of what each step may be off by:
+  * float32 operands are scaled by a power of two and taken as two float16 parts: x = hi + lo + e with |e| <= 2^-22 |x| or
+    2^-40 of the largest |x|, and of the four products of parts lo lo (2^-22) is dropped: 2^-20 |x y| in all, and 2^-39 of the
+    largest; 16-bit operands are multiplied exactly;
+  * float32 sums: at most one unit in the last place (2^-23 of what has been summed) for each step of 16 products -- with
+    float32 operands 48 such steps at most, then one for each 256 of the contraction -- and one for each part, of 64 of the contraction at least, of at most 600;
   * the gradient of the logits: its logit's and log sum's errors (each the largest of a row's logits'), the exponential's
-    (2^-20) and, between the products, one rounding (2^-8 bfloat16, 2^-11 float16; 2^-16 for two bfloat16 parts; 2^-25
-    absolutely below float16's normal range);
+    (2^-20) and, between the products, one rounding (2^-8 bfloat16; 2^-11 float16, or 2^-25 below its normal range; 2^-22 or
+    2^-40 for two parts);
   * the results' own rounding.
 """
 import ctypes as C
@@ -50,10 +50,11 @@ def _want(hidden, weight, labels, reduction="mean", scale=1.0):
     keep = (labels >= 0) & (labels < classes)
     h, w = hidden[keep].double(), weight.double()
     y, n = labels[keep], int(keep.sum())
-    rel = 2.0 ** -15 if f32 else 0.0
-    steps = lambda k: 2.0 ** -23 * ((3 if f32 else 1) * (k / 16 + 1) + 600)   # noqa: E731
+    rel, least = (2.0 ** -20, 2.0 ** -39) if f32 else (0.0, 0.0)
+    steps = lambda k: 2.0 ** -23 * ((min(3 * (k / 16 + 1), 48) + k / 256 if f32 else k / 16 + 1) + min(k / 64 + 1, 600))   # noqa: E731
+    most = lambda x: float(x.abs().max()) if x.numel() else 0.0   # noqa: E731
     logits = h @ w
-    elogit = (h.abs() @ w.abs()).mul_(rel + steps(dim))
+    elogit = (h.abs() @ w.abs()).mul_(rel + steps(dim)) + least * (most(h) * w.abs().sum(0) + most(w) * h.abs().sum(1, keepdim=True))
     erow = elogit.amax(1, keepdim=True) if n else elogit.sum(1, keepdim=True)
     lse = torch.logsumexp(logits, 1, keepdim=True)
     rows = (lse - logits.gather(1, y[:, None])).squeeze(1)
@@ -63,7 +64,8 @@ def _want(hidden, weight, labels, reduction="mean", scale=1.0):
     g = p - hot
     # the exponent's argument is rounded too: 2^-23 of the logit and of the log sum
     eg = p * (2 * erow + 2.0 ** -20 + 2.0 ** -22 * (logits.abs() + lse.abs())).expm1() + 2.0 ** -23 * hot
-    eg += g.abs() * (2.0 ** -16 if f32 else 2.0 ** -8 if hidden.dtype == torch.bfloat16 else 2.0 ** -11) + (0.0 if hidden.dtype != torch.float16 else 2.0 ** -25)
+    eg += g.abs() * (2.0 ** -22 if f32 else 2.0 ** -8 if hidden.dtype == torch.bfloat16 else 2.0 ** -11)
+    eg += 2.0 ** -40 if f32 else 0.0 if hidden.dtype == torch.bfloat16 else 2.0 ** -25
     if reduction == "mean" and n:
         scale = scale / n
     out = 2.0 ** -23 if f32 else torch.finfo(hidden.dtype).eps / 2
@@ -71,9 +73,9 @@ def _want(hidden, weight, labels, reduction="mean", scale=1.0):
     dh = torch.zeros(hidden.shape, dtype=torch.float64, device="cuda")
     eh = torch.zeros_like(dh)
     dh[keep] = scale * (g @ w.t())
-    eh[keep] = abs(scale) * (eg @ w.abs().t() + (g.abs() @ w.abs().t()) * (rel + steps(classes)))
+    eh[keep] = abs(scale) * (eg @ w.abs().t() + (g.abs() @ w.abs().t()) * (rel + steps(classes)) + least * most(w) * g.abs().sum(1, keepdim=True))
     dw = scale * (h.t() @ g)
-    ew = abs(scale) * (h.abs().t() @ eg + (h.abs().t() @ g.abs()) * (rel + steps(n)))
+    ew = abs(scale) * (h.abs().t() @ eg + (h.abs().t() @ g.abs()) * (rel + steps(n)) + least * most(h) * g.abs().sum(0))
     eh, ew = eh * 1.01 + out * dh.abs() + tiny * keep[:, None], ew * 1.01 + out * dw.abs() + tiny
     if reduction == "none":
         loss, eloss = torch.zeros(len(labels), dtype=torch.float64, device="cuda"), torch.zeros(len(labels), dtype=torch.float64, device="cuda")
@@ -180,7 +182,7 @@ def test_nan_in_a_labelled_row(classes):
 
 @gpu
 def test_large_and_small_logits():
-    """Logits of some thousands, and rows whose label is certain or out of the question."""
+    """Logits of some thousands beside rows of zeros, and rows whose label is certain or out of the question."""
     import torch
     for classes in (50, 600):
         hidden, weight, labels = _inputs(150, 64, classes, "f32", seed=9)
@@ -190,6 +192,15 @@ def test_large_and_small_logits():
         hidden[120] = 0.0
         got = _both(hidden, weight, labels, "none")
         assert bool(torch.isfinite(got[0]).all())
+
+
+@gpu
+@pytest.mark.parametrize("classes", [50, 600])
+@pytest.mark.parametrize("scale_h,scale_w", [(1e-30, 1e30), (1e25, 1e-26), (3e-39, 1.0), (1e-3, 1e3)])
+def test_operands_of_any_magnitude(scale_h, scale_w, classes):
+    """float32 operands far from 1, subnormal ones among them."""
+    hidden, weight, labels = _inputs(150, 64, classes, "f32", "dim", "some", seed=10)
+    _both(hidden * scale_h, weight * scale_w, labels, scale=1e-6)
 
 
 @gpu
