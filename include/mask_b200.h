@@ -446,6 +446,52 @@ typedef struct mask_head {
 size_t mask_linear_xent_scratch_bytes(const mask_head* head);   /* 0 for arguments that mask_linear_xent refuses */
 int mask_linear_xent(const mask_head* head, void* d_scratch, size_t scratch_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------
+ * Group norm with an activation over node features, channels last, of one graph or a batch of graphs
+ * (rows d_offsets[b] .. d_offsets[b+1] are graph b), and its gradients: what stands between a sparse
+ * product and the next layer where hidden features are normalised.  No counterpart in the reference.
+ *
+ * Statistics are those of a graph's rows and a group's channels / groups neighbouring channels:
+ *   y = act((x - mean) rstd weight + bias),  rstd = 1 / sqrt(variance + eps)
+ * mask_group_norm writes y, mean and rstd ([graphs, groups], float32); mask_group_norm_backward reads x,
+ * grad, mean and rstd and writes dx (d_y, NULL: not wanted), dweight and dbias (NULL: not wanted).  The
+ * gradient of ReLU is taken from the same 32-bit value as the forward pass's output.  The variance is a sum
+ * of squared differences, not a difference of squares; sums are 32 or 64 bits.  The same call gives the
+ * same bits.
+ *
+ * Offsets ascend and lie in [0, rows]; rows outside every graph are neither read nor written, a graph
+ * without rows has mean 0 and rstd 1 / sqrt(eps).  (Offsets that break this give wrong results, but nothing
+ * outside the arrays is touched.)  y may be x, and dx may be x or grad.  Scratch:
+ * mask_group_norm_scratch_bytes, 256-byte aligned, one call at a time.  Asynchronous on `stream`.
+ * ------------------------------------------------------------------------------------------ */
+typedef enum mask_activation { MASK_ACT_NONE = 0, MASK_ACT_RELU = 1, MASK_ACT_SILU = 2 } mask_activation;
+
+typedef struct mask_norm {
+    int32_t dtype;              /* mask_dtype of x, y, grad and dx */
+    int32_t activation;         /* mask_activation */
+    int64_t rows;               /* < 2^31 */
+    int32_t channels, groups;   /* channels a multiple of groups, at most 2^20 */
+    int32_t graphs;             /* 1 or more; 1 without offsets */
+    float eps;
+    const int32_t* d_offsets;   /* [graphs + 1], or NULL: one graph of all rows */
+    const void* d_x;            /* rows x_stride elements apart */
+    int64_t x_stride;
+    const float* d_weight;      /* [channels], or NULL: 1 */
+    const float* d_bias;        /* [channels], or NULL: 0 */
+    void* d_y;                  /* y, or dx */
+    int64_t y_stride;
+    float* d_mean;              /* [graphs, groups]; read by the backward pass */
+    float* d_rstd;
+    const void* d_grad;         /* backward: gradient of y */
+    int64_t grad_stride;
+    float* d_dweight;           /* backward, [channels], or NULL */
+    float* d_dbias;
+} mask_norm;
+
+size_t mask_group_norm_scratch_bytes(const mask_norm* norm, int backward);   /* 0 for arguments that the call refuses */
+int mask_group_norm(const mask_norm* norm, void* d_scratch, size_t scratch_bytes, void* stream);
+int mask_group_norm_backward(const mask_norm* norm, void* d_scratch, size_t scratch_bytes, void* stream);
+
 /* Development knobs for kernel variants, process-wide: "sweep" (1 = persistent tcgen05 kernel except
  * where the warp-level one measures faster (by N and the plan), 2 = always, 0 = warp-level kernels only),
  * "nslab" (tcgen05 kernel: 128-column slabs per sweep, 1 / 2 / 4; 0 = the plan table's choice),

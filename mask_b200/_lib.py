@@ -61,6 +61,9 @@ SIGNATURES = {
     "mask_spmm_srbcrs_static_scratch": (C.c_int, [vp, vp, vp, vp, i32, i32, i32, vp, i64, vp, i64, C.c_int, vp]),
     "mask_linear_xent_scratch_bytes": (sz, [vp]),
     "mask_linear_xent": (C.c_int, [vp, vp, sz, vp]),
+    "mask_group_norm_scratch_bytes": (sz, [vp, C.c_int]),
+    "mask_group_norm": (C.c_int, [vp, vp, sz, vp]),
+    "mask_group_norm_backward": (C.c_int, [vp, vp, sz, vp]),
     "mask_tune": (C.c_int, [C.c_char_p, C.c_int]),
     "mask_spmm_kernel_name": (C.c_int, [vp, C.c_int, i32, C.c_int, C.c_char_p, sz]),
     "mask_spmm_warp_shape": (C.c_int, [vp, C.c_int, i32, C.c_int, C.POINTER(i32), C.POINTER(i32)]),
@@ -75,6 +78,7 @@ SIGNATURES = {
 
 REORDER = {"none": 0, "row_rcm": 1, "first_col_sort": 2, "jaccard_greedy": 3}
 REDUCTION = {"none": 0, "mean": 1, "sum": 2}
+ACTIVATION = {"none": 0, "relu": 1, "silu": 2}
 POLICY = {"auto": 0, "row": 1, "strict_lb": 2, "multi_bind": 3, "ref_auto": 4}
 
 
@@ -89,6 +93,13 @@ class Head(C.Structure):
                 ("weight", vp), ("weight_dim_stride", i64), ("weight_class_stride", i64), ("labels", vp), ("loss", vp),
                 ("grad_scale", C.c_float), ("reserved", i32), ("dhidden", vp), ("dhidden_stride", i64), ("dweight", vp),
                 ("dweight_dim_stride", i64), ("dweight_class_stride", i64)]
+
+
+class Norm(C.Structure):
+    """mask_norm"""
+    _fields_ = [("dtype", i32), ("activation", i32), ("rows", i64), ("channels", i32), ("groups", i32), ("graphs", i32), ("eps", C.c_float),
+                ("offsets", vp), ("x", vp), ("x_stride", i64), ("weight", vp), ("bias", vp), ("y", vp), ("y_stride", i64), ("mean", vp),
+                ("rstd", vp), ("grad", vp), ("grad_stride", i64), ("dweight", vp), ("dbias", vp)]
 
 
 class Features(C.Structure):

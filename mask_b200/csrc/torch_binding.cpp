@@ -196,6 +196,132 @@ PyObject* linear_xent_checked(PyObject* const* args, Py_ssize_t n_args) {
     return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(loss)), THPVariable_Wrap(std::move(dhidden)), THPVariable_Wrap(std::move(dweight)));
 }
 
+// What both directions of group norm take: x, its result, the affine parameters and the batch's offsets.
+bool norm_operands(mask_norm& n, PyObject* px, PyObject* groups, PyObject* weight, PyObject* bias, PyObject* offsets, PyObject* activation, PyObject* out,
+                   int* device, const at::Tensor** x, at::Tensor& y) {
+    *x = device_tensor(px, "x", 2, device);
+    if (!*x) return false;
+    n.dtype = dtype_of(**x, "x");
+    if (n.dtype < 0) return false;
+    const int64_t rows = (*x)->size(0), channels = (*x)->size(1), g = PyLong_AsLong(groups);
+    n.activation = (int32_t)PyLong_AsLong(activation);
+    if (PyErr_Occurred()) return false;
+    if (channels < 1 || channels > (1 << 20) || rows >= ((int64_t)1 << 31)) return raise("x must have 1 to 2^20 columns and fewer than 2^31 rows"), false;
+    if (g < 1 || channels % g) {
+        PyErr_Format(PyExc_RuntimeError, "%lld channels are not a multiple of %lld groups", (long long)channels, (long long)g);
+        return false;
+    }
+    if (channels > 1 && (*x)->stride(1) != 1) return raise("rows of x must be contiguous"), false;
+    n.rows = rows;
+    n.channels = (int32_t)channels;
+    n.groups = (int32_t)g;
+    n.d_x = (*x)->const_data_ptr();
+    n.x_stride = (*x)->stride(0);
+    const char* names[2] = {"weight", "bias"};
+    PyObject* objects[2] = {weight, bias};
+    const float** to[2] = {&n.d_weight, &n.d_bias};
+    for (int i = 0; i < 2; i++) {
+        if (objects[i] == Py_None) continue;
+        const at::Tensor* t = device_tensor(objects[i], names[i], 1, device);
+        if (!t) return false;
+        if (t->scalar_type() != at::kFloat || t->size(0) != channels || !t->is_contiguous()) {
+            PyErr_Format(PyExc_RuntimeError, "%s must be contiguous float32 with one value per channel", names[i]);
+            return false;
+        }
+        *to[i] = t->const_data_ptr<float>();
+    }
+    n.graphs = 1;
+    if (offsets != Py_None) {
+        const at::Tensor* t = device_tensor(offsets, "offsets", 1, device);
+        if (!t) return false;
+        if (t->scalar_type() != at::kInt || !t->is_contiguous() || t->size(0) < 2 || t->size(0) > (1 << 24))
+            return raise("offsets must be contiguous int32 with one entry more than there are graphs"), false;
+        n.graphs = (int32_t)(t->size(0) - 1);
+        n.d_offsets = t->const_data_ptr<int32_t>();
+    }
+    if (out == Py_None) {
+        y = at::empty({rows, channels}, (*x)->options());
+    } else {
+        const at::Tensor* t = device_tensor(out, "out", 2, device);
+        if (!t) return false;
+        if (t->scalar_type() != (*x)->scalar_type() || t->size(0) != rows || t->size(1) != channels) return raise("out must have x's shape and dtype"), false;
+        if ((channels > 1 && t->stride(1) != 1) || (rows > 1 && t->stride(0) < channels)) return raise("rows of out must be contiguous and apart"), false;
+        y = *t;
+    }
+    n.d_y = y.mutable_data_ptr();
+    n.y_stride = y.stride(0);
+    return true;
+}
+
+int run_norm(const mask_norm& n, bool backward, const at::Tensor& x) {
+    const size_t need = mask_group_norm_scratch_bytes(&n, backward);
+    at::Tensor scratch = at::empty({(int64_t)need}, x.options().dtype(at::kByte));
+    cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = backward ? mask_group_norm_backward(&n, scratch.mutable_data_ptr(), need, stream) : mask_group_norm(&n, scratch.mutable_data_ptr(), need, stream);
+    Py_END_ALLOW_THREADS
+    return rc;
+}
+
+PyObject* result_of(PyObject* out, at::Tensor&& y) {
+    if (out == Py_None) return THPVariable_Wrap(std::move(y));
+    Py_INCREF(out);
+    return out;
+}
+
+// group_norm(x, groups, weight, bias, offsets, eps, activation, out) -> (y, mean, rstd), or the status of a call that failed
+PyObject* group_norm_checked(PyObject* const* args, Py_ssize_t n_args) {
+    if (n_args != 8) return raise("group_norm takes 8 arguments");
+    mask_norm n{};
+    int device = -1;
+    const at::Tensor* x;
+    at::Tensor y;
+    n.eps = (float)PyFloat_AsDouble(args[5]);
+    if (PyErr_Occurred()) return nullptr;
+    if (!(n.eps >= 0.f)) return raise("eps must not be negative");
+    if (!norm_operands(n, args[0], args[1], args[2], args[3], args[4], args[6], args[7], &device, &x, y)) return nullptr;
+    at::Tensor mean = at::empty({n.graphs, n.groups}, x->options().dtype(at::kFloat)), rstd = at::empty_like(mean);
+    n.d_mean = mean.mutable_data_ptr<float>();
+    n.d_rstd = rstd.mutable_data_ptr<float>();
+    const int rc = run_norm(n, false, *x);
+    if (rc != MASK_OK) return PyLong_FromLong(rc);
+    return Py_BuildValue("(NNN)", result_of(args[7], std::move(y)), THPVariable_Wrap(std::move(mean)), THPVariable_Wrap(std::move(rstd)));
+}
+
+// group_norm_backward(grad, x, mean, rstd, groups, weight, bias, offsets, activation, out) -> (dx, dweight, dbias), or a status
+PyObject* group_norm_backward_checked(PyObject* const* args, Py_ssize_t n_args) {
+    if (n_args != 10) return raise("group_norm_backward takes 10 arguments");
+    mask_norm n{};
+    int device = -1;
+    const at::Tensor* x;
+    at::Tensor dx;
+    if (!norm_operands(n, args[1], args[4], args[5], args[6], args[7], args[8], args[9], &device, &x, dx)) return nullptr;
+    const at::Tensor* grad = device_tensor(args[0], "grad", 2, &device);
+    if (!grad) return nullptr;
+    if (grad->scalar_type() != x->scalar_type() || grad->size(0) != n.rows || grad->size(1) != n.channels) return raise("grad must have x's shape and dtype");
+    if (n.channels > 1 && grad->stride(1) != 1) return raise("rows of grad must be contiguous");
+    n.d_grad = grad->const_data_ptr();
+    n.grad_stride = grad->stride(0);
+    const char* names[2] = {"mean", "rstd"};
+    float** to[2] = {&n.d_mean, &n.d_rstd};
+    for (int i = 0; i < 2; i++) {
+        const at::Tensor* t = device_tensor(args[2 + i], names[i], 2, &device);
+        if (!t) return nullptr;
+        if (t->scalar_type() != at::kFloat || t->size(0) != n.graphs || t->size(1) != n.groups || !t->is_contiguous()) {
+            PyErr_Format(PyExc_RuntimeError, "%s must be contiguous float32 [graphs, groups]", names[i]);
+            return nullptr;
+        }
+        *to[i] = const_cast<float*>(t->const_data_ptr<float>());   // read only
+    }
+    at::Tensor dweight = at::empty({n.channels}, x->options().dtype(at::kFloat)), dbias = at::empty_like(dweight);
+    n.d_dweight = dweight.mutable_data_ptr<float>();
+    n.d_dbias = dbias.mutable_data_ptr<float>();
+    const int rc = run_norm(n, true, *x);
+    if (rc != MASK_OK) return PyLong_FromLong(rc);
+    return Py_BuildValue("(NNN)", result_of(args[9], std::move(dx)), THPVariable_Wrap(std::move(dweight)), THPVariable_Wrap(std::move(dbias)));
+}
+
 // Tensors without storage or strides (sparse ones, those of torch.func's transforms) throw already when they are asked
 // for an address or whether they are contiguous.
 template <PyObject* (*Body)(PyObject* const*, Py_ssize_t)>
@@ -216,6 +342,8 @@ PyMethodDef method(const char* name, const char* doc) {
 PyMethodDef methods[] = {
     method<product>("spmm", "out = A @ dense, or a status"),
     method<linear_xent_checked>("linear_xent", "loss, or (loss, dhidden, dweight), or a status"),
+    method<group_norm_checked>("group_norm", "(y, mean, rstd), or a status"),
+    method<group_norm_backward_checked>("group_norm_backward", "(dx, dweight, dbias), or a status"),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

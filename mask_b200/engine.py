@@ -349,6 +349,36 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: tor
     return got
 
 
+def _activation(name):
+    if name not in _lib.ACTIVATION:
+        raise RuntimeError(f"activation must be one of {', '.join(_lib.ACTIVATION)}")
+    return _lib.ACTIVATION[name]
+
+
+def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               offsets: torch.Tensor | None = None, eps: float = 1e-5, activation: str = "none", out: torch.Tensor | None = None):
+    """Group norm of node features ``x[rows, channels]`` (float32, bfloat16 or float16) and an activation ("none", "relu",
+    "silu") on the current stream: returns (y, mean, rstd), the statistics float32 ``[graphs, groups]`` over a graph's rows
+    and a group's neighbouring channels.  ``offsets`` (int32, graphs + 1) are the batch's first rows, ascending; without them
+    all rows are one graph.  Rows outside every graph are not written.  ``weight`` and ``bias`` are float32 ``[channels]``.
+    ``x`` may have any distance between its rows; ``out`` may be ``x``."""
+    got = (_lib._binding or _lib.binding()).group_norm(x, groups, weight, bias, offsets, eps, _activation(activation), out)
+    if type(got) is int:
+        check(got, "mask_group_norm")
+    return got
+
+
+def group_norm_backward(grad: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, groups: int,
+                        weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, offsets: torch.Tensor | None = None,
+                        activation: str = "none", out: torch.Tensor | None = None):
+    """Gradients of ``group_norm`` from the gradient of y, x and the statistics it returned: (dx, dweight, dbias), the last
+    two float32.  ``out`` takes dx and may be ``grad`` or ``x``."""
+    got = (_lib._binding or _lib.binding()).group_norm_backward(grad, x, mean, rstd, groups, weight, bias, offsets, _activation(activation), out)
+    if type(got) is int:
+        check(got, "mask_group_norm_backward")
+    return got
+
+
 def kernel_signature(packed, N: int, plan: Plan, tf32x3: bool = False) -> tuple[str, int]:
     """(name of the kernel ``spmm`` launches for this matrix, plan and N; the library's kernel revision)."""
     fmt = 2 if isinstance(packed, PackedMCO) else (1 if isinstance(packed, PackedMETCF) else 0)
