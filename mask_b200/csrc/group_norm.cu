@@ -6,12 +6,18 @@
 //     du = dy act'(u),  xhat = (x - mean) rstd,  dbeta_c = sum du,  dgamma_c = sum du xhat   (over all rows),
 //     dx = rstd (du gamma - m1 - xhat m2),  m1 = sum du gamma / n,  m2 = sum du gamma xhat / n   (over graph and group).
 // Both directions are a pass of sums over the features, a join of the sums and a pass that writes.  Rows are dealt out in
-// chunks of one graph; a block takes a chunk and up to 32 vectors of 16 bytes of channels, so that its loads are whole
-// 512-byte stretches whatever the groups are, and leaves two numbers per channel.  They are joined in a fixed order: the
-// same call gives the same bits.  The variance is never taken as a difference of squares: 8 values at a time are centred on
-// their own mean, and (count, mean, sum of squares) triples are joined.  A batch's chunks need no table: chunk j of graph b
+// chunks of one graph; a block takes a chunk and a slab of up to 32 x 4 channels, so that its loads are whole stretches of
+// 256 or 512 bytes whatever the groups are, and leaves two numbers per channel.  A graph that is one chunk is finished by its
+// block at once (where slabs hold whole groups): small graphs are read from memory once.  Sums are joined in a fixed order:
+// the same call gives the same bits.  The variance is never taken as a difference of squares: 8 values at a time are centred
+// on their own mean, and (count, mean, sum of squares) triples are joined.  A batch's chunks need no table: chunk j of graph b
 // has number off[b] / chunk + b + j, which leaves room for every graph's last, shorter chunk.
+//
+// Bound by memory where nothing but sums is computed; SiLU costs two special-function operations a value, 8 values a clock
+// and SM.  Channels go in pairs through the packed float instructions, which halves what else is issued (9 instead of 26
+// instructions a value in the backward sums).
 #include <algorithm>
+#include <type_traits>
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -22,14 +28,15 @@
 namespace mask {
 
 constexpr int kNormThreads = 256;
-constexpr int kNormBatch = 8;       // rows a thread has in flight
+constexpr int kNormVec = 4;         // channels of a thread
 
 struct NormArgs {
     int64_t rows;
-    int32_t channels, groups, per_group, graphs, activation;
+    int32_t channels, groups, per_group, graphs;
     float eps;
     int32_t chunk;              // rows
     int32_t tx;                 // threads along the channels (a power of two), 256 / tx along the rows
+    int32_t whole;              // slabs hold whole groups
     const int32_t* offsets;     // or NULL: one graph
     const void* x;
     int64_t x_stride;
@@ -44,52 +51,123 @@ struct NormArgs {
     float* dweight;             // or NULL
     float* dbias;               // or NULL
     float2* part;               // [chunks][channels]: mean and sum of squares around it; backward: sums of du, du xhat
-    float2* sums;               // [graphs][channels], backward
+    float2* sums;               // [graphs][channels], backward, graphs of several chunks
 };
 
-template <typename T> __device__ __forceinline__ float to_float(T x);
-template <> __device__ __forceinline__ float to_float(float x) { return x; }
-template <> __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <> __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-template <typename T> __device__ __forceinline__ T from_float(float x);
-template <> __device__ __forceinline__ float from_float(float x) { return x; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float(float x) { return __float2bfloat16_rn(x); }
-template <> __device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x); }
-
-template <typename T, int VEC>
-struct Vec {
-    uint4 raw;
-    __device__ __forceinline__ void load(const T* from) {
-        if constexpr (VEC == 1) *reinterpret_cast<T*>(&raw) = *from;
-        else raw = *reinterpret_cast<const uint4*>(from);
+// ---- pairs -------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint64_t bits(float2 a) { return *reinterpret_cast<uint64_t*>(&a); }
+__device__ __forceinline__ float2 pair(uint64_t a) { return *reinterpret_cast<float2*>(&a); }
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+    return pair(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+    return pair(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+    return pair(r);
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 1 / (1 + exp(-u)); exp's overflow gives 0
+__device__ __forceinline__ float2 sigmoid2(float2 u) {
+    const float2 t = mul2(u, both(-1.4426950408889634f));
+    const float2 d = add2(make_float2(exp2_approx(t.x), exp2_approx(t.y)), both(1.f));
+    return make_float2(rcp_approx(d.x), rcp_approx(d.y));
+}
+template <int ACT>
+__device__ __forceinline__ float2 activate2(float2 u) {
+    if constexpr (ACT == MASK_ACT_RELU) {     // NaN stays NaN
+        float2 r;
+        asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r.x) : "f"(u.x));
+        asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r.y) : "f"(u.y));
+        return r;
     }
-    __device__ __forceinline__ void store(T* to) const {
-        if constexpr (VEC == 1) *to = *reinterpret_cast<const T*>(&raw);
-        else *reinterpret_cast<uint4*>(to) = raw;
-    }
-    __device__ __forceinline__ float get(int i) const { return to_float(reinterpret_cast<const T*>(&raw)[i]); }
-    __device__ __forceinline__ void set(int i, float v) { reinterpret_cast<T*>(&raw)[i] = from_float<T>(v); }
-};
-
-__device__ __forceinline__ float sigmoid(float u) { return __fdividef(1.f, 1.f + __expf(-u)); }   // exp overflows to inf: 0
-__device__ __forceinline__ float activate(float u, int activation) {
-    if (activation == MASK_ACT_RELU) return u < 0.f ? 0.f : u;      // NaN stays
-    if (activation == MASK_ACT_SILU) return u == -INFINITY ? 0.f : u * sigmoid(u);
+    if constexpr (ACT == MASK_ACT_SILU) return mul2(u, sigmoid2(u));
     return u;
 }
-__device__ __forceinline__ float activate_slope(float u, int activation) {
-    if (activation == MASK_ACT_RELU) return u > 0.f ? 1.f : (u <= 0.f ? 0.f : u);
-    if (activation == MASK_ACT_SILU) {
-        const float s = sigmoid(u);
-        return s == 0.f ? 0.f : s * (1.f + u * (1.f - s));
+// dy act'(u)
+template <int ACT>
+__device__ __forceinline__ float2 through_activation2(float2 dy, float2 u) {
+    if constexpr (ACT == MASK_ACT_RELU) {     // u of NaN: NaN
+        return make_float2(u.x > 0.f ? dy.x : (u.x <= 0.f ? 0.f : u.x), u.y > 0.f ? dy.y : (u.y <= 0.f ? 0.f : u.y));
     }
-    return 1.f;
+    if constexpr (ACT == MASK_ACT_SILU) {     // s + u s (1 - s)
+        const float2 s = sigmoid2(u);
+        return mul2(dy, fma2(mul2(u, s), fma2(s, both(-1.f), both(1.f)), s));
+    }
+    return dy;
 }
+
+// Four channels of a row, or one (VEC == 1, where the addresses or the channel count rule out vectors).
+template <typename T, int VEC>
+struct Row {
+    uint32_t raw[VEC == 1 ? 1 : (sizeof(T) == 4 ? 4 : 2)];
+    __device__ __forceinline__ void load(const T* from) {
+        if constexpr (VEC == 1) {
+            if constexpr (sizeof(T) == 4) raw[0] = *reinterpret_cast<const uint32_t*>(from);
+            else raw[0] = *reinterpret_cast<const uint16_t*>(from);
+        } else if constexpr (sizeof(T) == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(from);
+            raw[0] = v.x; raw[1] = v.y; raw[2] = v.z; raw[3] = v.w;
+        } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(from);
+            raw[0] = v.x; raw[1] = v.y;
+        }
+    }
+    __device__ __forceinline__ void store(T* to) const {
+        if constexpr (VEC == 1) {
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(to) = raw[0];
+            else *reinterpret_cast<uint16_t*>(to) = (uint16_t)raw[0];
+        } else if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<uint4*>(to) = make_uint4(raw[0], raw[1], raw[2], raw[3]);
+        } else {
+            *reinterpret_cast<uint2*>(to) = make_uint2(raw[0], raw[1]);
+        }
+    }
+    // channels 2i and 2i + 1; VEC == 1: the second is 0
+    __device__ __forceinline__ float2 get(int i) const {
+        if constexpr (sizeof(T) == 4) {
+            return make_float2(__uint_as_float(raw[2 * i]), VEC == 1 ? 0.f : __uint_as_float(raw[VEC == 1 ? 0 : 2 * i + 1]));
+        } else if constexpr (std::is_same<T, __half>::value) {
+            return __half22float2(*reinterpret_cast<const __half2*>(&raw[i]));
+        } else {
+            return make_float2(__uint_as_float(raw[i] << 16), __uint_as_float(raw[i] & 0xffff0000u));
+        }
+    }
+    __device__ __forceinline__ void set(int i, float2 v) {
+        if constexpr (sizeof(T) == 4) {
+            raw[2 * i] = __float_as_uint(v.x);
+            if constexpr (VEC > 1) raw[2 * i + 1] = __float_as_uint(v.y);
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const __half2 h = __float22half2_rn(v);
+            raw[i] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+            const __nv_bfloat162 h = __float22bfloat162_rn(v);
+            raw[i] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+    }
+};
 
 // ---- chunks ------------------------------------------------------------------------------------------------
 struct Graph {
     int64_t begin, end;     // rows, inside the array whatever the offsets hold
     int64_t first;          // its first chunk
+    __device__ __forceinline__ int chunks(int chunk) const { return (int)((end - begin + chunk - 1) / chunk); }
 };
 __device__ __forceinline__ Graph graph_of(const NormArgs& p, int b) {
     if (!p.offsets) return {0, p.rows, 0};
@@ -100,6 +178,7 @@ struct Chunk {
     int graph;
     int64_t row;
     int n;                  // rows, 0: no such chunk
+    bool alone;             // the graph's only one
 };
 // All lanes of a warp: 32 graphs are looked at at a time.
 __device__ __forceinline__ Chunk chunk_of(const NormArgs& p, int64_t number) {
@@ -115,374 +194,507 @@ __device__ __forceinline__ Chunk chunk_of(const NormArgs& p, int64_t number) {
     const Graph g = graph_of(p, lo);
     const int64_t row = g.begin + (number - g.first) * p.chunk;
     const bool real = number >= g.first && row < g.end;
-    return {lo, row, real ? (int)min((int64_t)p.chunk, g.end - row) : 0};
+    return {lo, row, real ? (int)min((int64_t)p.chunk, g.end - row) : 0, g.end - g.begin <= p.chunk};
 }
+
+struct Place {
+    int tx, ty, rows, c;        // threads along the rows; first channel
+    bool live;
+};
+template <int VEC>
+__device__ __forceinline__ Place place_of(const NormArgs& p) {
+    Place at;
+    at.tx = threadIdx.x & (p.tx - 1);
+    at.ty = threadIdx.x / p.tx;
+    at.rows = kNormThreads / p.tx;
+    at.c = (blockIdx.y * p.tx + at.tx) * VEC;
+    at.live = at.c < p.channels;
+    return at;
+}
+
+// What a thread keeps of its channels, in pairs: -mean, rstd gamma, beta.
+template <int VEC>
+struct Channels {
+    static constexpr int kPairs = (VEC + 1) / 2;
+    float2 minus_mean[kPairs], gain[kPairs], bias[kPairs];
+    template <typename Mean, typename Rstd>
+    __device__ __forceinline__ void load(const NormArgs& p, int c, Mean mean, Rstd rstd) {
+        float* to[3] = {&minus_mean[0].x, &gain[0].x, &bias[0].x};
+#pragma unroll
+        for (int i = 0; i < 2 * kPairs; i++) {
+            const bool real = i < VEC;
+            to[0][i] = real ? -mean(c + i) : 0.f;
+            to[1][i] = real ? rstd(c + i) * (p.weight ? p.weight[c + i] : 1.f) : 0.f;
+            to[2][i] = real && p.bias ? p.bias[c + i] : 0.f;
+        }
+    }
+    __device__ __forceinline__ void load(const NormArgs& p, int graph, int c) {
+        const int64_t at = (int64_t)graph * p.groups;
+        load(p, c, [&](int k) { return p.mean[at + k / p.per_group]; }, [&](int k) { return p.rstd[at + k / p.per_group]; });
+    }
+    __device__ __forceinline__ float2 centred(float2 x, int i) const { return add2(x, minus_mean[i]); }
+    __device__ __forceinline__ float2 linear(float2 centred, int i) const { return fma2(centred, gain[i], bias[i]); }
+};
 
 // ---- forward -------------------------------------------------------------------------------------------------
-struct Moments {
-    float n, mean, m2;
-};
-__device__ __forceinline__ void join(Moments& a, const Moments& b) {
-    const float n = a.n + b.n;
-    if (n == 0.f) return;
-    const float share = b.n / n, d = b.mean - a.mean;
-    a.mean += d * share;
-    a.m2 += b.m2 + d * d * a.n * share;
-    a.n = n;
+template <typename T, int VEC, int ACT>
+__device__ __forceinline__ void write_rows(const NormArgs& p, const Chunk& chunk, const Place& at, const Channels<VEC>& ch) {
+    constexpr int kBatch = 4;
+    const T* x = static_cast<const T*>(p.x) + chunk.row * p.x_stride + at.c;
+    T* y = static_cast<T*>(p.y) + chunk.row * p.y_stride + at.c;
+    for (int r = at.ty; r < chunk.n; r += kBatch * at.rows) {
+        Row<T, VEC> v[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; k++)
+            if (r + k * at.rows < chunk.n) v[k].load(x + (int64_t)(r + k * at.rows) * p.x_stride);
+#pragma unroll
+        for (int k = 0; k < kBatch; k++) {
+            if (r + k * at.rows >= chunk.n) break;
+#pragma unroll
+            for (int i = 0; i < Channels<VEC>::kPairs; i++) v[k].set(i, activate2<ACT>(ch.linear(ch.centred(v[k].get(i), i), i)));
+            v[k].store(y + (int64_t)(r + k * at.rows) * p.y_stride);
+        }
+    }
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kNormThreads) group_norm_moments_kernel(const NormArgs p) {
+// Joins `n2` values of mean `mean2` and squares `q2` to a pair of channels' first `n`; share = n2 / (n + n2).
+__device__ __forceinline__ void join2(float2& mean, float2& m2, float n, float2 mean2, float2 q2, float share) {
+    const float2 d = add2(mean2, mul2(mean, both(-1.f)));
+    mean = fma2(d, both(share), mean);
+    m2 = add2(m2, fma2(mul2(d, d), both(n * share), q2));
+}
+
+template <typename T, int VEC, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 4) group_norm_moments_kernel(const NormArgs p) {
+    constexpr int kPairs = Channels<VEC>::kPairs, kBatch = 8;
     wait_for_previous_kernel();
     let_next_kernel_start();
     const Chunk chunk = chunk_of(p, blockIdx.x);
     if (chunk.n == 0) return;
-    const int tx = threadIdx.x & (p.tx - 1), ty = threadIdx.x / p.tx, rows = kNormThreads / p.tx;
-    const int c = (blockIdx.y * p.tx + tx) * VEC;
-    const T* x = static_cast<const T*>(p.x) + chunk.row * p.x_stride + c;
-    float mean[VEC], m2[VEC], n = 0.f;
+    const Place at = place_of<VEC>(p);
+    const T* x = static_cast<const T*>(p.x) + chunk.row * p.x_stride + at.c;
+    float2 mean[kPairs], m2[kPairs];
+    float n = 0.f;
 #pragma unroll
-    for (int i = 0; i < VEC; i++) mean[i] = m2[i] = 0.f;
-    if (c < p.channels) {
-        for (int r = ty; r < chunk.n; r += kNormBatch * rows) {
-            Vec<T, VEC> v[kNormBatch];
-            const int have = min(kNormBatch, (chunk.n - r + rows - 1) / rows);
+    for (int i = 0; i < kPairs; i++) mean[i] = m2[i] = both(0.f);
+    if (at.live) {
+        for (int r = at.ty; r < chunk.n; r += kBatch * at.rows) {
+            Row<T, VEC> v[kBatch];
+            const int have = min(kBatch, (chunk.n - r + at.rows - 1) / at.rows);
 #pragma unroll
-            for (int k = 0; k < kNormBatch; k++)
-                if (k < have) v[k].load(x + (int64_t)(r + k * rows) * p.x_stride);
-            const float inv = 1.f / (float)have, share = (float)have / (n + (float)have);
+            for (int k = 0; k < kBatch; k++)
+                if (k < have) v[k].load(x + (int64_t)(r + k * at.rows) * p.x_stride);
+            const float share = __fdividef((float)have, n + (float)have);
+            if (have == kBatch) {
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                float s = 0.f, q = 0.f;
+                for (int i = 0; i < kPairs; i++) {
+                    float2 s = both(0.f), q = both(0.f);
 #pragma unroll
-                for (int k = 0; k < kNormBatch; k++)
-                    if (k < have) s += v[k].get(i);
-                s *= inv;
+                    for (int k = 0; k < kBatch; k++) s = add2(s, v[k].get(i));
+                    const float2 minus = mul2(s, both(-1.f / kBatch));
 #pragma unroll
-                for (int k = 0; k < kNormBatch; k++)
-                    if (k < have) {
-                        const float d = v[k].get(i) - s;
-                        q += d * d;
+                    for (int k = 0; k < kBatch; k++) {
+                        const float2 d = add2(v[k].get(i), minus);
+                        q = fma2(d, d, q);
                     }
-                const float d = s - mean[i];
-                mean[i] += d * share;
-                m2[i] += q + d * d * n * share;
+                    join2(mean[i], m2[i], n, mul2(s, both(1.f / kBatch)), q, share);
+                }
+            } else {
+                const float inv = 1.f / (float)have;
+#pragma unroll
+                for (int i = 0; i < kPairs; i++) {
+                    float2 s = both(0.f), q = both(0.f);
+#pragma unroll
+                    for (int k = 0; k < kBatch; k++)
+                        if (k < have) s = add2(s, v[k].get(i));
+                    s = mul2(s, both(inv));
+                    const float2 minus = mul2(s, both(-1.f));
+#pragma unroll
+                    for (int k = 0; k < kBatch; k++)
+                        if (k < have) {
+                            const float2 d = add2(v[k].get(i), minus);
+                            q = fma2(d, d, q);
+                        }
+                    join2(mean[i], m2[i], n, s, q, share);
+                }
             }
             n += (float)have;
         }
     }
-    __shared__ float all[2][VEC][kNormThreads];
+    __shared__ float2 all[2][kPairs][kNormThreads];
     __shared__ float counts[kNormThreads];
+    for (int s = at.rows / 2; s > 0; s >>= 1) {
+        if (at.ty >= s && at.ty < 2 * s) {
 #pragma unroll
-    for (int i = 0; i < VEC; i++) {
-        all[0][i][threadIdx.x] = mean[i];
-        all[1][i][threadIdx.x] = m2[i];
-    }
-    counts[threadIdx.x] = n;
-    for (int s = rows / 2; s > 0; s >>= 1) {
-        __syncthreads();
-        if (ty < s) {
-            const int other = threadIdx.x + s * p.tx;
-#pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                Moments a{n, mean[i], m2[i]};
-                join(a, {counts[other], all[0][i][other], all[1][i][other]});
-                all[0][i][threadIdx.x] = mean[i] = a.mean;
-                all[1][i][threadIdx.x] = m2[i] = a.m2;
+            for (int i = 0; i < kPairs; i++) {
+                all[0][i][threadIdx.x] = mean[i];
+                all[1][i][threadIdx.x] = m2[i];
             }
-            counts[threadIdx.x] = n = n + counts[other];
+            counts[threadIdx.x] = n;
+        }
+        __syncthreads();
+        if (at.ty < s) {
+            const int other = threadIdx.x + s * p.tx;
+            const float more = counts[other], share = n + more > 0.f ? more / (n + more) : 0.f;
+#pragma unroll
+            for (int i = 0; i < kPairs; i++) join2(mean[i], m2[i], n, all[0][i][other], all[1][i][other], share);
+            n += more;
         }
     }
-    if (ty == 0 && c < p.channels) {
-        float2* to = p.part + (int64_t)blockIdx.x * p.channels + c;
+    const bool finish = chunk.alone && p.whole;
+    if (at.ty == 0 && at.live && !finish) {
+        float2* to = p.part + (int64_t)blockIdx.x * p.channels + at.c;
 #pragma unroll
-        for (int i = 0; i < VEC; i++) to[i] = make_float2(mean[i], m2[i]);
+        for (int i = 0; i < kPairs; i++) {
+            to[2 * i] = make_float2(mean[i].x, m2[i].x);
+            if (VEC > 1) to[2 * i + 1] = make_float2(mean[i].y, m2[i].y);
+        }
     }
-}
+    if (!finish) return;
 
-__device__ __forceinline__ double block_sum(double v, double* room) {
+    // the whole graph: statistics of the slab's groups, then the rows once more (they are in the L1 or L2)
+    __shared__ float2 channel[32 * kNormVec];
+    if (at.ty == 0) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        for (int i = 0; i < kPairs; i++) {
+            channel[at.tx * VEC + 2 * i] = make_float2(mean[i].x, m2[i].x);
+            if (VEC > 1) channel[at.tx * VEC + 2 * i + 1] = make_float2(mean[i].y, m2[i].y);
+        }
+    }
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) room[threadIdx.x >> 5] = v;
+    const int width = p.tx * VEC, base = blockIdx.y * width, c = base + threadIdx.x;
+    float2 stats = make_float2(0.f, 0.f);
+    if ((int)threadIdx.x < width && c < p.channels) {
+        const int g0 = threadIdx.x / p.per_group * p.per_group;      // groups begin with the slab
+        float sum = 0.f, squares = 0.f;
+        for (int i = 0; i < p.per_group; i++) sum += channel[g0 + i].x;
+        const float m = sum / (float)p.per_group;
+        for (int i = 0; i < p.per_group; i++) {
+            const float d = channel[g0 + i].x - m;
+            squares += channel[g0 + i].y + (float)chunk.n * d * d;
+        }
+        stats = make_float2(m, rsqrtf(squares / ((float)chunk.n * (float)p.per_group) + p.eps));
+        if ((int)threadIdx.x == g0) {
+            const int64_t to = (int64_t)chunk.graph * p.groups + c / p.per_group;
+            p.mean[to] = stats.x;
+            p.rstd[to] = stats.y;
+        }
+    }
     __syncthreads();
-    v = 0.0;
-#pragma unroll
-    for (int w = 0; w < kNormThreads / 32; w++) v += room[w];
-    return v;
+    if ((int)threadIdx.x < width) channel[threadIdx.x] = stats;
+    __syncthreads();
+    if (!at.live) return;
+    Channels<VEC> ch;
+    ch.load(p, at.c, [&](int k) { return channel[k - base].x; }, [&](int k) { return channel[k - base].y; });
+    write_rows<T, VEC, ACT>(p, chunk, at, ch);
 }
 
 // One block per graph and group: mean and rstd from the chunks' channels.
 __global__ void __launch_bounds__(kNormThreads) group_norm_join_kernel(const NormArgs p) {
     wait_for_previous_kernel();
     let_next_kernel_start();
-    __shared__ double room[kNormThreads / 32];
     const int b = blockIdx.x / p.groups, g = blockIdx.x % p.groups;
     const Graph graph = graph_of(p, b);
-    const int64_t n = graph.end - graph.begin, chunks = (n + p.chunk - 1) / p.chunk, values = chunks * p.per_group;
+    const int64_t n = graph.end - graph.begin;
+    const int chunks = graph.chunks(p.chunk), last = (int)(n - (int64_t)(chunks - 1) * p.chunk);
+    if (chunks == 1 && p.whole) return;       // its block has done it
+    // threads along the group's channels, the rest along the chunks; four chunks in flight
+    int across = 1;
+    while (across < p.per_group && across < kNormThreads) across *= 2;
+    const int tx = threadIdx.x & (across - 1), ty = threadIdx.x / across, step = kNormThreads / across;
     const float2* part = p.part + graph.first * p.channels + g * p.per_group;
-    auto count = [&](int64_t j) { return (double)min((int64_t)p.chunk, n - j * p.chunk); };
-    double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < values; i += kNormThreads) {
-        const int64_t j = i / p.per_group;
-        sum += count(j) * part[j * p.channels + (i - j * p.per_group)].x;
+    float count = 0.f, mean = 0.f, m2 = 0.f;
+    auto join = [&](float n2, float mean2, float q2) {
+        if (n2 == 0.f) return;
+        const float share = n2 / (count + n2), d = mean2 - mean;
+        mean += d * share;
+        m2 += q2 + d * d * count * share;
+        count += n2;
+    };
+    for (int c = tx; c < p.per_group; c += across)
+        for (int j = ty; j < chunks; j += 4 * step) {
+            float2 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (j + k * step < chunks) v[k] = part[(int64_t)(j + k * step) * p.channels + c];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (j + k * step < chunks) join((float)(j + k * step == chunks - 1 ? last : p.chunk), v[k].x, v[k].y);
+        }
+    __shared__ float room[3][kNormThreads / 32];
+    auto join_lanes = [&](int from) {
+#pragma unroll
+        for (int o = from; o > 0; o >>= 1) {
+            const float n2 = __shfl_down_sync(0xffffffffu, count, o), mean_b = __shfl_down_sync(0xffffffffu, mean, o), q2 = __shfl_down_sync(0xffffffffu, m2, o);
+            join(n2, mean_b, q2);
+        }
+    };
+    join_lanes(16);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) {
+        room[0][warp] = count;
+        room[1][warp] = mean;
+        room[2][warp] = m2;
     }
-    const double total = (double)n * p.per_group, mean = n ? block_sum(sum, room) / total : 0.0;
-    double m2 = 0.0;
-    for (int64_t i = threadIdx.x; i < values; i += kNormThreads) {
-        const int64_t j = i / p.per_group;
-        const float2 v = part[j * p.channels + (i - j * p.per_group)];
-        const double d = v.x - mean;
-        m2 += v.y + count(j) * d * d;
-    }
-    m2 = block_sum(m2, room);
-    if (threadIdx.x == 0) {
-        p.mean[blockIdx.x] = (float)mean;
-        p.rstd[blockIdx.x] = (float)rsqrt((n ? m2 / total : 0.0) + (double)p.eps);
+    __syncthreads();
+    if (warp == 0) {
+        count = lane < kNormThreads / 32 ? room[0][lane] : 0.f;
+        mean = lane < kNormThreads / 32 ? room[1][lane] : 0.f;
+        m2 = lane < kNormThreads / 32 ? room[2][lane] : 0.f;
+        join_lanes(4);
+        if (lane == 0) {
+            p.mean[blockIdx.x] = mean;
+            p.rstd[blockIdx.x] = rsqrtf((n ? m2 / ((float)n * (float)p.per_group) : 0.f) + p.eps);
+        }
     }
 }
 
-// What a thread keeps of its channels.
-template <int VEC>
-struct Channels {
-    float mean[VEC], rstd[VEC], gain[VEC], bias[VEC];      // gain = rstd gamma
-    __device__ __forceinline__ void load(const NormArgs& p, int graph, int c) {
-#pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            const int64_t at = (int64_t)graph * p.groups + (c + i) / p.per_group;
-            mean[i] = p.mean[at];
-            rstd[i] = p.rstd[at];
-            gain[i] = rstd[i] * (p.weight ? p.weight[c + i] : 1.f);
-            bias[i] = p.bias ? p.bias[c + i] : 0.f;
-        }
-    }
-    __device__ __forceinline__ float centred(float x, int i) const { return x - mean[i]; }
-    __device__ __forceinline__ float linear(float centred, int i) const { return fmaf(centred, gain[i], bias[i]); }
-};
-
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kNormThreads) group_norm_apply_kernel(const NormArgs p) {
+template <typename T, int VEC, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 4) group_norm_apply_kernel(const NormArgs p) {
     wait_for_previous_kernel();
     let_next_kernel_start();
     // the last chunks first: the L2 still has them from the pass before
     const Chunk chunk = chunk_of(p, gridDim.x - 1 - blockIdx.x);
-    const int tx = threadIdx.x & (p.tx - 1), ty = threadIdx.x / p.tx, rows = kNormThreads / p.tx;
-    const int c = (blockIdx.y * p.tx + tx) * VEC;
-    if (chunk.n == 0 || c >= p.channels) return;
+    const Place at = place_of<VEC>(p);
+    if (chunk.n == 0 || (chunk.alone && p.whole) || !at.live) return;
     Channels<VEC> ch;
-    ch.load(p, chunk.graph, c);
-    const T* x = static_cast<const T*>(p.x) + chunk.row * p.x_stride + c;
-    T* y = static_cast<T*>(p.y) + chunk.row * p.y_stride + c;
-    constexpr int kBatch = kNormBatch / 2;
-    for (int r = ty; r < chunk.n; r += kBatch * rows) {
-        Vec<T, VEC> v[kBatch];
+    ch.load(p, chunk.graph, at.c);
+    write_rows<T, VEC, ACT>(p, chunk, at, ch);
+}
+
+// ---- backward ------------------------------------------------------------------------------------------------
+// Sums over a group's channels, of a graph's sums per channel: means of du gamma (times -rstd) and of du gamma xhat (times
+// -rstd^2), by all lanes of a warp.
+__device__ __forceinline__ float2 group_means(const NormArgs& p, const float2* sums, int g, int64_t graph, int64_t rows) {
+    float a = 0.f, b = 0.f;
+    for (int i = threadIdx.x & 31; i < p.per_group; i += 32) {
+        const int c = g * p.per_group + i;
+        const float2 s = sums[c];
+        const float w = p.weight ? p.weight[c] : 1.f;
+        a += w * s.x;
+        b += w * s.y;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
+    const float r = p.rstd[graph * p.groups + g], inv = -r / ((float)rows * (float)p.per_group);
+    return make_float2(a * inv, b * inv * r);
+}
+
+template <typename T, int VEC, int ACT>
+__device__ __forceinline__ void write_grads(const NormArgs& p, const Chunk& chunk, const Place& at, const Channels<VEC>& ch, const float2* means, int first) {
+    constexpr int kPairs = Channels<VEC>::kPairs, kBatch = 4;
+    float2 m1[kPairs], m2[kPairs];
+#pragma unroll
+    for (int i = 0; i < kPairs; i++) {
+        const float2 a = means[(at.c + 2 * i) / p.per_group - first], b = VEC > 1 ? means[(at.c + 2 * i + 1) / p.per_group - first] : a;
+        m1[i] = make_float2(a.x, b.x);
+        m2[i] = make_float2(a.y, b.y);
+    }
+    const T* x = static_cast<const T*>(p.x) + chunk.row * p.x_stride + at.c;
+    const T* dy = static_cast<const T*>(p.grad) + chunk.row * p.grad_stride + at.c;
+    T* dx = static_cast<T*>(p.y) + chunk.row * p.y_stride + at.c;
+    for (int r = at.ty; r < chunk.n; r += kBatch * at.rows) {
+        Row<T, VEC> v[kBatch], w[kBatch];
 #pragma unroll
         for (int k = 0; k < kBatch; k++)
-            if (r + k * rows < chunk.n) v[k].load(x + (int64_t)(r + k * rows) * p.x_stride);
+            if (r + k * at.rows < chunk.n) {
+                v[k].load(x + (int64_t)(r + k * at.rows) * p.x_stride);
+                w[k].load(dy + (int64_t)(r + k * at.rows) * p.grad_stride);
+            }
 #pragma unroll
         for (int k = 0; k < kBatch; k++) {
-            if (r + k * rows >= chunk.n) break;
+            if (r + k * at.rows >= chunk.n) break;
 #pragma unroll
-            for (int i = 0; i < VEC; i++) v[k].set(i, activate(ch.linear(ch.centred(v[k].get(i), i), i), p.activation));
-            v[k].store(y + (int64_t)(r + k * rows) * p.y_stride);
+            for (int i = 0; i < kPairs; i++) {
+                const float2 d = ch.centred(v[k].get(i), i), du = through_activation2<ACT>(w[k].get(i), ch.linear(d, i));
+                v[k].set(i, fma2(du, ch.gain[i], fma2(d, m2[i], m1[i])));
+            }
+            v[k].store(dx + (int64_t)(r + k * at.rows) * p.y_stride);
         }
     }
 }
 
-// ---- backward ------------------------------------------------------------------------------------------------
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kNormThreads) group_norm_grad_sums_kernel(const NormArgs p) {
+template <typename T, int VEC, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 4) group_norm_grad_sums_kernel(const NormArgs p) {
+    constexpr int kPairs = Channels<VEC>::kPairs, kBatch = 4;
     wait_for_previous_kernel();
     let_next_kernel_start();
     const Chunk chunk = chunk_of(p, blockIdx.x);
     if (chunk.n == 0) return;
-    const int tx = threadIdx.x & (p.tx - 1), ty = threadIdx.x / p.tx, rows = kNormThreads / p.tx;
-    const int c = (blockIdx.y * p.tx + tx) * VEC;
-    float s1[VEC], s2[VEC];
+    const Place at = place_of<VEC>(p);
+    float2 s1[kPairs], s2[kPairs];
 #pragma unroll
-    for (int i = 0; i < VEC; i++) s1[i] = s2[i] = 0.f;
-    if (c < p.channels) {
-        Channels<VEC> ch;
-        ch.load(p, chunk.graph, c);
-        const T* x = static_cast<const T*>(p.x) + chunk.row * p.x_stride + c;
-        const T* dy = static_cast<const T*>(p.grad) + chunk.row * p.grad_stride + c;
-        constexpr int kBatch = kNormBatch / 2;
-        for (int r = ty; r < chunk.n; r += kBatch * rows) {
-            Vec<T, VEC> v[kBatch], w[kBatch];
+    for (int i = 0; i < kPairs; i++) s1[i] = s2[i] = both(0.f);
+    Channels<VEC> ch;
+    if (at.live) {
+        ch.load(p, chunk.graph, at.c);
+        const T* x = static_cast<const T*>(p.x) + chunk.row * p.x_stride + at.c;
+        const T* dy = static_cast<const T*>(p.grad) + chunk.row * p.grad_stride + at.c;
+        for (int r = at.ty; r < chunk.n; r += kBatch * at.rows) {
+            Row<T, VEC> v[kBatch], w[kBatch];
 #pragma unroll
             for (int k = 0; k < kBatch; k++)
-                if (r + k * rows < chunk.n) {
-                    v[k].load(x + (int64_t)(r + k * rows) * p.x_stride);
-                    w[k].load(dy + (int64_t)(r + k * rows) * p.grad_stride);
+                if (r + k * at.rows < chunk.n) {
+                    v[k].load(x + (int64_t)(r + k * at.rows) * p.x_stride);
+                    w[k].load(dy + (int64_t)(r + k * at.rows) * p.grad_stride);
                 }
 #pragma unroll
             for (int k = 0; k < kBatch; k++) {
-                if (r + k * rows >= chunk.n) break;
+                if (r + k * at.rows >= chunk.n) break;
 #pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    const float d = ch.centred(v[k].get(i), i), du = w[k].get(i) * activate_slope(ch.linear(d, i), p.activation);
-                    s1[i] += du;
-                    s2[i] += du * (d * ch.rstd[i]);
+                for (int i = 0; i < kPairs; i++) {
+                    const float2 d = ch.centred(v[k].get(i), i), du = through_activation2<ACT>(w[k].get(i), ch.linear(d, i));
+                    s1[i] = add2(s1[i], du);
+                    s2[i] = fma2(du, d, s2[i]);
                 }
             }
         }
     }
-    __shared__ float all[2][VEC][kNormThreads];
-    for (int s = rows / 2; s > 0; s >>= 1) {
-        if (ty >= s && ty < 2 * s) {
+    __shared__ float2 all[2][kPairs][kNormThreads];
+    for (int s = at.rows / 2; s > 0; s >>= 1) {
+        if (at.ty >= s && at.ty < 2 * s) {
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
+            for (int i = 0; i < kPairs; i++) {
                 all[0][i][threadIdx.x] = s1[i];
                 all[1][i][threadIdx.x] = s2[i];
             }
         }
         __syncthreads();
-        if (ty < s) {
+        if (at.ty < s) {
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                s1[i] += all[0][i][threadIdx.x + s * p.tx];
-                s2[i] += all[1][i][threadIdx.x + s * p.tx];
+            for (int i = 0; i < kPairs; i++) {
+                s1[i] = add2(s1[i], all[0][i][threadIdx.x + s * p.tx]);
+                s2[i] = add2(s2[i], all[1][i][threadIdx.x + s * p.tx]);
             }
         }
     }
-    if (ty == 0 && c < p.channels) {
-        float2* to = p.part + (int64_t)blockIdx.x * p.channels + c;
+    float2* part = p.part + (int64_t)blockIdx.x * p.channels;
+    if (at.ty == 0 && at.live) {
+        const float* rstd = p.rstd + (int64_t)chunk.graph * p.groups;
 #pragma unroll
-        for (int i = 0; i < VEC; i++) to[i] = make_float2(s1[i], s2[i]);
+        for (int i = 0; i < kPairs; i++) {
+            const int c = at.c + 2 * i;
+            part[c] = make_float2(s1[i].x, s2[i].x * rstd[c / p.per_group]);
+            if (VEC > 1) part[c + 1] = make_float2(s1[i].y, s2[i].y * rstd[(c + 1) / p.per_group]);
+        }
     }
+    if (!chunk.alone || !p.whole || !p.y) return;
+    // the whole graph: its groups' means, then the rows once more
+    __shared__ float2 means[32 * kNormVec];
+    __syncthreads();
+    const int width = p.tx * VEC, first = (int)(blockIdx.y * width) / p.per_group, end = min((int)(blockIdx.y + 1) * width, p.channels);
+    for (int g = first + (threadIdx.x >> 5); g * p.per_group < end; g += kNormThreads / 32) {
+        const float2 m = group_means(p, part, g, chunk.graph, chunk.n);
+        if ((threadIdx.x & 31) == 0) means[g - first] = m;
+    }
+    __syncthreads();
+    if (at.live) write_grads<T, VEC, ACT>(p, chunk, at, ch, means, first);
 }
 
-// sums[graph][channel] over the graph's chunks: a block per graph and 32 channels, 8 threads a channel.
-__device__ __forceinline__ float2 sum_rows(const float2* from, int64_t n, int64_t stride, bool live, float2 (*room)[32]) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+// The sums of a graph: in its only chunk's place, or joined.
+__device__ __forceinline__ const float2* sums_of(const NormArgs& p, const Graph& g, int b) {
+    return g.end - g.begin <= p.chunk ? p.part + g.first * p.channels : p.sums + (int64_t)b * p.channels;
+}
+
+// Sums of 8 channels by a block, 32 threads a channel, four values in flight each; every thread gets its channel's.
+template <typename Value>
+__device__ __forceinline__ float2 sum_of_channel(int n, Value value, float2 (*room)[8]) {
+    const int c = threadIdx.x & 7, w = threadIdx.x >> 3;
     double a = 0.0, b = 0.0;
-    if (live)
-        for (int64_t j = w; j < n; j += kNormThreads / 32) {
-            const float2 v = from[j * stride];
-            a += v.x;
-            b += v.y;
+    for (int j = w; j < n; j += 4 * 32) {
+        float2 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = j + 32 * k < n ? value(j + 32 * k) : make_float2(0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            a += v[k].x;
+            b += v[k].y;
         }
+    }
     __syncthreads();
-    room[w][lane] = make_float2((float)a, (float)b);
+    room[w][c] = make_float2((float)a, (float)b);
     __syncthreads();
     float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < kNormThreads / 32; i++) {
-        s.x += room[i][lane].x;
-        s.y += room[i][lane].y;
-    }
+    for (int i = 0; i < 32; i++) s = add2(s, room[i][c]);
     return s;
 }
 __global__ void __launch_bounds__(kNormThreads) group_norm_grad_join_kernel(const NormArgs p) {
     wait_for_previous_kernel();
     let_next_kernel_start();
-    __shared__ float2 room[kNormThreads / 32][32];
-    const int c = blockIdx.y * 32 + (threadIdx.x & 31);
-    const Graph graph = graph_of(p, blockIdx.x);
-    const int64_t chunks = (graph.end - graph.begin + p.chunk - 1) / p.chunk;
-    const float2 s = sum_rows(p.part + graph.first * p.channels + c, chunks, p.channels, c < p.channels, room);
-    if (threadIdx.x < 32 && c < p.channels) p.sums[(int64_t)blockIdx.x * p.channels + c] = s;
+    __shared__ float2 room[32][8];
+    const int c = blockIdx.x * 8 + (threadIdx.x & 7);
+    for (int b = blockIdx.y; b < p.graphs; b += gridDim.y) {
+        const Graph graph = graph_of(p, b);
+        const int chunks = graph.chunks(p.chunk);
+        if (chunks < 2) continue;
+        const float2* part = p.part + graph.first * p.channels + c;
+        const float2 s = sum_of_channel(chunks, [&](int j) { return c < p.channels ? part[(int64_t)j * p.channels] : make_float2(0.f, 0.f); }, room);
+        if (threadIdx.x < 8 && c < p.channels) p.sums[(int64_t)b * p.channels + c] = s;
+    }
 }
 
 // Writes dx; the last blocks along x sum the graphs' channels up to dgamma and dbeta.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kNormThreads) group_norm_grad_apply_kernel(const NormArgs p, int64_t chunks) {
+template <typename T, int VEC, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 4) group_norm_grad_apply_kernel(const NormArgs p, int64_t chunks) {
     wait_for_previous_kernel();
     let_next_kernel_start();
-    __shared__ float2 room[kNormThreads / 32][32];
     if (blockIdx.x >= chunks) {
-        const int64_t block = (blockIdx.x - chunks) * gridDim.y + blockIdx.y;
-        const int64_t c = block * 32 + (threadIdx.x & 31);
-        if (block * 32 >= p.channels) return;
-        const float2 s = sum_rows(p.sums + c, p.graphs, p.channels, c < p.channels, room);
-        if (threadIdx.x < 32 && c < p.channels) {
+        __shared__ float2 room[32][8];
+        const int64_t c0 = ((blockIdx.x - chunks) * gridDim.y + blockIdx.y) * 8, c = c0 + (threadIdx.x & 7);
+        if (c0 >= p.channels) return;
+        const float2 s = sum_of_channel(p.graphs, [&](int b) {
+            const Graph g = graph_of(p, b);
+            return c < p.channels && g.end > g.begin ? sums_of(p, g, b)[c] : make_float2(0.f, 0.f);
+        }, room);
+        if (threadIdx.x < 8 && c < p.channels) {
             if (p.dbias) p.dbias[c] = s.x;
             if (p.dweight) p.dweight[c] = s.y;
         }
         return;
     }
-    if (!p.y) return;
     const Chunk chunk = chunk_of(p, chunks - 1 - blockIdx.x);
-    if (chunk.n == 0) return;
-    // the block's groups' means of du gamma and du gamma xhat
-    __shared__ float2 means[32 * 8];
-    const int width = p.tx * VEC, first = (int)(blockIdx.y * width) / p.per_group;
-    const int last = min((int)(blockIdx.y * width) + width, p.channels) - 1;
+    if (chunk.n == 0 || !p.y || (chunk.alone && p.whole)) return;
+    __shared__ float2 means[32 * kNormVec];
+    const int width = p.tx * VEC, first = (int)(blockIdx.y * width) / p.per_group, end = min((int)(blockIdx.y + 1) * width, p.channels);
     const Graph graph = graph_of(p, chunk.graph);
-    const float inv = 1.f / ((float)(graph.end - graph.begin) * (float)p.per_group);
-    for (int g = first + (threadIdx.x >> 5); g <= last / p.per_group; g += kNormThreads / 32) {
-        float a = 0.f, b = 0.f;
-        for (int i = threadIdx.x & 31; i < p.per_group; i += 32) {
-            const int c = g * p.per_group + i;
-            const float2 s = p.sums[(int64_t)chunk.graph * p.channels + c];
-            const float w = p.weight ? p.weight[c] : 1.f;
-            a += w * s.x;
-            b += w * s.y;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            a += __shfl_xor_sync(0xffffffffu, a, o);
-            b += __shfl_xor_sync(0xffffffffu, b, o);
-        }
-        if ((threadIdx.x & 31) == 0) means[g - first] = make_float2(a * inv, b * inv);
+    const float2* sums = sums_of(p, graph, chunk.graph);
+    for (int g = first + (threadIdx.x >> 5); g * p.per_group < end; g += kNormThreads / 32) {
+        const float2 m = group_means(p, sums, g, chunk.graph, graph.end - graph.begin);
+        if ((threadIdx.x & 31) == 0) means[g - first] = m;
     }
     __syncthreads();
-    const int tx = threadIdx.x & (p.tx - 1), ty = threadIdx.x / p.tx, rows = kNormThreads / p.tx;
-    const int c = (blockIdx.y * p.tx + tx) * VEC;
-    if (c >= p.channels) return;
+    const Place at = place_of<VEC>(p);
+    if (!at.live) return;
     Channels<VEC> ch;
-    ch.load(p, chunk.graph, c);
-    float m1[VEC], m2[VEC];      // times rstd
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
-        const float2 m = means[(c + i) / p.per_group - first];
-        m1[i] = m.x * ch.rstd[i];
-        m2[i] = m.y * ch.rstd[i] * ch.rstd[i];
-    }
-    const T* x = static_cast<const T*>(p.x) + chunk.row * p.x_stride + c;
-    const T* dy = static_cast<const T*>(p.grad) + chunk.row * p.grad_stride + c;
-    T* dx = static_cast<T*>(p.y) + chunk.row * p.y_stride + c;
-    constexpr int kBatch = kNormBatch / 2;
-    for (int r = ty; r < chunk.n; r += kBatch * rows) {
-        Vec<T, VEC> v[kBatch], w[kBatch];
-#pragma unroll
-        for (int k = 0; k < kBatch; k++)
-            if (r + k * rows < chunk.n) {
-                v[k].load(x + (int64_t)(r + k * rows) * p.x_stride);
-                w[k].load(dy + (int64_t)(r + k * rows) * p.grad_stride);
-            }
-#pragma unroll
-        for (int k = 0; k < kBatch; k++) {
-            if (r + k * rows >= chunk.n) break;
-#pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                const float d = ch.centred(v[k].get(i), i), du = w[k].get(i) * activate_slope(ch.linear(d, i), p.activation);
-                v[k].set(i, fmaf(du, ch.gain[i], -fmaf(d, m2[i], m1[i])));
-            }
-            v[k].store(dx + (int64_t)(r + k * rows) * p.y_stride);
-        }
-    }
+    ch.load(p, chunk.graph, at.c);
+    write_grads<T, VEC, ACT>(p, chunk, at, ch, means, first);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------
 struct NormPlan {
     int vec, tx, slabs, chunk;
+    bool whole;
     int64_t chunks;
     size_t part, sums, bytes;
 };
 
 static NormPlan plan_norm(const mask_norm& n, bool backward) {
     NormPlan p = {};
-    const int element = n.dtype == MASK_F32 ? 4 : 2, wide = 16 / element;
-    auto fits = [&](const void* data, int64_t stride) { return stride % wide == 0 && (reinterpret_cast<uintptr_t>(data) & 15) == 0; };
-    const bool vec = n.channels % wide == 0 && fits(n.d_x, n.x_stride) && (!n.d_y || fits(n.d_y, n.y_stride)) && (!backward || fits(n.d_grad, n.grad_stride));
-    p.vec = vec ? wide : 1;
+    const int bytes = (n.dtype == MASK_F32 ? 4 : 2) * kNormVec;
+    auto fits = [&](const void* data, int64_t stride) { return stride % kNormVec == 0 && reinterpret_cast<uintptr_t>(data) % bytes == 0; };
+    const bool vec = n.channels % kNormVec == 0 && fits(n.d_x, n.x_stride) && (!n.d_y || fits(n.d_y, n.y_stride)) && (!backward || fits(n.d_grad, n.grad_stride));
+    p.vec = vec ? kNormVec : 1;
     const int vectors = n.channels / p.vec;
     p.tx = 1;
     while (p.tx < 32 && p.tx < vectors) p.tx *= 2;
     p.slabs = (vectors + p.tx - 1) / p.tx;
-    // six blocks an SM, chunks of 8 rows a thread to 1024 rows
-    const int64_t want = 6 * (int64_t)sm_count(), least = std::max<int64_t>(16, std::min<int64_t>(8 * (kNormThreads / p.tx), 256));
+    p.whole = p.slabs == 1 || p.tx * p.vec % (n.channels / n.groups) == 0;
+    // six blocks an SM, chunks of 16 rows a thread to 1024 rows
+    const int64_t want = 6 * (int64_t)sm_count(), least = std::min<int64_t>(16 * (kNormThreads / p.tx), 256);
     p.chunk = (int)std::min<int64_t>(std::max<int64_t>(n.rows * p.slabs / want, least), 1024);
     p.chunks = n.rows / p.chunk + n.graphs;
     auto take = [&](size_t bytes) {
@@ -521,25 +733,36 @@ static const char* refuse_norm(const mask_norm* n, bool backward) {
     return nullptr;
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, int ACT>
 static int launch_norm(const NormArgs& a, const NormPlan& p, bool backward, cudaStream_t st) {
     const dim3 grid((unsigned)p.chunks, (unsigned)p.slabs);
+    const bool one_chunk = p.whole && a.graphs == 1 && a.rows > 0 && a.rows <= p.chunk && !a.offsets;    // its block does everything
     int rc;
     if (!backward) {
-        if ((rc = launch_overlapped(group_norm_moments_kernel<T, VEC>, grid, kNormThreads, 0, st, a))) return rc;
+        if ((rc = launch_overlapped(group_norm_moments_kernel<T, VEC, ACT>, grid, kNormThreads, 0, st, a)) || one_chunk) return rc;
         if ((rc = launch_overlapped(group_norm_join_kernel, dim3((unsigned)(a.graphs * a.groups)), kNormThreads, 0, st, a))) return rc;
-        return launch_overlapped(group_norm_apply_kernel<T, VEC>, grid, kNormThreads, 0, st, a);
+        return launch_overlapped(group_norm_apply_kernel<T, VEC, ACT>, grid, kNormThreads, 0, st, a);
     }
-    const int32_t parts = (a.channels + 31) / 32;
-    if ((rc = launch_overlapped(group_norm_grad_sums_kernel<T, VEC>, grid, kNormThreads, 0, st, a))) return rc;
-    if ((rc = launch_overlapped(group_norm_grad_join_kernel, dim3((unsigned)a.graphs, (unsigned)parts), kNormThreads, 0, st, a))) return rc;
+    const int32_t parts = (a.channels + 7) / 8;
+    if ((rc = launch_overlapped(group_norm_grad_sums_kernel<T, VEC, ACT>, grid, kNormThreads, 0, st, a))) return rc;
+    if (a.rows > p.chunk) {       // else no graph has two chunks
+        if ((rc = launch_overlapped(group_norm_grad_join_kernel, dim3((unsigned)parts, (unsigned)std::min(a.graphs, 256)), kNormThreads, 0, st, a)))
+            return rc;
+    }
     const unsigned more = a.dweight || a.dbias ? (unsigned)((parts + p.slabs - 1) / p.slabs) : 0;
-    return launch_overlapped(group_norm_grad_apply_kernel<T, VEC>, dim3(grid.x + more, grid.y), kNormThreads, 0, st, a, p.chunks);
+    return launch_overlapped(group_norm_grad_apply_kernel<T, VEC, ACT>, dim3(grid.x + more, grid.y), kNormThreads, 0, st, a, p.chunks);
 }
 
-template <typename T, int WIDE>
-static int launch_norm_as(const NormArgs& a, const NormPlan& p, bool backward, cudaStream_t st) {
-    return p.vec == 1 ? launch_norm<T, 1>(a, p, backward, st) : launch_norm<T, WIDE>(a, p, backward, st);
+template <typename T, int VEC>
+static int launch_norm_act(const NormArgs& a, const NormPlan& p, int activation, bool backward, cudaStream_t st) {
+    if (activation == MASK_ACT_RELU) return launch_norm<T, VEC, MASK_ACT_RELU>(a, p, backward, st);
+    if (activation == MASK_ACT_SILU) return launch_norm<T, VEC, MASK_ACT_SILU>(a, p, backward, st);
+    return launch_norm<T, VEC, MASK_ACT_NONE>(a, p, backward, st);
+}
+
+template <typename T>
+static int launch_norm_as(const NormArgs& a, const NormPlan& p, int activation, bool backward, cudaStream_t st) {
+    return p.vec == 1 ? launch_norm_act<T, 1>(a, p, activation, backward, st) : launch_norm_act<T, kNormVec>(a, p, activation, backward, st);
 }
 
 static int run_norm(const mask_norm* n, bool backward, void* d_scratch, size_t scratch_bytes, cudaStream_t st) {
@@ -549,15 +772,15 @@ static int run_norm(const mask_norm* n, bool backward, void* d_scratch, size_t s
     if (scratch_bytes < p.bytes) return fail(MASK_ERR_SCRATCH_TOO_SMALL, "scratch is smaller than mask_group_norm_scratch_bytes");
     NormArgs a = {};
     a.rows = n->rows; a.channels = n->channels; a.groups = n->groups; a.per_group = n->channels / n->groups; a.graphs = n->graphs;
-    a.activation = n->activation; a.eps = n->eps; a.chunk = p.chunk; a.tx = p.tx;
+    a.eps = n->eps; a.chunk = p.chunk; a.tx = p.tx; a.whole = p.whole;
     a.offsets = n->d_offsets; a.x = n->d_x; a.x_stride = n->x_stride; a.weight = n->d_weight; a.bias = n->d_bias;
     a.y = n->d_y; a.y_stride = n->y_stride; a.mean = n->d_mean; a.rstd = n->d_rstd;
     a.grad = n->d_grad; a.grad_stride = n->grad_stride; a.dweight = n->d_dweight; a.dbias = n->d_dbias;
     a.part = reinterpret_cast<float2*>(static_cast<char*>(d_scratch) + p.part);
     a.sums = reinterpret_cast<float2*>(static_cast<char*>(d_scratch) + p.sums);
-    if (n->dtype == MASK_F32) return launch_norm_as<float, 4>(a, p, backward, st);
-    if (n->dtype == MASK_BF16) return launch_norm_as<__nv_bfloat16, 8>(a, p, backward, st);
-    return launch_norm_as<__half, 8>(a, p, backward, st);
+    if (n->dtype == MASK_F32) return launch_norm_as<float>(a, p, n->activation, backward, st);
+    if (n->dtype == MASK_BF16) return launch_norm_as<__nv_bfloat16>(a, p, n->activation, backward, st);
+    return launch_norm_as<__half>(a, p, n->activation, backward, st);
 }
 
 }  // namespace mask
