@@ -35,6 +35,7 @@ struct NormArgs {
     int32_t channels, groups, per_group, graphs;
     float eps;
     int32_t chunk;              // rows
+    uint64_t chunk_inverse;     // 2^64 / chunk, rounded up: the high half of a product with it is a quotient (rows < 2^31)
     int32_t tx;                 // threads along the channels (a power of two), 256 / tx along the rows
     int32_t whole;              // slabs hold whole groups
     const int32_t* offsets;     // or NULL: one graph
@@ -117,15 +118,19 @@ __device__ __forceinline__ float2 through_activation2(float2 dy, float2 u) {
 template <typename T, int VEC>
 struct Row {
     uint32_t raw[VEC == 1 ? 1 : (sizeof(T) == 4 ? 4 : 2)];
+    // kLast: nobody reads it again, so that the cache may give its room to others first
+    template <bool kLast = false>
     __device__ __forceinline__ void load(const T* from) {
         if constexpr (VEC == 1) {
             if constexpr (sizeof(T) == 4) raw[0] = *reinterpret_cast<const uint32_t*>(from);
             else raw[0] = *reinterpret_cast<const uint16_t*>(from);
         } else if constexpr (sizeof(T) == 4) {
-            const uint4 v = *reinterpret_cast<const uint4*>(from);
+            const uint4* at = reinterpret_cast<const uint4*>(from);
+            const uint4 v = kLast ? __ldcs(at) : *at;
             raw[0] = v.x; raw[1] = v.y; raw[2] = v.z; raw[3] = v.w;
         } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(from);
+            const uint2* at = reinterpret_cast<const uint2*>(from);
+            const uint2 v = kLast ? __ldcs(at) : *at;
             raw[0] = v.x; raw[1] = v.y;
         }
     }
@@ -134,9 +139,9 @@ struct Row {
             if constexpr (sizeof(T) == 4) *reinterpret_cast<uint32_t*>(to) = raw[0];
             else *reinterpret_cast<uint16_t*>(to) = (uint16_t)raw[0];
         } else if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<uint4*>(to) = make_uint4(raw[0], raw[1], raw[2], raw[3]);
+            __stcs(reinterpret_cast<uint4*>(to), make_uint4(raw[0], raw[1], raw[2], raw[3]));
         } else {
-            *reinterpret_cast<uint2*>(to) = make_uint2(raw[0], raw[1]);
+            __stcs(reinterpret_cast<uint2*>(to), make_uint2(raw[0], raw[1]));
         }
     }
     // channels 2i and 2i + 1; VEC == 1: the second is 0
@@ -167,13 +172,13 @@ struct Row {
 struct Graph {
     int64_t begin, end;     // rows, inside the array whatever the offsets hold
     int64_t first;          // its first chunk
-    __device__ __forceinline__ int chunks(int chunk) const { return (int)((end - begin + chunk - 1) / chunk); }
 };
 __device__ __forceinline__ Graph graph_of(const NormArgs& p, int b) {
     if (!p.offsets) return {0, p.rows, 0};
     const int64_t begin = min(max((int64_t)p.offsets[b], (int64_t)0), p.rows), end = min(max((int64_t)p.offsets[b + 1], begin), p.rows);
-    return {begin, end, begin / p.chunk + b};
+    return {begin, end, (int64_t)__umul64hi((uint64_t)begin, p.chunk_inverse) + b};
 }
+__device__ __forceinline__ int chunks_of(const NormArgs& p, const Graph& g) { return (int)__umul64hi((uint64_t)(g.end - g.begin + p.chunk - 1), p.chunk_inverse); }
 struct Chunk {
     int graph;
     int64_t row;
@@ -246,7 +251,7 @@ __device__ __forceinline__ void write_rows(const NormArgs& p, const Chunk& chunk
         Row<T, VEC> v[kBatch];
 #pragma unroll
         for (int k = 0; k < kBatch; k++)
-            if (r + k * at.rows < chunk.n) v[k].load(x + (int64_t)(r + k * at.rows) * p.x_stride);
+            if (r + k * at.rows < chunk.n) v[k].template load<true>(x + (int64_t)(r + k * at.rows) * p.x_stride);
 #pragma unroll
         for (int k = 0; k < kBatch; k++) {
             if (r + k * at.rows >= chunk.n) break;
@@ -396,7 +401,7 @@ __global__ void __launch_bounds__(kNormThreads) group_norm_join_kernel(const Nor
     const int b = blockIdx.x / p.groups, g = blockIdx.x % p.groups;
     const Graph graph = graph_of(p, b);
     const int64_t n = graph.end - graph.begin;
-    const int chunks = graph.chunks(p.chunk), last = (int)(n - (int64_t)(chunks - 1) * p.chunk);
+    const int chunks = chunks_of(p, graph), last = (int)(n - (int64_t)(chunks - 1) * p.chunk);
     if (chunks == 1 && p.whole) return;       // its block has done it
     // threads along the group's channels, the rest along the chunks; four chunks in flight
     int across = 1;
@@ -453,8 +458,7 @@ template <typename T, int VEC, int ACT>
 __global__ void __launch_bounds__(kNormThreads, 4) group_norm_apply_kernel(const NormArgs p) {
     wait_for_previous_kernel();
     let_next_kernel_start();
-    // the last chunks first: the L2 still has them from the pass before
-    const Chunk chunk = chunk_of(p, gridDim.x - 1 - blockIdx.x);
+    const Chunk chunk = chunk_of(p, blockIdx.x);
     const Place at = place_of<VEC>(p);
     if (chunk.n == 0 || (chunk.alone && p.whole) || !at.live) return;
     Channels<VEC> ch;
@@ -501,8 +505,8 @@ __device__ __forceinline__ void write_grads(const NormArgs& p, const Chunk& chun
 #pragma unroll
         for (int k = 0; k < kBatch; k++)
             if (r + k * at.rows < chunk.n) {
-                v[k].load(x + (int64_t)(r + k * at.rows) * p.x_stride);
-                w[k].load(dy + (int64_t)(r + k * at.rows) * p.grad_stride);
+                v[k].template load<true>(x + (int64_t)(r + k * at.rows) * p.x_stride);
+                w[k].template load<true>(dy + (int64_t)(r + k * at.rows) * p.grad_stride);
             }
 #pragma unroll
         for (int k = 0; k < kBatch; k++) {
@@ -629,7 +633,7 @@ __global__ void __launch_bounds__(kNormThreads) group_norm_grad_join_kernel(cons
     const int c = blockIdx.x * 8 + (threadIdx.x & 7);
     for (int b = blockIdx.y; b < p.graphs; b += gridDim.y) {
         const Graph graph = graph_of(p, b);
-        const int chunks = graph.chunks(p.chunk);
+        const int chunks = chunks_of(p, graph);
         if (chunks < 2) continue;
         const float2* part = p.part + graph.first * p.channels + c;
         const float2 s = sum_of_channel(chunks, [&](int j) { return c < p.channels ? part[(int64_t)j * p.channels] : make_float2(0.f, 0.f); }, room);
@@ -656,7 +660,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) group_norm_grad_apply_kernel(
         }
         return;
     }
-    const Chunk chunk = chunk_of(p, chunks - 1 - blockIdx.x);
+    const Chunk chunk = chunk_of(p, blockIdx.x);
     if (chunk.n == 0 || !p.y || (chunk.alone && p.whole)) return;
     __shared__ float2 means[32 * kNormVec];
     const int width = p.tx * VEC, first = (int)(blockIdx.y * width) / p.per_group, end = min((int)(blockIdx.y + 1) * width, p.channels);
@@ -689,13 +693,16 @@ static NormPlan plan_norm(const mask_norm& n, bool backward) {
     const bool vec = n.channels % kNormVec == 0 && fits(n.d_x, n.x_stride) && (!n.d_y || fits(n.d_y, n.y_stride)) && (!backward || fits(n.d_grad, n.grad_stride));
     p.vec = vec ? kNormVec : 1;
     const int vectors = n.channels / p.vec;
+    // threads along the channels: a whole row where it has up to 32 vectors, else 32 or the 16 that leave fewer idle
     p.tx = 1;
     while (p.tx < 32 && p.tx < vectors) p.tx *= 2;
+    if (vectors > 32 && (vectors + 15) / 16 * 16 < (vectors + 31) / 32 * 32) p.tx = 16;
     p.slabs = (vectors + p.tx - 1) / p.tx;
     p.whole = p.slabs == 1 || p.tx * p.vec % (n.channels / n.groups) == 0;
-    // six blocks an SM, chunks of 16 rows a thread to 1024 rows
-    const int64_t want = 6 * (int64_t)sm_count(), least = std::min<int64_t>(16 * (kNormThreads / p.tx), 256);
-    p.chunk = (int)std::min<int64_t>(std::max<int64_t>(n.rows * p.slabs / want, least), 1024);
+    // Four blocks an SM are resident: as many chunks as that, in whole batches of rows.  (300007 x 256 bf16 backward: 159 us;
+    // twice as many 164, four times 199, since every chunk leaves sums to join and blocks have a start and an end.)
+    const int64_t want = 4 * (int64_t)sm_count(), batch = 8 * (kNormThreads / p.tx), most = 4096 / batch * batch;
+    p.chunk = (int)std::min<int64_t>(std::max<int64_t>((n.rows * p.slabs + want * batch - 1) / (want * batch) * batch, std::min<int64_t>(batch, 256)), std::max<int64_t>(most, batch));
     p.chunks = n.rows / p.chunk + n.graphs;
     auto take = [&](size_t bytes) {
         const size_t at = p.bytes;
@@ -746,7 +753,7 @@ static int launch_norm(const NormArgs& a, const NormPlan& p, bool backward, cuda
     const int32_t parts = (a.channels + 7) / 8;
     if ((rc = launch_overlapped(group_norm_grad_sums_kernel<T, VEC, ACT>, grid, kNormThreads, 0, st, a))) return rc;
     if (a.rows > p.chunk) {       // else no graph has two chunks
-        if ((rc = launch_overlapped(group_norm_grad_join_kernel, dim3((unsigned)parts, (unsigned)std::min(a.graphs, 256)), kNormThreads, 0, st, a)))
+        if ((rc = launch_overlapped(group_norm_grad_join_kernel, dim3((unsigned)parts, (unsigned)std::max(1, std::min(a.graphs, 4 * sm_count() / parts))), kNormThreads, 0, st, a)))
             return rc;
     }
     const unsigned more = a.dweight || a.dbias ? (unsigned)((parts + p.slabs - 1) / p.slabs) : 0;
@@ -772,7 +779,7 @@ static int run_norm(const mask_norm* n, bool backward, void* d_scratch, size_t s
     if (scratch_bytes < p.bytes) return fail(MASK_ERR_SCRATCH_TOO_SMALL, "scratch is smaller than mask_group_norm_scratch_bytes");
     NormArgs a = {};
     a.rows = n->rows; a.channels = n->channels; a.groups = n->groups; a.per_group = n->channels / n->groups; a.graphs = n->graphs;
-    a.eps = n->eps; a.chunk = p.chunk; a.tx = p.tx; a.whole = p.whole;
+    a.eps = n->eps; a.chunk = p.chunk; a.chunk_inverse = ~(uint64_t)0 / (uint64_t)p.chunk + 1; a.tx = p.tx; a.whole = p.whole;
     a.offsets = n->d_offsets; a.x = n->d_x; a.x_stride = n->x_stride; a.weight = n->d_weight; a.bias = n->d_bias;
     a.y = n->d_y; a.y_stride = n->y_stride; a.mean = n->d_mean; a.rstd = n->d_rstd;
     a.grad = n->d_grad; a.grad_stride = n->grad_stride; a.dweight = n->d_dweight; a.dbias = n->d_dbias;
