@@ -383,15 +383,17 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             if constexpr (P == 1) return next_accumulator();
             for (int k = k0; k < k1; k += kXentSegment) {
                 if (!next_accumulator()) return false;
+                if (k == k0) {
 #pragma unroll
-                for (int c = 0; c < kChunks; c++) {
-                    uint32_t u[32];
-                    tmem_ld32(acc + 32 * c, u);
+                    for (int j = 0; j < (P == 2 ? kHalf : 0); j++) total[j] = 0.f;
+                }
 #pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const float x = __uint_as_float(u[j]);
-                        total[P == 2 ? 32 * c + j : 0] = k == k0 ? x : total[P == 2 ? 32 * c + j : 0] + x;
-                    }
+                for (int c = 0; c < 2 * kChunks; c++) {
+                    uint32_t u[16];
+                    tmem_ld16(acc + 16 * c, u);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                    for (int j = 0; j < 16; j++) total[P == 2 ? 16 * c + j : 0] += __uint_as_float(u[j]);
                 }
                 release();
             }
