@@ -28,6 +28,8 @@ __device__ __forceinline__ bool labelled(int64_t y, int32_t classes) { return y 
 // One block per chunk of rows: how many of them are labelled.
 __global__ void __launch_bounds__(kXentCountThreads) xent_count_kernel(const int64_t* __restrict__ labels, int64_t rows, int32_t classes, int64_t chunk,
                                                                        int32_t* __restrict__ counts) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
     __shared__ int sums[32];
     const int64_t r0 = blockIdx.x * chunk, r1 = min(rows, r0 + chunk);
     int n = 0;
@@ -48,6 +50,8 @@ __global__ void __launch_bounds__(kXentCountThreads) xent_number_kernel(const in
                                                                         int32_t* __restrict__ label, int32_t* __restrict__ total,
                                                                         int32_t* __restrict__ status, uint32_t* __restrict__ range,
                                                                         float* __restrict__ row_loss) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
     __shared__ int sums[32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int at = 0;
@@ -110,6 +114,8 @@ __device__ __forceinline__ uint32_t finite_magnitude(float x) {
 
 // The largest finite magnitudes of both operands (FP32 input).  A maximum does not depend on the order.
 __global__ void __launch_bounds__(256) xent_range_kernel(const XentPackArgs p) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
     const int lane = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * 8, w0 = grid_warp();
     const float* hidden = static_cast<const float*>(p.hidden);
@@ -195,6 +201,8 @@ constexpr int kXentPackThreads = 256;
 
 template <bool kFloat>
 __global__ void __launch_bounds__(kXentPackThreads) xent_pack_kernel(const XentPackArgs p) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
     constexpr int kBytes = kFloat ? 4 : 2;
     const int lane = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * (kXentPackThreads / 32), w0 = grid_warp();
@@ -260,6 +268,8 @@ __global__ void __launch_bounds__(kXentPackThreads) xent_pack_kernel(const XentP
 // ---- joining -----------------------------------------------------------------------------------------------
 // Log sums and losses of the rows from the parts of the classes, in the parts' order.
 __global__ void __launch_bounds__(256) xent_join_kernel(const XentArgs p) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
     const int count = *p.count, lane = threadIdx.x & 31;
     const int64_t end = ((int64_t)count + 31) / 32 * 32;
     const float f = logit_factor(p.range);
@@ -303,6 +313,8 @@ struct XentReduceArgs {
 };
 
 __global__ void __launch_bounds__(256) xent_reduce_kernel(const XentReduceArgs p) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
     const int count = *p.count;
     const int64_t m_end = p.m_is_count ? count : p.m, n_vec = (p.n + 3) / 4;
     const ProductScale scale = product_scale(p.scale, p.mean, count, p.range, p.operand);
@@ -329,6 +341,8 @@ __global__ void __launch_bounds__(256) xent_reduce_kernel(const XentReduceArgs p
 // The loss of all rows, in a fixed order and 64 bits; NaN where a kernel gave up on a wait.
 __global__ void __launch_bounds__(1024) xent_loss_kernel(const int32_t* count_, const float* __restrict__ warp_loss, const int32_t* status, float* loss,
                                                          int64_t rows, int reduction) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
     const int count = *count_;
     if (*status) {
         const int64_t n = reduction == MASK_REDUCE_NONE ? rows : 1;
@@ -369,11 +383,17 @@ struct XentPlan {
     size_t counts, row_of, label, total, stats, label_logit, lse2, warp_loss, h_planes, w_planes, g, part_dh, part_dw, bytes;
 };
 
-// Parts to cut `units` of work per tile into, so that `tiles` tiles fill the SMs: the fewest rounds of the longest part.
-// A part costs two units beside its own (the accumulator's way out).
-static int best_splits(int64_t tiles, int64_t units, int64_t sms) {
+// `rows`: of the product.  Returns the blocks that share a tile of `bn` columns.
+static int tile_blocks(int bn, int64_t rows) { return bn == 256 && rows > kXentTileM ? 2 : 1; }
+
+// Parts to cut each tile's `units` of work into (tiles: those of `rows` rows, `others` of them side by side), so that they
+// fill the SMs: the fewest rounds of the longest part, `rounds` at most.  A part costs two units beside its own (the
+// accumulator's way out).
+static int best_splits(int64_t rows, int bn, int64_t others, int64_t units, int rounds) {
+    const int cg = tile_blocks(bn, rows);
+    const int64_t sms = sm_count() / cg, tiles = (rows + cg * kXentTileM - 1) / (cg * kXentTileM) * others;
     int64_t best = 1, best_cost = INT64_MAX;
-    const int64_t most = std::min<int64_t>(units, std::max<int64_t>(1, 4 * sms / std::max<int64_t>(tiles, 1)));
+    const int64_t most = std::min<int64_t>(units, std::max<int64_t>(1, rounds * sms / std::max<int64_t>(tiles, 1)));
     for (int64_t s = 1; s <= most; s++) {
         const int64_t cost = (tiles * s + sms - 1) / sms * ((units + s - 1) / s + 2);
         if (cost < best_cost) { best_cost = cost; best = s; }
@@ -388,7 +408,6 @@ static int tile_width(int n) {
 
 static XentPlan plan_xent(const mask_head& h) {
     XentPlan p = {};
-    const int64_t sms = sm_count();
     p.planes = h.dtype == MASK_F32 ? 2 : 1;
     p.dim_pad = (int)round_up(h.dim, 8);
     p.rows_pad = round_up(std::max<int64_t>(h.rows, 1), kXentTileM);
@@ -401,8 +420,7 @@ static XentPlan plan_xent(const mask_head& h) {
     p.bn_dim = tile_width(h.dim);
     // one tile of all classes: 256 columns, with two planes of G in shared memory 128
     p.one_pass = p.grads && h.classes <= (p.planes == 2 ? 128 : 256);
-    const int64_t m_tiles = p.rows_pad / kXentTileM;
-    p.stats_splits = p.one_pass ? 1 : best_splits(m_tiles, (h.classes + p.bn_logits - 1) / p.bn_logits, sms);
+    p.stats_splits = p.one_pass ? 1 : best_splits(p.rows_pad, p.bn_logits, 1, (h.classes + p.bn_logits - 1) / p.bn_logits, 16);
     if (p.grads) {
         if (p.one_pass) {
             p.piece = h.classes;
@@ -415,12 +433,12 @@ static XentPlan plan_xent(const mask_head& h) {
         const int64_t n_tiles = (h.dim + p.bn_dim - 1) / p.bn_dim;
         p.part_ld = (int)(n_tiles * p.bn_dim);
         if (h.d_dhidden) {
-            p.dh_splits = best_splits(m_tiles * n_tiles, (p.piece + kXentTileK - 1) / kXentTileK, sms);
+            p.dh_splits = best_splits(p.rows_pad, p.bn_dim, n_tiles, (p.piece + kXentTileK - 1) / kXentTileK, 4);
             p.dh_parts = p.dh_splits > 1 || p.n_pieces > 1;
             p.part_dh_rows = p.rows_pad;
         }
         if (h.d_dweight) {
-            p.dw_splits = best_splits((p.piece + kXentTileM - 1) / kXentTileM * n_tiles, (p.rows_pad + kXentTileK - 1) / kXentTileK, sms);
+            p.dw_splits = best_splits(p.piece, p.bn_dim, n_tiles, (p.rows_pad + kXentTileK - 1) / kXentTileK, 4);
             p.dw_parts = p.dw_splits > 1;
             p.part_dw_rows = round_up(p.piece, kXentTileM);
         }
@@ -469,30 +487,32 @@ static int plane_map(CUtensorMap* map, const void* data, int64_t cols, int64_t r
     return MASK_OK;
 }
 
-template <int BN, int P, int MODE>
+template <int BN, int P, int MODE, int CG>
 static int launch_xent_gemm_as(const XentArgs& a, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mg, int64_t items, cudaStream_t st) {
-    using L = XentLayout<BN, P, MODE>;
+    using L = XentLayout<BN, P, MODE, CG>;
     static std::atomic<uint64_t> done{0};
-    const int rc = opt_in_shared_memory(reinterpret_cast<const void*>(xent_gemm_kernel<BN, P, MODE>), L::kDynamicBytes, done);
+    const int rc = opt_in_shared_memory(reinterpret_cast<const void*>(xent_gemm_kernel<BN, P, MODE, CG>), L::kDynamicBytes, done);
     if (rc != MASK_OK) return rc;
-    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(items, sm_count()));
-    xent_gemm_kernel<BN, P, MODE><<<grid, xent_threads(P), L::kDynamicBytes, st>>>(a, ma, mb, mg);
-    MASK_CUDA_TRY(cudaGetLastError());
-    return MASK_OK;
+    const unsigned grid = CG * (unsigned)std::max<int64_t>(1, std::min<int64_t>(items, sm_count() / CG));
+    return launch_overlapped_clusters(CG, xent_gemm_kernel<BN, P, MODE, CG>, dim3(grid), xent_threads(P), L::kDynamicBytes, st, a, ma, mb, mg);
+}
+
+template <int MODE, int P>
+static int launch_xent_gemm_planes(int bn, int cg, const XentArgs& a, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mg, int64_t items,
+                                   cudaStream_t st) {
+    if (bn == 64) return launch_xent_gemm_as<64, P, MODE, 1>(a, ma, mb, mg, items, st);
+    if (bn == 128) return launch_xent_gemm_as<128, P, MODE, 1>(a, ma, mb, mg, items, st);
+    if constexpr (P == 2 && MODE == kXentGradOne) return fail(MASK_ERR_INVALID_ARGUMENT, "no such kernel");
+    else if (cg == 1) return launch_xent_gemm_as<256, P, MODE, 1>(a, ma, mb, mg, items, st);
+    else return launch_xent_gemm_as<256, P, MODE, 2>(a, ma, mb, mg, items, st);
 }
 
 template <int MODE>
-static int launch_xent_gemm(int bn, int planes, const XentArgs& a, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mg, int64_t items,
-                            cudaStream_t st) {
-    if (planes == 1) {
-        if (bn == 64) return launch_xent_gemm_as<64, 1, MODE>(a, ma, mb, mg, items, st);
-        if (bn == 128) return launch_xent_gemm_as<128, 1, MODE>(a, ma, mb, mg, items, st);
-        return launch_xent_gemm_as<256, 1, MODE>(a, ma, mb, mg, items, st);
-    }
-    if (bn == 64) return launch_xent_gemm_as<64, 2, MODE>(a, ma, mb, mg, items, st);
-    if (bn == 128) return launch_xent_gemm_as<128, 2, MODE>(a, ma, mb, mg, items, st);
-    if constexpr (MODE == kXentGradOne) return fail(MASK_ERR_INVALID_ARGUMENT, "no such kernel");
-    else return launch_xent_gemm_as<256, 2, MODE>(a, ma, mb, mg, items, st);
+static int launch_xent_gemm(int bn, int planes, const XentArgs& a, int64_t rows, int64_t parts, const CUtensorMap& ma, const CUtensorMap& mb,
+                            const CUtensorMap& mg, cudaStream_t st) {
+    const int cg = tile_blocks(bn, rows);
+    const int64_t items = (rows + cg * kXentTileM - 1) / (cg * kXentTileM) * parts;
+    return planes == 1 ? launch_xent_gemm_planes<MODE, 1>(bn, cg, a, ma, mb, mg, items, st) : launch_xent_gemm_planes<MODE, 2>(bn, cg, a, ma, mb, mg, items, st);
 }
 
 static const char* refuse_head(const mask_head* h) {
@@ -525,11 +545,15 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
     uint32_t* range = reinterpret_cast<uint32_t*>(total + 2);
     float* row_loss = h.reduction == MASK_REDUCE_NONE ? h.d_loss : nullptr;
     const int P = plan.planes;
-    const int64_t rp = plan.rows_pad, m_tiles = rp / kXentTileM;
+    const int64_t rp = plan.rows_pad;
 
-    if (plan.n_chunks > 1) xent_count_kernel<<<plan.n_chunks, kXentCountThreads, 0, st>>>(h.d_labels, h.rows, h.classes, plan.chunk, counts);
-    xent_number_kernel<<<plan.n_chunks, kXentCountThreads, 0, st>>>(h.d_labels, h.rows, h.classes, plan.chunk, counts, row_of, label, total, total + 1, range, row_loss);
-    MASK_CUDA_TRY(cudaGetLastError());
+    const dim3 chunks((unsigned)plan.n_chunks);
+    int rc = MASK_OK;
+    if (plan.n_chunks > 1 && (rc = launch_overlapped(xent_count_kernel, chunks, kXentCountThreads, 0, st, h.d_labels, h.rows, h.classes, plan.chunk, counts)))
+        return rc;
+    if ((rc = launch_overlapped(xent_number_kernel, chunks, kXentCountThreads, 0, st, h.d_labels, h.rows, h.classes, plan.chunk, counts, row_of, label,
+                                total, total + 1, range, row_loss)))
+        return rc;
 
     XentPackArgs pk = {};
     pk.dtype = h.dtype; pk.dim = h.dim; pk.dim_pad = plan.dim_pad; pk.classes = h.classes; pk.rows = h.rows;
@@ -545,20 +569,18 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
     const int64_t pack_rows = rp + (plan.pack_weight ? h.classes : 0);
     const unsigned pack_grid = (unsigned)std::min<int64_t>((pack_rows + 7) / 8, 8 * (int64_t)sm_count());
     if (h.dtype == MASK_F32) {
-        xent_range_kernel<<<pack_grid, 256, 0, st>>>(pk);
-        xent_pack_kernel<true><<<pack_grid, kXentPackThreads, 0, st>>>(pk);
+        if ((rc = launch_overlapped(xent_range_kernel, dim3(pack_grid), 256, 0, st, pk))) return rc;
+        if ((rc = launch_overlapped(xent_pack_kernel<true>, dim3(pack_grid), kXentPackThreads, 0, st, pk))) return rc;
     } else {
-        xent_pack_kernel<false><<<pack_grid, kXentPackThreads, 0, st>>>(pk);
+        if ((rc = launch_overlapped(xent_pack_kernel<false>, dim3(pack_grid), kXentPackThreads, 0, st, pk))) return rc;
     }
-    MASK_CUDA_TRY(cudaGetLastError());
 
     const void* w_data = plan.pack_weight ? (const void*)pk.w_planes : h.d_weight;
     const int64_t w_ld = plan.pack_weight ? plan.dim_pad : h.weight_class_stride, w_plane = plan.pack_weight ? pk.w_plane : w_ld * h.classes;
     const int w_cols = plan.pack_weight ? plan.dim_pad : h.dim;
-    int rc;
     CUtensorMap h_k, w_k, none = {};     // K-major, contracted over dim
     if ((rc = plane_map(&h_k, pk.h_planes, plan.dim_pad, rp, P, plan.dim_pad, pk.h_plane, 64, kXentTileM))) return rc;
-    if ((rc = plane_map(&w_k, w_data, w_cols, h.classes, P, w_ld, w_plane, 64, plan.bn_logits))) return rc;
+    if ((rc = plane_map(&w_k, w_data, w_cols, h.classes, P, w_ld, w_plane, 64, plan.bn_logits / tile_blocks(plan.bn_logits, rp)))) return rc;
 
     XentArgs a = {};
     a.count = total; a.status = total + 1;
@@ -574,9 +596,8 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
 
     if (!plan.one_pass) {
         a.splits = plan.stats_splits;
-        if ((rc = launch_xent_gemm<kXentStats>(plan.bn_logits, P, a, h_k, w_k, none, m_tiles * a.splits, st))) return rc;
-        xent_join_kernel<<<(unsigned)std::min<int64_t>((rp + 255) / 256, 4 * (int64_t)sm_count()), 256, 0, st>>>(a);
-        MASK_CUDA_TRY(cudaGetLastError());
+        if ((rc = launch_xent_gemm<kXentStats>(plan.bn_logits, P, a, rp, a.splits, h_k, w_k, none, st))) return rc;
+        if ((rc = launch_overlapped(xent_join_kernel, dim3((unsigned)std::min<int64_t>((rp + 255) / 256, 4 * (int64_t)sm_count())), 256, 0, st, a))) return rc;
     }
     if (plan.grads) {
         char* g = at(plan.g);
@@ -596,8 +617,8 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
             a.v0 = piece * plan.piece;
             a.vc = std::min(plan.piece, h.classes - a.v0);
             const int64_t v_tiles = (a.vc + plan.bn_logits - 1) / plan.bn_logits;
-            if (plan.one_pass) rc = launch_xent_gemm<kXentGradOne>(plan.bn_logits, P, a, h_k, w_k, g_st, m_tiles, st);
-            else rc = launch_xent_gemm<kXentGrad>(plan.bn_logits, P, a, h_k, w_k, g_st, m_tiles * v_tiles, st);
+            if (plan.one_pass) rc = launch_xent_gemm<kXentGradOne>(plan.bn_logits, P, a, rp, 1, h_k, w_k, g_st, st);
+            else rc = launch_xent_gemm<kXentGrad>(plan.bn_logits, P, a, rp, v_tiles, h_k, w_k, g_st, st);
             if (rc) return rc;
             if (h.d_dhidden) {
                 XentArgs b = a;
@@ -606,7 +627,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
                 b.part = reinterpret_cast<float*>(at(plan.part_dh)); b.part_rows = plan.part_dh_rows; b.part_ld = plan.part_ld;
                 b.out = h.d_dhidden; b.out_m = h.dhidden_stride; b.out_n = 1;
                 b.out_vec = h.dhidden_stride % (int64_t)vec == 0 && (reinterpret_cast<uintptr_t>(h.d_dhidden) & 15) == 0;
-                if ((rc = launch_xent_gemm<kXentDHidden>(plan.bn_dim, P, b, g_k, w_mn, none, m_tiles * n_tiles * b.splits, st))) return rc;
+                if ((rc = launch_xent_gemm<kXentDHidden>(plan.bn_dim, P, b, rp, n_tiles * b.splits, g_k, w_mn, none, st))) return rc;
             }
             if (h.d_dweight) {
                 XentArgs b = a;
@@ -615,15 +636,13 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
                 b.part = reinterpret_cast<float*>(at(plan.part_dw)); b.part_rows = plan.part_dw_rows; b.part_ld = plan.part_ld;
                 b.out = h.d_dweight; b.out_m = h.dweight_class_stride; b.out_n = h.dweight_dim_stride;
                 b.out_vec = b.out_n == 1 && b.out_m % (int64_t)vec == 0 && (reinterpret_cast<uintptr_t>(h.d_dweight) & 15) == 0;
-                const int64_t wm_tiles = (a.vc + kXentTileM - 1) / kXentTileM;
-                if ((rc = launch_xent_gemm<kXentDWeight>(plan.bn_dim, P, b, g_mn, h_mn, none, wm_tiles * n_tiles * b.splits, st))) return rc;
+                if ((rc = launch_xent_gemm<kXentDWeight>(plan.bn_dim, P, b, a.vc, n_tiles * b.splits, g_mn, h_mn, none, st))) return rc;
                 if (plan.dw_parts) {
                     XentReduceArgs w = r;
                     w.part = b.part; w.part_rows = b.part_rows; w.splits = b.splits; w.m = a.vc; w.m0 = a.v0;
                     w.out = b.out; w.out_m = b.out_m; w.out_n = b.out_n;
                     const int64_t n = (int64_t)w.m * ((w.n + 3) / 4);
-                    xent_reduce_kernel<<<std::min(blocks_for(n, 256), most_blocks), 256, 0, st>>>(w);
-                    MASK_CUDA_TRY(cudaGetLastError());
+                    if ((rc = launch_overlapped(xent_reduce_kernel, dim3(std::min(blocks_for(n, 256), most_blocks)), 256, 0, st, w))) return rc;
                 }
             }
         }
@@ -632,12 +651,10 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
             r.m_is_count = 1; r.operand = 1;
             r.out = h.d_dhidden; r.out_m = h.dhidden_stride; r.out_n = 1;
             const int64_t n = rp * ((r.n + 3) / 4);
-            xent_reduce_kernel<<<(unsigned)std::min<int64_t>((n + 255) / 256, most_blocks), 256, 0, st>>>(r);
-            MASK_CUDA_TRY(cudaGetLastError());
+            if ((rc = launch_overlapped(xent_reduce_kernel, dim3((unsigned)std::min<int64_t>((n + 255) / 256, most_blocks)), 256, 0, st, r))) return rc;
         }
     }
-    xent_loss_kernel<<<1, 1024, 0, st>>>(total, a.warp_loss, total + 1, h.d_loss, h.rows, h.reduction);
-    MASK_CUDA_TRY(cudaGetLastError());
+    if ((rc = launch_overlapped(xent_loss_kernel, dim3(1), 1024, 0, st, total, a.warp_loss, total + 1, h.d_loss, h.rows, h.reduction))) return rc;
     return MASK_OK;
 }
 

@@ -25,7 +25,7 @@
 namespace mask {
 
 constexpr int kXentTileM = 128, kXentTileK = 64;
-constexpr int kXentSegment = 4;                     // blocks of the contraction that an accumulator takes (FP32 input)
+constexpr int kXentSegment = 2;                     // blocks of the contraction that an accumulator takes (FP32 input)
 constexpr int kXentWarps = 8;                       // epilogue warps: 4 quarters of 32 rows x 2 halves of the columns
 // + producer + MMA issuer; with segments summed in registers (P == 2) two warps more make three whole warpgroups, whose
 // 168 registers a thread are dealt again: 216 to the two that take accumulators apart, 72 to the third (3 x 168 in all).
@@ -98,10 +98,12 @@ __device__ __forceinline__ float logit_factor(const uint32_t* range) {
     return range ? ldexpf(kLog2e, min(plane_exponent(range[0]) + plane_exponent(range[1]) - 28, 126)) : kLog2e;   // finite: 0 stays 0
 }
 
-template <int BN, int P, int MODE>
+// CG: blocks that share a tile.  2: a cluster of two takes 256 rows, each block 128 of them and half of the columns' operand,
+// and the first issues the MMAs for both.
+template <int BN, int P, int MODE, int CG>
 struct XentLayout {
     static constexpr bool kWritesG = MODE == kXentGrad || MODE == kXentGradOne;
-    static constexpr int kTileA = kXentTileM * kXentTileK * 2, kTileB = BN * kXentTileK * 2;
+    static constexpr int kTileA = kXentTileM * kXentTileK * 2, kTileB = BN / CG * kXentTileK * 2;
     static constexpr int kStage = P * (kTileA + kTileB);
     static constexpr int kStaging = kWritesG ? kXentWarps * 4096 : 0;      // 32 rows x 32 columns x 2 planes or buffers a warp
     static constexpr int kMost = 227 * 1024 - 1024 - 256 - kStaging - (MODE == kXentGradOne ? 2 * 2 * 128 * 12 : 0);
@@ -119,12 +121,56 @@ struct XentLayout {
     static_assert(S >= 2 && kDynamicBytes <= 227 * 1024 && kTmemCols <= 512, "tile does not fit");
 };
 
-__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
+// Descriptors as their two halves: stepping through an operand is one 32-bit addition.
+template <int CG>
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+    if constexpr (CG == 1)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %5, p;\n\t}"
+            ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %2};\n\tmov.b64 db, {%3, %4};\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %5, p;\n\t}"
+            ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+// Bounded wait of a whole warp: a probe first, which is enough where the phase is over already.
+__device__ __forceinline__ bool wait_all_lanes(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    if (__all_sync(0xffffffffu, mbar_probe(bar, parity))) return true;
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+// Arrives on `bar`, of both blocks of a pair, when the MMAs issued so far are done.
+template <int CG>
+__device__ __forceinline__ void xent_commit(uint32_t bar) {
+    if constexpr (CG == 1) umma_commit(bar);
+    else
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+                     ::"r"(bar), "h"((uint16_t)3)
+                     : "memory");
+}
+// The address of the same shared memory in the first block of the pair.
+template <int CG>
+__device__ __forceinline__ uint32_t in_leader(uint32_t at) {
+    if constexpr (CG == 1) return at;
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(at));
+    return r;
+}
+template <int CG>
+__device__ __forceinline__ void arrive_at_leader(uint32_t bar) {
+    if constexpr (CG == 1) mbar_arrive(bar);
+    else asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_leader<CG>(bar)) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
     asm volatile(
@@ -138,10 +184,17 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
         : "memory");
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+// Completes on `bar`, which with CG == 2 is the first block's.
+template <int CG>
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
-                 : "memory");
+    if constexpr (CG == 1)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+                     : "memory");
 }
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
@@ -178,11 +231,11 @@ __device__ __forceinline__ void online_softmax(const float (&v)[32], float f, fl
     top = now;
 }
 
-template <int BN, int P, int MODE>
+template <int BN, int P, int MODE, int CG>
 __global__ void __launch_bounds__(xent_threads(P), 1)
 xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const __grid_constant__ CUtensorMap map_g) {
-    using L = XentLayout<BN, P, MODE>;
+    using L = XentLayout<BN, P, MODE, CG>;
     constexpr int S = L::S;
     constexpr bool kLogits = MODE == kXentStats || MODE == kXentGrad || MODE == kXentGradOne;
     constexpr bool kAmn = MODE == kXentDWeight, kBmn = !kLogits;
@@ -199,7 +252,10 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
     auto exchange_bar = [&](int q) { return bars + 8u * (2 * S + 5 + q); };
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kAbort);
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + L::kTmemSlot);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    uint32_t rank = 0;                                  // within the pair
+    if constexpr (CG == 2) asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const int64_t group = blockIdx.x / CG, groups = gridDim.x / CG;
 
     if (tid == 0) {
         *abort_flag = 0;
@@ -209,27 +265,36 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(accf_bar(b), 1);
-            mbar_init(acce_bar(b), kXentWarps);
+            mbar_init(acce_bar(b), CG * kXentWarps);
         }
         for (int q = 0; q < 4; q++) mbar_init(exchange_bar(q), 2);
         mbar_init(drain_bar, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kXentWarps + 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kTmemSlot), "r"(L::kTmemCols) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kTmemSlot), "r"(L::kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kTmemSlot), "r"(L::kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if constexpr (CG == 2) cluster_sync();             // both blocks' barriers and tensor memory are there
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
+
+    wait_for_previous_kernel();
+    let_next_kernel_start();
 
     // ---- work: an item is a tile of rows with a range of column tiles and a range of blocks of the contraction ----------
     const int count = *p.count;
     const int m_extent = MODE == kXentDWeight ? p.vc : count;
     const int n_extent = kLogits ? p.vc : p.dim;
     const int k_extent = kLogits ? p.dim : (MODE == kXentDHidden ? p.vc : count);
-    const int m_tiles = (m_extent + kXentTileM - 1) / kXentTileM, n_tiles = (n_extent + BN - 1) / BN;
+    const int m_tiles = (m_extent + CG * kXentTileM - 1) / (CG * kXentTileM), n_tiles = (n_extent + BN - 1) / BN;
     const int k_blocks = (k_extent + kXentTileK - 1) / kXentTileK;
     // stats: parts of the column tiles; G: every tile an item; products: every tile once for each part of the contraction
     const int64_t items = (int64_t)m_tiles * (MODE == kXentStats ? p.splits : (kLogits ? n_tiles : n_tiles * p.splits));
@@ -264,29 +329,30 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 int s = 0;
                 uint32_t round = 0;
                 bool ok = true;
-                for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+                for (int64_t i = group; i < items && ok; i += groups) {
                     const Item t = item_of(i);
                     for (int n = t.n0; n < t.n1 && ok; n++) {
                         for (int k = t.k0; k < t.k1; k++) {
                             if (round > 0 && !mbar_wait(empty_bar(s), (round - 1) & 1, abort_flag)) { ok = false; break; }
-                            const uint32_t bar = full_bar(s), at = base + s * L::kStage;
-                            xent_expect_tx(bar, L::kStage);
-    #pragma unroll
+                            const uint32_t bar = in_leader<CG>(full_bar(s)), at = base + s * L::kStage;
+                            if (rank == 0) xent_expect_tx(full_bar(s), CG * L::kStage);
+                            const int am = (t.m * CG + (int)rank) * kXentTileM, bn = n * BN + (int)rank * (BN / CG);
+#pragma unroll
                             for (int z = 0; z < P; z++) {
                                 const uint32_t a = at + z * L::kTileA, b = at + P * L::kTileA + z * L::kTileB;
                                 if constexpr (kAmn) {
-    #pragma unroll
+#pragma unroll
                                     for (int j = 0; j < kXentTileM / 64; j++)
-                                        tma_load_3d(a + j * 8192, &map_a, bar, t.m * kXentTileM + j * 64, k * kXentTileK, z);
+                                        tma_load_3d<CG>(a + j * 8192, &map_a, bar, am + j * 64, k * kXentTileK, z);
                                 } else {
-                                    tma_load_3d(a, &map_a, bar, k * kXentTileK, t.m * kXentTileM, z);
+                                    tma_load_3d<CG>(a, &map_a, bar, k * kXentTileK, am, z);
                                 }
                                 if constexpr (kBmn) {
-    #pragma unroll
-                                    for (int j = 0; j < BN / 64; j++)
-                                        tma_load_3d(b + j * 8192, &map_b, bar, n * BN + j * 64, (MODE == kXentDHidden ? p.v0 : 0) + k * kXentTileK, z);
+#pragma unroll
+                                    for (int j = 0; j < BN / CG / 64; j++)
+                                        tma_load_3d<CG>(b + j * 8192, &map_b, bar, bn + j * 64, (MODE == kXentDHidden ? p.v0 : 0) + k * kXentTileK, z);
                                 } else {
-                                    tma_load_3d(b, &map_b, bar, k * kXentTileK, p.v0 + n * BN, z);
+                                    tma_load_3d<CG>(b, &map_b, bar, k * kXentTileK, p.v0 + bn, z);
                                 }
                             }
                             if (++s == S) { s = 0; round++; }
@@ -296,55 +362,65 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             }
             __syncwarp();
         } else if (warp == kXentWarps + 1) {
-            // ------------------------------ MMA issuer ---------------------------------------------------------------------
-            if (lane == 0) {
+            // ------------------------------ MMA issuer, of the pair's first block ----------------------------------------------
+            // The whole warp goes through the loop and one elected lane issues, so that descriptors live in uniform registers:
+            // from within a branch of one lane, four MMAs of 512 clocks took 790 to issue.
+            if (rank == 0) {
+                const bool elected = elect_one();
                 const uint32_t fmt = p.half_type ? 0u : 1u;
-                // instruction descriptor: D = F32, A and B bf16 or fp16, M = 128
+                // instruction descriptor: D = F32, A and B bf16 or fp16, M = 128 a block
                 const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (kAmn ? 1u << 15 : 0u) | (kBmn ? 1u << 16 : 0u) |
-                                       ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kXentTileM >> 4) << 24);
+                                       ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(CG * kXentTileM >> 4) << 24);
                 // 128-byte swizzle; K-major: groups of 8 rows 1024 bytes apart; MN-major: 64-wide atoms 8192 bytes apart, groups of 8 k 1024
                 const uint64_t a0 = umma_smem_desc(base, kAmn ? 512 : 1, 64, 2);
                 const uint64_t b0 = umma_smem_desc(base + P * L::kTileA, kBmn ? 512 : 1, 64, 2);
+                const uint32_t a_hi = (uint32_t)(a0 >> 32), b_hi = (uint32_t)(b0 >> 32);
                 constexpr uint32_t kStepA = kAmn ? 128 : 2, kStepB = kBmn ? 128 : 2;   // 16 of the contraction, in 16 bytes
+                uint32_t a_lo = (uint32_t)a0, b_lo = (uint32_t)b0;                     // of stage s
                 int s = 0;
                 uint32_t round = 0, acc_it = 0;
                 bool ok = true;
-                for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+                for (int64_t i = group; i < items && ok; i += groups) {
                     const Item t = item_of(i);
                     if (t.k0 >= t.k1) continue;
                     for (int n = t.n0; n < t.n1 && ok; n++) {
                         uint32_t buf = 0, acc = 0, open = 0;
+                        int left = 0;                        // blocks that the open accumulator still takes
                         for (int k = t.k0; k < t.k1; k++) {
                             if (!open) {
                                 buf = acc_it & 1;
                                 acc = tmem_base + buf * BN;
-                                if (acc_it >= 2 && !mbar_wait(acce_bar(buf), ((acc_it >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
-                                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                                left = P == 2 ? min(kXentSegment, t.k1 - k) : t.k1 - k;
+                                if (acc_it >= 2 && !wait_all_lanes(acce_bar(buf), ((acc_it >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
                             }
-                            if (!mbar_wait_spin(full_bar(s), round & 1, abort_flag)) { ok = false; break; }
+                            if (!wait_all_lanes(full_bar(s), round & 1, abort_flag)) { ok = false; break; }
                             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                            const uint64_t a = a0 + (uint64_t)(s * L::kStage >> 4), b = b0 + (uint64_t)(s * L::kStage >> 4);
-    #pragma unroll
-                            for (int c = 0; c < (P == 2 ? 3 : 1); c++) {     // hi hi, hi lo, lo hi
-                                const uint64_t ac = a + (c == 2 ? L::kTileA >> 4 : 0), bc = b + (c == 1 ? L::kTileB >> 4 : 0);
-    #pragma unroll
-                                for (int j = 0; j < kXentTileK / 16; j++) {
-                                    umma_f16(acc, ac + j * kStepA, bc + j * kStepB, idesc, open);
-                                    open = 1;
+                            if (elected) {
+#pragma unroll
+                                for (int c = 0; c < (P == 2 ? 3 : 1); c++) {     // hi hi, hi lo, lo hi
+#pragma unroll
+                                    for (int j = 0; j < kXentTileK / 16; j++)
+                                        umma_f16<CG>(acc, a_lo + (c == 2 ? L::kTileA >> 4 : 0) + j * kStepA, a_hi, b_lo + (c == 1 ? L::kTileB >> 4 : 0) + j * kStepB,
+                                                     b_hi, idesc, c + j ? 1u : open);
                                 }
+                                xent_commit<CG>(empty_bar(s));
+                                if (left == 1) xent_commit<CG>(accf_bar(buf));
                             }
-                            umma_commit(empty_bar(s));
-                            if (++s == S) { s = 0; round++; }
-                            if (k + 1 == t.k1 || (P == 2 && (k + 1 - t.k0) % kXentSegment == 0)) {
-                                umma_commit(accf_bar(buf));
-                                acc_it++;
-                                open = 0;
+                            __syncwarp();
+                            open = --left > 0;
+                            if (left == 0) acc_it++;
+                            a_lo += L::kStage >> 4;
+                            b_lo += L::kStage >> 4;
+                            if (++s == S) {
+                                s = 0; round++;
+                                a_lo = (uint32_t)a0; b_lo = (uint32_t)b0;
                             }
                         }
-                        if (!ok) break;
                     }
                 }
-                umma_commit(drain_bar);
+                // whatever was issued must have finished before shared and tensor memory go away
+                if (elected) xent_commit<CG>(drain_bar);
+                __syncwarp();
                 const long long start = clock64();
                 while (!mbar_test(drain_bar, 0)) {
                     if (clock64() - start > kUmmaWaitCycles) { *abort_flag = 1; break; }
@@ -368,7 +444,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
         auto release = [&]() {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) mbar_arrive(acce_bar(acc_it & 1));
+            if (lane == 0) arrive_at_leader<CG>(acce_bar(acc_it & 1));
             acc_it++;
         };
         auto next_accumulator = [&]() -> bool {
@@ -414,8 +490,9 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             }
         };
         // G of 32 columns to global memory through this warp's staging buffer
-        [[maybe_unused]] auto write_g = [&](const float (&g)[32], int m, int col) {
+        [[maybe_unused]] auto write_g = [&](const float (&g)[32], int row0, int col) {
             if constexpr (L::kWritesG) {
+                if (row0 >= p.rows_pad) return;            // a pair's second tile may lie behind the last row
                 // P == 1: two buffers in turn, so the older copy may still be read; P == 2: both planes at once
                 if (lane == 0) {
                     if constexpr (P == 1) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
@@ -443,7 +520,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 __syncwarp();
                 if (lane == 0) {
 #pragma unroll
-                    for (int z = 0; z < P; z++) tma_store_3d(&map_g, staging + first + z * 2048, col, m * kXentTileM + 32 * quarter, z);
+                    for (int z = 0; z < P; z++) tma_store_3d(&map_g, staging + first + z * 2048, col, row0, z);
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
                 stage_it++;
@@ -504,9 +581,9 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 v[j] = !live || col + j >= classes ? 0.f : unit * (y == col + j ? e - 1.f : e);
             }
         };
-        for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+        for (int64_t i = group; i < items && ok; i += groups) {
             const Item t = item_of(i);
-            const int r = t.m * kXentTileM + 32 * quarter + lane;     // row of the tile that this thread holds
+            const int r = (t.m * CG + (int)rank) * kXentTileM + 32 * quarter + lane;     // row of the tile that this thread holds
             if constexpr (MODE == kXentStats) {
                 const int y = r < count ? p.label[r] : -1;
                 float top = -INFINITY, sum = 0.f, picked = 0.f;
@@ -548,7 +625,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     float v[32];
                     values(c, v);
                     gradient(v, col, p.vc, live, y, lse2);
-                    write_g(v, t.m, col);
+                    write_g(v, r - lane, col);
                 }
                 done();
             } else if constexpr (MODE == kXentGradOne) {
@@ -593,7 +670,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     float w = loss;
 #pragma unroll
                     for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-                    if (lane == 0) p.warp_loss[t.m * (kXentTileM / 32) + quarter] = w;
+                    if (lane == 0 && r < p.rows_pad) p.warp_loss[r >> 5] = w;
                 }
 #pragma unroll(kUnroll)
                 for (int c = 0; c < kChunks; c++) {
@@ -601,7 +678,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     float v[32];
                     values(c, v);
                     gradient(v, col, p.classes, live, y, lse2);
-                    write_g(v, t.m, col);
+                    write_g(v, r - lane, col);
                 }
                 done();
             } else {
@@ -635,6 +712,8 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
     // ---- teardown: everybody gets here, aborting or not ---------------------------------------------------------------
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    // The pair's first block has waited for all its MMAs; the other one may still be reading or signalling this one.
+    if constexpr (CG == 2) cluster_sync();
     if (*abort_flag) {
         // copies that were issued but never consumed may still be landing in this block's shared memory
         const long long start = clock64();
@@ -644,7 +723,8 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
     }
     if (warp == kXentWarps + 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(L::kTmemCols) : "memory");
+        if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(L::kTmemCols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(L::kTmemCols) : "memory");
     }
     if (tid == 0 && *abort_flag) atomicExch(p.status, 1);
 }
