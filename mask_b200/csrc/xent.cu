@@ -266,31 +266,43 @@ __global__ void __launch_bounds__(kXentPackThreads) xent_pack_kernel(const XentP
 }
 
 // ---- joining -----------------------------------------------------------------------------------------------
-// Log sums and losses of the rows from the parts of the classes, in the parts' order.
-__global__ void __launch_bounds__(256) xent_join_kernel(const XentArgs p) {
+// Log sums and losses of the rows from the parts of the classes: a block takes 32 rows, 32 threads each, whose shares of
+// the parts are joined in their order.
+__global__ void __launch_bounds__(1024) xent_join_kernel(const XentArgs p, int parts) {
     wait_for_previous_kernel();
     let_next_kernel_start();
-    const int count = *p.count, lane = threadIdx.x & 31;
-    const int64_t end = ((int64_t)count + 31) / 32 * 32;
+    __shared__ float2 room[32][33];
+    const int count = *p.count, lane = threadIdx.x & 31, share = threadIdx.x >> 5;
     const float f = logit_factor(p.range);
-    for (int64_t r = grid_thread(); r < end; r += (int64_t)gridDim.x * blockDim.x) {
-        float loss = 0.f;
-        if (r < count) {
-            float top = -INFINITY, sum = 0.f;
-            for (int i = 0; i < 2 * p.splits; i++) top = fmaxf(top, p.stats[(int64_t)i * p.rows_pad + r].x);
-            const float base = top == -INFINITY ? 0.f : top * f;
-            for (int i = 0; i < 2 * p.splits; i++) {
-                const float2 s = p.stats[(int64_t)i * p.rows_pad + r];
-                sum += s.y * fast_exp2(fmaf(s.x, f, -base));
-            }
-            const float lse2 = base + log2f(sum);
-            p.lse2[r] = lse2;
-            loss = kLn2 * fmaf(-p.label_logit[r], f, lse2);
-            if (p.row_loss) p.row_loss[p.row_of[r]] = loss;
+    for (int64_t r0 = 32 * (int64_t)blockIdx.x; r0 < count; r0 += 32 * (int64_t)gridDim.x) {
+        const int64_t r = r0 + lane;
+        float top = -INFINITY, sum = 0.f;
+        for (int i = share; i < parts; i += 32) {
+            const float2 s = r < count ? p.stats[(int64_t)i * p.rows_pad + r] : make_float2(-INFINITY, 0.f);
+            const float now = fmaxf(top, s.x), base = now == -INFINITY ? 0.f : now * f;
+            sum = sum * fast_exp2(fmaf(top, f, -base)) + s.y * fast_exp2(fmaf(s.x, f, -base));
+            top = now;
         }
+        __syncthreads();
+        room[share][lane] = make_float2(top, sum);
+        __syncthreads();
+        if (share == 0) {
+            top = -INFINITY;
+            for (int i = 0; i < 32; i++) top = fmaxf(top, room[i][lane].x);
+            const float base = top == -INFINITY ? 0.f : top * f;
+            sum = 0.f;
+            for (int i = 0; i < 32; i++) sum += room[i][lane].y * fast_exp2(fmaf(room[i][lane].x, f, -base));
+            float loss = 0.f;
+            if (r < count) {
+                const float lse2 = base + log2f(sum);
+                p.lse2[r] = lse2;
+                loss = kLn2 * fmaf(-p.label_logit[r], f, lse2);
+                if (p.row_loss) p.row_loss[p.row_of[r]] = loss;
+            }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
-        if (lane == 0) p.warp_loss[r >> 5] = loss;
+            for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+            if (lane == 0) p.warp_loss[r0 >> 5] = loss;
+        }
     }
 }
 
@@ -372,7 +384,7 @@ struct XentPlan {
     int n_chunks;
     bool grads, one_pass, pack_weight;
     int bn_logits, bn_dim;
-    int stats_splits;
+    int stats_splits, stats_parts;       // parts of the classes' tiles, and numbers a row gets from them
     int piece, n_pieces;                 // classes of a piece (a multiple of 256 unless one tile holds all), pieces
     int g_ld;
     int dh_splits, dw_splits;
@@ -421,6 +433,7 @@ static XentPlan plan_xent(const mask_head& h) {
     // one tile of all classes: 256 columns, with two planes of G in shared memory 128
     p.one_pass = p.grads && h.classes <= (p.planes == 2 ? 128 : 256);
     p.stats_splits = p.one_pass ? 1 : best_splits(p.rows_pad, p.bn_logits, 1, (h.classes + p.bn_logits - 1) / p.bn_logits, 16);
+    p.stats_parts = p.stats_splits * (p.planes == 1 && p.bn_logits >= 128 ? XentLayout<256, 1, kXentStats, 1>::kParts : XentLayout<64, 1, kXentStats, 1>::kParts);
     if (p.grads) {
         if (p.one_pass) {
             p.piece = h.classes;
@@ -454,7 +467,7 @@ static XentPlan plan_xent(const mask_head& h) {
     p.counts = take(4 * (size_t)p.n_chunks);
     p.row_of = take(4 * rp);
     p.label = take(4 * rp);
-    p.stats = p.one_pass ? 0 : take(16 * rp * p.stats_splits);
+    p.stats = p.one_pass ? 0 : take(8 * rp * p.stats_parts);
     p.label_logit = take(4 * rp);
     p.lse2 = take(4 * rp);
     p.warp_loss = take(rp / 8);
@@ -494,7 +507,7 @@ static int launch_xent_gemm_as(const XentArgs& a, const CUtensorMap& ma, const C
     const int rc = opt_in_shared_memory(reinterpret_cast<const void*>(xent_gemm_kernel<BN, P, MODE, CG>), L::kDynamicBytes, done);
     if (rc != MASK_OK) return rc;
     const unsigned grid = CG * (unsigned)std::max<int64_t>(1, std::min<int64_t>(items, sm_count() / CG));
-    return launch_overlapped_clusters(CG, xent_gemm_kernel<BN, P, MODE, CG>, dim3(grid), xent_threads(P), L::kDynamicBytes, st, a, ma, mb, mg);
+    return launch_overlapped_clusters(CG, xent_gemm_kernel<BN, P, MODE, CG>, dim3(grid), L::kThreads, L::kDynamicBytes, st, a, ma, mb, mg);
 }
 
 template <int MODE, int P>
@@ -597,7 +610,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
     if (!plan.one_pass) {
         a.splits = plan.stats_splits;
         if ((rc = launch_xent_gemm<kXentStats>(plan.bn_logits, P, a, rp, a.splits, h_k, w_k, none, st))) return rc;
-        if ((rc = launch_overlapped(xent_join_kernel, dim3((unsigned)std::min<int64_t>((rp + 255) / 256, 4 * (int64_t)sm_count())), 256, 0, st, a))) return rc;
+        if ((rc = launch_overlapped(xent_join_kernel, dim3((unsigned)std::min<int64_t>(rp / 32, 2 * (int64_t)sm_count())), 1024, 0, st, a, plan.stats_parts))) return rc;
     }
     if (plan.grads) {
         char* g = at(plan.g);

@@ -26,11 +26,6 @@ namespace mask {
 
 constexpr int kXentTileM = 128, kXentTileK = 64;
 constexpr int kXentSegment = 2;                     // blocks of the contraction that an accumulator takes (FP32 input)
-constexpr int kXentWarps = 8;                       // epilogue warps: 4 quarters of 32 rows x 2 halves of the columns
-// + producer + MMA issuer; with segments summed in registers (P == 2) two warps more make three whole warpgroups, whose
-// 168 registers a thread are dealt again: 216 to the two that take accumulators apart, 72 to the third (3 x 168 in all).
-constexpr int xent_threads(int planes) { return 32 * (kXentWarps + (planes == 2 ? 4 : 2)); }
-
 enum XentMode {
     kXentStats,      // logits -> running maximum and sum of each row over a range of classes
     kXentGrad,       // logits -> G of a piece of the classes, with the rows' log sums known
@@ -50,7 +45,7 @@ struct XentArgs {
     int32_t half_type;         // planes hold fp16, not bf16
     const int32_t* label;      // [labelled row]
     const int32_t* row_of;     // [labelled row] -> row of the caller's arrays
-    float2* stats;             // [2 * splits][rows_pad]: maximum, sum of exp(logit - maximum)
+    float2* stats;             // [splits * epilogue parts][rows_pad]: maximum, sum of exp(logit - maximum)
     float* label_logit;        // [labelled row]
     float* lse2;               // [labelled row]: log2 of the row's sum of exponentials
     float* row_loss;           // caller's, or NULL
@@ -102,16 +97,24 @@ __device__ __forceinline__ float logit_factor(const uint32_t* range) {
 // and the first issues the MMAs for both.
 template <int BN, int P, int MODE, int CG>
 struct XentLayout {
+    // Epilogue warps: 4 quarters of 32 rows, each for so many parts of the columns.  Where every logit costs an exponential,
+    // four (16 warps): with two, a warp's waits for tensor memory and the special-function unit left the SM idle.
+    static constexpr int kParts = P == 1 && MODE <= kXentGradOne && BN >= 128 ? 4 : 2;
+    static constexpr int kWarps = 4 * kParts;
+    // + producer + MMA issuer; where segments are summed in registers (P == 2) two warps more make three whole warpgroups, whose
+    // 168 registers a thread are dealt again: 216 to the two that take accumulators apart, 72 to the third (3 x 168 in all).
+    static constexpr int kThreads = 32 * (kWarps + (P == 2 ? 4 : 2));
     static constexpr bool kWritesG = MODE == kXentGrad || MODE == kXentGradOne;
     static constexpr int kTileA = kXentTileM * kXentTileK * 2, kTileB = BN / CG * kXentTileK * 2;
     static constexpr int kStage = P * (kTileA + kTileB);
-    static constexpr int kStaging = kWritesG ? kXentWarps * 4096 : 0;      // 32 rows x 32 columns x 2 planes or buffers a warp
-    static constexpr int kMost = 227 * 1024 - 1024 - 256 - kStaging - (MODE == kXentGradOne ? 2 * 2 * 128 * 12 : 0);
+    static constexpr int kStagingBuffer = (kParts == 4 ? 1 : 2) * 2048;    // a warp's 32 rows x 32 columns, of two planes or two in turn
+    static constexpr int kStaging = kWritesG ? kWarps * kStagingBuffer : 0;
+    static constexpr int kExchangeBytes = MODE == kXentGradOne ? 2 * kParts * 128 * 12 : 0;   // one-pass mode: [2 turns][parts][128 rows]
+    static constexpr int kMost = 227 * 1024 - 1024 - 256 - kStaging - kExchangeBytes;
     static constexpr int S = kMost / kStage < 8 ? kMost / kStage : 8;
     static constexpr int kTmemCols = 2 * BN;
     static constexpr int kStagingAt = S * kStage;
-    static constexpr int kExchange = kStagingAt + kStaging;                // one-pass mode: [2 turns][2 halves][128 rows] x 12 bytes
-    static constexpr int kExchangeBytes = MODE == kXentGradOne ? 2 * 2 * 128 * 12 : 0;
+    static constexpr int kExchange = kStagingAt + kStaging;
     static constexpr int kBars = kExchange + kExchangeBytes;
     static constexpr int kNumBars = 2 * S + 4 + 1 + 4;
     static constexpr int kTmemSlot = kBars + kNumBars * 8;
@@ -232,7 +235,7 @@ __device__ __forceinline__ void online_softmax(const float (&v)[32], float f, fl
 }
 
 template <int BN, int P, int MODE, int CG>
-__global__ void __launch_bounds__(xent_threads(P), 1)
+__global__ void __launch_bounds__((XentLayout<BN, P, MODE, CG>::kThreads), 1)
 xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const __grid_constant__ CUtensorMap map_g) {
     using L = XentLayout<BN, P, MODE, CG>;
@@ -265,13 +268,13 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(accf_bar(b), 1);
-            mbar_init(acce_bar(b), CG * kXentWarps);
+            mbar_init(acce_bar(b), CG * L::kWarps);
         }
-        for (int q = 0; q < 4; q++) mbar_init(exchange_bar(q), 2);
+        for (int q = 0; q < 4; q++) mbar_init(exchange_bar(q), L::kParts);
         mbar_init(drain_bar, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kXentWarps + 1) {
+    if (warp == L::kWarps + 1) {
         if constexpr (CG == 1) {
             asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::kTmemSlot), "r"(L::kTmemCols) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -321,9 +324,9 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
         return t;
     };
 
-    if (warp >= kXentWarps) {
+    if (warp >= L::kWarps) {
         if constexpr (P == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == kXentWarps) {
+        if (warp == L::kWarps) {
             // ------------------------------ producer -----------------------------------------------------------------------
             if (lane == 0) {
                 int s = 0;
@@ -361,7 +364,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 }
             }
             __syncwarp();
-        } else if (warp == kXentWarps + 1) {
+        } else if (warp == L::kWarps + 1) {
             // ------------------------------ MMA issuer, of the pair's first block ----------------------------------------------
             // The whole warp goes through the loop and one elected lane issues, so that descriptors live in uniform registers:
             // from within a branch of one lane, four MMAs of 512 clocks took 790 to issue.
@@ -431,16 +434,16 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
     } else {
         // ------------------------------ epilogue -----------------------------------------------------------------------
         if constexpr (P == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-        constexpr int kHalf = BN / 2;
-        constexpr int kChunks = kHalf / 32, kUnroll = P == 2 ? kChunks : 1;
-        const int quarter = warp & 3, half = warp >> 2;
+        constexpr int kWidth = BN / L::kParts;             // columns of a warp
+        constexpr int kChunks = kWidth / 32, kUnroll = P == 2 ? kChunks : 1;
+        const int quarter = warp & 3, part = warp >> 2;
         uint32_t acc_it = 0;
         bool ok = true;
         const bool half_type = p.half_type != 0;
-        [[maybe_unused]] const uint32_t staging = base + L::kStagingAt + warp * 4096;
+        [[maybe_unused]] const uint32_t staging = base + L::kStagingAt + warp * L::kStagingBuffer;
         [[maybe_unused]] uint32_t stage_it = 0;
         uint32_t acc = 0;                                // the tile's accumulator in tensor memory (P == 1)
-        [[maybe_unused]] float total[P == 2 ? kHalf : 1];   // or its sum so far
+        [[maybe_unused]] float total[P == 2 ? kWidth : 1];   // or its sum so far
         auto release = [&]() {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -451,7 +454,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             const uint32_t buf = acc_it & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(accf_bar(buf), (acc_it >> 1) & 1, abort_flag))) return false;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            acc = tmem_base + ((uint32_t)(32 * quarter) << 16) + buf * BN + half * kHalf;
+            acc = tmem_base + ((uint32_t)(32 * quarter) << 16) + buf * BN + part * kWidth;
             return true;
         };
         // The tile's columns of this warp: left in tensor memory, or summed up from its segments.
@@ -461,7 +464,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 if (!next_accumulator()) return false;
                 if (k == k0) {
 #pragma unroll
-                    for (int j = 0; j < (P == 2 ? kHalf : 0); j++) total[j] = 0.f;
+                    for (int j = 0; j < (P == 2 ? kWidth : 0); j++) total[j] = 0.f;
                 }
 #pragma unroll
                 for (int c = 0; c < 2 * kChunks; c++) {
@@ -493,14 +496,15 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
         [[maybe_unused]] auto write_g = [&](const float (&g)[32], int row0, int col) {
             if constexpr (L::kWritesG) {
                 if (row0 >= p.rows_pad) return;            // a pair's second tile may lie behind the last row
-                // P == 1: two buffers in turn, so the older copy may still be read; P == 2: both planes at once
+                // two buffers in turn: the older copy may still be read; one buffer, or both for the two planes: none may
+                constexpr bool kTwo = P == 1 && L::kStagingBuffer == 4096;
                 if (lane == 0) {
-                    if constexpr (P == 1) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                    if constexpr (kTwo) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
                     else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 }
                 __syncwarp();
                 const uint32_t row = staging + lane * 64, x = (lane >> 1) & 3;
-                const uint32_t first = P == 1 ? (stage_it & 1) * 2048 : 0;
+                const uint32_t first = kTwo ? (stage_it & 1) * 2048 : 0;
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     uint32_t h[4], l[4];
@@ -572,13 +576,23 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             }
         };
         const float f = kLogits ? logit_factor(p.range) : 0.f;
-        [[maybe_unused]] const float unit = P == 2 ? (float)(1 << kGradExponent) : 1.f;
-        // exp(logit) over the row's sum, less 1 at its label; 0 outside the rows and classes
-        [[maybe_unused]] auto gradient = [&](float (&v)[32], int col, int classes, bool live, int y, float lse2) {
+        // exp(logit) over the row's sum, less 1 at its label; 0 outside the classes and, where lse2 is infinite, the rows
+        [[maybe_unused]] auto gradient = [&](float (&v)[32], int col, int classes, int y, float lse2) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-                const float e = fast_exp2(fmaf(v[j], f, -lse2));
-                v[j] = !live || col + j >= classes ? 0.f : unit * (y == col + j ? e - 1.f : e);
+            for (int j = 0; j < 32; j++) v[j] = fast_exp2(fmaf(v[j], f, -lse2));
+            if (col + 32 > classes) {
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                    if (col + j >= classes) v[j] = 0.f;
+            }
+            if (__any_sync(0xffffffffu, (uint32_t)(y - col) < 32u)) {
+#pragma unroll
+                for (int j = 0; j < 32; j++)
+                    if (y - col == j && y < classes) v[j] -= 1.f;
+            }
+            if constexpr (P == 2) {
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] *= (float)(1 << kGradExponent);
             }
         };
         for (int64_t i = group; i < items && ok; i += groups) {
@@ -592,7 +606,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     if (!acquire(t.k0, t.k1)) { ok = false; break; }
 #pragma unroll(kUnroll)
                     for (int c = 0; c < kChunks; c++) {
-                        const int col = n * BN + half * kHalf + 32 * c;
+                        const int col = n * BN + part * kWidth + 32 * c;
                         if (col >= p.classes) break;
                         float v[32];
                         values(c, v);
@@ -611,20 +625,20 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     done();
                 }
                 if (ok && r < count) {
-                    p.stats[(int64_t)(2 * t.split + half) * p.rows_pad + r] = make_float2(top, sum);
+                    p.stats[(int64_t)(L::kParts * t.split + part) * p.rows_pad + r] = make_float2(top, sum);
                     if (have) p.label_logit[r] = picked;
                 }
             } else if constexpr (MODE == kXentGrad) {
                 const bool live = r < count;
                 const int y = live ? p.label[r] - p.v0 : -1;
-                const float lse2 = live ? p.lse2[r] : 0.f;
+                const float lse2 = live ? p.lse2[r] : INFINITY;
                 if (!acquire(t.k0, t.k1)) { ok = false; break; }
 #pragma unroll(kUnroll)
                 for (int c = 0; c < kChunks; c++) {
-                    const int col = t.n0 * BN + half * kHalf + 32 * c;     // within the piece
+                    const int col = t.n0 * BN + part * kWidth + 32 * c;     // within the piece
                     float v[32];
                     values(c, v);
-                    gradient(v, col, p.vc, live, y, lse2);
+                    gradient(v, col, p.vc, y, lse2);
                     write_g(v, r - lane, col);
                 }
                 done();
@@ -635,7 +649,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 float top = -INFINITY, sum = 0.f, picked = 0.f;
 #pragma unroll(kUnroll)
                 for (int c = 0; c < kChunks; c++) {
-                    const int col = half * kHalf + 32 * c;
+                    const int col = part * kWidth + 32 * c;
                     if (col >= p.classes) break;
                     float v[32];
                     values(c, v);
@@ -647,25 +661,29 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     for (int j = 0; j < 32; j++)
                         if (y - col == j) picked = v[j];
                 }
-                // The two warps that hold halves of the same rows tell each other.  Two turns' worth of room: a warp writes
-                // turn i + 2 after the other has arrived at turn i + 1, hence read turn i.
-                float* ex = reinterpret_cast<float*>(gbase + L::kExchange) + (turn & 1) * 2 * 128 * 3;
-                float* mine = ex + (half * 128 + 32 * quarter + lane) * 3;
-                mine[0] = top;
-                mine[1] = sum;
-                mine[2] = picked;
+                // The warps that hold parts of the same rows tell one another.  Two turns' worth of room: a warp writes turn i + 2
+                // after all others have arrived at turn i + 1, hence read turn i.
+                float* ex = reinterpret_cast<float*>(gbase + L::kExchange) + (turn & 1) * L::kParts * 128 * 3 + (32 * quarter + lane) * 3;
+                ex[part * 128 * 3] = top;
+                ex[part * 128 * 3 + 1] = sum;
+                ex[part * 128 * 3 + 2] = picked;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(exchange_bar(quarter));
                 if (!__all_sync(0xffffffffu, mbar_wait(exchange_bar(quarter), turn & 1, abort_flag))) { ok = false; break; }
                 turn++;
-                // both halves in the same order on both sides, so that both get the same bits
-                const float* a = ex + (32 * quarter + lane) * 3;
-                const float* b = a + 128 * 3;
-                const float most = fmaxf(a[0], b[0]);
+                // all parts in the same order everywhere, so that everybody gets the same bits
+                float most = ex[0], all = 0.f, at_label = 0.f;
+#pragma unroll
+                for (int i = 1; i < L::kParts; i++) most = fmaxf(most, ex[i * 128 * 3]);
                 const float bs = most == -INFINITY ? 0.f : most * f;
-                const float lse2 = bs + log2f(a[1] * fast_exp2(fmaf(a[0], f, -bs)) + b[1] * fast_exp2(fmaf(b[0], f, -bs)));
-                if (half == 0) {
-                    const float loss = live ? kLn2 * fmaf(-(a[2] + b[2]), f, lse2) : 0.f;
+#pragma unroll
+                for (int i = 0; i < L::kParts; i++) {
+                    all += ex[i * 128 * 3 + 1] * fast_exp2(fmaf(ex[i * 128 * 3], f, -bs));
+                    at_label += ex[i * 128 * 3 + 2];
+                }
+                const float lse2 = bs + log2f(all);
+                if (part == 0) {
+                    const float loss = live ? kLn2 * fmaf(-at_label, f, lse2) : 0.f;
                     if (live && p.row_loss) p.row_loss[p.row_of[r]] = loss;
                     float w = loss;
 #pragma unroll
@@ -674,10 +692,10 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 }
 #pragma unroll(kUnroll)
                 for (int c = 0; c < kChunks; c++) {
-                    const int col = half * kHalf + 32 * c;
+                    const int col = part * kWidth + 32 * c;
                     float v[32];
                     values(c, v);
-                    gradient(v, col, p.classes, live, y, lse2);
+                    gradient(v, col, p.classes, y, live ? lse2 : INFINITY);
                     write_g(v, r - lane, col);
                 }
                 done();
@@ -688,7 +706,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 const bool live = r < m_extent;
 #pragma unroll(kUnroll)
                 for (int c = 0; c < kChunks; c++) {
-                    const int col = t.n0 * BN + half * kHalf + 32 * c;
+                    const int col = t.n0 * BN + part * kWidth + 32 * c;
                     if (col >= n_extent) break;
                     float v[32];
                     if (!empty) {
@@ -721,7 +739,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
         }
         __syncthreads();
     }
-    if (warp == kXentWarps + 1) {
+    if (warp == L::kWarps + 1) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(L::kTmemCols) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(L::kTmemCols) : "memory");
