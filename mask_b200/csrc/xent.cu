@@ -144,11 +144,16 @@ __global__ void __launch_bounds__(256) xent_range_kernel(const XentPackArgs p) {
     } else {
         for (int64_t v = w0; v < p.classes; v += warps) scan(weight + v * p.w_class_stride, p.dim, p.w_dim_stride, most[1]);
     }
+    __shared__ uint32_t room[2];
+    if (threadIdx.x < 2) room[threadIdx.x] = 0;
+    __syncthreads();
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         const uint32_t m = __reduce_max_sync(0xffffffffu, most[k]);
-        if (lane == 0 && m) atomicMax(p.range + k, m);
+        if (lane == 0 && m) atomicMax(room + k, m);
     }
+    __syncthreads();
+    if (threadIdx.x < 2 && room[threadIdx.x]) atomicMax(p.range + threadIdx.x, room[threadIdx.x]);
 }
 
 // hi and lo of a scaled float; an infinite or NaN hi has no lo
@@ -215,12 +220,21 @@ __global__ void __launch_bounds__(kXentPackThreads) xent_pack_kernel(const XentP
         pack_row<kFloat>(src, 1, p.dim, p.dim_pad, p.h_planes + i * p.dim_pad, p.h_plane, h_scale, lane);
     }
     if (p.dhidden && count < p.rows) {
-        for (int64_t r = w0; r < p.rows; r += warps) {
-            if (labelled(p.labels[r], p.classes)) continue;
-            char* to = static_cast<char*>(p.dhidden) + r * p.dhidden_stride * kBytes;
-            for (int d = lane; d < p.dim; d += 32) {
-                if constexpr (kFloat) reinterpret_cast<float*>(to)[d] = 0.f;
-                else reinterpret_cast<uint16_t*>(to)[d] = 0;
+        // a warp looks at 32 labels and then clears the rows without one
+        const bool vec = (reinterpret_cast<uintptr_t>(p.dhidden) & 15) == 0 && p.dhidden_stride * kBytes % 16 == 0 && p.dim * kBytes % 16 == 0;
+        for (int64_t r0 = 32 * w0; r0 < p.rows; r0 += 32 * warps) {
+            const int64_t r = r0 + lane;
+            unsigned clear = __ballot_sync(0xffffffffu, r < p.rows && !labelled(p.labels[min(r, p.rows - 1)], p.classes));
+            for (; clear; clear &= clear - 1) {
+                char* to = static_cast<char*>(p.dhidden) + (r0 + __ffs(clear) - 1) * p.dhidden_stride * kBytes;
+                if (vec) {
+                    for (int d = 16 * lane; d < p.dim * kBytes; d += 512) *reinterpret_cast<uint4*>(to + d) = make_uint4(0u, 0u, 0u, 0u);
+                } else {
+                    for (int d = lane; d < p.dim; d += 32) {
+                        if constexpr (kFloat) reinterpret_cast<float*>(to)[d] = 0.f;
+                        else reinterpret_cast<uint16_t*>(to)[d] = 0;
+                    }
+                }
             }
         }
     }
@@ -306,12 +320,13 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const XentArgs p, int p
     }
 }
 
-// Parts of a product summed in their order, scaled and written where the caller wants them: 4 values a thread, neighbouring
-// threads along the axis that is contiguous in the output.
+// Parts of a product summed up, scaled and written where the caller wants them.  A block takes 256 / shares vectors of four
+// values, neighbouring threads along the axis that is contiguous in the output, and `shares` threads a vector (many parts of
+// a small product), whose sums are added in their order.
 struct XentReduceArgs {
     const float* part;
     int64_t part_rows;
-    int32_t part_ld, splits;
+    int32_t part_ld, splits, shares;
     int32_t m, n;
     const int32_t* count;      // labelled rows (for the scale)
     int32_t m_is_count;        // as many rows as are labelled, each to row_of[m]
@@ -331,13 +346,32 @@ __global__ void __launch_bounds__(256) xent_reduce_kernel(const XentReduceArgs p
     const int64_t m_end = p.m_is_count ? count : p.m, n_vec = (p.n + 3) / 4;
     const ProductScale scale = product_scale(p.scale, p.mean, count, p.range, p.operand);
     const bool m_fast = p.out_m == 1 && p.out_n != 1;
-    for (int64_t i = grid_thread(); i < m_end * n_vec; i += (int64_t)gridDim.x * blockDim.x) {
+    __shared__ float4 room[256];
+    const int per_block = 256 / p.shares, share = threadIdx.x / per_block;
+    const int64_t most = m_end * n_vec;
+    for (int64_t i0 = (int64_t)blockIdx.x * per_block; i0 < most; i0 += (int64_t)gridDim.x * per_block) {
+        const int64_t i = i0 + threadIdx.x % per_block;
         const int64_t m = m_fast ? i % m_end : i / n_vec, n = 4 * (m_fast ? i / m_end : i % n_vec);
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < p.splits; s++) {
-            const float4 v = *reinterpret_cast<const float4*>(p.part + (s * p.part_rows + m) * p.part_ld + n);
-            a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+        if (i < most) {
+#pragma unroll 4
+            for (int s = share; s < p.splits; s += p.shares) {
+                const float4 v = *reinterpret_cast<const float4*>(p.part + (s * p.part_rows + m) * p.part_ld + n);
+                a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+            }
         }
+        if (p.shares > 1) {
+            __syncthreads();
+            room[threadIdx.x] = a;
+            __syncthreads();
+            if (share == 0) {
+                for (int s = 1; s < p.shares; s++) {
+                    const float4 v = room[s * per_block + threadIdx.x];
+                    a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+                }
+            }
+        }
+        if (share > 0 || i >= most) continue;
         const float v[4] = {scale(a.x), scale(a.y), scale(a.z), scale(a.w)};
         const int64_t at = (p.m_is_count ? (int64_t)p.row_of[m] : p.m0 + m) * p.out_m + n * p.out_n;
 #pragma unroll
@@ -395,14 +429,16 @@ struct XentPlan {
     size_t counts, row_of, label, total, stats, label_logit, lse2, warp_loss, h_planes, w_planes, g, part_dh, part_dw, bytes;
 };
 
-// `rows`: of the product.  Returns the blocks that share a tile of `bn` columns.
-static int tile_blocks(int bn, int64_t rows) { return bn == 256 && rows > kXentTileM ? 2 : 1; }
+// Blocks that share a tile of `bn` columns of a product with so many rows.  Pairs load a third less (dH of 16384 x 16384 x 512:
+// 171 us instead of 195), but wait for one another's epilogue: logits, whose epilogue takes as long as contracting 500
+// (16384 x 256 x 16384: 110 and 139 us a block alone, 144 and 182 in pairs; over 512 they take the same), are left to pairs only
+// where more than that is contracted.
+static int tile_blocks(int bn, int64_t rows, int contracted = 1 << 30) { return bn == 256 && rows > kXentTileM && contracted > 512 ? 2 : 1; }
 
 // Parts to cut each tile's `units` of work into (tiles: those of `rows` rows, `others` of them side by side), so that they
 // fill the SMs: the fewest rounds of the longest part, `rounds` at most.  A part costs two units beside its own (the
 // accumulator's way out).
-static int best_splits(int64_t rows, int bn, int64_t others, int64_t units, int rounds) {
-    const int cg = tile_blocks(bn, rows);
+static int best_splits(int64_t rows, int cg, int64_t others, int64_t units, int rounds) {
     const int64_t sms = sm_count() / cg, tiles = (rows + cg * kXentTileM - 1) / (cg * kXentTileM) * others;
     int64_t best = 1, best_cost = INT64_MAX;
     const int64_t most = std::min<int64_t>(units, std::max<int64_t>(1, rounds * sms / std::max<int64_t>(tiles, 1)));
@@ -432,7 +468,7 @@ static XentPlan plan_xent(const mask_head& h) {
     p.bn_dim = tile_width(h.dim);
     // one tile of all classes: 256 columns, with two planes of G in shared memory 128
     p.one_pass = p.grads && h.classes <= (p.planes == 2 ? 128 : 256);
-    p.stats_splits = p.one_pass ? 1 : best_splits(p.rows_pad, p.bn_logits, 1, (h.classes + p.bn_logits - 1) / p.bn_logits, 16);
+    p.stats_splits = p.one_pass ? 1 : best_splits(p.rows_pad, tile_blocks(p.bn_logits, p.rows_pad, h.dim), 1, (h.classes + p.bn_logits - 1) / p.bn_logits, 16);
     p.stats_parts = p.stats_splits * (p.planes == 1 && p.bn_logits >= 128 ? XentLayout<256, 1, kXentStats, 1>::kParts : XentLayout<64, 1, kXentStats, 1>::kParts);
     if (p.grads) {
         if (p.one_pass) {
@@ -446,12 +482,12 @@ static XentPlan plan_xent(const mask_head& h) {
         const int64_t n_tiles = (h.dim + p.bn_dim - 1) / p.bn_dim;
         p.part_ld = (int)(n_tiles * p.bn_dim);
         if (h.d_dhidden) {
-            p.dh_splits = best_splits(p.rows_pad, p.bn_dim, n_tiles, (p.piece + kXentTileK - 1) / kXentTileK, 4);
+            p.dh_splits = best_splits(p.rows_pad, tile_blocks(p.bn_dim, p.rows_pad), n_tiles, (p.piece + kXentTileK - 1) / kXentTileK, 4);
             p.dh_parts = p.dh_splits > 1 || p.n_pieces > 1;
             p.part_dh_rows = p.rows_pad;
         }
         if (h.d_dweight) {
-            p.dw_splits = best_splits(p.piece, p.bn_dim, n_tiles, (p.rows_pad + kXentTileK - 1) / kXentTileK, 4);
+            p.dw_splits = best_splits(p.piece, tile_blocks(p.bn_dim, p.piece), n_tiles, (p.rows_pad + kXentTileK - 1) / kXentTileK, 4);
             p.dw_parts = p.dw_splits > 1;
             p.part_dw_rows = round_up(p.piece, kXentTileM);
         }
@@ -523,9 +559,19 @@ static int launch_xent_gemm_planes(int bn, int cg, const XentArgs& a, const CUte
 template <int MODE>
 static int launch_xent_gemm(int bn, int planes, const XentArgs& a, int64_t rows, int64_t parts, const CUtensorMap& ma, const CUtensorMap& mb,
                             const CUtensorMap& mg, cudaStream_t st) {
-    const int cg = tile_blocks(bn, rows);
+    const int cg = MODE <= kXentGradOne ? tile_blocks(bn, rows, a.dim) : tile_blocks(bn, rows);
     const int64_t items = (rows + cg * kXentTileM - 1) / (cg * kXentTileM) * parts;
     return planes == 1 ? launch_xent_gemm_planes<MODE, 1>(bn, cg, a, ma, mb, mg, items, st) : launch_xent_gemm_planes<MODE, 2>(bn, cg, a, ma, mb, mg, items, st);
+}
+
+// `rows`: of the product, at most.
+static int launch_xent_reduce(XentReduceArgs r, int64_t rows, cudaStream_t st) {
+    const int64_t vectors = rows * ((r.n + 3) / 4);
+    // 16 parts or more and not enough vectors for two blocks an SM: up to 32 threads a vector
+    r.shares = 1;
+    while (r.shares < 32 && 8 * r.shares < r.splits && vectors * r.shares < 512 * (int64_t)sm_count()) r.shares *= 2;
+    const int64_t blocks = (vectors * r.shares + 255) / 256;
+    return launch_overlapped(xent_reduce_kernel, dim3((unsigned)std::min<int64_t>(blocks, 8 * (int64_t)sm_count())), 256, 0, st, r);
 }
 
 static const char* refuse_head(const mask_head* h) {
@@ -593,7 +639,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
     const int w_cols = plan.pack_weight ? plan.dim_pad : h.dim;
     CUtensorMap h_k, w_k, none = {};     // K-major, contracted over dim
     if ((rc = plane_map(&h_k, pk.h_planes, plan.dim_pad, rp, P, plan.dim_pad, pk.h_plane, 64, kXentTileM))) return rc;
-    if ((rc = plane_map(&w_k, w_data, w_cols, h.classes, P, w_ld, w_plane, 64, plan.bn_logits / tile_blocks(plan.bn_logits, rp)))) return rc;
+    if ((rc = plane_map(&w_k, w_data, w_cols, h.classes, P, w_ld, w_plane, 64, plan.bn_logits / tile_blocks(plan.bn_logits, rp, h.dim)))) return rc;
 
     XentArgs a = {};
     a.count = total; a.status = total + 1;
@@ -616,16 +662,16 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
         char* g = at(plan.g);
         const int64_t g_plane = rp * plan.g_ld;
         CUtensorMap g_st, g_k, g_mn, w_mn, h_mn;
-        if ((rc = plane_map(&g_st, g, plan.g_ld, rp, P, plan.g_ld, g_plane, 32, 32))) return rc;
+        if ((rc = plane_map(&g_st, g, plan.g_ld, rp, P, plan.g_ld, g_plane, P == 1 && plan.bn_logits == 256 ? XentLayout<256, 1, kXentGrad, 1>::kBox : 32, 32))) return rc;
         if ((rc = plane_map(&g_k, g, plan.g_ld, rp, P, plan.g_ld, g_plane, 64, kXentTileM))) return rc;
         if ((rc = plane_map(&g_mn, g, plan.g_ld, rp, P, plan.g_ld, g_plane, 64, 64))) return rc;
         if ((rc = plane_map(&w_mn, w_data, w_cols, h.classes, P, w_ld, w_plane, 64, 64))) return rc;
         if ((rc = plane_map(&h_mn, pk.h_planes, plan.dim_pad, rp, P, plan.dim_pad, pk.h_plane, 64, 64))) return rc;
         const int64_t n_tiles = plan.part_ld / plan.bn_dim;
-        const unsigned most_blocks = (unsigned)(8 * sm_count());
         XentReduceArgs r = {};
         r.part_ld = plan.part_ld; r.n = h.dim; r.count = total; r.row_of = row_of; r.out_type = h.dtype; r.scale = a.scale; r.mean = a.mean; r.range = a.range;
-        const uintptr_t vec = h.dtype == MASK_F32 ? 4 : 8;      // elements of 16 bytes
+        const int64_t vec = 8;      // elements of a vector: 32 bytes of FP32, 16 of the others
+        const uintptr_t aligned = h.dtype == MASK_F32 ? 31 : 15;
         for (int piece = 0; piece < plan.n_pieces; piece++) {
             a.v0 = piece * plan.piece;
             a.vc = std::min(plan.piece, h.classes - a.v0);
@@ -639,7 +685,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
                 b.store = !plan.dh_parts ? kXentFinal : (piece == 0 ? kXentPartial : kXentAccumulate);
                 b.part = reinterpret_cast<float*>(at(plan.part_dh)); b.part_rows = plan.part_dh_rows; b.part_ld = plan.part_ld;
                 b.out = h.d_dhidden; b.out_m = h.dhidden_stride; b.out_n = 1;
-                b.out_vec = h.dhidden_stride % (int64_t)vec == 0 && (reinterpret_cast<uintptr_t>(h.d_dhidden) & 15) == 0;
+                b.out_vec = h.dhidden_stride % vec == 0 && (reinterpret_cast<uintptr_t>(h.d_dhidden) & aligned) == 0;
                 if ((rc = launch_xent_gemm<kXentDHidden>(plan.bn_dim, P, b, rp, n_tiles * b.splits, g_k, w_mn, none, st))) return rc;
             }
             if (h.d_dweight) {
@@ -648,14 +694,13 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
                 b.store = plan.dw_parts ? kXentPartial : kXentFinal;
                 b.part = reinterpret_cast<float*>(at(plan.part_dw)); b.part_rows = plan.part_dw_rows; b.part_ld = plan.part_ld;
                 b.out = h.d_dweight; b.out_m = h.dweight_class_stride; b.out_n = h.dweight_dim_stride;
-                b.out_vec = b.out_n == 1 && b.out_m % (int64_t)vec == 0 && (reinterpret_cast<uintptr_t>(h.d_dweight) & 15) == 0;
+                b.out_vec = b.out_n == 1 && b.out_m % vec == 0 && (reinterpret_cast<uintptr_t>(h.d_dweight) & aligned) == 0;
                 if ((rc = launch_xent_gemm<kXentDWeight>(plan.bn_dim, P, b, a.vc, n_tiles * b.splits, g_mn, h_mn, none, st))) return rc;
                 if (plan.dw_parts) {
                     XentReduceArgs w = r;
                     w.part = b.part; w.part_rows = b.part_rows; w.splits = b.splits; w.m = a.vc; w.m0 = a.v0;
                     w.out = b.out; w.out_m = b.out_m; w.out_n = b.out_n;
-                    const int64_t n = (int64_t)w.m * ((w.n + 3) / 4);
-                    if ((rc = launch_overlapped(xent_reduce_kernel, dim3(std::min(blocks_for(n, 256), most_blocks)), 256, 0, st, w))) return rc;
+                    if ((rc = launch_xent_reduce(w, w.m, st))) return rc;
                 }
             }
         }
@@ -663,8 +708,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
             r.part = reinterpret_cast<float*>(at(plan.part_dh)); r.part_rows = plan.part_dh_rows; r.splits = plan.dh_splits;
             r.m_is_count = 1; r.operand = 1;
             r.out = h.d_dhidden; r.out_m = h.dhidden_stride; r.out_n = 1;
-            const int64_t n = rp * ((r.n + 3) / 4);
-            if ((rc = launch_overlapped(xent_reduce_kernel, dim3((unsigned)std::min<int64_t>((n + 255) / 256, most_blocks)), 256, 0, st, r))) return rc;
+            if ((rc = launch_xent_reduce(r, rp, st))) return rc;
         }
     }
     if ((rc = launch_overlapped(xent_loss_kernel, dim3(1), 1024, 0, st, total, a.warp_loss, total + 1, h.d_loss, h.rows, h.reduction))) return rc;

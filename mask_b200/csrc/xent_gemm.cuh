@@ -57,7 +57,7 @@ struct XentArgs {
     void* out;                 // final store: element (m, n) at m * out_m + n * out_n
     int64_t out_m, out_n;
     int32_t out_type;          // MASK_F32 / MASK_BF16 / MASK_F16
-    int32_t out_vec;           // rows of 32 values may be written as 16-byte vectors
+    int32_t out_vec;           // rows of 32 values may be written as 32-byte (FP32) or 16-byte vectors
     float scale;
     int32_t mean;              // scale / count
     const uint32_t* range;     // bits of the largest finite magnitudes of hidden and weight, or NULL: planes are the operands themselves
@@ -107,7 +107,10 @@ struct XentLayout {
     static constexpr bool kWritesG = MODE == kXentGrad || MODE == kXentGradOne;
     static constexpr int kTileA = kXentTileM * kXentTileK * 2, kTileB = BN / CG * kXentTileK * 2;
     static constexpr int kStage = P * (kTileA + kTileB);
-    static constexpr int kStagingBuffer = (kParts == 4 ? 1 : 2) * 2048;    // a warp's 32 rows x 32 columns, of two planes or two in turn
+    // G leaves through a warp's staging buffer of 4 KB: 32 rows of 64 columns where the warp has as many, else of 32, for both
+    // planes or two in turn.
+    static constexpr int kBox = P == 1 && BN / kParts >= 64 ? 64 : 32;
+    static constexpr int kStagingBuffer = 4096;
     static constexpr int kStaging = kWritesG ? kWarps * kStagingBuffer : 0;
     static constexpr int kExchangeBytes = MODE == kXentGradOne ? 2 * kParts * 128 * 12 : 0;   // one-pass mode: [2 turns][parts][128 rows]
     static constexpr int kMost = 227 * 1024 - 1024 - 256 - kStaging - kExchangeBytes;
@@ -211,6 +214,12 @@ __device__ __forceinline__ void st_shared_v4(uint32_t at, uint32_t a, uint32_t b
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// A whole 32-byte sector by one thread: pieces of 16 bytes of 32 different rows cost the L2 twice the requests.
+__device__ __forceinline__ void st_global_v8(float* at, const float* v) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(at), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                 : "memory");
+}
 __device__ __forceinline__ uint32_t pack_half2(float a, float b, bool half_type) {
     if (half_type) {
         const __half2 h = __floats2half2_rn(a, b);
@@ -492,42 +501,47 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 for (int j = 0; j < 32; j++) v[j] = total[32 * c + j];
             }
         };
-        // G of 32 columns to global memory through this warp's staging buffer
-        [[maybe_unused]] auto write_g = [&](const float (&g)[32], int row0, int col) {
+        // G of the warp's 32 columns number c to global memory, through its staging buffer
+        [[maybe_unused]] auto write_g = [&](const float (&g)[32], int row0, int col, int c) {
             if constexpr (L::kWritesG) {
                 if (row0 >= p.rows_pad) return;            // a pair's second tile may lie behind the last row
-                // two buffers in turn: the older copy may still be read; one buffer, or both for the two planes: none may
-                constexpr bool kTwo = P == 1 && L::kStagingBuffer == 4096;
-                if (lane == 0) {
-                    if constexpr (kTwo) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-                    else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                constexpr bool kWide = L::kBox == 64;
+                const bool begins = !kWide || (c & 1) == 0, ends = !kWide || (c & 1) == 1;
+                // what the buffer held must have been read, but for the other one of two in turn
+                if (begins) {
+                    if (lane == 0) {
+                        if constexpr (P == 1 && !kWide) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                        else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
-                const uint32_t row = staging + lane * 64, x = (lane >> 1) & 3;
-                const uint32_t first = kTwo ? (stage_it & 1) * 2048 : 0;
+                const uint32_t row = staging + lane * (kWide ? 128 : 64), x = kWide ? lane & 7 : (lane >> 1) & 3;
+                const uint32_t first = P == 1 && !kWide ? (stage_it & 1) * 2048 : 0, chunk0 = kWide ? (c & 1) * 4 : 0;
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
+                for (uint32_t i = 0; i < 4; i++) {
                     uint32_t h[4], l[4];
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const float u = g[8 * c + 2 * j], w = g[8 * c + 2 * j + 1];
+                        const float u = g[8 * i + 2 * j], w = g[8 * i + 2 * j + 1];
                         h[j] = pack_half2(u, w, half_type);
                         if constexpr (P == 2) {
                             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
                             l[j] = pack_half2(u - f.x, w - f.y, true);
                         }
                     }
-                    st_shared_v4(row + first + ((c ^ x) << 4), h[0], h[1], h[2], h[3]);
-                    if constexpr (P == 2) st_shared_v4(row + 2048 + ((c ^ x) << 4), l[0], l[1], l[2], l[3]);
+                    st_shared_v4(row + first + (((chunk0 + i) ^ x) << 4), h[0], h[1], h[2], h[3]);
+                    if constexpr (P == 2) st_shared_v4(row + 2048 + ((i ^ x) << 4), l[0], l[1], l[2], l[3]);
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
+                if (ends) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
 #pragma unroll
-                    for (int z = 0; z < P; z++) tma_store_3d(&map_g, staging + first + z * 2048, col, row0, z);
-                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                        for (int z = 0; z < P; z++) tma_store_3d(&map_g, staging + first + z * 2048, kWide ? col - 32 : col, row0, z);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                    stage_it++;
                 }
-                stage_it++;
             }
         };
 
@@ -535,15 +549,19 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
         // 32 values of row r of a product, from column col, to the parts or to the caller
         [[maybe_unused]] auto write_out = [&](const float (&v)[32], const ProductScale& scale, int split, int r, int col) {
             if (p.store != kXentFinal) {
-                float4* to = reinterpret_cast<float4*>(p.part + ((int64_t)split * p.part_rows + r) * p.part_ld + col);
+                float* to = p.part + ((int64_t)split * p.part_rows + r) * p.part_ld + col;
+                if (p.store == kXentAccumulate) {
+                    float sum[32];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    float4 x = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-                    if (p.store == kXentAccumulate) {
-                        const float4 w = to[j];
-                        x.x += w.x; x.y += w.y; x.z += w.z; x.w += w.w;
+                    for (int j = 0; j < 8; j++) {
+                        const float4 w = reinterpret_cast<const float4*>(to)[j];
+                        sum[4 * j] = v[4 * j] + w.x; sum[4 * j + 1] = v[4 * j + 1] + w.y; sum[4 * j + 2] = v[4 * j + 2] + w.z; sum[4 * j + 3] = v[4 * j + 3] + w.w;
                     }
-                    to[j] = x;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) st_global_v8(to + 8 * j, sum + 8 * j);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) st_global_v8(to + 8 * j, v + 8 * j);
                 }
                 return;
             }
@@ -551,9 +569,14 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             const int64_t at = row * p.out_m + (int64_t)col * p.out_n;
             if (p.out_vec && col + 32 <= n_extent) {
                 if (p.out_type == MASK_F32) {
-                    float4* to = reinterpret_cast<float4*>(static_cast<float*>(p.out) + at);
+                    float* to = static_cast<float*>(p.out) + at;
 #pragma unroll
-                    for (int j = 0; j < 8; j++) to[j] = make_float4(scale(v[4 * j]), scale(v[4 * j + 1]), scale(v[4 * j + 2]), scale(v[4 * j + 3]));
+                    for (int j = 0; j < 4; j++) {
+                        float x[8];
+#pragma unroll
+                        for (int i = 0; i < 8; i++) x[i] = scale(v[8 * j + i]);
+                        st_global_v8(to + 8 * j, x);
+                    }
                 } else {
                     uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
 #pragma unroll
@@ -639,7 +662,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     float v[32];
                     values(c, v);
                     gradient(v, col, p.vc, y, lse2);
-                    write_g(v, r - lane, col);
+                    write_g(v, r - lane, col, c);
                 }
                 done();
             } else if constexpr (MODE == kXentGradOne) {
@@ -696,7 +719,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     float v[32];
                     values(c, v);
                     gradient(v, col, p.classes, y, live ? lse2 : INFINITY);
-                    write_g(v, r - lane, col);
+                    write_g(v, r - lane, col, c);
                 }
                 done();
             } else {
