@@ -419,7 +419,7 @@ int mask_spmm_srbcrs_static_scratch(const mask_plan* plan, const int32_t* d_val_
  *
  * Scratch: mask_linear_xent_scratch_bytes(head) bytes, 256-byte aligned, one call at a time (two captured graphs
  * that may run at once need two).  Asynchronous on `stream`.  Should a kernel give up on one of its bounded
- * waits, every loss is NaN.
+ * waits, the losses (of the labelled rows, where they are all that is asked for) are NaN.
  * ------------------------------------------------------------------------------------------ */
 typedef enum mask_dtype { MASK_F32 = 0, MASK_BF16 = 1, MASK_F16 = 2 } mask_dtype;
 typedef enum mask_reduction { MASK_REDUCE_NONE = 0, MASK_REDUCE_MEAN = 1, MASK_REDUCE_SUM = 2 } mask_reduction;
@@ -428,7 +428,7 @@ typedef struct mask_head {
     int32_t dtype;              /* mask_dtype of hidden, weight and their gradients */
     int32_t reduction;          /* mask_reduction */
     int64_t rows;               /* < 2^31 - 256 */
-    int32_t dim, classes;       /* 1 or more, < 2^31 - 256 */
+    int32_t dim, classes;       /* dim 1 to 2^20, classes 1 or more and < 2^31 - 256 */
     const void* d_hidden;       /* [rows, dim], rows hidden_stride elements apart */
     int64_t hidden_stride;
     const void* d_weight;       /* element (d, v) at d * weight_dim_stride + v * weight_class_stride */

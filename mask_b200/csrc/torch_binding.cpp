@@ -155,8 +155,8 @@ PyObject* linear_xent_checked(PyObject* const* args, Py_ssize_t n_args) {
     if (rows > 1 && labels->stride(0) != 1) return raise("labels must be contiguous");
     if (dim > 1 && hidden->stride(1) != 1) return raise("rows of hidden must be contiguous");
     constexpr int64_t most = ((int64_t)1 << 31) - 256;
-    if (dim < 1 || classes < 1 || rows >= most || dim >= most || classes >= most)
-        return raise("hidden and weight must have at least one column and fewer than 2^31 - 256 rows and columns");
+    if (dim < 1 || classes < 1 || dim > (1 << 20) || rows >= most || classes >= most)
+        return raise("hidden must have 1 to 2^20 columns, weight at least one, both fewer than 2^31 - 256 rows and columns");
     h.reduction = (int32_t)PyLong_AsLong(args[3]);
     h.grad_scale = (float)PyFloat_AsDouble(args[4]);
     const bool grads = PyObject_IsTrue(args[5]) == 1;

@@ -20,6 +20,9 @@
 namespace mask {
 
 constexpr int kXentCountThreads = 1024;
+// Rows and values (of hidden and of a weight that has to be packed) up to which one block prepares them: 2708 x 16 x 7 takes
+// it about 7 us, the four kernels 12.
+constexpr int64_t kXentSmallRows = 4096, kXentSmallValues = 65536;
 constexpr size_t kXentPieceBytes = (size_t)512 << 20;   // what a piece of G may take
 
 // ---- numbering of the labelled rows ------------------------------------------------------------------
@@ -43,28 +46,35 @@ __global__ void __launch_bounds__(kXentCountThreads) xent_count_kernel(const int
     }
 }
 
-// Writes row_of and label of the chunk's labelled rows behind those of the chunks before it; the last block leaves the
+struct XentNumberArgs {
+    const int64_t* labels;
+    int64_t rows, chunk;
+    int32_t classes;
+    const int32_t* counts;
+    int32_t* row_of;
+    int32_t* label;
+    int32_t* total;
+    int32_t* status;
+    uint32_t* range;
+    float* row_loss;
+};
+
+// Writes row_of and label of the block's chunk of rows behind those of the chunks before it; the last block leaves the
 // total.  Losses of rows without a label are set to 0 here.
-__global__ void __launch_bounds__(kXentCountThreads) xent_number_kernel(const int64_t* __restrict__ labels, int64_t rows, int32_t classes, int64_t chunk,
-                                                                        const int32_t* __restrict__ counts, int32_t* __restrict__ row_of,
-                                                                        int32_t* __restrict__ label, int32_t* __restrict__ total,
-                                                                        int32_t* __restrict__ status, uint32_t* __restrict__ range,
-                                                                        float* __restrict__ row_loss) {
-    wait_for_previous_kernel();
-    let_next_kernel_start();
+__device__ __forceinline__ void number_rows(const XentNumberArgs& p) {
     __shared__ int sums[32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int at = 0;
-    for (int b = threadIdx.x; b < (int)blockIdx.x; b += kXentCountThreads) at += counts[b];
+    for (int b = threadIdx.x; b < (int)blockIdx.x; b += kXentCountThreads) at += p.counts[b];
     at = __reduce_add_sync(0xffffffffu, at);
     if (lane == 0) sums[warp] = at;
     __syncthreads();
     at = __reduce_add_sync(0xffffffffu, sums[lane]);
-    const int64_t r0 = blockIdx.x * chunk, r1 = min(rows, r0 + chunk);
+    const int64_t r0 = blockIdx.x * p.chunk, r1 = min(p.rows, r0 + p.chunk);
     for (int64_t rb = r0; rb < r1; rb += kXentCountThreads) {
         const int64_t r = rb + threadIdx.x;
-        const int64_t y = r < r1 ? labels[r] : -1;
-        const bool mine = labelled(y, classes);
+        const int64_t y = r < r1 ? p.labels[r] : -1;
+        const bool mine = labelled(y, p.classes);
         const unsigned ballot = __ballot_sync(0xffffffffu, mine);
         __syncthreads();
         if (lane == 0) sums[warp] = __popc(ballot);
@@ -73,18 +83,23 @@ __global__ void __launch_bounds__(kXentCountThreads) xent_number_kernel(const in
         const int before = __reduce_add_sync(0xffffffffu, lane < warp ? in_warp : 0);
         if (mine) {
             const int to = at + before + __popc(ballot & ((1u << lane) - 1));
-            row_of[to] = (int32_t)r;
-            label[to] = (int32_t)y;
-        } else if (r < r1 && row_loss) {
-            row_loss[r] = 0.f;
+            p.row_of[to] = (int32_t)r;
+            p.label[to] = (int32_t)y;
+        } else if (r < r1 && p.row_loss) {
+            p.row_loss[r] = 0.f;
         }
         at += __reduce_add_sync(0xffffffffu, in_warp);
     }
     if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
-        *total = at;
-        *status = 0;
-        range[0] = range[1] = 0;
+        *p.total = at;
+        *p.status = 0;
+        p.range[0] = p.range[1] = 0;
     }
+}
+__global__ void __launch_bounds__(kXentCountThreads) xent_number_kernel(const XentNumberArgs p) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    number_rows(p);
 }
 
 // ---- planes ----------------------------------------------------------------------------------------------
@@ -112,37 +127,43 @@ __device__ __forceinline__ uint32_t finite_magnitude(float x) {
     return b < 0x7f800000u ? b : 0u;
 }
 
-// The largest finite magnitudes of both operands (FP32 input).  A maximum does not depend on the order.
-__global__ void __launch_bounds__(256) xent_range_kernel(const XentPackArgs p) {
-    wait_for_previous_kernel();
-    let_next_kernel_start();
+// Lanes for a row of n values, four to a lane: a power of two, so that a warp takes several short rows at a time.
+__device__ __forceinline__ int lanes_for(int n) {
+    int g = 1;
+    while (g < 32 && 4 * g < n) g *= 2;
+    return g;
+}
+
+// The largest finite magnitudes of both operands (FP32 input) to p.range.  A maximum does not depend on the order.
+__device__ __forceinline__ void find_range(const XentPackArgs& p, int64_t w0, int64_t warps) {
     const int lane = threadIdx.x & 31;
-    const int64_t warps = (int64_t)gridDim.x * 8, w0 = grid_warp();
     const float* hidden = static_cast<const float*>(p.hidden);
     const float* weight = static_cast<const float*>(p.weight);
     uint32_t most[2] = {0, 0};
-    auto scan = [&](const float* row, int64_t n, int64_t stride, uint32_t& m) {
+    auto scan = [&](const float* row, int64_t n, int64_t stride, uint32_t& m, int lane, int lanes) {
         if (stride == 1 && (reinterpret_cast<uintptr_t>(row) & 15) == 0) {
             int64_t d = 4 * lane;
-            for (; d + 4 <= n; d += 128) {
+            for (; d + 4 <= n; d += 4 * lanes) {
                 const float4 v = __ldg(reinterpret_cast<const float4*>(row + d));
                 m = max(m, max(max(finite_magnitude(v.x), finite_magnitude(v.y)), max(finite_magnitude(v.z), finite_magnitude(v.w))));
             }
             for (; d < n; d++) m = max(m, finite_magnitude(__ldg(row + d)));
         } else {
-            for (int64_t d = lane; d < n; d += 32) m = max(m, finite_magnitude(__ldg(row + d * stride)));
+            for (int64_t d = lane; d < n; d += lanes) m = max(m, finite_magnitude(__ldg(row + d * stride)));
         }
     };
     const int count = *p.count;
-    for (int64_t i = w0; i < count; i += warps) scan(hidden + p.row_of[i] * p.hidden_stride, p.dim, 1, most[0]);
+    const int lanes = lanes_for(p.dim), rows = 32 / lanes, sub = lane & (lanes - 1);
+#pragma unroll 2
+    for (int64_t i = w0 * rows + lane / lanes; i < count; i += warps * rows) scan(hidden + p.row_of[i] * p.hidden_stride, p.dim, 1, most[0], sub, lanes);
     if (p.w_class_stride == 1) {       // in stretches of at most 4096 along the axis that is contiguous
         const int64_t parts = (p.classes + 4095) / 4096;
         for (int64_t i = w0; i < p.dim * parts; i += warps) {
             const int64_t v = i % parts * 4096;
-            scan(weight + i / parts * p.w_dim_stride + v, min((int64_t)4096, p.classes - v), 1, most[1]);
+            scan(weight + i / parts * p.w_dim_stride + v, min((int64_t)4096, p.classes - v), 1, most[1], lane, 32);
         }
     } else {
-        for (int64_t v = w0; v < p.classes; v += warps) scan(weight + v * p.w_class_stride, p.dim, p.w_dim_stride, most[1]);
+        for (int64_t v = w0 * rows + lane / lanes; v < p.classes; v += warps * rows) scan(weight + v * p.w_class_stride, p.dim, p.w_dim_stride, most[1], sub, lanes);
     }
     __shared__ uint32_t room[2];
     if (threadIdx.x < 2) room[threadIdx.x] = 0;
@@ -155,6 +176,11 @@ __global__ void __launch_bounds__(256) xent_range_kernel(const XentPackArgs p) {
     __syncthreads();
     if (threadIdx.x < 2 && room[threadIdx.x]) atomicMax(p.range + threadIdx.x, room[threadIdx.x]);
 }
+__global__ void __launch_bounds__(256) xent_range_kernel(const XentPackArgs p) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    find_range(p, grid_warp(), (int64_t)gridDim.x * 8);
+}
 
 // hi and lo of a scaled float; an infinite or NaN hi has no lo
 __device__ __forceinline__ void split_half(float x, uint32_t& hi, uint32_t& lo) {
@@ -164,11 +190,11 @@ __device__ __forceinline__ void split_half(float x, uint32_t& hi, uint32_t& lo) 
     lo = __half_as_ushort(__float2half_rn(isfinite(hf) ? x - hf : 0.f));
 }
 
-// One row of `dim` elements `stride` apart to the planes, by a warp; `src` NULL writes zeros.
+// One row of `dim` elements `stride` apart to the planes, by `lanes` lanes of which this is number `lane`; `src` NULL writes zeros.
 template <bool kFloat>
-__device__ __forceinline__ void pack_row(const void* src, int64_t stride, int dim, int dim_pad, uint16_t* to, int64_t plane, float scale, int lane) {
+__device__ __forceinline__ void pack_row(const void* src, int64_t stride, int dim, int dim_pad, uint16_t* to, int64_t plane, float scale, int lane, int lanes) {
     const bool vec = stride == 1 && (reinterpret_cast<uintptr_t>(src) & (kFloat ? 15 : 7)) == 0;
-    for (int d = 4 * lane; d < dim_pad; d += 128) {
+    for (int d = 4 * lane; d < dim_pad; d += 4 * lanes) {
         if constexpr (kFloat) {
             float x[4] = {0.f, 0.f, 0.f, 0.f};
             const float* f = static_cast<const float*>(src);
@@ -202,49 +228,75 @@ __device__ __forceinline__ void pack_row(const void* src, int64_t stride, int di
     }
 }
 
+template <bool kFloat>
+__device__ __forceinline__ float plane_scale(const XentPackArgs& p, int operand) { return kFloat ? exp2f((float)(14 - plane_exponent(__ldcg(p.range + operand)))) : 1.f; }
+
+// The labelled rows to their planes; zeros to dhidden's other rows.
+template <bool kFloat>
+__device__ __forceinline__ void pack_hidden(const XentPackArgs& p, int64_t w0, int64_t warps) {
+    constexpr int kBytes = kFloat ? 4 : 2;
+    const int lane = threadIdx.x & 31, count = *p.count;
+    const float h_scale = plane_scale<kFloat>(p, 0);
+    // labelled rows, and zeros up to a whole tile
+    const int64_t end = ((int64_t)count + kXentTileM - 1) / kXentTileM * kXentTileM;
+    const int lanes = lanes_for(p.dim_pad), rows = 32 / lanes;
+#pragma unroll 2
+    for (int64_t i = w0 * rows + lane / lanes; i < end; i += warps * rows) {
+        const void* src = i < count ? static_cast<const char*>(p.hidden) + (int64_t)p.row_of[i] * p.hidden_stride * kBytes : nullptr;
+        pack_row<kFloat>(src, 1, p.dim, p.dim_pad, p.h_planes + i * p.dim_pad, p.h_plane, h_scale, lane & (lanes - 1), lanes);
+    }
+    if (p.dhidden && count < p.rows) {
+        // a warp looks at 32 labels and then clears the rows without one
+        const int bytes = p.dim * kBytes;
+        const bool vec = (reinterpret_cast<uintptr_t>(p.dhidden) & 15) == 0 && p.dhidden_stride * kBytes % 16 == 0 && bytes % 16 == 0;
+        for (int64_t r0 = 32 * w0; r0 < p.rows; r0 += 32 * warps) {
+            const int64_t r = r0 + lane;
+            const unsigned clear = __ballot_sync(0xffffffffu, r < p.rows && !labelled(p.labels[min(r, p.rows - 1)], p.classes));
+            if (!clear) continue;
+            char* to = static_cast<char*>(p.dhidden) + r0 * p.dhidden_stride * kBytes;
+            const int pieces = vec ? bytes / 16 : p.dim;       // of a row
+            int row = lane / pieces, piece = lane % pieces;    // lanes go through the rows' pieces one after the other
+            const int rows_on = 32 / pieces, pieces_on = 32 % pieces;
+            while (row < 32) {
+                if (clear >> row & 1) {
+                    char* at = to + row * p.dhidden_stride * kBytes;
+                    if (vec) *reinterpret_cast<uint4*>(at + 16 * piece) = make_uint4(0u, 0u, 0u, 0u);
+                    else if constexpr (kFloat) reinterpret_cast<float*>(at)[piece] = 0.f;
+                    else reinterpret_cast<uint16_t*>(at)[piece] = 0;
+                }
+                row += rows_on;
+                piece += pieces_on;
+                if (piece >= pieces) { piece -= pieces; row++; }
+            }
+        }
+    }
+}
+
+// The weight to its planes, class by class.
+template <bool kFloat>
+__device__ __forceinline__ void pack_weight(const XentPackArgs& p, int64_t w0, int64_t warps) {
+    const float w_scale = plane_scale<kFloat>(p, 1);
+    const int lane = threadIdx.x & 31, lanes = lanes_for(p.dim_pad), rows = 32 / lanes;
+    for (int64_t v = w0 * rows + lane / lanes; v < p.classes; v += warps * rows)
+        pack_row<kFloat>(static_cast<const char*>(p.weight) + v * p.w_class_stride * (kFloat ? 4 : 2), p.w_dim_stride, p.dim, p.dim_pad,
+                         p.w_planes + v * p.dim_pad, p.w_plane, w_scale, lane & (lanes - 1), lanes);
+}
+
 constexpr int kXentPackThreads = 256;
 
 template <bool kFloat>
 __global__ void __launch_bounds__(kXentPackThreads) xent_pack_kernel(const XentPackArgs p) {
     wait_for_previous_kernel();
     let_next_kernel_start();
-    constexpr int kBytes = kFloat ? 4 : 2;
     const int lane = threadIdx.x & 31;
     const int64_t warps = (int64_t)gridDim.x * (kXentPackThreads / 32), w0 = grid_warp();
-    const int count = *p.count;
-    const float h_scale = kFloat ? exp2f((float)(14 - plane_exponent(p.range[0]))) : 1.f, w_scale = kFloat ? exp2f((float)(14 - plane_exponent(p.range[1]))) : 1.f;
-    // labelled rows, and zeros up to a whole tile
-    const int64_t end = ((int64_t)count + kXentTileM - 1) / kXentTileM * kXentTileM;
-    for (int64_t i = w0; i < end; i += warps) {
-        const void* src = i < count ? static_cast<const char*>(p.hidden) + (int64_t)p.row_of[i] * p.hidden_stride * kBytes : nullptr;
-        pack_row<kFloat>(src, 1, p.dim, p.dim_pad, p.h_planes + i * p.dim_pad, p.h_plane, h_scale, lane);
-    }
-    if (p.dhidden && count < p.rows) {
-        // a warp looks at 32 labels and then clears the rows without one
-        const bool vec = (reinterpret_cast<uintptr_t>(p.dhidden) & 15) == 0 && p.dhidden_stride * kBytes % 16 == 0 && p.dim * kBytes % 16 == 0;
-        for (int64_t r0 = 32 * w0; r0 < p.rows; r0 += 32 * warps) {
-            const int64_t r = r0 + lane;
-            unsigned clear = __ballot_sync(0xffffffffu, r < p.rows && !labelled(p.labels[min(r, p.rows - 1)], p.classes));
-            for (; clear; clear &= clear - 1) {
-                char* to = static_cast<char*>(p.dhidden) + (r0 + __ffs(clear) - 1) * p.dhidden_stride * kBytes;
-                if (vec) {
-                    for (int d = 16 * lane; d < p.dim * kBytes; d += 512) *reinterpret_cast<uint4*>(to + d) = make_uint4(0u, 0u, 0u, 0u);
-                } else {
-                    for (int d = lane; d < p.dim; d += 32) {
-                        if constexpr (kFloat) reinterpret_cast<float*>(to)[d] = 0.f;
-                        else reinterpret_cast<uint16_t*>(to)[d] = 0;
-                    }
-                }
-            }
-        }
-    }
+    pack_hidden<kFloat>(p, w0, warps);
     if (!p.weight) return;
     if (p.w_dim_stride == 1 || p.w_class_stride != 1) {
-        for (int64_t v = w0; v < p.classes; v += warps)
-            pack_row<kFloat>(static_cast<const char*>(p.weight) + v * p.w_class_stride * kBytes, p.w_dim_stride, p.dim, p.dim_pad,
-                             p.w_planes + v * p.dim_pad, p.w_plane, w_scale, lane);
+        pack_weight<kFloat>(p, w0, warps);
         return;
     }
+    const float w_scale = plane_scale<kFloat>(p, 1);
     // classes are contiguous: tiles of 32 x 32 turned over in shared memory
     __shared__ uint32_t tile[kXentPackThreads / 32][32][33];
     uint32_t(*t)[33] = tile[threadIdx.x >> 5];
@@ -279,44 +331,62 @@ __global__ void __launch_bounds__(kXentPackThreads) xent_pack_kernel(const XentP
     }
 }
 
-// ---- joining -----------------------------------------------------------------------------------------------
-// Log sums and losses of the rows from the parts of the classes: a block takes 32 rows, 32 threads each, whose shares of
-// the parts are joined in their order.
-__global__ void __launch_bounds__(1024) xent_join_kernel(const XentArgs p, int parts) {
+// All of the above by one block, for heads so small that launches count (kXentSmallRows, kXentSmallValues).
+template <bool kFloat>
+__global__ void __launch_bounds__(kXentCountThreads) xent_prepare_kernel(const XentNumberArgs n, const XentPackArgs p) {
     wait_for_previous_kernel();
     let_next_kernel_start();
-    __shared__ float2 room[32][33];
-    const int count = *p.count, lane = threadIdx.x & 31, share = threadIdx.x >> 5;
+    number_rows(n);
+    __syncthreads();
+    const int64_t w0 = threadIdx.x >> 5, warps = kXentCountThreads / 32;
+    if constexpr (kFloat) {
+        find_range(p, w0, warps);
+        __syncthreads();
+    }
+    pack_hidden<kFloat>(p, w0, warps);
+    if (p.weight) pack_weight<kFloat>(p, w0, warps);
+}
+
+// ---- joining -----------------------------------------------------------------------------------------------
+// Log sums and losses of the rows from the parts of the classes: a block takes 1024 / shares rows, a warp 32 of them, and
+// `shares` (a power of two) threads a row, whose shares of the parts are joined in their order.
+__global__ void __launch_bounds__(1024) xent_join_kernel(const XentArgs p, int parts, int shares) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    __shared__ float2 room[1024];
+    const int count = *p.count, rows = 1024 / shares, share = threadIdx.x / rows, at = threadIdx.x & (rows - 1);
     const float f = logit_factor(p.range);
-    for (int64_t r0 = 32 * (int64_t)blockIdx.x; r0 < count; r0 += 32 * (int64_t)gridDim.x) {
-        const int64_t r = r0 + lane;
+    const bool lost = *p.status != 0;
+    for (int64_t r0 = rows * (int64_t)blockIdx.x; r0 < count; r0 += rows * (int64_t)gridDim.x) {
+        const int64_t r = r0 + at;
         float top = -INFINITY, sum = 0.f;
-        for (int i = share; i < parts; i += 32) {
-            const float2 s = r < count ? p.stats[(int64_t)i * p.rows_pad + r] : make_float2(-INFINITY, 0.f);
+        auto join = [&](float2 s) {
             const float now = fmaxf(top, s.x), base = now == -INFINITY ? 0.f : now * f;
             sum = sum * fast_exp2(fmaf(top, f, -base)) + s.y * fast_exp2(fmaf(s.x, f, -base));
             top = now;
+        };
+        if (r < count) {
+#pragma unroll 4
+            for (int i = share; i < parts; i += shares) join(p.stats[(int64_t)i * p.rows_pad + r]);
         }
-        __syncthreads();
-        room[share][lane] = make_float2(top, sum);
-        __syncthreads();
-        if (share == 0) {
-            top = -INFINITY;
-            for (int i = 0; i < 32; i++) top = fmaxf(top, room[i][lane].x);
-            const float base = top == -INFINITY ? 0.f : top * f;
-            sum = 0.f;
-            for (int i = 0; i < 32; i++) sum += room[i][lane].y * fast_exp2(fmaf(room[i][lane].x, f, -base));
-            float loss = 0.f;
-            if (r < count) {
-                const float lse2 = base + log2f(sum);
-                p.lse2[r] = lse2;
-                loss = kLn2 * fmaf(-p.label_logit[r], f, lse2);
-                if (p.row_loss) p.row_loss[p.row_of[r]] = loss;
-            }
+        if (shares > 1) {
+            __syncthreads();
+            room[threadIdx.x] = make_float2(top, sum);
+            __syncthreads();
+        }
+        if (share > 0) continue;
+        for (int i = 1; i < shares; i++) join(room[i * rows + at]);
+        float loss = 0.f;
+        if (r < count) {
+            const float lse2 = (top == -INFINITY ? 0.f : top * f) + log2f(sum);
+            p.lse2[r] = lse2;
+            loss = lost ? NAN : kLn2 * fmaf(-p.label_logit[r], f, lse2);
+            if (p.row_loss) p.row_loss[p.row_of[r]] = loss;
+        }
+        const bool any = __any_sync(0xffffffffu, r < count);
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
-            if (lane == 0) p.warp_loss[r0 >> 5] = loss;
-        }
+        for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
+        if ((threadIdx.x & 31) == 0 && any) p.warp_loss[r >> 5] = loss;
     }
 }
 
@@ -339,9 +409,7 @@ struct XentReduceArgs {
     const uint32_t* range;
 };
 
-__global__ void __launch_bounds__(256) xent_reduce_kernel(const XentReduceArgs p) {
-    wait_for_previous_kernel();
-    let_next_kernel_start();
+__device__ __forceinline__ void reduce_parts(const XentReduceArgs& p) {
     const int count = *p.count;
     const int64_t m_end = p.m_is_count ? count : p.m, n_vec = (p.n + 3) / 4;
     const ProductScale scale = product_scale(p.scale, p.mean, count, p.range, p.operand);
@@ -384,28 +452,49 @@ __global__ void __launch_bounds__(256) xent_reduce_kernel(const XentReduceArgs p
     }
 }
 
+struct XentLossArgs {
+    const int32_t* count;
+    const float* warp_loss;
+    const int32_t* status;
+    float* loss;               // NULL: not now
+    int64_t rows;
+    int32_t reduction;
+};
+
 // The loss of all rows, in a fixed order and 64 bits; NaN where a kernel gave up on a wait.
-__global__ void __launch_bounds__(1024) xent_loss_kernel(const int32_t* count_, const float* __restrict__ warp_loss, const int32_t* status, float* loss,
-                                                         int64_t rows, int reduction) {
-    wait_for_previous_kernel();
-    let_next_kernel_start();
-    const int count = *count_;
-    if (*status) {
-        const int64_t n = reduction == MASK_REDUCE_NONE ? rows : 1;
-        for (int64_t r = threadIdx.x; r < n; r += 1024) loss[r] = NAN;
+__device__ __forceinline__ void sum_losses(const XentLossArgs& p) {
+    const int count = *p.count;
+    if (*p.status) {
+        const int64_t n = p.reduction == MASK_REDUCE_NONE ? p.rows : 1;
+        for (int64_t r = threadIdx.x; r < n; r += 256) p.loss[r] = NAN;
         return;
     }
-    if (reduction == MASK_REDUCE_NONE) return;
-    __shared__ double sums[32];
+    if (p.reduction == MASK_REDUCE_NONE) return;
+    __shared__ double sums[8];
     double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < ((int64_t)count + 31) / 32; i += 1024) sum += warp_loss[i];
+#pragma unroll 8
+    for (int64_t i = threadIdx.x; i < ((int64_t)count + 31) / 32; i += 256) sum += p.warp_loss[i];
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
     __syncthreads();
-    if (threadIdx.x < 32) {
-        sum = sums[threadIdx.x];
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (threadIdx.x == 0) *loss = count == 0 ? 0.f : (float)(reduction == MASK_REDUCE_MEAN ? sum / count : sum);
+    if (threadIdx.x == 0) {
+        sum = 0.0;
+        for (int i = 0; i < 8; i++) sum += sums[i];
+        *p.loss = count == 0 ? 0.f : (float)(p.reduction == MASK_REDUCE_MEAN ? sum / count : sum);
+    }
+}
+
+// What is left of a call (grid.y: dweight's parts, dhidden's); a block that has no other part of it sums the losses.
+__global__ void __launch_bounds__(256) xent_finish_kernel(const XentReduceArgs dw, const XentReduceArgs dh, const XentLossArgs loss) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    if (blockIdx.y == 2) {
+        if (blockIdx.x == 0 && loss.loss) sum_losses(loss);
+        return;
+    }
+    if (blockIdx.y == 0 ? dw.part != nullptr : dh.part != nullptr) {
+        if (blockIdx.y == 0) reduce_parts(dw);
+        else reduce_parts(dh);
     }
 }
 
@@ -416,7 +505,7 @@ struct XentPlan {
     int planes, dim_pad;
     int64_t rows_pad, chunk;
     int n_chunks;
-    bool grads, one_pass, pack_weight;
+    bool grads, one_pass, pack_weight, small;
     int bn_logits, bn_dim;
     int stats_splits, stats_parts;       // parts of the classes' tiles, and numbers a row gets from them
     int piece, n_pieces;                 // classes of a piece (a multiple of 256 unless one tile holds all), pieces
@@ -464,6 +553,8 @@ static XentPlan plan_xent(const mask_head& h) {
     p.grads = h.d_dhidden || h.d_dweight;
     p.pack_weight = p.planes == 2 || h.weight_dim_stride != 1 || h.weight_class_stride % 8 || h.weight_class_stride < h.dim ||
                     (reinterpret_cast<uintptr_t>(h.d_weight) & 15);
+    p.small = h.rows <= kXentSmallRows && h.rows * h.dim + (p.pack_weight ? (int64_t)h.dim * h.classes : 0) <= kXentSmallValues;
+    if (p.small) p.chunk = kXentSmallRows, p.n_chunks = 1;
     p.bn_logits = h.classes <= 64 ? 64 : (h.classes <= 128 ? 128 : 256);
     p.bn_dim = tile_width(h.dim);
     // one tile of all classes: 256 columns, with two planes of G in shared memory 128
@@ -564,14 +655,18 @@ static int launch_xent_gemm(int bn, int planes, const XentArgs& a, int64_t rows,
     return planes == 1 ? launch_xent_gemm_planes<MODE, 1>(bn, cg, a, ma, mb, mg, items, st) : launch_xent_gemm_planes<MODE, 2>(bn, cg, a, ma, mb, mg, items, st);
 }
 
-// `rows`: of the product, at most.
-static int launch_xent_reduce(XentReduceArgs r, int64_t rows, cudaStream_t st) {
+// Blocks for a product's parts (0: it has none), `rows` of them at most, and the threads that share a vector.
+static int64_t share_parts(XentReduceArgs& r, int64_t rows) {
+    if (!r.part) return 0;
     const int64_t vectors = rows * ((r.n + 3) / 4);
     // 16 parts or more and not enough vectors for two blocks an SM: up to 32 threads a vector
     r.shares = 1;
     while (r.shares < 32 && 8 * r.shares < r.splits && vectors * r.shares < 512 * (int64_t)sm_count()) r.shares *= 2;
-    const int64_t blocks = (vectors * r.shares + 255) / 256;
-    return launch_overlapped(xent_reduce_kernel, dim3((unsigned)std::min<int64_t>(blocks, 8 * (int64_t)sm_count())), 256, 0, st, r);
+    return std::min<int64_t>((vectors * r.shares + 255) / 256, 8 * (int64_t)sm_count());
+}
+static int launch_xent_finish(XentReduceArgs dw, int64_t dw_rows, XentReduceArgs dh, int64_t dh_rows, const XentLossArgs& loss, cudaStream_t st) {
+    const int64_t blocks = std::max<int64_t>(1, std::max(share_parts(dw, dw_rows), share_parts(dh, dh_rows)));
+    return launch_overlapped(xent_finish_kernel, dim3((unsigned)blocks, 3), 256, 0, st, dw, dh, loss);
 }
 
 static const char* refuse_head(const mask_head* h) {
@@ -580,7 +675,8 @@ static const char* refuse_head(const mask_head* h) {
     if (h->reduction < MASK_REDUCE_NONE || h->reduction > MASK_REDUCE_SUM) return "reduction must be MASK_REDUCE_NONE, _MEAN or _SUM";
     constexpr int64_t most = ((int64_t)1 << 31) - 256;
     if (h->rows < 0 || h->rows >= most) return "rows out of range";
-    if (h->dim < 1 || h->dim >= most || h->classes < 1 || h->classes >= most) return "dim and classes must be at least 1 and below 2^31 - 256";
+    if (h->dim < 1 || h->dim > (1 << 20)) return "dim must be 1 to 2^20";
+    if (h->classes < 1 || h->classes >= most) return "classes must be at least 1 and below 2^31 - 256";
     if (h->hidden_stride < 0 || h->weight_dim_stride < 0 || h->weight_class_stride < 0 || h->dhidden_stride < 0 || h->dweight_dim_stride < 0 ||
         h->dweight_class_stride < 0)
         return "strides must not be negative";
@@ -606,14 +702,8 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
     const int P = plan.planes;
     const int64_t rp = plan.rows_pad;
 
-    const dim3 chunks((unsigned)plan.n_chunks);
     int rc = MASK_OK;
-    if (plan.n_chunks > 1 && (rc = launch_overlapped(xent_count_kernel, chunks, kXentCountThreads, 0, st, h.d_labels, h.rows, h.classes, plan.chunk, counts)))
-        return rc;
-    if ((rc = launch_overlapped(xent_number_kernel, chunks, kXentCountThreads, 0, st, h.d_labels, h.rows, h.classes, plan.chunk, counts, row_of, label,
-                                total, total + 1, range, row_loss)))
-        return rc;
-
+    const XentNumberArgs number = {h.d_labels, h.rows, plan.chunk, h.classes, counts, row_of, label, total, total + 1, range, row_loss};
     XentPackArgs pk = {};
     pk.dtype = h.dtype; pk.dim = h.dim; pk.dim_pad = plan.dim_pad; pk.classes = h.classes; pk.rows = h.rows;
     pk.count = total; pk.row_of = row_of; pk.labels = h.d_labels;
@@ -625,13 +715,24 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
         pk.w_planes = reinterpret_cast<uint16_t*>(at(plan.w_planes)); pk.w_plane = (int64_t)h.classes * plan.dim_pad;
     }
     pk.range = range;
-    const int64_t pack_rows = rp + (plan.pack_weight ? h.classes : 0);
-    const unsigned pack_grid = (unsigned)std::min<int64_t>((pack_rows + 7) / 8, 8 * (int64_t)sm_count());
-    if (h.dtype == MASK_F32) {
-        if ((rc = launch_overlapped(xent_range_kernel, dim3(pack_grid), 256, 0, st, pk))) return rc;
-        if ((rc = launch_overlapped(xent_pack_kernel<true>, dim3(pack_grid), kXentPackThreads, 0, st, pk))) return rc;
+    if (plan.small) {
+        if (h.dtype == MASK_F32) rc = launch_overlapped(xent_prepare_kernel<true>, dim3(1), kXentCountThreads, 0, st, number, pk);
+        else rc = launch_overlapped(xent_prepare_kernel<false>, dim3(1), kXentCountThreads, 0, st, number, pk);
+        if (rc) return rc;
     } else {
-        if ((rc = launch_overlapped(xent_pack_kernel<false>, dim3(pack_grid), kXentPackThreads, 0, st, pk))) return rc;
+        const dim3 chunks((unsigned)plan.n_chunks);
+        if (plan.n_chunks > 1 && (rc = launch_overlapped(xent_count_kernel, chunks, kXentCountThreads, 0, st, h.d_labels, h.rows, h.classes, plan.chunk, counts)))
+            return rc;
+        if ((rc = launch_overlapped(xent_number_kernel, chunks, kXentCountThreads, 0, st, number))) return rc;
+        const int64_t pack_rows = rp + (plan.pack_weight ? h.classes : 0);
+        const dim3 pack_grid((unsigned)std::min<int64_t>((pack_rows + 7) / 8, 8 * (int64_t)sm_count()));
+        if (h.dtype == MASK_F32) {
+            if ((rc = launch_overlapped(xent_range_kernel, pack_grid, 256, 0, st, pk))) return rc;
+            rc = launch_overlapped(xent_pack_kernel<true>, pack_grid, kXentPackThreads, 0, st, pk);
+        } else {
+            rc = launch_overlapped(xent_pack_kernel<false>, pack_grid, kXentPackThreads, 0, st, pk);
+        }
+        if (rc) return rc;
     }
 
     const void* w_data = plan.pack_weight ? (const void*)pk.w_planes : h.d_weight;
@@ -656,8 +757,12 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
     if (!plan.one_pass) {
         a.splits = plan.stats_splits;
         if ((rc = launch_xent_gemm<kXentStats>(plan.bn_logits, P, a, rp, a.splits, h_k, w_k, none, st))) return rc;
-        if ((rc = launch_overlapped(xent_join_kernel, dim3((unsigned)std::min<int64_t>(rp / 32, 2 * (int64_t)sm_count())), 1024, 0, st, a, plan.stats_parts))) return rc;
+        int shares = 1;
+        while (shares < 32 && 8 * shares < plan.stats_parts) shares *= 2;
+        const int64_t blocks = std::min<int64_t>((rp * shares + 1023) / 1024, 2 * (int64_t)sm_count());
+        if ((rc = launch_overlapped(xent_join_kernel, dim3((unsigned)blocks), 1024, 0, st, a, plan.stats_parts, shares))) return rc;
     }
+    XentReduceArgs dw = {}, dh = {};
     if (plan.grads) {
         char* g = at(plan.g);
         const int64_t g_plane = rp * plan.g_ld;
@@ -700,7 +805,8 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
                     XentReduceArgs w = r;
                     w.part = b.part; w.part_rows = b.part_rows; w.splits = b.splits; w.m = a.vc; w.m0 = a.v0;
                     w.out = b.out; w.out_m = b.out_m; w.out_n = b.out_n;
-                    if ((rc = launch_xent_reduce(w, w.m, st))) return rc;
+                    if (plan.n_pieces == 1) dw = w;
+                    else if ((rc = launch_xent_finish(w, w.m, {}, 0, {}, st))) return rc;
                 }
             }
         }
@@ -708,11 +814,12 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
             r.part = reinterpret_cast<float*>(at(plan.part_dh)); r.part_rows = plan.part_dh_rows; r.splits = plan.dh_splits;
             r.m_is_count = 1; r.operand = 1;
             r.out = h.d_dhidden; r.out_m = h.dhidden_stride; r.out_n = 1;
-            if ((rc = launch_xent_reduce(r, rp, st))) return rc;
+            dh = r;
         }
     }
-    if ((rc = launch_overlapped(xent_loss_kernel, dim3(1), 1024, 0, st, total, a.warp_loss, total + 1, h.d_loss, h.rows, h.reduction))) return rc;
-    return MASK_OK;
+    if (!plan.grads && h.reduction == MASK_REDUCE_NONE) return MASK_OK;      // the join has written every loss
+    const XentLossArgs loss = {total, a.warp_loss, total + 1, h.d_loss, h.rows, h.reduction};
+    return launch_xent_finish(dw, dw.m, dh, rp, loss, st);
 }
 
 }  // namespace mask
