@@ -140,31 +140,39 @@ __device__ __forceinline__ void find_range(const XentPackArgs& p, int64_t w0, in
     const float* hidden = static_cast<const float*>(p.hidden);
     const float* weight = static_cast<const float*>(p.weight);
     uint32_t most[2] = {0, 0};
-    auto scan = [&](const float* row, int64_t n, int64_t stride, uint32_t& m, int lane, int lanes) {
-        if (stride == 1 && (reinterpret_cast<uintptr_t>(row) & 15) == 0) {
-            int64_t d = 4 * lane;
-            for (; d + 4 <= n; d += 4 * lanes) {
-                const float4 v = __ldg(reinterpret_cast<const float4*>(row + d));
-                m = max(m, max(max(finite_magnitude(v.x), finite_magnitude(v.y)), max(finite_magnitude(v.z), finite_magnitude(v.w))));
+    // rows i of n values, `stride` apart, at base(i); a thread has four rows in flight
+    auto scan = [&](int64_t rows, int64_t n, int64_t stride, int lanes, auto base, uint32_t& m) {
+        const int sub = lane & (lanes - 1), side = 32 / lanes;
+        const int64_t step = warps * side;
+        for (int64_t i = w0 * side + lane / lanes; i < rows; i += 4 * step) {
+            const float* row[4];
+            bool vec = stride == 1;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                row[k] = base(min(i + k * step, rows - 1));
+                vec = vec && (reinterpret_cast<uintptr_t>(row[k]) & 15) == 0;
             }
-            for (; d < n; d++) m = max(m, finite_magnitude(__ldg(row + d)));
-        } else {
-            for (int64_t d = lane; d < n; d += lanes) m = max(m, finite_magnitude(__ldg(row + d * stride)));
+            int64_t d = 4 * sub;
+            if (vec) {
+                for (; d + 4 <= n; d += 4 * lanes) {
+                    float4 v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) v[k] = __ldg(reinterpret_cast<const float4*>(row[k] + d));
+#pragma unroll
+                    for (int k = 0; k < 4; k++) m = max(m, max(max(finite_magnitude(v[k].x), finite_magnitude(v[k].y)), max(finite_magnitude(v[k].z), finite_magnitude(v[k].w))));
+                }
+            }
+            for (; d < n; d += 4 * lanes)
+                for (int64_t e = d; e < min(d + 4, n); e++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) m = max(m, finite_magnitude(__ldg(row[k] + e * stride)));
         }
     };
-    const int count = *p.count;
-    const int lanes = lanes_for(p.dim), rows = 32 / lanes, sub = lane & (lanes - 1);
-#pragma unroll 2
-    for (int64_t i = w0 * rows + lane / lanes; i < count; i += warps * rows) scan(hidden + p.row_of[i] * p.hidden_stride, p.dim, 1, most[0], sub, lanes);
-    if (p.w_class_stride == 1) {       // in stretches of at most 4096 along the axis that is contiguous
-        const int64_t parts = (p.classes + 4095) / 4096;
-        for (int64_t i = w0; i < p.dim * parts; i += warps) {
-            const int64_t v = i % parts * 4096;
-            scan(weight + i / parts * p.w_dim_stride + v, min((int64_t)4096, p.classes - v), 1, most[1], lane, 32);
-        }
-    } else {
-        for (int64_t v = w0 * rows + lane / lanes; v < p.classes; v += warps * rows) scan(weight + v * p.w_class_stride, p.dim, p.w_dim_stride, most[1], sub, lanes);
-    }
+    scan(*p.count, p.dim, 1, lanes_for(p.dim), [&](int64_t i) { return hidden + p.row_of[i] * p.hidden_stride; }, most[0]);
+    if (p.w_class_stride == 1)
+        scan(p.dim, p.classes, 1, 32, [&](int64_t d) { return weight + d * p.w_dim_stride; }, most[1]);
+    else
+        scan(p.classes, p.dim, p.w_dim_stride, lanes_for(p.dim), [&](int64_t v) { return weight + v * p.w_class_stride; }, most[1]);
     __shared__ uint32_t room[2];
     if (threadIdx.x < 2) room[threadIdx.x] = 0;
     __syncthreads();
@@ -194,6 +202,7 @@ __device__ __forceinline__ void split_half(float x, uint32_t& hi, uint32_t& lo) 
 template <bool kFloat>
 __device__ __forceinline__ void pack_row(const void* src, int64_t stride, int dim, int dim_pad, uint16_t* to, int64_t plane, float scale, int lane, int lanes) {
     const bool vec = stride == 1 && (reinterpret_cast<uintptr_t>(src) & (kFloat ? 15 : 7)) == 0;
+#pragma unroll 4
     for (int d = 4 * lane; d < dim_pad; d += 4 * lanes) {
         if constexpr (kFloat) {
             float x[4] = {0.f, 0.f, 0.f, 0.f};
@@ -240,10 +249,16 @@ __device__ __forceinline__ void pack_hidden(const XentPackArgs& p, int64_t w0, i
     // labelled rows, and zeros up to a whole tile
     const int64_t end = ((int64_t)count + kXentTileM - 1) / kXentTileM * kXentTileM;
     const int lanes = lanes_for(p.dim_pad), rows = 32 / lanes;
-#pragma unroll 2
-    for (int64_t i = w0 * rows + lane / lanes; i < end; i += warps * rows) {
-        const void* src = i < count ? static_cast<const char*>(p.hidden) + (int64_t)p.row_of[i] * p.hidden_stride * kBytes : nullptr;
-        pack_row<kFloat>(src, 1, p.dim, p.dim_pad, p.h_planes + i * p.dim_pad, p.h_plane, h_scale, lane & (lanes - 1), lanes);
+    const int64_t step = warps * rows;
+    auto source = [&](int64_t i) -> const void* {
+        return i < count ? static_cast<const char*>(p.hidden) + (int64_t)p.row_of[i] * p.hidden_stride * kBytes : nullptr;
+    };
+    for (int64_t i = w0 * rows + lane / lanes; i < end; i += 2 * step) {
+        const void* a = source(i);
+        const void* b = i + step < end ? source(i + step) : nullptr;
+        pack_row<kFloat>(a, 1, p.dim, p.dim_pad, p.h_planes + i * p.dim_pad, p.h_plane, h_scale, lane & (lanes - 1), lanes);
+        if (i + step < end)
+            pack_row<kFloat>(b, 1, p.dim, p.dim_pad, p.h_planes + (i + step) * p.dim_pad, p.h_plane, h_scale, lane & (lanes - 1), lanes);
     }
     if (p.dhidden && count < p.rows) {
         // a warp looks at 32 labels and then clears the rows without one
