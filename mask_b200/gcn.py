@@ -1,4 +1,5 @@
-"""Row-sharded 2-layer GCN forward: ``out = A·(ReLU(A·(X·W1))·W2)`` over P ranks.
+"""2-layer GCNs: the row-sharded forward ``out = A·(ReLU(A·(X·W1))·W2)`` over P ranks, and training on one device
+(``GCN2``: loss and gradients, with group norm between the layers and the classifier head without its logits in memory).
 
 The reference project is single-GPU (its GCN driver, end2end/gcn/eva_gcn_sparsene.py:316-343,
 calls one SpMM per layer on one device); this module is the multi-GPU harness the benchmark
@@ -134,6 +135,7 @@ class FusedGCN2:
       ops.shared_h1(rows, cols) -> list of two objects with ``.local`` (this rank's full copy)
       ops.spmm_to_all(packed, dense, h1_buffer, r0, r1)   # ReLU(A_panel·dense) -> rows [r0,r1) of EVERY rank's copy
       ops.spmm(packed, dense) -> Tensor                    # plain product of the panel
+      ops.linear_cross_entropy(rows, W2, labels, reduction) -> Tensor   # for ``loss`` only
       ops.close()
     """
 
@@ -168,8 +170,8 @@ class FusedGCN2:
     def plans(self):
         return getattr(self.ops, "plans", [])
 
-    def forward(self, X: torch.Tensor, W1: torch.Tensor, W2: torch.Tensor) -> torch.Tensor:
-        """Returns this rank's rows [bounds[rank], bounds[rank+1]) of the output."""
+    def _aggregated(self, X: torch.Tensor, W1: torch.Tensor) -> torch.Tensor:
+        """This rank's rows of ``A·H1``."""
         if W1.shape[1] != self.hidden:
             raise RuntimeError("W1 does not match the hidden width this object was built for")
         XW1 = X @ W1
@@ -180,8 +182,22 @@ class FusedGCN2:
         if self.world > 1:
             dist.all_reduce(self.flag, group=self.group)   # (stream-ordered) barrier: every panel of H1 has landed
         if self.packed is None:
-            return X.new_zeros((0, W2.shape[1]))
-        return self.ops.spmm(self.packed, buf.local) @ W2
+            return X.new_zeros((0, self.hidden))
+        return self.ops.spmm(self.packed, buf.local)
+
+    def forward(self, X: torch.Tensor, W1: torch.Tensor, W2: torch.Tensor) -> torch.Tensor:
+        """Returns this rank's rows [bounds[rank], bounds[rank+1]) of the output."""
+        return self._aggregated(X, W1) @ W2
+
+    def loss(self, X: torch.Tensor, W1: torch.Tensor, W2: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
+        """Mean softmax cross entropy over all ranks' labelled rows, on every rank (0 without any), with no rank's logits in
+        memory.  ``labels`` (int64) are those of this rank's rows; a label that is no class leaves its row out."""
+        rows = self._aggregated(X, W1)
+        labelled = (labels >= 0) & (labels < W2.shape[1])
+        both = torch.stack([self.ops.linear_cross_entropy(rows, W2, labels, "sum").double(), labelled.sum().double()])
+        if self.world > 1:
+            dist.all_reduce(both, group=self.group)
+        return (both[0] / both[1].clamp(min=1)).float()
 
     def close(self) -> None:
         self.ops.close()
@@ -217,11 +233,83 @@ class _FusedDeviceOps:
     def spmm(self, packed, dense):
         return self.engine.spmm(packed, dense)
 
+    def linear_cross_entropy(self, rows, weight, labels, reduction):
+        return self.engine.linear_cross_entropy(rows, weight, labels, reduction)
+
     def close(self):
         self.plans, self._by_buffer = [], {}
         for b in self.buffers:
             b.close()
         self.buffers = []
+
+
+@dataclass
+class GCN2Gradients:
+    W1: torch.Tensor
+    weight: torch.Tensor     # group norm's gain and bias
+    bias: torch.Tensor
+    W2: torch.Tensor
+    X: torch.Tensor | None = None
+
+
+class GCN2:
+    """Two-layer GCN of one device, trained: with ``H = act(norm(A·(X·W1)))`` the head's logits are ``(A·H)·W2``, and
+
+        loss = mean over the labelled nodes of the softmax cross entropy
+
+    The reference's driver trains such a network from its tensor library's pieces (end2end/gcn/eva_gcn_sparsene.py:316-343,
+    599-781).  Here everything between the dense products ``X·W1`` and its gradient is this library's: sparse products with A
+    and A^T, group norm with the activation (per graph of a batch: ``offsets``), and the head with its gradients, which keeps
+    neither the logits nor their gradient in memory.
+
+    ``graph``: square CSR with ``rowptr``, ``colind``, ``values`` (NumPy) and ``M``.  ``ops`` supplies the device's pieces
+    (``_TrainOps``), so that the chain of gradients can be checked without one.  ``tf32x3`` as in ``engine.spmm``."""
+
+    def __init__(self, graph, device, groups: int, activation: str = "relu", offsets=None, eps: float = 1e-5, tf32x3: bool = False, ops=None):
+        if graph.M != graph.K:
+            raise RuntimeError("the GCN needs a square adjacency matrix")
+        self.groups, self.activation, self.eps = groups, activation, eps
+        self.ops = ops if ops is not None else _TrainOps(device, tf32x3)
+        self.offsets = None if offsets is None else torch.as_tensor(np.asarray(offsets), dtype=torch.int32).to(device)
+        self.A, self.At = self.ops.pack(graph), self.ops.pack(_transposed(graph))
+
+    def _forward(self, X, W1, weight, bias):
+        Z = self.ops.spmm(self.A, X @ W1)
+        H, mean, rstd = self.ops.group_norm(Z, self.groups, weight, bias, self.offsets, self.eps, self.activation)
+        return Z, mean, rstd, self.ops.spmm(self.A, H)
+
+    def loss(self, X, W1, weight, bias, W2, labels, reduction: str = "mean") -> torch.Tensor:
+        return self.ops.linear_cross_entropy(self._forward(X, W1, weight, bias)[3], W2, labels, reduction)
+
+    def loss_and_gradients(self, X, W1, weight, bias, W2, labels, input_gradient: bool = False) -> tuple[torch.Tensor, GCN2Gradients]:
+        """Mean loss and its gradients (that of X on request)."""
+        Z, mean, rstd, S = self._forward(X, W1, weight, bias)
+        loss, dS, dW2 = self.ops.linear_cross_entropy(S, W2, labels, "mean", True)
+        dH = self.ops.spmm(self.At, dS)
+        dZ, dweight, dbias = self.ops.group_norm_backward(dH, Z, mean, rstd, self.groups, weight, bias, self.offsets, self.activation)
+        dY = self.ops.spmm(self.At, dZ)
+        return loss, GCN2Gradients(X.t() @ dY, dweight, dbias, dW2, dY @ W1.t() if input_gradient else None)
+
+
+class _TrainOps:
+    """The product path of GCN2."""
+
+    def __init__(self, device, tf32x3):
+        from . import engine
+        self.pack = device_ops(device)[0]
+        self.spmm = lambda packed, dense: engine.spmm_any_width(packed, dense, tf32x3=tf32x3)
+        self.group_norm, self.group_norm_backward = engine.group_norm, engine.group_norm_backward
+        self.linear_cross_entropy = engine.linear_cross_entropy
+
+
+def _transposed(csr):
+    """The CSR of the transposed matrix (host, NumPy)."""
+    from .generators import CSR
+    rows = np.repeat(np.arange(csr.M, dtype=np.int32), np.diff(csr.rowptr))
+    order = np.argsort(csr.colind, kind="stable")
+    rowptr = np.zeros(csr.K + 1, dtype=csr.rowptr.dtype)
+    np.cumsum(np.bincount(csr.colind, minlength=csr.K), out=rowptr[1:])
+    return CSR(csr.K, csr.M, rowptr, rows[order], csr.values[order])
 
 
 class _null:
