@@ -12,6 +12,7 @@
 // Few classes (up to 256, FP32 128) fit one tile, and steps 2 and 3 share one product.  Contractions that leave SMs idle are split and
 // their parts summed in a fixed order.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tensor_map.h"
@@ -22,7 +23,8 @@ namespace mask {
 constexpr int kXentCountThreads = 1024;
 // Rows and values (of hidden and of a weight that has to be packed) up to which one block prepares them: 2708 x 16 x 7 takes
 // it about 7 us, the four kernels 12.
-constexpr int64_t kXentSmallRows = 4096, kXentSmallValues = 65536;
+constexpr int kXentSmallRows = 4096;
+constexpr int64_t kXentSmallValues = 65536;
 constexpr size_t kXentPieceBytes = (size_t)512 << 20;   // what a piece of G may take
 
 // ---- numbering of the labelled rows ------------------------------------------------------------------
@@ -362,6 +364,177 @@ __global__ void __launch_bounds__(kXentCountThreads) xent_prepare_kernel(const X
     if (p.weight) pack_weight<kFloat>(p, w0, warps);
 }
 
+// ---- tiny heads --------------------------------------------------------------------------------------------
+// The whole head by one block and without tensor cores, for problems that are smaller than their launches (kXentTiny...): a
+// warp per labelled row, its lanes along the classes for the logits and along the features for dH; then dW with the rows of a
+// product dealt to 1024 / (dim classes) threads, whose sums are added in their order.  Labelled rows and G stay in shared
+// memory where they fit.  2708 x 16 x 7, one row in twenty labelled: one launch instead of five.
+struct XentTinyArgs {
+    const void* hidden;
+    int64_t hidden_stride;
+    const void* weight;
+    int64_t w_dim_stride, w_class_stride;
+    void* dhidden;             // or NULL
+    int64_t dhidden_stride;
+    void* dweight;             // or NULL
+    int64_t dw_dim_stride, dw_class_stride;
+    int32_t dim;
+    float* g;                  // [rows][classes], where shared memory has no room
+    float* loss;
+    int32_t reduction;
+    float scale;
+};
+constexpr int kXentTinyProduct = 1024;                  // dim * classes
+constexpr int kXentTinyKept = 4096;                     // values of labelled rows, and of G, in shared memory
+constexpr int kXentTinyBytes = 4 * (kXentSmallRows + 2 * kXentTinyKept + kXentTinyProduct + kXentCountThreads);
+constexpr int64_t kXentTinyWork = (int64_t)1 << 19;     // rows * dim * classes
+
+template <typename T> __device__ __forceinline__ float load_float(const void* p, int64_t i) {
+    if constexpr (std::is_same<T, float>::value) return static_cast<const float*>(p)[i];
+    else if constexpr (std::is_same<T, __half>::value) return __half2float(static_cast<const __half*>(p)[i]);
+    else return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+template <typename T> __device__ __forceinline__ void store_float(void* p, int64_t i, float v) {
+    if constexpr (std::is_same<T, float>::value) static_cast<float*>(p)[i] = v;
+    else if constexpr (std::is_same<T, __half>::value) static_cast<__half*>(p)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kXentCountThreads) xent_tiny_kernel(const XentNumberArgs n, const XentTinyArgs p) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    constexpr int kTurns = kXentSmallRows / kXentCountThreads;
+    extern __shared__ float tiny_smem[];
+    uint32_t* info = reinterpret_cast<uint32_t*>(tiny_smem);         // [labelled row]: row, label << 16
+    float* h_kept = tiny_smem + kXentSmallRows;
+    float* g_kept = h_kept + kXentTinyKept;
+    float* w = g_kept + kXentTinyKept;                                // [dim][classes]
+    float* room = w + kXentTinyProduct;
+    __shared__ int sums[kTurns][32];
+    __shared__ double losses_of[32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.dim, V = n.classes, rows = (int)n.rows;
+    // labels, and the rows without one
+    int y[kTurns];
+    unsigned ballot[kTurns];
+#pragma unroll
+    for (int k = 0; k < kTurns; k++) {
+        const int r = k * kXentCountThreads + threadIdx.x;
+        const int64_t label = r < rows ? n.labels[r] : -1;
+        y[k] = labelled(label, V) ? (int)label : -1;
+    }
+    for (int i = threadIdx.x; i < D * V; i += kXentCountThreads) {
+        const int d = i / V, v = i - d * V;
+        w[i] = load_float<T>(p.weight, d * p.w_dim_stride + v * p.w_class_stride);
+    }
+#pragma unroll
+    for (int k = 0; k < kTurns; k++) {
+        ballot[k] = __ballot_sync(0xffffffffu, y[k] >= 0);
+        if (lane == 0) sums[k][warp] = __popc(ballot[k]);
+    }
+    __syncthreads();
+    int count = 0;
+#pragma unroll
+    for (int k = 0; k < kTurns; k++) {
+        const int r = k * kXentCountThreads + threadIdx.x, in_warp = sums[k][lane];
+        const int before = __reduce_add_sync(0xffffffffu, lane < warp ? in_warp : 0);
+        if (y[k] >= 0) {
+            info[count + before + __popc(ballot[k] & ((1u << lane) - 1))] = (uint32_t)r | (uint32_t)y[k] << 16;
+        } else if (r < rows) {
+            if (n.row_loss) n.row_loss[r] = 0.f;
+            if (p.dhidden) {
+                T* to = static_cast<T*>(p.dhidden) + r * p.dhidden_stride;
+                int d = 0;
+                if ((reinterpret_cast<uintptr_t>(to) & 15) == 0)
+                    for (; d + 16 / (int)sizeof(T) <= D; d += 16 / (int)sizeof(T)) *reinterpret_cast<uint4*>(to + d) = make_uint4(0u, 0u, 0u, 0u);
+                for (; d < D; d++) store_float<T>(to, d, 0.f);
+            }
+        }
+        count += __reduce_add_sync(0xffffffffu, in_warp);
+    }
+    __syncthreads();
+    const float scale = xent_scale(p.scale, p.reduction == MASK_REDUCE_MEAN, count);
+    const bool keep = count * D <= kXentTinyKept && count * V <= kXentTinyKept;
+    if (keep) {
+        for (int i = threadIdx.x; i < count * D; i += kXentCountThreads) {
+            const int at = i / D;
+            h_kept[i] = load_float<T>(p.hidden, (int64_t)(info[at] & 0xffff) * p.hidden_stride + (i - at * D));
+        }
+        __syncthreads();
+    }
+    float* g_all = keep ? g_kept : p.g;
+    auto feature = [&](int i, int d) { return keep ? h_kept[i * D + d] : load_float<T>(p.hidden, (int64_t)(info[i] & 0xffff) * p.hidden_stride + d); };
+    double losses = 0.0;
+    for (int i = warp; i < count; i += 32) {
+        const int r = (int)(info[i] & 0xffff), label = (int)(info[i] >> 16);
+        float* g = g_all + i * V;
+        float top = -INFINITY, picked = 0.f;
+        for (int v = lane; v < V; v += 32) {
+            float s = 0.f;
+#pragma unroll 4
+            for (int d = 0; d < D; d++) s = fmaf(feature(i, d), w[d * V + v], s);
+            g[v] = s;
+            top = fmaxf(top, s);
+            if (v == label) picked = s;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            picked += __shfl_xor_sync(0xffffffffu, picked, o);
+        }
+        float sum = 0.f;
+        for (int v = lane; v < V; v += 32) sum += fast_exp2((g[v] - top) * kLog2e);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float loss = kLn2 * (fmaf(top - picked, kLog2e, log2f(sum)));
+        losses += loss;
+        if (lane == 0 && n.row_loss) n.row_loss[r] = loss;
+        if (!p.dhidden && !p.dweight) continue;
+        for (int v = lane; v < V; v += 32) {
+            const float e = fast_exp2((g[v] - top) * kLog2e) / sum;
+            g[v] = v == label ? e - 1.f : e;
+        }
+        __syncwarp();
+        if (p.dhidden) {
+            for (int d = lane; d < D; d += 32) {
+                float s = 0.f;
+#pragma unroll 4
+                for (int v = 0; v < V; v++) s = fmaf(g[v], w[d * V + v], s);
+                store_float<T>(p.dhidden, r * p.dhidden_stride + d, scale * s);
+            }
+        }
+    }
+    if (lane == 0) losses_of[warp] = losses;
+    __syncthreads();
+    if (threadIdx.x == 0 && !n.row_loss) {
+        double s = 0.0;
+        for (int i = 0; i < 32; i++) s += losses_of[i];
+        *p.loss = count == 0 ? 0.f : (float)(p.reduction == MASK_REDUCE_MEAN ? s / count : s);
+    }
+    if (!p.dweight) return;
+    const int shares = kXentCountThreads / (D * V), share = threadIdx.x / (D * V), pair = threadIdx.x - share * (D * V);
+    const int d = pair / V, v = pair - d * V;
+    float s = 0.f;
+    if (share < shares) {
+#pragma unroll 4
+        for (int i = share; i < count; i += shares) s = fmaf(g_all[i * V + v], feature(i, d), s);
+    }
+    room[threadIdx.x] = s;
+    __syncthreads();
+    if (share == 0) {
+        for (int i = 1; i < shares; i++) s += room[i * D * V + pair];
+        store_float<T>(p.dweight, d * p.dw_dim_stride + v * p.dw_class_stride, scale * s);
+    }
+}
+
+template <typename T>
+static int launch_xent_tiny(const XentNumberArgs& n, const XentTinyArgs& t, cudaStream_t st) {
+    static std::atomic<uint64_t> done{0};
+    const int rc = opt_in_shared_memory(reinterpret_cast<const void*>(xent_tiny_kernel<T>), kXentTinyBytes, done);
+    if (rc != MASK_OK) return rc;
+    return launch_overlapped(xent_tiny_kernel<T>, dim3(1), kXentCountThreads, kXentTinyBytes, st, n, t);
+}
+
 // ---- joining -----------------------------------------------------------------------------------------------
 // Log sums and losses of the rows from the parts of the classes: a block takes 1024 / shares rows, a warp 32 of them, and
 // `shares` (a power of two) threads a row, whose shares of the parts are joined in their order.
@@ -520,7 +693,7 @@ struct XentPlan {
     int planes, dim_pad;
     int64_t rows_pad, chunk;
     int n_chunks;
-    bool grads, one_pass, pack_weight, small;
+    bool grads, one_pass, pack_weight, small, tiny;
     int bn_logits, bn_dim;
     int stats_splits, stats_parts;       // parts of the classes' tiles, and numbers a row gets from them
     int piece, n_pieces;                 // classes of a piece (a multiple of 256 unless one tile holds all), pieces
@@ -598,6 +771,7 @@ static XentPlan plan_xent(const mask_head& h) {
             p.part_dw_rows = round_up(p.piece, kXentTileM);
         }
     }
+    p.tiny = h.rows <= kXentSmallRows && (int64_t)h.dim * h.classes <= kXentTinyProduct && h.rows * h.dim * h.classes <= kXentTinyWork;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -609,6 +783,13 @@ static XentPlan plan_xent(const mask_head& h) {
     p.counts = take(4 * (size_t)p.n_chunks);
     p.row_of = take(4 * rp);
     p.label = take(4 * rp);
+    if (p.tiny) {
+        p.chunk = kXentSmallRows;
+        p.n_chunks = 1;
+        p.g = take(4 * (size_t)(h.rows * h.classes));
+        p.bytes = at;
+        return p;
+    }
     p.stats = p.one_pass ? 0 : take(8 * rp * p.stats_parts);
     p.label_logit = take(4 * rp);
     p.lse2 = take(4 * rp);
@@ -719,6 +900,14 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
 
     int rc = MASK_OK;
     const XentNumberArgs number = {h.d_labels, h.rows, plan.chunk, h.classes, counts, row_of, label, total, total + 1, range, row_loss};
+    if (plan.tiny) {
+        const XentTinyArgs t = {h.d_hidden, h.hidden_stride, h.d_weight, h.weight_dim_stride, h.weight_class_stride, h.d_dhidden, h.dhidden_stride, h.d_dweight,
+                                h.dweight_dim_stride, h.dweight_class_stride, h.dim, reinterpret_cast<float*>(at(plan.g)), h.d_loss, h.reduction, h.grad_scale};
+        if (h.dtype == MASK_F32) return launch_xent_tiny<float>(number, t, st);
+        if (h.dtype == MASK_F16) return launch_xent_tiny<__half>(number, t, st);
+        return launch_xent_tiny<__nv_bfloat16>(number, t, st);
+    }
+
     XentPackArgs pk = {};
     pk.dtype = h.dtype; pk.dim = h.dim; pk.dim_pad = plan.dim_pad; pk.classes = h.classes; pk.rows = h.rows;
     pk.count = total; pk.row_of = row_of; pk.labels = h.d_labels;

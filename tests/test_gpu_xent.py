@@ -131,6 +131,15 @@ def test_labels(reduction, labelled, classes):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,dim,classes", [(2708, 16, 7), (512, 64, 16), (512, 16, 64), (512, 1024, 1), (1, 1, 1024), (4096, 2, 64), (4097, 2, 60), (700, 5, 150)])
+def test_few_products(rows, dim, classes, dtype):
+    """Around the sizes up to which one block takes the whole head."""
+    for labelled in ("some", "all"):
+        _both(*_inputs(rows, dim, classes, dtype, "class" if labelled == "some" else "dim", labelled, seed=6), scale=256.0 if dtype == "f16" else 1.0)
+
+
+@gpu
 @pytest.mark.parametrize("rows", [3000, 70001])
 def test_many_chunks_of_labels(rows):
     """More rows than one block numbers, in unequal chunks."""
