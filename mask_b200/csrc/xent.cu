@@ -400,110 +400,68 @@ template <typename T> __device__ __forceinline__ void store_float(void* p, int64
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kXentCountThreads) xent_tiny_kernel(const XentNumberArgs n, const XentTinyArgs p) {
-    wait_for_previous_kernel();
-    let_next_kernel_start();
-    constexpr int kTurns = kXentSmallRows / kXentCountThreads;
-    extern __shared__ float tiny_smem[];
-    uint32_t* info = reinterpret_cast<uint32_t*>(tiny_smem);         // [labelled row]: row, label << 16
-    float* h_kept = tiny_smem + kXentSmallRows;
-    float* g_kept = h_kept + kXentTinyKept;
-    float* w = g_kept + kXentTinyKept;                                // [dim][classes]
-    float* room = w + kXentTinyProduct;
-    __shared__ int sums[kTurns][32];
+// Loss, G and gradients of `count` labelled rows (info: row, label << 16); kKept: their features and G are in shared memory.
+template <typename T, bool kKept>
+__device__ __forceinline__ void tiny_rows(const XentNumberArgs& n, const XentTinyArgs& p, int count, const uint32_t* info, const float* h_kept, float* g_all,
+                                          const float* w, float* room) {
     __shared__ double losses_of[32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.dim, V = n.classes, rows = (int)n.rows;
-    // labels, and the rows without one
-    int y[kTurns];
-    unsigned ballot[kTurns];
-#pragma unroll
-    for (int k = 0; k < kTurns; k++) {
-        const int r = k * kXentCountThreads + threadIdx.x;
-        const int64_t label = r < rows ? n.labels[r] : -1;
-        y[k] = labelled(label, V) ? (int)label : -1;
-    }
-    for (int i = threadIdx.x; i < D * V; i += kXentCountThreads) {
-        const int d = i / V, v = i - d * V;
-        w[i] = load_float<T>(p.weight, d * p.w_dim_stride + v * p.w_class_stride);
-    }
-#pragma unroll
-    for (int k = 0; k < kTurns; k++) {
-        ballot[k] = __ballot_sync(0xffffffffu, y[k] >= 0);
-        if (lane == 0) sums[k][warp] = __popc(ballot[k]);
-    }
-    __syncthreads();
-    int count = 0;
-#pragma unroll
-    for (int k = 0; k < kTurns; k++) {
-        const int r = k * kXentCountThreads + threadIdx.x, in_warp = sums[k][lane];
-        const int before = __reduce_add_sync(0xffffffffu, lane < warp ? in_warp : 0);
-        if (y[k] >= 0) {
-            info[count + before + __popc(ballot[k] & ((1u << lane) - 1))] = (uint32_t)r | (uint32_t)y[k] << 16;
-        } else if (r < rows) {
-            if (n.row_loss) n.row_loss[r] = 0.f;
-            if (p.dhidden) {
-                T* to = static_cast<T*>(p.dhidden) + r * p.dhidden_stride;
-                int d = 0;
-                if ((reinterpret_cast<uintptr_t>(to) & 15) == 0)
-                    for (; d + 16 / (int)sizeof(T) <= D; d += 16 / (int)sizeof(T)) *reinterpret_cast<uint4*>(to + d) = make_uint4(0u, 0u, 0u, 0u);
-                for (; d < D; d++) store_float<T>(to, d, 0.f);
-            }
-        }
-        count += __reduce_add_sync(0xffffffffu, in_warp);
-    }
-    __syncthreads();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.dim, V = n.classes;
     const float scale = xent_scale(p.scale, p.reduction == MASK_REDUCE_MEAN, count);
-    const bool keep = count * D <= kXentTinyKept && count * V <= kXentTinyKept;
-    if (keep) {
-        for (int i = threadIdx.x; i < count * D; i += kXentCountThreads) {
-            const int at = i / D;
-            h_kept[i] = load_float<T>(p.hidden, (int64_t)(info[at] & 0xffff) * p.hidden_stride + (i - at * D));
-        }
-        __syncthreads();
-    }
-    float* g_all = keep ? g_kept : p.g;
-    auto feature = [&](int i, int d) { return keep ? h_kept[i * D + d] : load_float<T>(p.hidden, (int64_t)(info[i] & 0xffff) * p.hidden_stride + d); };
+    auto feature = [&](int i, int d) {
+        if constexpr (kKept) return h_kept[i * D + d];
+        else return load_float<T>(p.hidden, (int64_t)(info[i] & 0xffff) * p.hidden_stride + d);
+    };
+    // a warp takes as many rows at a time as have room for their classes side by side
+    int width = 1;
+    while (width < 32 && width < V) width *= 2;
+    const int sub = lane & (width - 1), at_once = 32 / width;
     double losses = 0.0;
-    for (int i = warp; i < count; i += 32) {
-        const int r = (int)(info[i] & 0xffff), label = (int)(info[i] >> 16);
-        float* g = g_all + i * V;
-        float top = -INFINITY, picked = 0.f;
-        for (int v = lane; v < V; v += 32) {
+    for (int i0 = warp * at_once; i0 < count; i0 += 32 * at_once) {
+        const int i = i0 + lane / width;
+        const bool live = i < count;
+        const int row = live ? i : 0, label = (int)(info[row] >> 16);
+        float* g = g_all + row * V;
+        float top = -INFINITY, picked = 0.f, first = 0.f;
+        for (int v = sub; v < V; v += width) {
             float s = 0.f;
-#pragma unroll 4
-            for (int d = 0; d < D; d++) s = fmaf(feature(i, d), w[d * V + v], s);
-            g[v] = s;
+#pragma unroll 8
+            for (int d = 0; d < D; d++) s = fmaf(feature(row, d), w[d * V + v], s);
+            if (v == sub) first = s;
+            else if (live) g[v] = s;
             top = fmaxf(top, s);
             if (v == label) picked = s;
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
+        for (int o = width / 2; o > 0; o >>= 1) {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             picked += __shfl_xor_sync(0xffffffffu, picked, o);
         }
-        float sum = 0.f;
-        for (int v = lane; v < V; v += 32) sum += fast_exp2((g[v] - top) * kLog2e);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float loss = kLn2 * (fmaf(top - picked, kLog2e, log2f(sum)));
-        losses += loss;
-        if (lane == 0 && n.row_loss) n.row_loss[r] = loss;
+        float sum = sub < V ? fast_exp2((first - top) * kLog2e) : 0.f;
+        const float e_first = sum;
+        for (int v = sub + width; v < V; v += width) sum += fast_exp2((g[v] - top) * kLog2e);
+        for (int o = width / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float loss = live ? kLn2 * fmaf(top - picked, kLog2e, log2f(sum)) : 0.f;
+        if (sub == 0) {
+            losses += loss;
+            if (live && n.row_loss) n.row_loss[info[row] & 0xffff] = loss;
+        }
         if (!p.dhidden && !p.dweight) continue;
-        for (int v = lane; v < V; v += 32) {
-            const float e = fast_exp2((g[v] - top) * kLog2e) / sum;
-            g[v] = v == label ? e - 1.f : e;
+        const float inv = 1.f / sum;
+        for (int v = sub; v < V; v += width) {
+            const float e = (v == sub ? e_first : fast_exp2((g[v] - top) * kLog2e)) * inv;
+            if (live) g[v] = v == label ? e - 1.f : e;
         }
         __syncwarp();
-        if (p.dhidden) {
-            for (int d = lane; d < D; d += 32) {
+        if (p.dhidden && live) {
+            const int64_t to = (int64_t)(info[row] & 0xffff) * p.dhidden_stride;
+            for (int d = sub; d < D; d += width) {
                 float s = 0.f;
-#pragma unroll 4
+#pragma unroll 8
                 for (int v = 0; v < V; v++) s = fmaf(g[v], w[d * V + v], s);
-                store_float<T>(p.dhidden, r * p.dhidden_stride + d, scale * s);
+                store_float<T>(p.dhidden, to + d, scale * s);
             }
         }
     }
+    for (int o = 16; o > 0; o >>= 1) losses += __shfl_xor_sync(0xffffffffu, losses, o);
     if (lane == 0) losses_of[warp] = losses;
     __syncthreads();
     if (threadIdx.x == 0 && !n.row_loss) {
@@ -524,6 +482,80 @@ __global__ void __launch_bounds__(kXentCountThreads) xent_tiny_kernel(const Xent
     if (share == 0) {
         for (int i = 1; i < shares; i++) s += room[i * D * V + pair];
         store_float<T>(p.dweight, d * p.dw_dim_stride + v * p.dw_class_stride, scale * s);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kXentCountThreads) xent_tiny_kernel(const XentNumberArgs n, const XentTinyArgs p) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    constexpr int kTurns = kXentSmallRows / kXentCountThreads;
+    extern __shared__ float tiny_smem[];
+    uint32_t* info = reinterpret_cast<uint32_t*>(tiny_smem);         // [labelled row]: row, label << 16
+    float* h_kept = tiny_smem + kXentSmallRows;
+    float* g_kept = h_kept + kXentTinyKept;
+    float* w = g_kept + kXentTinyKept;                                // [dim][classes]
+    float* room = w + kXentTinyProduct;
+    __shared__ int sums[kTurns][32];
+    __shared__ uint32_t have[kXentSmallRows / 32];                    // a bit for each row: labelled
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.dim, V = n.classes, rows = (int)n.rows;
+    // labels, and the rows without one
+    int y[kTurns];
+    unsigned ballot[kTurns];
+#pragma unroll
+    for (int k = 0; k < kTurns; k++) {
+        const int r = k * kXentCountThreads + threadIdx.x;
+        const int64_t label = r < rows ? n.labels[r] : -1;
+        y[k] = labelled(label, V) ? (int)label : -1;
+    }
+    for (int i = threadIdx.x; i < D * V; i += kXentCountThreads) {
+        const int d = i / V, v = i - d * V;
+        w[i] = load_float<T>(p.weight, d * p.w_dim_stride + v * p.w_class_stride);
+    }
+#pragma unroll
+    for (int k = 0; k < kTurns; k++) {
+        ballot[k] = __ballot_sync(0xffffffffu, y[k] >= 0);
+        if (lane == 0) {
+            sums[k][warp] = __popc(ballot[k]);
+            have[k * 32 + warp] = ballot[k];
+        }
+    }
+    __syncthreads();
+    int count = 0;
+#pragma unroll
+    for (int k = 0; k < kTurns; k++) {
+        const int r = k * kXentCountThreads + threadIdx.x, in_warp = sums[k][lane];
+        const int before = __reduce_add_sync(0xffffffffu, lane < warp ? in_warp : 0);
+        if (y[k] >= 0) {
+            info[count + before + __popc(ballot[k] & ((1u << lane) - 1))] = (uint32_t)r | (uint32_t)y[k] << 16;
+        } else if (r < rows && n.row_loss) {
+            n.row_loss[r] = 0.f;
+        }
+        count += __reduce_add_sync(0xffffffffu, in_warp);
+    }
+    __syncthreads();
+    if (p.dhidden) {
+        // rows without a label, neighbouring threads at neighbouring addresses
+        constexpr int kWide = 16 / (int)sizeof(T);
+        const bool vec = (reinterpret_cast<uintptr_t>(p.dhidden) & 15) == 0 && p.dhidden_stride % kWide == 0 && D % kWide == 0;
+        const int pieces = vec ? D / kWide : D;
+        for (int i = threadIdx.x; i < rows * pieces; i += kXentCountThreads) {
+            const int r = i / pieces, piece = i - r * pieces;
+            if (have[r >> 5] >> (r & 31) & 1) continue;
+            T* to = static_cast<T*>(p.dhidden) + r * p.dhidden_stride;
+            if (vec) reinterpret_cast<uint4*>(to)[piece] = make_uint4(0u, 0u, 0u, 0u);
+            else store_float<T>(to, piece, 0.f);
+        }
+    }
+    if (count * D <= kXentTinyKept && count * V <= kXentTinyKept) {
+        for (int i = threadIdx.x; i < count * D; i += kXentCountThreads) {
+            const int at = i / D;
+            h_kept[i] = load_float<T>(p.hidden, (int64_t)(info[at] & 0xffff) * p.hidden_stride + (i - at * D));
+        }
+        __syncthreads();
+        tiny_rows<T, true>(n, p, count, info, h_kept, g_kept, w, room);
+    } else {
+        tiny_rows<T, false>(n, p, count, info, nullptr, p.g, w, room);
     }
 }
 
