@@ -30,24 +30,6 @@ constexpr size_t kXentPieceBytes = (size_t)512 << 20;   // what a piece of G may
 // ---- numbering of the labelled rows ------------------------------------------------------------------
 __device__ __forceinline__ bool labelled(int64_t y, int32_t classes) { return y >= 0 && y < classes; }
 
-// One block per chunk of rows: how many of them are labelled.
-__global__ void __launch_bounds__(kXentCountThreads) xent_count_kernel(const int64_t* __restrict__ labels, int64_t rows, int32_t classes, int64_t chunk,
-                                                                       int32_t* __restrict__ counts) {
-    wait_for_previous_kernel();
-    let_next_kernel_start();
-    __shared__ int sums[32];
-    const int64_t r0 = blockIdx.x * chunk, r1 = min(rows, r0 + chunk);
-    int n = 0;
-    for (int64_t r = r0 + threadIdx.x; r < r1; r += kXentCountThreads) n += labelled(labels[r], classes);
-    n = __reduce_add_sync(0xffffffffu, n);
-    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = n;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        n = __reduce_add_sync(0xffffffffu, sums[threadIdx.x]);
-        if (threadIdx.x == 0) counts[blockIdx.x] = n;
-    }
-}
-
 struct XentNumberArgs {
     const int64_t* labels;
     int64_t rows, chunk;
@@ -58,8 +40,27 @@ struct XentNumberArgs {
     int32_t* total;
     int32_t* status;
     uint32_t* range;
+    const uint2* ranges;       // what the scan's blocks found, or NULL: to be found later
+    int32_t n_ranges;
     float* row_loss;
 };
+
+// The largest of all threads' values, for thread 0.
+__device__ __forceinline__ void block_max(uint32_t (&most)[2]) {
+    __shared__ uint32_t room[2];
+    if (threadIdx.x < 2) room[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, most[k]);
+        if ((threadIdx.x & 31) == 0 && m) atomicMax(room + k, m);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        most[0] = room[0];
+        most[1] = room[1];
+    }
+}
 
 // Writes row_of and label of the block's chunk of rows behind those of the chunks before it; the last block leaves the
 // total.  Losses of rows without a label are set to 0 here.
@@ -92,10 +93,21 @@ __device__ __forceinline__ void number_rows(const XentNumberArgs& p) {
         }
         at += __reduce_add_sync(0xffffffffu, in_warp);
     }
-    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) {
+    if (blockIdx.x < gridDim.x - 1) return;
+    uint32_t most[2] = {0, 0};
+    if (p.ranges) {
+        for (int i = threadIdx.x; i < p.n_ranges; i += kXentCountThreads) {
+            const uint2 m = p.ranges[i];
+            most[0] = max(most[0], m.x);
+            most[1] = max(most[1], m.y);
+        }
+        block_max(most);
+    }
+    if (threadIdx.x == 0) {
         *p.total = at;
         *p.status = 0;
-        p.range[0] = p.range[1] = 0;
+        p.range[0] = most[0];
+        p.range[1] = most[1];
     }
 }
 __global__ void __launch_bounds__(kXentCountThreads) xent_number_kernel(const XentNumberArgs p) {
@@ -121,6 +133,7 @@ struct XentPackArgs {
     int64_t w_plane;
     void* dhidden;             // rows without a label are set to 0
     int64_t dhidden_stride;
+    bool cleared;
     uint32_t* range;           // FP32: bits of the largest finite magnitude of the labelled rows of hidden, and of weight
 };
 
@@ -136,60 +149,122 @@ __device__ __forceinline__ int lanes_for(int n) {
     return g;
 }
 
+// Rows base(i) of n values, `stride` apart: the largest finite magnitude.  A thread has four rows in flight.
+template <typename Base>
+__device__ __forceinline__ void scan_rows(int64_t rows, int64_t n, int64_t stride, int lanes, int64_t w0, int64_t warps, Base base, uint32_t& m) {
+    const int lane = threadIdx.x & 31, sub = lane & (lanes - 1), side = 32 / lanes;
+    const int64_t step = warps * side;
+    for (int64_t i = w0 * side + lane / lanes; i < rows; i += 4 * step) {
+        const float* row[4];
+        bool vec = stride == 1;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            row[k] = base(min(i + k * step, rows - 1));
+            vec = vec && (reinterpret_cast<uintptr_t>(row[k]) & 15) == 0;
+        }
+        int64_t d = 4 * sub;
+        if (vec) {
+            for (; d + 4 <= n; d += 4 * lanes) {
+                float4 v[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = __ldg(reinterpret_cast<const float4*>(row[k] + d));
+#pragma unroll
+                for (int k = 0; k < 4; k++) m = max(m, max(max(finite_magnitude(v[k].x), finite_magnitude(v[k].y)), max(finite_magnitude(v[k].z), finite_magnitude(v[k].w))));
+            }
+        }
+        for (; d < n; d += 4 * lanes)
+            for (int64_t e = d; e < min(d + 4, n); e++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) m = max(m, finite_magnitude(__ldg(row[k] + e * stride)));
+    }
+}
+__device__ __forceinline__ void scan_weight(const XentPackArgs& p, int64_t w0, int64_t warps, uint32_t& m) {
+    const float* weight = static_cast<const float*>(p.weight);
+    if (p.w_class_stride == 1)
+        scan_rows(p.dim, p.classes, 1, 32, w0, warps, [&](int64_t d) { return weight + d * p.w_dim_stride; }, m);
+    else
+        scan_rows(p.classes, p.dim, p.w_dim_stride, lanes_for(p.dim), w0, warps, [&](int64_t v) { return weight + v * p.w_class_stride; }, m);
+}
+
 // The largest finite magnitudes of both operands (FP32 input) to p.range.  A maximum does not depend on the order.
 __device__ __forceinline__ void find_range(const XentPackArgs& p, int64_t w0, int64_t warps) {
-    const int lane = threadIdx.x & 31;
     const float* hidden = static_cast<const float*>(p.hidden);
-    const float* weight = static_cast<const float*>(p.weight);
     uint32_t most[2] = {0, 0};
-    // rows i of n values, `stride` apart, at base(i); a thread has four rows in flight
-    auto scan = [&](int64_t rows, int64_t n, int64_t stride, int lanes, auto base, uint32_t& m) {
-        const int sub = lane & (lanes - 1), side = 32 / lanes;
-        const int64_t step = warps * side;
-        for (int64_t i = w0 * side + lane / lanes; i < rows; i += 4 * step) {
-            const float* row[4];
-            bool vec = stride == 1;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                row[k] = base(min(i + k * step, rows - 1));
-                vec = vec && (reinterpret_cast<uintptr_t>(row[k]) & 15) == 0;
-            }
-            int64_t d = 4 * sub;
-            if (vec) {
-                for (; d + 4 <= n; d += 4 * lanes) {
-                    float4 v[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) v[k] = __ldg(reinterpret_cast<const float4*>(row[k] + d));
-#pragma unroll
-                    for (int k = 0; k < 4; k++) m = max(m, max(max(finite_magnitude(v[k].x), finite_magnitude(v[k].y)), max(finite_magnitude(v[k].z), finite_magnitude(v[k].w))));
-                }
-            }
-            for (; d < n; d += 4 * lanes)
-                for (int64_t e = d; e < min(d + 4, n); e++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) m = max(m, finite_magnitude(__ldg(row[k] + e * stride)));
-        }
-    };
-    scan(*p.count, p.dim, 1, lanes_for(p.dim), [&](int64_t i) { return hidden + p.row_of[i] * p.hidden_stride; }, most[0]);
-    if (p.w_class_stride == 1)
-        scan(p.dim, p.classes, 1, 32, [&](int64_t d) { return weight + d * p.w_dim_stride; }, most[1]);
-    else
-        scan(p.classes, p.dim, p.w_dim_stride, lanes_for(p.dim), [&](int64_t v) { return weight + v * p.w_class_stride; }, most[1]);
-    __shared__ uint32_t room[2];
-    if (threadIdx.x < 2) room[threadIdx.x] = 0;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 2; k++) {
-        const uint32_t m = __reduce_max_sync(0xffffffffu, most[k]);
-        if (lane == 0 && m) atomicMax(room + k, m);
+    scan_rows(*p.count, p.dim, 1, lanes_for(p.dim), w0, warps, [&](int64_t i) { return hidden + p.row_of[i] * p.hidden_stride; }, most[0]);
+    scan_weight(p, w0, warps, most[1]);
+    block_max(most);
+    if (threadIdx.x == 0) {
+        if (most[0]) atomicMax(p.range, most[0]);
+        if (most[1]) atomicMax(p.range + 1, most[1]);
     }
-    __syncthreads();
-    if (threadIdx.x < 2 && room[threadIdx.x]) atomicMax(p.range + threadIdx.x, room[threadIdx.x]);
 }
 __global__ void __launch_bounds__(256) xent_range_kernel(const XentPackArgs p) {
     wait_for_previous_kernel();
     let_next_kernel_start();
     find_range(p, grid_warp(), (int64_t)gridDim.x * 8);
+}
+
+// Zeros to the rows of dhidden, among the 32 from r0, that `clear` has a bit for; by a warp.
+template <bool kFloat>
+__device__ __forceinline__ void clear_rows(const XentPackArgs& p, int64_t r0, unsigned clear) {
+    constexpr int kBytes = kFloat ? 4 : 2;
+    if (!clear) return;
+    const int lane = threadIdx.x & 31, bytes = p.dim * kBytes;
+    const bool vec = (reinterpret_cast<uintptr_t>(p.dhidden) & 15) == 0 && p.dhidden_stride * kBytes % 16 == 0 && bytes % 16 == 0;
+    char* to = static_cast<char*>(p.dhidden) + r0 * p.dhidden_stride * kBytes;
+    const int pieces = vec ? bytes / 16 : p.dim;       // of a row
+    int row = lane / pieces, piece = lane % pieces;    // lanes go through the rows' pieces one after the other
+    const int rows_on = 32 / pieces, pieces_on = 32 % pieces;
+    while (row < 32) {
+        if (clear >> row & 1) {
+            char* at = to + row * p.dhidden_stride * kBytes;
+            if (vec) *reinterpret_cast<uint4*>(at + 16 * piece) = make_uint4(0u, 0u, 0u, 0u);
+            else if constexpr (kFloat) reinterpret_cast<float*>(at)[piece] = 0.f;
+            else reinterpret_cast<uint16_t*>(at)[piece] = 0;
+        }
+        row += rows_on;
+        piece += pieces_on;
+        if (piece >= pieces) { piece -= pieces; row++; }
+    }
+}
+
+// What of many rows needs no numbers yet, in one pass: a block per chunk counts its labelled rows, takes their largest
+// magnitude (FP32) and clears the other rows of dhidden; the blocks behind those take the weight's.
+template <bool kFloat>
+__global__ void __launch_bounds__(kXentCountThreads) xent_scan_kernel(const XentPackArgs p, int64_t chunk, int n_chunks, int32_t* __restrict__ counts,
+                                                                      uint2* __restrict__ ranges) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t most[2] = {0, 0};
+    if ((int)blockIdx.x < n_chunks) {
+        __shared__ int sums[32];
+        const float* hidden = static_cast<const float*>(p.hidden);
+        const int64_t r1 = min(p.rows, (blockIdx.x + 1) * chunk);
+        const int lanes = lanes_for(p.dim);
+        int n = 0;
+        for (int64_t rb = blockIdx.x * chunk + 32 * warp; rb < r1; rb += kXentCountThreads) {
+            const int64_t r = rb + lane;
+            const bool mine = r < r1 && labelled(p.labels[min(r, r1 - 1)], p.classes);
+            const unsigned have = __ballot_sync(0xffffffffu, mine), clear = __ballot_sync(0xffffffffu, !mine && r < r1);
+            n += __popc(have);
+            if constexpr (kFloat)
+                scan_rows(__popc(have), p.dim, 1, lanes, 0, 1, [&](int64_t i) { return hidden + (rb + __fns(have, 0, (int)i + 1)) * p.hidden_stride; }, most[0]);
+            if (p.dhidden) clear_rows<kFloat>(p, rb, clear);
+        }
+        if (lane == 0) sums[warp] = n;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            n = __reduce_add_sync(0xffffffffu, sums[threadIdx.x]);
+            if (threadIdx.x == 0) counts[blockIdx.x] = n;
+        }
+    } else if constexpr (kFloat) {
+        scan_weight(p, (int64_t)(blockIdx.x - n_chunks) * 32 + warp, (int64_t)(gridDim.x - n_chunks) * 32, most[1]);
+    }
+    if constexpr (kFloat) {
+        block_max(most);
+        if (threadIdx.x == 0) ranges[blockIdx.x] = make_uint2(most[0], most[1]);
+    }
 }
 
 // hi and lo of a scaled float; an infinite or NaN hi has no lo
@@ -242,7 +317,7 @@ __device__ __forceinline__ void pack_row(const void* src, int64_t stride, int di
 template <bool kFloat>
 __device__ __forceinline__ float plane_scale(const XentPackArgs& p, int operand) { return kFloat ? exp2f((float)(14 - plane_exponent(__ldcg(p.range + operand)))) : 1.f; }
 
-// The labelled rows to their planes; zeros to dhidden's other rows.
+// The labelled rows to their planes; zeros to dhidden's other rows, unless they have been cleared.
 template <bool kFloat>
 __device__ __forceinline__ void pack_hidden(const XentPackArgs& p, int64_t w0, int64_t warps) {
     constexpr int kBytes = kFloat ? 4 : 2;
@@ -262,29 +337,10 @@ __device__ __forceinline__ void pack_hidden(const XentPackArgs& p, int64_t w0, i
         if (i + step < end)
             pack_row<kFloat>(b, 1, p.dim, p.dim_pad, p.h_planes + (i + step) * p.dim_pad, p.h_plane, h_scale, lane & (lanes - 1), lanes);
     }
-    if (p.dhidden && count < p.rows) {
-        // a warp looks at 32 labels and then clears the rows without one
-        const int bytes = p.dim * kBytes;
-        const bool vec = (reinterpret_cast<uintptr_t>(p.dhidden) & 15) == 0 && p.dhidden_stride * kBytes % 16 == 0 && bytes % 16 == 0;
+    if (p.dhidden && !p.cleared && count < p.rows) {
         for (int64_t r0 = 32 * w0; r0 < p.rows; r0 += 32 * warps) {
             const int64_t r = r0 + lane;
-            const unsigned clear = __ballot_sync(0xffffffffu, r < p.rows && !labelled(p.labels[min(r, p.rows - 1)], p.classes));
-            if (!clear) continue;
-            char* to = static_cast<char*>(p.dhidden) + r0 * p.dhidden_stride * kBytes;
-            const int pieces = vec ? bytes / 16 : p.dim;       // of a row
-            int row = lane / pieces, piece = lane % pieces;    // lanes go through the rows' pieces one after the other
-            const int rows_on = 32 / pieces, pieces_on = 32 % pieces;
-            while (row < 32) {
-                if (clear >> row & 1) {
-                    char* at = to + row * p.dhidden_stride * kBytes;
-                    if (vec) *reinterpret_cast<uint4*>(at + 16 * piece) = make_uint4(0u, 0u, 0u, 0u);
-                    else if constexpr (kFloat) reinterpret_cast<float*>(at)[piece] = 0.f;
-                    else reinterpret_cast<uint16_t*>(at)[piece] = 0;
-                }
-                row += rows_on;
-                piece += pieces_on;
-                if (piece >= pieces) { piece -= pieces; row++; }
-            }
+            clear_rows<kFloat>(p, r0, __ballot_sync(0xffffffffu, r < p.rows && !labelled(p.labels[min(r, p.rows - 1)], p.classes)));
         }
     }
 }
@@ -724,7 +780,7 @@ static int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 struct XentPlan {
     int planes, dim_pad;
     int64_t rows_pad, chunk;
-    int n_chunks;
+    int n_chunks, weight_blocks;
     bool grads, one_pass, pack_weight, small, tiny;
     int bn_logits, bn_dim;
     int stats_splits, stats_parts;       // parts of the classes' tiles, and numbers a row gets from them
@@ -735,7 +791,7 @@ struct XentPlan {
     int64_t part_dh_rows, part_dw_rows;
     int part_ld;
     // byte offsets into the scratch
-    size_t counts, row_of, label, total, stats, label_logit, lse2, warp_loss, h_planes, w_planes, g, part_dh, part_dw, bytes;
+    size_t counts, ranges, row_of, label, total, stats, label_logit, lse2, warp_loss, h_planes, w_planes, g, part_dh, part_dw, bytes;
 };
 
 // Blocks that share a tile of `bn` columns of a product with so many rows.  Pairs load a third less (dH of 16384 x 16384 x 512:
@@ -813,6 +869,8 @@ static XentPlan plan_xent(const mask_head& h) {
     const size_t rp = (size_t)p.rows_pad;
     p.total = take(256);
     p.counts = take(4 * (size_t)p.n_chunks);
+    p.weight_blocks = (int)std::min<int64_t>(sm_count(), ((int64_t)h.dim * h.classes + 32767) / 32768);
+    p.ranges = take(8 * (size_t)(p.n_chunks + p.weight_blocks));
     p.row_of = take(4 * rp);
     p.label = take(4 * rp);
     if (p.tiny) {
@@ -931,7 +989,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
     const int64_t rp = plan.rows_pad;
 
     int rc = MASK_OK;
-    const XentNumberArgs number = {h.d_labels, h.rows, plan.chunk, h.classes, counts, row_of, label, total, total + 1, range, row_loss};
+    XentNumberArgs number = {h.d_labels, h.rows, plan.chunk, h.classes, counts, row_of, label, total, total + 1, range, nullptr, 0, row_loss};
     if (plan.tiny) {
         const XentTinyArgs t = {h.d_hidden, h.hidden_stride, h.d_weight, h.weight_dim_stride, h.weight_class_stride, h.d_dhidden, h.dhidden_stride, h.d_dweight,
                                 h.dweight_dim_stride, h.dweight_class_stride, h.dim, reinterpret_cast<float*>(at(plan.g)), h.d_loss, h.reduction, h.grad_scale};
@@ -957,13 +1015,21 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
         if (rc) return rc;
     } else {
         const dim3 chunks((unsigned)plan.n_chunks);
-        if (plan.n_chunks > 1 && (rc = launch_overlapped(xent_count_kernel, chunks, kXentCountThreads, 0, st, h.d_labels, h.rows, h.classes, plan.chunk, counts)))
-            return rc;
+        if (plan.n_chunks > 1) {
+            // a block per chunk, and for the weight at most one an SM
+            const int blocks = plan.n_chunks + (P == 2 ? plan.weight_blocks : 0);
+            uint2* ranges = reinterpret_cast<uint2*>(at(plan.ranges));
+            if (P == 2) rc = launch_overlapped(xent_scan_kernel<true>, dim3((unsigned)blocks), kXentCountThreads, 0, st, pk, plan.chunk, plan.n_chunks, counts, ranges);
+            else rc = launch_overlapped(xent_scan_kernel<false>, dim3((unsigned)blocks), kXentCountThreads, 0, st, pk, plan.chunk, plan.n_chunks, counts, ranges);
+            if (rc) return rc;
+            pk.cleared = true;
+            if (P == 2) number.ranges = ranges, number.n_ranges = blocks;
+        }
         if ((rc = launch_overlapped(xent_number_kernel, chunks, kXentCountThreads, 0, st, number))) return rc;
         const int64_t pack_rows = rp + (plan.pack_weight ? h.classes : 0);
         const dim3 pack_grid((unsigned)std::min<int64_t>((pack_rows + 7) / 8, 8 * (int64_t)sm_count()));
-        if (h.dtype == MASK_F32) {
-            if ((rc = launch_overlapped(xent_range_kernel, pack_grid, 256, 0, st, pk))) return rc;
+        if (P == 2) {
+            if (plan.n_chunks == 1 && (rc = launch_overlapped(xent_range_kernel, pack_grid, 256, 0, st, pk))) return rc;
             rc = launch_overlapped(xent_pack_kernel<true>, pack_grid, kXentPackThreads, 0, st, pk);
         } else {
             rc = launch_overlapped(xent_pack_kernel<false>, pack_grid, kXentPackThreads, 0, st, pk);
