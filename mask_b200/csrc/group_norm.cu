@@ -36,8 +36,8 @@ struct NormArgs {
     float eps;
     int32_t chunk;              // rows
     uint64_t chunk_inverse;     // 2^64 / chunk, rounded up: the high half of a product with it is a quotient (rows < 2^31)
-    int32_t tx;                 // threads along the channels (a power of two), 256 / tx along the rows
-    int32_t whole;              // slabs hold whole groups
+    int32_t tx;                 // threads along the channels, 256 / tx along the rows
+    int64_t handled;            // graphs of up to so many rows are finished by the first kernel (slabs hold whole groups)
     const int32_t* offsets;     // or NULL: one graph
     const void* x;
     int64_t x_stride;
@@ -183,7 +183,7 @@ struct Chunk {
     int graph;
     int64_t row;
     int n;                  // rows, 0: no such chunk
-    bool alone;             // the graph's only one
+    bool handled;           // the graph is one that the first kernel finishes
 };
 // All lanes of a warp: 32 graphs are looked at at a time.
 __device__ __forceinline__ Chunk chunk_of(const NormArgs& p, int64_t number) {
@@ -199,7 +199,7 @@ __device__ __forceinline__ Chunk chunk_of(const NormArgs& p, int64_t number) {
     const Graph g = graph_of(p, lo);
     const int64_t row = g.begin + (number - g.first) * p.chunk;
     const bool real = number >= g.first && row < g.end;
-    return {lo, row, real ? (int)min((int64_t)p.chunk, g.end - row) : 0, g.end - g.begin <= p.chunk};
+    return {lo, row, real ? (int)min((int64_t)p.chunk, g.end - row) : 0, g.end - g.begin <= p.handled};
 }
 
 struct Place {
@@ -209,11 +209,11 @@ struct Place {
 template <int VEC>
 __device__ __forceinline__ Place place_of(const NormArgs& p) {
     Place at;
-    at.tx = threadIdx.x & (p.tx - 1);
     at.ty = threadIdx.x / p.tx;
+    at.tx = threadIdx.x - at.ty * p.tx;
     at.rows = kNormThreads / p.tx;
     at.c = (blockIdx.y * p.tx + at.tx) * VEC;
-    at.live = at.c < p.channels;
+    at.live = at.c < p.channels && at.ty < at.rows;
     return at;
 }
 
@@ -269,16 +269,15 @@ __device__ __forceinline__ void join2(float2& mean, float2& m2, float n, float2 
     m2 = add2(m2, fma2(mul2(d, d), both(n * share), q2));
 }
 
-template <typename T, int VEC, int ACT>
-__global__ void __launch_bounds__(kNormThreads, 4) group_norm_moments_kernel(const NormArgs p) {
+// The power of two below n, from which a tree over n goes down (0 for 1).
+__device__ __forceinline__ int half_of(int n) { return n > 1 ? 1 << (31 - __clz(n - 1)) : 0; }
+
+// Mean and squares around it of the chunk's channels; all of the block's rows end up with the threads of ty == 0.
+template <typename T, int VEC>
+__device__ __forceinline__ void chunk_moments(const NormArgs& p, const Chunk& chunk, const Place& at, float2 (&mean)[Channels<VEC>::kPairs],
+                                              float2 (&m2)[Channels<VEC>::kPairs]) {
     constexpr int kPairs = Channels<VEC>::kPairs, kBatch = 8;
-    wait_for_previous_kernel();
-    let_next_kernel_start();
-    const Chunk chunk = chunk_of(p, blockIdx.x);
-    if (chunk.n == 0) return;
-    const Place at = place_of<VEC>(p);
     const T* x = static_cast<const T*>(p.x) + chunk.row * p.x_stride + at.c;
-    float2 mean[kPairs], m2[kPairs];
     float n = 0.f;
 #pragma unroll
     for (int i = 0; i < kPairs; i++) mean[i] = m2[i] = both(0.f);
@@ -328,8 +327,8 @@ __global__ void __launch_bounds__(kNormThreads, 4) group_norm_moments_kernel(con
     }
     __shared__ float2 all[2][kPairs][kNormThreads];
     __shared__ float counts[kNormThreads];
-    for (int s = at.rows / 2; s > 0; s >>= 1) {
-        if (at.ty >= s && at.ty < 2 * s) {
+    for (int s = half_of(at.rows); s > 0; s >>= 1) {
+        if (at.ty >= s && at.ty < min(2 * s, at.rows)) {
 #pragma unroll
             for (int i = 0; i < kPairs; i++) {
                 all[0][i][threadIdx.x] = mean[i];
@@ -338,7 +337,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) group_norm_moments_kernel(con
             counts[threadIdx.x] = n;
         }
         __syncthreads();
-        if (at.ty < s) {
+        if (at.ty < s && at.ty + s < at.rows) {
             const int other = threadIdx.x + s * p.tx;
             const float more = counts[other], share = n + more > 0.f ? more / (n + more) : 0.f;
 #pragma unroll
@@ -346,27 +345,20 @@ __global__ void __launch_bounds__(kNormThreads, 4) group_norm_moments_kernel(con
             n += more;
         }
     }
-    const bool finish = chunk.alone && p.whole;
-    if (at.ty == 0 && at.live && !finish) {
-        float2* to = p.part + (int64_t)blockIdx.x * p.channels + at.c;
+}
+template <int VEC>
+__device__ __forceinline__ void put_channels(float2* to, const float2 (&a)[Channels<VEC>::kPairs], const float2 (&b)[Channels<VEC>::kPairs]) {
 #pragma unroll
-        for (int i = 0; i < kPairs; i++) {
-            to[2 * i] = make_float2(mean[i].x, m2[i].x);
-            if (VEC > 1) to[2 * i + 1] = make_float2(mean[i].y, m2[i].y);
-        }
+    for (int i = 0; i < Channels<VEC>::kPairs; i++) {
+        to[2 * i] = make_float2(a[i].x, b[i].x);
+        if (VEC > 1) to[2 * i + 1] = make_float2(a[i].y, b[i].y);
     }
-    if (!finish) return;
+}
 
-    // the whole graph: statistics of the slab's groups, then the rows once more (they are in the L1 or L2)
-    __shared__ float2 channel[32 * kNormVec];
-    if (at.ty == 0) {
-#pragma unroll
-        for (int i = 0; i < kPairs; i++) {
-            channel[at.tx * VEC + 2 * i] = make_float2(mean[i].x, m2[i].x);
-            if (VEC > 1) channel[at.tx * VEC + 2 * i + 1] = make_float2(mean[i].y, m2[i].y);
-        }
-    }
-    __syncthreads();
+// The rest of a graph whose `rows` rows the slab's channels' moments (`channel`, complete and the block's own) are of: its
+// groups' statistics, then this block's rows once more (they are in the L1 or L2).
+template <typename T, int VEC, int ACT>
+__device__ __forceinline__ void finish_graph(const NormArgs& p, const Chunk& chunk, float rows, const Place& at, float2* channel, bool writes_stats) {
     const int width = p.tx * VEC, base = blockIdx.y * width, c = base + threadIdx.x;
     float2 stats = make_float2(0.f, 0.f);
     if ((int)threadIdx.x < width && c < p.channels) {
@@ -376,10 +368,10 @@ __global__ void __launch_bounds__(kNormThreads, 4) group_norm_moments_kernel(con
         const float m = sum / (float)p.per_group;
         for (int i = 0; i < p.per_group; i++) {
             const float d = channel[g0 + i].x - m;
-            squares += channel[g0 + i].y + (float)chunk.n * d * d;
+            squares += channel[g0 + i].y + rows * d * d;
         }
-        stats = make_float2(m, rsqrtf(squares / ((float)chunk.n * (float)p.per_group) + p.eps));
-        if ((int)threadIdx.x == g0) {
+        stats = make_float2(m, rsqrtf(squares / (rows * (float)p.per_group) + p.eps));
+        if ((int)threadIdx.x == g0 && writes_stats) {
             const int64_t to = (int64_t)chunk.graph * p.groups + c / p.per_group;
             p.mean[to] = stats.x;
             p.rstd[to] = stats.y;
@@ -394,6 +386,95 @@ __global__ void __launch_bounds__(kNormThreads, 4) group_norm_moments_kernel(con
     write_rows<T, VEC, ACT>(p, chunk, at, ch);
 }
 
+template <typename T, int VEC, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 4) group_norm_moments_kernel(const NormArgs p) {
+    constexpr int kPairs = Channels<VEC>::kPairs;
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    const Chunk chunk = chunk_of(p, blockIdx.x);
+    if (chunk.n == 0) return;
+    const Place at = place_of<VEC>(p);
+    float2 mean[kPairs], m2[kPairs];
+    chunk_moments<T, VEC>(p, chunk, at, mean, m2);
+    if (!chunk.handled) {
+        if (at.ty == 0 && at.live) put_channels<VEC>(p.part + (int64_t)blockIdx.x * p.channels + at.c, mean, m2);
+        return;
+    }
+    __shared__ float2 channel[32 * kNormVec];
+    if (at.ty == 0) put_channels<VEC>(channel + at.tx * VEC, mean, m2);
+    __syncthreads();
+    finish_graph<T, VEC, ACT>(p, chunk, (float)chunk.n, at, channel, true);
+}
+
+// ---- clusters --------------------------------------------------------------------------------------------------
+// One graph of middling size by a cluster of eight blocks for each slab of its channels, which take an eighth of the rows
+// each and read one another's sums from shared memory: one launch, whose second pass over the rows finds them in the L2.
+constexpr int kNormCluster = 8;
+// Rows of a thread up to which that is faster than three launches over all SMs.  Forward 2708 x 64 (21 rows): 9.3 us, streamed
+// 12.5; 8000 x 64 (62): 19.3 and 18.4; backward 1000 x 64 (8): 9.9 and 14.2; 2708 x 64: 18.8 and 14.5.  (Of batches of such
+// graphs none gained: 16 of about 1000 x 128 took 23.8 us and 14.4 streamed.)
+constexpr int kNormClusterForward = 28, kNormClusterBackward = 12;
+
+__device__ __forceinline__ void norm_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float2 load_of_rank(const float2* own, uint32_t rank) {
+    float2 v;
+    asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %2, %3;\n\tld.shared::cluster.v2.f32 {%0, %1}, [a];\n\t}"
+                 : "=f"(v.x), "=f"(v.y)
+                 : "r"((uint32_t)__cvta_generic_to_shared(own)), "r"(rank)
+                 : "memory");
+    return v;
+}
+// This block's share of the only graph's rows (0 behind the last); n: the graph's.
+__device__ __forceinline__ Chunk share_of_cluster(const NormArgs& p, int64_t& n) {
+    const Graph g = graph_of(p, 0);
+    n = g.end - g.begin;
+    const int64_t share = (n + kNormCluster - 1) / kNormCluster, row = g.begin + blockIdx.x * share;
+    return {0, row, row < g.end ? (int)min(share, g.end - row) : 0, true};
+}
+
+template <typename T, int VEC, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 4) __cluster_dims__(kNormCluster, 1, 1) group_norm_cluster_kernel(const NormArgs p) {
+    constexpr int kPairs = Channels<VEC>::kPairs;
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    int64_t n;
+    const Chunk chunk = share_of_cluster(p, n);
+    const Place at = place_of<VEC>(p);
+    float2 mean[kPairs], m2[kPairs];
+    chunk_moments<T, VEC>(p, chunk, at, mean, m2);
+    __shared__ float2 mine[32 * kNormVec], channel[32 * kNormVec];
+    if (at.ty == 0) put_channels<VEC>(mine + at.tx * VEC, mean, m2);
+    norm_cluster_sync();
+    if ((int)threadIdx.x < p.tx * VEC) {
+        const int64_t share = (n + kNormCluster - 1) / kNormCluster;
+        float count = 0.f, mu = 0.f, squares = 0.f;
+#pragma unroll
+        for (uint32_t r = 0; r < kNormCluster; r++) {
+            const float2 v = load_of_rank(mine + threadIdx.x, r);
+            const float more = (float)max((int64_t)0, min(share, n - (int64_t)r * share));
+            if (more > 0.f) {
+                const float part = more / (count + more), d = v.x - mu;
+                mu += d * part;
+                squares += v.y + d * d * count * part;
+                count += more;
+            }
+        }
+        channel[threadIdx.x] = make_float2(mu, squares);
+    }
+    norm_cluster_sync();                     // nobody reads this block's sums any more; and the block's own barrier
+    if (n == 0) {
+        const int width = p.tx * VEC, c = blockIdx.y * width + threadIdx.x;
+        if (blockIdx.x == 0 && (int)threadIdx.x < width && c < p.channels && c % p.per_group == 0) {
+            p.mean[c / p.per_group] = 0.f;
+            p.rstd[c / p.per_group] = rsqrtf(p.eps);
+        }
+        return;
+    }
+    finish_graph<T, VEC, ACT>(p, chunk, (float)n, at, channel, blockIdx.x == 0);
+}
+
 // One block per graph and group: mean and rstd from the chunks' channels.
 __global__ void __launch_bounds__(kNormThreads) group_norm_join_kernel(const NormArgs p) {
     wait_for_previous_kernel();
@@ -402,7 +483,7 @@ __global__ void __launch_bounds__(kNormThreads) group_norm_join_kernel(const Nor
     const Graph graph = graph_of(p, b);
     const int64_t n = graph.end - graph.begin;
     const int chunks = chunks_of(p, graph), last = (int)(n - (int64_t)(chunks - 1) * p.chunk);
-    if (chunks == 1 && p.whole) return;       // its block has done it
+    if (chunks > 0 && n <= p.handled) return;       // finished
     // threads along the group's channels, the rest along the chunks; four chunks in flight
     int across = 1;
     while (across < p.per_group && across < kNormThreads) across *= 2;
@@ -460,7 +541,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) group_norm_apply_kernel(const
     let_next_kernel_start();
     const Chunk chunk = chunk_of(p, blockIdx.x);
     const Place at = place_of<VEC>(p);
-    if (chunk.n == 0 || (chunk.alone && p.whole) || !at.live) return;
+    if (chunk.n == 0 || chunk.handled || !at.live) return;
     Channels<VEC> ch;
     ch.load(p, chunk.graph, at.c);
     write_rows<T, VEC, ACT>(p, chunk, at, ch);
@@ -521,18 +602,13 @@ __device__ __forceinline__ void write_grads(const NormArgs& p, const Chunk& chun
     }
 }
 
+// Sums of du and du xhat of the chunk's channels; all of the block's rows end up with the threads of ty == 0.
 template <typename T, int VEC, int ACT>
-__global__ void __launch_bounds__(kNormThreads, 4) group_norm_grad_sums_kernel(const NormArgs p) {
+__device__ __forceinline__ void chunk_grad_sums(const NormArgs& p, const Chunk& chunk, const Place& at, Channels<VEC>& ch, float2 (&s1)[Channels<VEC>::kPairs],
+                                                float2 (&s2)[Channels<VEC>::kPairs]) {
     constexpr int kPairs = Channels<VEC>::kPairs, kBatch = 4;
-    wait_for_previous_kernel();
-    let_next_kernel_start();
-    const Chunk chunk = chunk_of(p, blockIdx.x);
-    if (chunk.n == 0) return;
-    const Place at = place_of<VEC>(p);
-    float2 s1[kPairs], s2[kPairs];
 #pragma unroll
     for (int i = 0; i < kPairs; i++) s1[i] = s2[i] = both(0.f);
-    Channels<VEC> ch;
     if (at.live) {
         ch.load(p, chunk.graph, at.c);
         const T* x = static_cast<const T*>(p.x) + chunk.row * p.x_stride + at.c;
@@ -558,8 +634,8 @@ __global__ void __launch_bounds__(kNormThreads, 4) group_norm_grad_sums_kernel(c
         }
     }
     __shared__ float2 all[2][kPairs][kNormThreads];
-    for (int s = at.rows / 2; s > 0; s >>= 1) {
-        if (at.ty >= s && at.ty < 2 * s) {
+    for (int s = half_of(at.rows); s > 0; s >>= 1) {
+        if (at.ty >= s && at.ty < min(2 * s, at.rows)) {
 #pragma unroll
             for (int i = 0; i < kPairs; i++) {
                 all[0][i][threadIdx.x] = s1[i];
@@ -567,7 +643,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) group_norm_grad_sums_kernel(c
             }
         }
         __syncthreads();
-        if (at.ty < s) {
+        if (at.ty < s && at.ty + s < at.rows) {
 #pragma unroll
             for (int i = 0; i < kPairs; i++) {
                 s1[i] = add2(s1[i], all[0][i][threadIdx.x + s * p.tx]);
@@ -575,32 +651,83 @@ __global__ void __launch_bounds__(kNormThreads, 4) group_norm_grad_sums_kernel(c
             }
         }
     }
-    float2* part = p.part + (int64_t)blockIdx.x * p.channels;
     if (at.ty == 0 && at.live) {
         const float* rstd = p.rstd + (int64_t)chunk.graph * p.groups;
 #pragma unroll
         for (int i = 0; i < kPairs; i++) {
             const int c = at.c + 2 * i;
-            part[c] = make_float2(s1[i].x, s2[i].x * rstd[c / p.per_group]);
-            if (VEC > 1) part[c + 1] = make_float2(s1[i].y, s2[i].y * rstd[(c + 1) / p.per_group]);
+            s2[i].x *= rstd[c / p.per_group];
+            if (VEC > 1) s2[i].y *= rstd[(c + 1) / p.per_group];
         }
     }
-    if (!chunk.alone || !p.whole || !p.y) return;
-    // the whole graph: its groups' means, then the rows once more
+}
+
+// dx of this block's rows of a graph of `rows` rows, from the graph's sums of the slab's channels (`sums`, from the slab's first).
+template <typename T, int VEC, int ACT>
+__device__ __forceinline__ void finish_grads(const NormArgs& p, const Chunk& chunk, int64_t rows, const Place& at, const Channels<VEC>& ch, const float2* sums) {
+    if (!p.y) return;
     __shared__ float2 means[32 * kNormVec];
-    __syncthreads();
-    const int width = p.tx * VEC, first = (int)(blockIdx.y * width) / p.per_group, end = min((int)(blockIdx.y + 1) * width, p.channels);
+    const int width = p.tx * VEC, base = blockIdx.y * width, first = base / p.per_group, end = min(base + width, p.channels);
     for (int g = first + (threadIdx.x >> 5); g * p.per_group < end; g += kNormThreads / 32) {
-        const float2 m = group_means(p, part, g, chunk.graph, chunk.n);
+        const float2 m = group_means(p, sums - base, g, chunk.graph, rows);
         if ((threadIdx.x & 31) == 0) means[g - first] = m;
     }
     __syncthreads();
     if (at.live) write_grads<T, VEC, ACT>(p, chunk, at, ch, means, first);
 }
 
-// The sums of a graph: in its only chunk's place, or joined.
-__device__ __forceinline__ const float2* sums_of(const NormArgs& p, const Graph& g, int b) {
-    return g.end - g.begin <= p.chunk ? p.part + g.first * p.channels : p.sums + (int64_t)b * p.channels;
+template <typename T, int VEC, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 4) group_norm_grad_sums_kernel(const NormArgs p) {
+    constexpr int kPairs = Channels<VEC>::kPairs;
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    const Chunk chunk = chunk_of(p, blockIdx.x);
+    if (chunk.n == 0) return;
+    const Place at = place_of<VEC>(p);
+    float2 s1[kPairs], s2[kPairs];
+    Channels<VEC> ch;
+    chunk_grad_sums<T, VEC, ACT>(p, chunk, at, ch, s1, s2);
+    if (!chunk.handled) {
+        if (at.ty == 0 && at.live) put_channels<VEC>(p.part + (int64_t)blockIdx.x * p.channels + at.c, s1, s2);
+        return;
+    }
+    // the whole graph
+    __shared__ float2 channel[32 * kNormVec];
+    if (at.ty == 0) {
+        put_channels<VEC>(channel + at.tx * VEC, s1, s2);
+        if (at.live) put_channels<VEC>(p.sums + (int64_t)chunk.graph * p.channels + at.c, s1, s2);
+    }
+    __syncthreads();
+    finish_grads<T, VEC, ACT>(p, chunk, chunk.n, at, ch, channel);
+}
+
+template <typename T, int VEC, int ACT>
+__global__ void __launch_bounds__(kNormThreads, 4) __cluster_dims__(kNormCluster, 1, 1) group_norm_grad_cluster_kernel(const NormArgs p) {
+    constexpr int kPairs = Channels<VEC>::kPairs;
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    int64_t n;
+    const Chunk chunk = share_of_cluster(p, n);
+    const Place at = place_of<VEC>(p);
+    float2 s1[kPairs], s2[kPairs];
+    Channels<VEC> ch;
+    chunk_grad_sums<T, VEC, ACT>(p, chunk, at, ch, s1, s2);
+    __shared__ float2 mine[32 * kNormVec], channel[32 * kNormVec];
+    if (at.ty == 0) put_channels<VEC>(mine + at.tx * VEC, s1, s2);
+    norm_cluster_sync();
+    const int width = p.tx * VEC, c = blockIdx.y * width + threadIdx.x;
+    if ((int)threadIdx.x < width) {
+        float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+        for (uint32_t r = 0; r < kNormCluster; r++) s = add2(s, load_of_rank(mine + threadIdx.x, r));
+        channel[threadIdx.x] = s;
+        if (c < p.channels && blockIdx.x == 0) {          // the only graph's sums are the result
+            if (p.dbias) p.dbias[c] = s.x;
+            if (p.dweight) p.dweight[c] = s.y;
+        }
+    }
+    norm_cluster_sync();                     // nobody reads this block's sums any more; and the block's own barrier
+    if (n > 0) finish_grads<T, VEC, ACT>(p, chunk, n, at, ch, channel);
 }
 
 // Sums of 8 channels by a block, 32 threads a channel, four values in flight each; every thread gets its channel's.
@@ -634,7 +761,7 @@ __global__ void __launch_bounds__(kNormThreads) group_norm_grad_join_kernel(cons
     for (int b = blockIdx.y; b < p.graphs; b += gridDim.y) {
         const Graph graph = graph_of(p, b);
         const int chunks = chunks_of(p, graph);
-        if (chunks < 2) continue;
+        if (graph.end - graph.begin <= p.handled) continue;      // finished
         const float2* part = p.part + graph.first * p.channels + c;
         const float2 s = sum_of_channel(chunks, [&](int j) { return c < p.channels ? part[(int64_t)j * p.channels] : make_float2(0.f, 0.f); }, room);
         if (threadIdx.x < 8 && c < p.channels) p.sums[(int64_t)b * p.channels + c] = s;
@@ -652,7 +779,7 @@ __global__ void __launch_bounds__(kNormThreads, 4) group_norm_grad_apply_kernel(
         if (c0 >= p.channels) return;
         const float2 s = sum_of_channel(p.graphs, [&](int b) {
             const Graph g = graph_of(p, b);
-            return c < p.channels && g.end > g.begin ? sums_of(p, g, b)[c] : make_float2(0.f, 0.f);
+            return c < p.channels && g.end > g.begin ? p.sums[(int64_t)b * p.channels + c] : make_float2(0.f, 0.f);
         }, room);
         if (threadIdx.x < 8 && c < p.channels) {
             if (p.dbias) p.dbias[c] = s.x;
@@ -661,27 +788,19 @@ __global__ void __launch_bounds__(kNormThreads, 4) group_norm_grad_apply_kernel(
         return;
     }
     const Chunk chunk = chunk_of(p, blockIdx.x);
-    if (chunk.n == 0 || !p.y || (chunk.alone && p.whole)) return;
-    __shared__ float2 means[32 * kNormVec];
-    const int width = p.tx * VEC, first = (int)(blockIdx.y * width) / p.per_group, end = min((int)(blockIdx.y + 1) * width, p.channels);
-    const Graph graph = graph_of(p, chunk.graph);
-    const float2* sums = sums_of(p, graph, chunk.graph);
-    for (int g = first + (threadIdx.x >> 5); g * p.per_group < end; g += kNormThreads / 32) {
-        const float2 m = group_means(p, sums, g, chunk.graph, graph.end - graph.begin);
-        if ((threadIdx.x & 31) == 0) means[g - first] = m;
-    }
-    __syncthreads();
+    if (chunk.n == 0 || !p.y || chunk.handled) return;
     const Place at = place_of<VEC>(p);
-    if (!at.live) return;
     Channels<VEC> ch;
-    ch.load(p, chunk.graph, at.c);
-    write_grads<T, VEC, ACT>(p, chunk, at, ch, means, first);
+    if (at.live) ch.load(p, chunk.graph, at.c);
+    const Graph graph = graph_of(p, chunk.graph);
+    finish_grads<T, VEC, ACT>(p, chunk, graph.end - graph.begin, at, ch, p.sums + (int64_t)chunk.graph * p.channels + blockIdx.y * p.tx * VEC);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------
 struct NormPlan {
     int vec, tx, slabs, chunk;
-    bool whole;
+    int64_t handled;
+    bool clusters;
     int64_t chunks;
     size_t part, sums, bytes;
 };
@@ -693,16 +812,30 @@ static NormPlan plan_norm(const mask_norm& n, bool backward) {
     const bool vec = n.channels % kNormVec == 0 && fits(n.d_x, n.x_stride) && (!n.d_y || fits(n.d_y, n.y_stride)) && (!backward || fits(n.d_grad, n.grad_stride));
     p.vec = vec ? kNormVec : 1;
     const int vectors = n.channels / p.vec;
-    // threads along the channels: a whole row where it has up to 32 vectors, else 32 or the 16 that leave fewer idle
-    p.tx = 1;
-    while (p.tx < 32 && p.tx < vectors) p.tx *= 2;
-    if (vectors > 32 && (vectors + 15) / 16 * 16 < (vectors + 31) / 32 * 32) p.tx = 16;
+    // Threads along the channels: up to 32, of those that make slabs of whole groups (where there are any) the ones that leave
+    // fewest idle; more where that is even.
+    const int per_group = n.channels / n.groups;
+    int unit = per_group;                       // vectors that hold whole groups
+    while (unit % p.vec) unit += per_group;
+    unit /= p.vec;
+    const bool whole = unit <= 32 || unit >= vectors;
+    if (vectors <= 32) unit = vectors;
+    else if (unit > 32) unit = 16;
+    int64_t least_cost = INT64_MAX;
+    for (int tx = unit; tx <= 32; tx += unit) {
+        const int64_t slabs = (vectors + tx - 1) / tx, cost = slabs * 256 / (kNormThreads / tx);     // threads' time for a row
+        const bool wide = tx * (p.vec == 1 ? bytes / kNormVec : bytes) >= 128 || tx + unit > 32;          // 128 bytes of a row, or what there is
+        if (wide && cost <= least_cost) { least_cost = cost; p.tx = tx; }
+    }
     p.slabs = (vectors + p.tx - 1) / p.tx;
-    p.whole = p.slabs == 1 || p.tx * p.vec % (n.channels / n.groups) == 0;
     // Four blocks an SM are resident: as many chunks as that, in whole batches of rows.  (300007 x 256 bf16 backward: 159 us;
     // twice as many 164, four times 199, since every chunk leaves sums to join and blocks have a start and an end.)
-    const int64_t want = 4 * (int64_t)sm_count(), batch = 8 * (kNormThreads / p.tx), most = 4096 / batch * batch;
-    p.chunk = (int)std::min<int64_t>(std::max<int64_t>((n.rows * p.slabs + want * batch - 1) / (want * batch) * batch, std::min<int64_t>(batch, 256)), std::max<int64_t>(most, batch));
+    const int64_t want = 4 * (int64_t)sm_count(), batch = 8 * (kNormThreads / p.tx), most = std::max<int64_t>(4096 / batch, 1) * batch;
+    p.chunk = (int)std::min(std::max((n.rows * p.slabs + want * batch - 1) / (want * batch) * batch, std::min<int64_t>(batch, 256)), most);
+    // Graphs of a chunk are finished by its block, one that is not much longer by clusters.
+    p.handled = whole ? p.chunk : 0;
+    const int64_t share = (int64_t)kNormCluster * (kNormThreads / p.tx) * (backward ? kNormClusterBackward : kNormClusterForward);
+    p.clusters = whole && n.graphs == 1 && n.rows > p.chunk && n.rows <= share;
     p.chunks = n.rows / p.chunk + n.graphs;
     auto take = [&](size_t bytes) {
         const size_t at = p.bytes;
@@ -743,19 +876,21 @@ static const char* refuse_norm(const mask_norm* n, bool backward) {
 template <typename T, int VEC, int ACT>
 static int launch_norm(const NormArgs& a, const NormPlan& p, bool backward, cudaStream_t st) {
     const dim3 grid((unsigned)p.chunks, (unsigned)p.slabs);
-    const bool one_chunk = p.whole && a.graphs == 1 && a.rows > 0 && a.rows <= p.chunk && !a.offsets;    // its block does everything
+    const dim3 clusters(kNormCluster, (unsigned)p.slabs);
+    const bool all_handled = a.rows > 0 && a.rows <= p.handled;        // none can be longer
     int rc;
     if (!backward) {
-        if ((rc = launch_overlapped(group_norm_moments_kernel<T, VEC, ACT>, grid, kNormThreads, 0, st, a)) || one_chunk) return rc;
+        if (p.clusters) return launch_overlapped(group_norm_cluster_kernel<T, VEC, ACT>, clusters, kNormThreads, 0, st, a);
+        if ((rc = launch_overlapped(group_norm_moments_kernel<T, VEC, ACT>, grid, kNormThreads, 0, st, a)) || (all_handled && !a.offsets)) return rc;
         if ((rc = launch_overlapped(group_norm_join_kernel, dim3((unsigned)(a.graphs * a.groups)), kNormThreads, 0, st, a))) return rc;
         return launch_overlapped(group_norm_apply_kernel<T, VEC, ACT>, grid, kNormThreads, 0, st, a);
     }
+    if (p.clusters) return launch_overlapped(group_norm_grad_cluster_kernel<T, VEC, ACT>, clusters, kNormThreads, 0, st, a);
     const int32_t parts = (a.channels + 7) / 8;
     if ((rc = launch_overlapped(group_norm_grad_sums_kernel<T, VEC, ACT>, grid, kNormThreads, 0, st, a))) return rc;
-    if (a.rows > p.chunk) {       // else no graph has two chunks
-        if ((rc = launch_overlapped(group_norm_grad_join_kernel, dim3((unsigned)parts, (unsigned)std::max(1, std::min(a.graphs, 4 * sm_count() / parts))), kNormThreads, 0, st, a)))
-            return rc;
-    }
+    if (!all_handled && (rc = launch_overlapped(group_norm_grad_join_kernel, dim3((unsigned)parts, (unsigned)std::max(1, std::min(a.graphs, 4 * sm_count() / parts))),
+                                                kNormThreads, 0, st, a)))
+        return rc;
     const unsigned more = a.dweight || a.dbias ? (unsigned)((parts + p.slabs - 1) / p.slabs) : 0;
     return launch_overlapped(group_norm_grad_apply_kernel<T, VEC, ACT>, dim3(grid.x + more, grid.y), kNormThreads, 0, st, a, p.chunks);
 }
@@ -779,7 +914,7 @@ static int run_norm(const mask_norm* n, bool backward, void* d_scratch, size_t s
     if (scratch_bytes < p.bytes) return fail(MASK_ERR_SCRATCH_TOO_SMALL, "scratch is smaller than mask_group_norm_scratch_bytes");
     NormArgs a = {};
     a.rows = n->rows; a.channels = n->channels; a.groups = n->groups; a.per_group = n->channels / n->groups; a.graphs = n->graphs;
-    a.eps = n->eps; a.chunk = p.chunk; a.chunk_inverse = ~(uint64_t)0 / (uint64_t)p.chunk + 1; a.tx = p.tx; a.whole = p.whole;
+    a.eps = n->eps; a.chunk = p.chunk; a.chunk_inverse = ~(uint64_t)0 / (uint64_t)p.chunk + 1; a.tx = p.tx; a.handled = p.handled;
     a.offsets = n->d_offsets; a.x = n->d_x; a.x_stride = n->x_stride; a.weight = n->d_weight; a.bias = n->d_bias;
     a.y = n->d_y; a.y_stride = n->y_stride; a.mean = n->d_mean; a.rstd = n->d_rstd;
     a.grad = n->d_grad; a.grad_stride = n->grad_stride; a.dweight = n->d_dweight; a.dbias = n->d_dbias;
