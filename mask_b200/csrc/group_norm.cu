@@ -818,7 +818,7 @@ static NormPlan plan_norm(const mask_norm& n, bool backward) {
     int unit = per_group;                       // vectors that hold whole groups
     while (unit % p.vec) unit += per_group;
     unit /= p.vec;
-    const bool whole = unit <= 32 || unit >= vectors;
+    const bool whole = vectors <= 32 || unit <= 32;
     if (vectors <= 32) unit = vectors;
     else if (unit > 32) unit = 16;
     int64_t least_cost = INT64_MAX;

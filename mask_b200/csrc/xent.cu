@@ -654,9 +654,10 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const XentArgs p, int p
         for (int i = 1; i < shares; i++) join(room[i * rows + at]);
         float loss = 0.f;
         if (r < count) {
-            const float lse2 = (top == -INFINITY ? 0.f : top * f) + log2f(sum);
-            p.lse2[r] = lse2;
-            loss = lost ? NAN : kLn2 * fmaf(-p.label_logit[r], f, lse2);
+            const float base = top == -INFINITY ? 0.f : top * f, log_sum = log2f(sum);
+            p.shift[r] = p.range ? base : base + log_sum;
+            p.factor[r] = (float)(1 << kGradExponent) / sum;
+            loss = lost ? NAN : kLn2 * (fmaf(-p.label_logit[r], f, base) + log_sum);
             if (p.row_loss) p.row_loss[p.row_of[r]] = loss;
         }
         const bool any = __any_sync(0xffffffffu, r < count);
@@ -791,7 +792,7 @@ struct XentPlan {
     int64_t part_dh_rows, part_dw_rows;
     int part_ld;
     // byte offsets into the scratch
-    size_t counts, ranges, row_of, label, total, stats, label_logit, lse2, warp_loss, h_planes, w_planes, g, part_dh, part_dw, bytes;
+    size_t counts, ranges, row_of, label, total, stats, label_logit, shift, factor, warp_loss, h_planes, w_planes, g, part_dh, part_dw, bytes;
 };
 
 // Blocks that share a tile of `bn` columns of a product with so many rows.  Pairs load a third less (dH of 16384 x 16384 x 512:
@@ -882,7 +883,8 @@ static XentPlan plan_xent(const mask_head& h) {
     }
     p.stats = p.one_pass ? 0 : take(8 * rp * p.stats_parts);
     p.label_logit = take(4 * rp);
-    p.lse2 = take(4 * rp);
+    p.shift = take(4 * rp);
+    p.factor = take(4 * rp);
     p.warp_loss = take(rp / 8);
     p.h_planes = take(2 * (size_t)p.planes * rp * p.dim_pad);
     p.w_planes = p.pack_weight ? take(2 * (size_t)p.planes * h.classes * p.dim_pad) : 0;
@@ -1051,7 +1053,8 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
     a.label = label; a.row_of = row_of; a.row_loss = row_loss;
     a.stats = reinterpret_cast<float2*>(at(plan.stats));
     a.label_logit = reinterpret_cast<float*>(at(plan.label_logit));
-    a.lse2 = reinterpret_cast<float*>(at(plan.lse2));
+    a.shift = reinterpret_cast<float*>(at(plan.shift));
+    a.factor = reinterpret_cast<float*>(at(plan.factor));
     a.warp_loss = reinterpret_cast<float*>(at(plan.warp_loss));
     a.scale = h.grad_scale; a.mean = h.reduction == MASK_REDUCE_MEAN;
     a.out_type = h.dtype;

@@ -47,7 +47,8 @@ struct XentArgs {
     const int32_t* row_of;     // [labelled row] -> row of the caller's arrays
     float2* stats;             // [splits * epilogue parts][rows_pad]: maximum, sum of exp(logit - maximum)
     float* label_logit;        // [labelled row]
-    float* lse2;               // [labelled row]: log2 of the row's sum of exponentials
+    float* shift;              // [labelled row]: 16-bit input: log2 of the row's sum of exponentials; FP32: what the sum's
+    float* factor;             //   exponents were taken less, and 2^15 over the sum (a log sum rounded to 32 bits would put 1e-6 on a whole row)
     float* row_loss;           // caller's, or NULL
     float* warp_loss;          // [rows_pad / 32]: sums of 32 rows' losses
     float* part;               // [splits][m_pad][n_pad]
@@ -599,10 +600,11 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             }
         };
         const float f = kLogits ? logit_factor(p.range) : 0.f;
-        // exp(logit) over the row's sum, less 1 at its label; 0 outside the classes and, where lse2 is infinite, the rows
-        [[maybe_unused]] auto gradient = [&](float (&v)[32], int col, int classes, int y, float lse2) {
+        // exp(logit) over the row's sum, less 1 at its label; 0 outside the classes and, where shift is infinite, the rows.
+        // FP32 input: times 2^15.
+        [[maybe_unused]] auto gradient = [&](float (&v)[32], int col, int classes, int y, float shift, float factor) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) v[j] = fast_exp2(fmaf(v[j], f, -lse2));
+            for (int j = 0; j < 32; j++) v[j] = fast_exp2(fmaf(v[j], f, -shift)) * (P == 2 ? factor : 1.f);
             if (col + 32 > classes) {
 #pragma unroll
                 for (int j = 0; j < 32; j++)
@@ -611,11 +613,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             if (__any_sync(0xffffffffu, (uint32_t)(y - col) < 32u)) {
 #pragma unroll
                 for (int j = 0; j < 32; j++)
-                    if (y - col == j && y < classes) v[j] -= 1.f;
-            }
-            if constexpr (P == 2) {
-#pragma unroll
-                for (int j = 0; j < 32; j++) v[j] *= (float)(1 << kGradExponent);
+                    if (y - col == j && y < classes) v[j] -= P == 2 ? (float)(1 << kGradExponent) : 1.f;
             }
         };
         for (int64_t i = group; i < items && ok; i += groups) {
@@ -654,14 +652,14 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             } else if constexpr (MODE == kXentGrad) {
                 const bool live = r < count;
                 const int y = live ? p.label[r] - p.v0 : -1;
-                const float lse2 = live ? p.lse2[r] : INFINITY;
+                const float shift = live ? p.shift[r] : INFINITY, factor = P == 2 && live ? p.factor[r] : 0.f;
                 if (!acquire(t.k0, t.k1)) { ok = false; break; }
 #pragma unroll(kUnroll)
                 for (int c = 0; c < kChunks; c++) {
                     const int col = t.n0 * BN + part * kWidth + 32 * c;     // within the piece
                     float v[32];
                     values(c, v);
-                    gradient(v, col, p.vc, y, lse2);
+                    gradient(v, col, p.vc, y, shift, factor);
                     write_g(v, r - lane, col, c);
                 }
                 done();
@@ -704,9 +702,10 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     all += ex[i * 128 * 3 + 1] * fast_exp2(fmaf(ex[i * 128 * 3], f, -bs));
                     at_label += ex[i * 128 * 3 + 2];
                 }
-                const float lse2 = bs + log2f(all);
+                const float log_sum = log2f(all), shift = !live ? INFINITY : (P == 2 ? bs : bs + log_sum);
+                const float factor = P == 2 && live ? (float)(1 << kGradExponent) / all : 0.f;
                 if (part == 0) {
-                    const float loss = live ? kLn2 * fmaf(-at_label, f, lse2) : 0.f;
+                    const float loss = live ? kLn2 * (fmaf(-at_label, f, bs) + log_sum) : 0.f;
                     if (live && p.row_loss) p.row_loss[p.row_of[r]] = loss;
                     float w = loss;
 #pragma unroll
@@ -718,7 +717,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     const int col = part * kWidth + 32 * c;
                     float v[32];
                     values(c, v);
-                    gradient(v, col, p.classes, y, live ? lse2 : INFINITY);
+                    gradient(v, col, p.classes, y, shift, factor);
                     write_g(v, r - lane, col, c);
                 }
                 done();

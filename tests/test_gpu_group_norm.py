@@ -152,6 +152,17 @@ def test_sizes(rows, channels, groups, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("rows,channels,groups", [(4, 194, 1), (2, 328, 1), (30, 1000, 2), (40, 592, 16), (900, 129, 1), (900, 132, 1), (2000, 320, 32), (64, 4096, 1),
+                                                  (1500, 66, 22), (5, 3, 3), (2700, 12, 2), (130, 160, 32)])
+def test_groups_and_slabs(rows, channels, groups):
+    """Groups wider than what a block takes of a row, groups that do not divide it, and the sizes of graph between the ways of
+    taking one."""
+    for dtype in ("f32", "bf16"):
+        _both(rows, channels, groups, dtype, activation="silu", seed=21)
+        _both(rows, channels, groups, dtype, [0, 0, rows // 3, rows], "none", seed=22)
+
+
+@gpu
 @pytest.mark.parametrize("activation", ["none", "relu", "silu"])
 @pytest.mark.parametrize("affine", [True, False])
 def test_activations(activation, affine):
