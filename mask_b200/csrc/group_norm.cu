@@ -778,8 +778,10 @@ __global__ void __launch_bounds__(kNormThreads, 4) group_norm_grad_apply_kernel(
         const int64_t c0 = ((blockIdx.x - chunks) * gridDim.y + blockIdx.y) * 8, c = c0 + (threadIdx.x & 7);
         if (c0 >= p.channels) return;
         const float2 s = sum_of_channel(p.graphs, [&](int b) {
+            // graphs without rows have no sums: what is read for them is dropped, so that no load waits for another
+            const float2 v = p.sums[(int64_t)b * p.channels + min(c, (int64_t)p.channels - 1)];
             const Graph g = graph_of(p, b);
-            return c < p.channels && g.end > g.begin ? p.sums[(int64_t)b * p.channels + c] : make_float2(0.f, 0.f);
+            return c < p.channels && g.end > g.begin ? v : make_float2(0.f, 0.f);
         }, room);
         if (threadIdx.x < 8 && c < p.channels) {
             if (p.dbias) p.dbias[c] = s.x;

@@ -637,8 +637,8 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const XentArgs p, int p
         const int64_t r = r0 + at;
         float top = -INFINITY, sum = 0.f;
         auto join = [&](float2 s) {
-            const float now = fmaxf(top, s.x), base = now == -INFINITY ? 0.f : now * f;
-            sum = sum * fast_exp2(fmaf(top, f, -base)) + s.y * fast_exp2(fmaf(s.x, f, -base));
+            const float now = fmaxf(top, s.x), base = exponent_base(now, f);
+            sum = sum * rebase(top, f, base) + s.y * rebase(s.x, f, base);
             top = now;
         };
         if (r < count) {
@@ -654,7 +654,7 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const XentArgs p, int p
         for (int i = 1; i < shares; i++) join(room[i * rows + at]);
         float loss = 0.f;
         if (r < count) {
-            const float base = top == -INFINITY ? 0.f : top * f, log_sum = log2f(sum);
+            const float base = exponent_base(top, f), log_sum = log2f(sum);
             p.shift[r] = p.range ? base : base + log_sum;
             p.factor[r] = (float)(1 << kGradExponent) / sum;
             loss = lost ? NAN : kLn2 * (fmaf(-p.label_logit[r], f, base) + log_sum);

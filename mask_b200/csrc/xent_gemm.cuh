@@ -230,14 +230,20 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b, bool half_type)
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// What a row's exponents are taken less: its maximum in bits, rounded.  Going from one to another multiplies the sum by
+// exp2 of the difference of the two rounded numbers -- exactly 1 where they are the same; with an exact product on one side
+// the sum drifts by a rounding with every 32 logits.
+__device__ __forceinline__ float exponent_base(float top, float f) { return top == -INFINITY ? 0.f : __fmul_rn(top, f); }    // a row that has seen only -inf
+__device__ __forceinline__ float rebase(float top, float f, float base) { return fast_exp2(__fsub_rn(__fmul_rn(top, f), base)); }
+
 // Adds 32 logits of a row, in units of 1 / f bits, to its running maximum and sum.
 __device__ __forceinline__ void online_softmax(const float (&v)[32], float f, float& top, float& sum) {
     float t[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
     for (int i = 4; i < 32; i++) t[i & 3] = fmaxf(t[i & 3], v[i]);
     const float now = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
-    const float base = now == -INFINITY ? 0.f : now * f;         // a row that has seen only -inf
-    float s[4] = {sum * fast_exp2(fmaf(top, f, -base)), 0.f, 0.f, 0.f};
+    const float base = exponent_base(now, f);
+    float s[4] = {sum * rebase(top, f, base), 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 32; i++) s[i & 3] += fast_exp2(fmaf(v[i], f, -base));
     sum = (s[0] + s[1]) + (s[2] + s[3]);
@@ -696,10 +702,10 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 float most = ex[0], all = 0.f, at_label = 0.f;
 #pragma unroll
                 for (int i = 1; i < L::kParts; i++) most = fmaxf(most, ex[i * 128 * 3]);
-                const float bs = most == -INFINITY ? 0.f : most * f;
+                const float bs = exponent_base(most, f);
 #pragma unroll
                 for (int i = 0; i < L::kParts; i++) {
-                    all += ex[i * 128 * 3 + 1] * fast_exp2(fmaf(ex[i * 128 * 3], f, -bs));
+                    all += ex[i * 128 * 3 + 1] * rebase(ex[i * 128 * 3], f, bs);
                     at_label += ex[i * 128 * 3 + 2];
                 }
                 const float log_sum = log2f(all), shift = !live ? INFINITY : (P == 2 ? bs : bs + log_sum);

@@ -275,6 +275,19 @@ def test_pieces_of_the_classes():
 
 
 @gpu
+def test_sums_of_many_classes_do_not_drift():
+    """A loss is formed from numbers below 32 in bits, rounded twice: 2^-20 ln 2 each.  The sums behind it take thousands of
+    steps, none of which may leave a trace of its own: root mean square below 2^-19, small logits that are exact to 2^-22."""
+    import torch
+    from mask_b200 import engine
+    for classes in (20000, 53055):
+        hidden, weight, labels = _inputs(95, 18, classes, "f32", seed=27)
+        got = engine.linear_cross_entropy(hidden, weight, labels, reduction="none")
+        off = got.double() - _want(hidden, weight, labels, "none")[0][0]
+        assert float(off.square().mean().sqrt()) < 2.0 ** -19
+
+
+@gpu
 def test_same_call_same_bits():
     import torch
     from mask_b200 import engine
