@@ -241,15 +241,20 @@ __global__ void __launch_bounds__(kXentCountThreads) xent_scan_kernel(const Xent
         __shared__ int sums[32];
         const float* hidden = static_cast<const float*>(p.hidden);
         const int64_t r1 = min(p.rows, (blockIdx.x + 1) * chunk);
+        __shared__ uint8_t numbers[32][32];        // of a warp's labelled rows
         const int lanes = lanes_for(p.dim);
         int n = 0;
         for (int64_t rb = blockIdx.x * chunk + 32 * warp; rb < r1; rb += kXentCountThreads) {
             const int64_t r = rb + lane;
-            const bool mine = r < r1 && labelled(p.labels[min(r, r1 - 1)], p.classes);
-            const unsigned have = __ballot_sync(0xffffffffu, mine), clear = __ballot_sync(0xffffffffu, !mine && r < r1);
+            const bool real = r < r1, mine = real && labelled(p.labels[r], p.classes);
+            const unsigned have = __ballot_sync(0xffffffffu, mine), clear = __ballot_sync(0xffffffffu, real && !mine);
             n += __popc(have);
-            if constexpr (kFloat)
-                scan_rows(__popc(have), p.dim, 1, lanes, 0, 1, [&](int64_t i) { return hidden + (rb + __fns(have, 0, (int)i + 1)) * p.hidden_stride; }, most[0]);
+            if constexpr (kFloat) {
+                if (mine) numbers[warp][__popc(have & ((1u << lane) - 1))] = (uint8_t)lane;
+                __syncwarp();
+                scan_rows(__popc(have), p.dim, 1, lanes, 0, 1, [&](int64_t i) { return hidden + (rb + numbers[warp][i]) * p.hidden_stride; }, most[0]);
+                __syncwarp();
+            }
             if (p.dhidden) clear_rows<kFloat>(p, rb, clear);
         }
         if (lane == 0) sums[warp] = n;
@@ -837,11 +842,11 @@ static XentPlan plan_xent(const mask_head& h) {
     // one tile of all classes: 256 columns, with two planes of G in shared memory 128
     p.one_pass = p.grads && h.classes <= (p.planes == 2 ? 128 : 256);
     p.stats_splits = p.one_pass ? 1 : best_splits(p.rows_pad, tile_blocks(p.bn_logits, p.rows_pad, h.dim), 1, (h.classes + p.bn_logits - 1) / p.bn_logits, 16);
-    p.stats_parts = p.stats_splits * (p.planes == 1 && p.bn_logits >= 128 ? XentLayout<256, 1, kXentStats, 1>::kParts : XentLayout<64, 1, kXentStats, 1>::kParts);
+    p.stats_parts = p.stats_splits * xent_parts(p.bn_logits, p.planes, true);
     if (p.grads) {
         if (p.one_pass) {
             p.piece = h.classes;
-            p.g_ld = (int)round_up(p.bn_logits, 128);
+            p.g_ld = p.bn_logits;
         } else {
             const int64_t fit = (int64_t)(kXentPieceBytes / (size_t)(2 * p.planes * p.rows_pad)) / 256 * 256;
             p.piece = p.g_ld = (int)std::min<int64_t>(round_up(h.classes, 256), std::max<int64_t>(fit, 256));
@@ -1072,7 +1077,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
         char* g = at(plan.g);
         const int64_t g_plane = rp * plan.g_ld;
         CUtensorMap g_st, g_k, g_mn, w_mn, h_mn;
-        if ((rc = plane_map(&g_st, g, plan.g_ld, rp, P, plan.g_ld, g_plane, P == 1 && plan.bn_logits == 256 ? XentLayout<256, 1, kXentGrad, 1>::kBox : 32, 32))) return rc;
+        if ((rc = plane_map(&g_st, g, plan.g_ld, rp, P, plan.g_ld, g_plane, xent_box(plan.bn_logits, P), 32))) return rc;
         if ((rc = plane_map(&g_k, g, plan.g_ld, rp, P, plan.g_ld, g_plane, 64, kXentTileM))) return rc;
         if ((rc = plane_map(&g_mn, g, plan.g_ld, rp, P, plan.g_ld, g_plane, 64, 64))) return rc;
         if ((rc = plane_map(&w_mn, w_data, w_cols, h.classes, P, w_ld, w_plane, 64, 64))) return rc;

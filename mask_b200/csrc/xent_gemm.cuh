@@ -96,12 +96,20 @@ __device__ __forceinline__ float logit_factor(const uint32_t* range) {
 
 // CG: blocks that share a tile.  2: a cluster of two takes 256 rows, each block 128 of them and half of the columns' operand,
 // and the first issues the MMAs for both.
+// Parts of a tile's columns that different epilogue warps take.  Where every logit costs an exponential, four (16 warps): with
+// two, a warp's waits for tensor memory and the special-function unit left the SM idle.
+constexpr int xent_parts(int bn, int planes, bool logits) { return bn == 64 ? 1 : (planes == 1 && logits ? 4 : 2); }
+// Columns that a warp writes of G at a time.
+constexpr int xent_box(int bn, int planes) { return planes == 1 && bn / xent_parts(bn, planes, true) >= 64 ? 64 : 32; }
+
 template <int BN, int P, int MODE, int CG>
 struct XentLayout {
-    // Epilogue warps: 4 quarters of 32 rows, each for so many parts of the columns.  Where every logit costs an exponential,
-    // four (16 warps): with two, a warp's waits for tensor memory and the special-function unit left the SM idle.
-    static constexpr int kParts = P == 1 && MODE <= kXentGradOne && BN >= 128 ? 4 : 2;
-    static constexpr int kWarps = 4 * kParts;
+    // Epilogue warps: 4 quarters of 32 rows, each for so many parts of the columns -- and for narrow tiles groups of such warps
+    // that take tiles in turn, since one such tile is all waiting (300000 x 64 x 40 bf16: xx us with groups, 37 with one).
+    static constexpr int kParts = xent_parts(BN, P, MODE <= kXentGradOne);
+    static constexpr int kGroups = BN == 64 ? (P == 1 ? 4 : 2) : 1;
+    static constexpr int kWarps = 4 * kParts * kGroups;
+    static constexpr int kBuffers = 2 * kGroups;                          // accumulators, two a group
     // + producer + MMA issuer; where segments are summed in registers (P == 2) two warps more make three whole warpgroups, whose
     // 168 registers a thread are dealt again: 216 to the two that take accumulators apart, 72 to the third (3 x 168 in all).
     static constexpr int kThreads = 32 * (kWarps + (P == 2 ? 4 : 2));
@@ -110,17 +118,17 @@ struct XentLayout {
     static constexpr int kStage = P * (kTileA + kTileB);
     // G leaves through a warp's staging buffer of 4 KB: 32 rows of 64 columns where the warp has as many, else of 32, for both
     // planes or two in turn.
-    static constexpr int kBox = P == 1 && BN / kParts >= 64 ? 64 : 32;
+    static constexpr int kBox = xent_box(BN, P);
     static constexpr int kStagingBuffer = 4096;
     static constexpr int kStaging = kWritesG ? kWarps * kStagingBuffer : 0;
     static constexpr int kExchangeBytes = MODE == kXentGradOne ? 2 * kParts * 128 * 12 : 0;   // one-pass mode: [2 turns][parts][128 rows]
     static constexpr int kMost = 227 * 1024 - 1024 - 256 - kStaging - kExchangeBytes;
     static constexpr int S = kMost / kStage < 8 ? kMost / kStage : 8;
-    static constexpr int kTmemCols = 2 * BN;
+    static constexpr int kTmemCols = kBuffers * BN;
     static constexpr int kStagingAt = S * kStage;
     static constexpr int kExchange = kStagingAt + kStaging;
     static constexpr int kBars = kExchange + kExchangeBytes;
-    static constexpr int kNumBars = 2 * S + 4 + 1 + 4;
+    static constexpr int kNumBars = 2 * S + 2 * kBuffers + 1 + 4;
     static constexpr int kTmemSlot = kBars + kNumBars * 8;
     static constexpr int kAbort = kTmemSlot + 8;
     static constexpr int kBytes = kAbort + 8;
@@ -266,9 +274,9 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (S + s); };
     auto accf_bar = [&](int b) { return bars + 8u * (2 * S + b); };
-    auto acce_bar = [&](int b) { return bars + 8u * (2 * S + 2 + b); };
-    const uint32_t drain_bar = bars + 8u * (2 * S + 4);
-    auto exchange_bar = [&](int q) { return bars + 8u * (2 * S + 5 + q); };
+    auto acce_bar = [&](int b) { return bars + 8u * (2 * S + L::kBuffers + b); };
+    const uint32_t drain_bar = bars + 8u * (2 * S + 2 * L::kBuffers);
+    auto exchange_bar = [&](int q) { return bars + 8u * (2 * S + 2 * L::kBuffers + 1 + q); };
     volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + L::kAbort);
     volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + L::kTmemSlot);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -282,9 +290,9 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), 1);
         }
-        for (int b = 0; b < 2; b++) {
+        for (int b = 0; b < L::kBuffers; b++) {
             mbar_init(accf_bar(b), 1);
-            mbar_init(acce_bar(b), CG * L::kWarps);
+            mbar_init(acce_bar(b), CG * L::kWarps / L::kGroups);
         }
         for (int q = 0; q < 4; q++) mbar_init(exchange_bar(q), L::kParts);
         mbar_init(drain_bar, 1);
@@ -397,17 +405,24 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 constexpr uint32_t kStepA = kAmn ? 128 : 2, kStepB = kBmn ? 128 : 2;   // 16 of the contraction, in 16 bytes
                 uint32_t a_lo = (uint32_t)a0, b_lo = (uint32_t)b0;                     // of stage s
                 int s = 0;
-                uint32_t round = 0, acc_it = 0;
+                uint32_t round = 0, turn = 0;
+                uint32_t uses[L::kGroups];                                             // of the groups' accumulators
+#pragma unroll
+                for (int g = 0; g < L::kGroups; g++) uses[g] = 0;
                 bool ok = true;
-                for (int64_t i = group; i < items && ok; i += groups) {
+                for (int64_t i = group; i < items && ok; i += groups, turn++) {
                     const Item t = item_of(i);
                     if (t.k0 >= t.k1) continue;
+                    const uint32_t g = turn % L::kGroups;
+                    uint32_t acc_it = uses[0];
+#pragma unroll
+                    for (int q = 1; q < L::kGroups; q++) acc_it = g == q ? uses[q] : acc_it;
                     for (int n = t.n0; n < t.n1 && ok; n++) {
                         uint32_t buf = 0, acc = 0, open = 0;
                         int left = 0;                        // blocks that the open accumulator still takes
                         for (int k = t.k0; k < t.k1; k++) {
                             if (!open) {
-                                buf = acc_it & 1;
+                                buf = 2 * g + (acc_it & 1);
                                 acc = tmem_base + buf * BN;
                                 left = P == 2 ? min(kXentSegment, t.k1 - k) : t.k1 - k;
                                 if (acc_it >= 2 && !wait_all_lanes(acce_bar(buf), ((acc_it >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
@@ -436,6 +451,8 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                             }
                         }
                     }
+#pragma unroll
+                    for (int q = 0; q < L::kGroups; q++) uses[q] = g == q ? acc_it : uses[q];
                 }
                 // whatever was issued must have finished before shared and tensor memory go away
                 if (elected) xent_commit<CG>(drain_bar);
@@ -452,7 +469,8 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
         if constexpr (P == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         constexpr int kWidth = BN / L::kParts;             // columns of a warp
         constexpr int kChunks = kWidth / 32, kUnroll = P == 2 ? kChunks : 1;
-        const int quarter = warp & 3, part = warp >> 2;
+        const int quarter = warp & 3, part = (warp >> 2) % L::kParts;
+        const uint32_t mine = (warp >> 2) / L::kParts;       // the group
         uint32_t acc_it = 0;
         bool ok = true;
         const bool half_type = p.half_type != 0;
@@ -463,11 +481,11 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
         auto release = [&]() {
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
-            if (lane == 0) arrive_at_leader<CG>(acce_bar(acc_it & 1));
+            if (lane == 0) arrive_at_leader<CG>(acce_bar(2 * mine + (acc_it & 1)));
             acc_it++;
         };
         auto next_accumulator = [&]() -> bool {
-            const uint32_t buf = acc_it & 1;
+            const uint32_t buf = 2 * mine + (acc_it & 1);
             if (!__all_sync(0xffffffffu, mbar_wait(accf_bar(buf), (acc_it >> 1) & 1, abort_flag))) return false;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             acc = tmem_base + ((uint32_t)(32 * quarter) << 16) + buf * BN + part * kWidth;
@@ -552,7 +570,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             }
         };
 
-        [[maybe_unused]] uint32_t turn = 0;
+        [[maybe_unused]] uint32_t turn = 0, count_of_items = 0;
         // 32 values of row r of a product, from column col, to the parts or to the caller
         [[maybe_unused]] auto write_out = [&](const float (&v)[32], const ProductScale& scale, int split, int r, int col) {
             if (p.store != kXentFinal) {
@@ -623,6 +641,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             }
         };
         for (int64_t i = group; i < items && ok; i += groups) {
+            if (L::kGroups > 1 && count_of_items++ % L::kGroups != mine) continue;
             const Item t = item_of(i);
             const int r = (t.m * CG + (int)rank) * kXentTileM + 32 * quarter + lane;     // row of the tile that this thread holds
             if constexpr (MODE == kXentStats) {
@@ -691,22 +710,30 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 // The warps that hold parts of the same rows tell one another.  Two turns' worth of room: a warp writes turn i + 2
                 // after all others have arrived at turn i + 1, hence read turn i.
                 float* ex = reinterpret_cast<float*>(gbase + L::kExchange) + (turn & 1) * L::kParts * 128 * 3 + (32 * quarter + lane) * 3;
-                ex[part * 128 * 3] = top;
-                ex[part * 128 * 3 + 1] = sum;
-                ex[part * 128 * 3 + 2] = picked;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(exchange_bar(quarter));
-                if (!__all_sync(0xffffffffu, mbar_wait(exchange_bar(quarter), turn & 1, abort_flag))) { ok = false; break; }
-                turn++;
+                if constexpr (L::kParts > 1) {
+                    ex[part * 128 * 3] = top;
+                    ex[part * 128 * 3 + 1] = sum;
+                    ex[part * 128 * 3 + 2] = picked;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(exchange_bar(quarter));
+                    if (!__all_sync(0xffffffffu, mbar_wait(exchange_bar(quarter), turn & 1, abort_flag))) { ok = false; break; }
+                    turn++;
+                }
                 // all parts in the same order everywhere, so that everybody gets the same bits
-                float most = ex[0], all = 0.f, at_label = 0.f;
+                float most = top, all = sum, at_label = picked;
+                if constexpr (L::kParts > 1) {
+                    most = ex[0];
 #pragma unroll
-                for (int i = 1; i < L::kParts; i++) most = fmaxf(most, ex[i * 128 * 3]);
+                    for (int i = 1; i < L::kParts; i++) most = fmaxf(most, ex[i * 128 * 3]);
+                    all = at_label = 0.f;
+                }
                 const float bs = exponent_base(most, f);
+                if constexpr (L::kParts > 1) {
 #pragma unroll
-                for (int i = 0; i < L::kParts; i++) {
-                    all += ex[i * 128 * 3 + 1] * rebase(ex[i * 128 * 3], f, bs);
-                    at_label += ex[i * 128 * 3 + 2];
+                    for (int i = 0; i < L::kParts; i++) {
+                        all += ex[i * 128 * 3 + 1] * rebase(ex[i * 128 * 3], f, bs);
+                        at_label += ex[i * 128 * 3 + 2];
+                    }
                 }
                 const float log_sum = log2f(all), shift = !live ? INFINITY : (P == 2 ? bs : bs + log_sum);
                 const float factor = P == 2 && live ? (float)(1 << kGradExponent) / all : 0.f;
