@@ -335,12 +335,29 @@ __device__ __forceinline__ void pack_hidden(const XentPackArgs& p, int64_t w0, i
     auto source = [&](int64_t i) -> const void* {
         return i < count ? static_cast<const char*>(p.hidden) + (int64_t)p.row_of[i] * p.hidden_stride * kBytes : nullptr;
     };
-    for (int64_t i = w0 * rows + lane / lanes; i < end; i += 2 * step) {
-        const void* a = source(i);
-        const void* b = i + step < end ? source(i + step) : nullptr;
-        pack_row<kFloat>(a, 1, p.dim, p.dim_pad, p.h_planes + i * p.dim_pad, p.h_plane, h_scale, lane & (lanes - 1), lanes);
-        if (i + step < end)
-            pack_row<kFloat>(b, 1, p.dim, p.dim_pad, p.h_planes + (i + step) * p.dim_pad, p.h_plane, h_scale, lane & (lanes - 1), lanes);
+    if (!kFloat && p.dim % 8 == 0 && p.hidden_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p.hidden) & 15) == 0 && end * (p.dim / 8) < ((int64_t)1 << 31)) {
+        // nothing but a copy, in vectors of 16 bytes, four of a thread's in flight
+        const int per_row = p.dim / 8, total = (int)end * per_row, threads = (int)warps * 32;
+        for (int i0 = (int)w0 * 32 + lane; i0 < total; i0 += 4 * threads) {
+            uint4 v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int i = min(i0 + k * threads, total - 1), row = i / per_row;
+                const uint4* from = static_cast<const uint4*>(source(row));
+                v[k] = from ? __ldg(from + (i - row * per_row)) : make_uint4(0u, 0u, 0u, 0u);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (i0 + k * threads < total) reinterpret_cast<uint4*>(p.h_planes)[i0 + k * threads] = v[k];
+        }
+    } else {
+        for (int64_t i = w0 * rows + lane / lanes; i < end; i += 2 * step) {
+            const void* a = source(i);
+            const void* b = i + step < end ? source(i + step) : nullptr;
+            pack_row<kFloat>(a, 1, p.dim, p.dim_pad, p.h_planes + i * p.dim_pad, p.h_plane, h_scale, lane & (lanes - 1), lanes);
+            if (i + step < end)
+                pack_row<kFloat>(b, 1, p.dim, p.dim_pad, p.h_planes + (i + step) * p.dim_pad, p.h_plane, h_scale, lane & (lanes - 1), lanes);
+        }
     }
     if (p.dhidden && !p.cleared && count < p.rows) {
         for (int64_t r0 = 32 * w0; r0 < p.rows; r0 += 32 * warps) {

@@ -223,6 +223,9 @@ __device__ __forceinline__ void st_shared_v4(uint32_t at, uint32_t a, uint32_t b
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+__device__ __forceinline__ void st_shared_u16(uint32_t at, uint16_t v) {
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
+}
 // A whole 32-byte sector by one thread: pieces of 16 bytes of 32 different rows cost the L2 twice the requests.
 __device__ __forceinline__ void st_global_v8(float* at, const float* v) {
     asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
@@ -256,6 +259,20 @@ __device__ __forceinline__ void online_softmax(const float (&v)[32], float f, fl
     for (int i = 0; i < 32; i++) s[i & 3] += fast_exp2(fmaf(v[i], f, -base));
     sum = (s[0] + s[1]) + (s[2] + s[3]);
     top = now;
+}
+
+// v[i] for an index of the thread's own, 0 <= i < 32: 31 selections.
+__device__ __forceinline__ float pick(const float (&v)[32], int i) {
+    float t[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++) t[j] = i & 1 ? v[2 * j + 1] : v[2 * j];
+#pragma unroll
+    for (int j = 0; j < 8; j++) t[j] = i & 2 ? t[2 * j + 1] : t[2 * j];
+#pragma unroll
+    for (int j = 0; j < 4; j++) t[j] = i & 4 ? t[2 * j + 1] : t[2 * j];
+    t[0] = i & 8 ? t[1] : t[0];
+    t[1] = i & 8 ? t[3] : t[2];
+    return i & 16 ? t[1] : t[0];
 }
 
 template <int BN, int P, int MODE, int CG>
@@ -527,7 +544,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             }
         };
         // G of the warp's 32 columns number c to global memory, through its staging buffer
-        [[maybe_unused]] auto write_g = [&](const float (&g)[32], int row0, int col, int c) {
+        [[maybe_unused]] auto write_g = [&](const float (&g)[32], int row0, int col, int c, int y, float at_label) {
             if constexpr (L::kWritesG) {
                 if (row0 >= p.rows_pad) return;            // a pair's second tile may lie behind the last row
                 constexpr bool kWide = L::kBox == 64;
@@ -556,6 +573,13 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     }
                     st_shared_v4(row + first + (((chunk0 + i) ^ x) << 4), h[0], h[1], h[2], h[3]);
                     if constexpr (P == 2) st_shared_v4(row + 2048 + ((i ^ x) << 4), l[0], l[1], l[2], l[3]);
+                }
+                if ((uint32_t)(y - col) < 32u) {           // this row's label is among the columns
+                    const uint32_t i = y - col;
+                    const uint16_t h = (uint16_t)pack_half2(at_label, 0.f, half_type);
+                    st_shared_u16(row + first + (((chunk0 + (i >> 3)) ^ x) << 4) + 2 * (i & 7), h);
+                    if constexpr (P == 2)
+                        st_shared_u16(row + 2048 + (((i >> 3) ^ x) << 4) + 2 * (i & 7), (uint16_t)pack_half2(at_label - __half2float(__ushort_as_half(h)), 0.f, true));
                 }
                 if (ends) {
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -624,9 +648,8 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             }
         };
         const float f = kLogits ? logit_factor(p.range) : 0.f;
-        // exp(logit) over the row's sum, less 1 at its label; 0 outside the classes and, where shift is infinite, the rows.
-        // FP32 input: times 2^15.
-        [[maybe_unused]] auto gradient = [&](float (&v)[32], int col, int classes, int y, float shift, float factor) {
+        // exp(logit) over the row's sum; 0 outside the classes and, where shift is infinite, the rows.  FP32 input: times 2^15.
+        [[maybe_unused]] auto gradient = [&](float (&v)[32], int col, int classes, float shift, float factor) {
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = fast_exp2(fmaf(v[j], f, -shift)) * (P == 2 ? factor : 1.f);
             if (col + 32 > classes) {
@@ -634,11 +657,11 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 for (int j = 0; j < 32; j++)
                     if (col + j >= classes) v[j] = 0.f;
             }
-            if (__any_sync(0xffffffffu, (uint32_t)(y - col) < 32u)) {
-#pragma unroll
-                for (int j = 0; j < 32; j++)
-                    if (y - col == j && y < classes) v[j] -= P == 2 ? (float)(1 << kGradExponent) : 1.f;
-            }
+        };
+        // the same less 1 at the row's label, whose logit is `picked`
+        [[maybe_unused]] auto label_gradient = [&](float picked, float shift, float factor) {
+            const float e = fast_exp2(fmaf(picked, f, -shift));
+            return P == 2 ? e * factor - (float)(1 << kGradExponent) : e - 1.f;
         };
         for (int64_t i = group; i < items && ok; i += groups) {
             if (L::kGroups > 1 && count_of_items++ % L::kGroups != mine) continue;
@@ -663,9 +686,8 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                         }
                         online_softmax(v, f, top, sum);
                         if (__any_sync(0xffffffffu, (uint32_t)(y - col) < 32u)) {
-#pragma unroll
-                            for (int j = 0; j < 32; j++)
-                                if (y - col == j) { picked = v[j]; have = true; }
+                            const float x = pick(v, y - col);
+                            if ((uint32_t)(y - col) < 32u) { picked = x; have = true; }
                         }
                     }
                     done();
@@ -676,16 +698,17 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 }
             } else if constexpr (MODE == kXentGrad) {
                 const bool live = r < count;
-                const int y = live ? p.label[r] - p.v0 : -1;
+                const int label = live ? p.label[r] - p.v0 : -1, y = label < p.vc ? label : -1;       // within the piece
                 const float shift = live ? p.shift[r] : INFINITY, factor = P == 2 && live ? p.factor[r] : 0.f;
+                const float at_label = y >= 0 ? label_gradient(p.label_logit[r], shift, factor) : 0.f;
                 if (!acquire(t.k0, t.k1)) { ok = false; break; }
 #pragma unroll(kUnroll)
                 for (int c = 0; c < kChunks; c++) {
                     const int col = t.n0 * BN + part * kWidth + 32 * c;     // within the piece
                     float v[32];
                     values(c, v);
-                    gradient(v, col, p.vc, y, shift, factor);
-                    write_g(v, r - lane, col, c);
+                    gradient(v, col, p.vc, shift, factor);
+                    write_g(v, r - lane, col, c, y, at_label);
                 }
                 done();
             } else if constexpr (MODE == kXentGradOne) {
@@ -699,13 +722,14 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     if (col >= p.classes) break;
                     float v[32];
                     values(c, v);
+                    if (col + 32 > p.classes) {
 #pragma unroll
-                    for (int j = 0; j < 32; j++)
-                        if (col + j >= p.classes) v[j] = -INFINITY;
+                        for (int j = 0; j < 32; j++)
+                            if (col + j >= p.classes) v[j] = -INFINITY;
+                    }
                     online_softmax(v, f, top, sum);
-#pragma unroll
-                    for (int j = 0; j < 32; j++)
-                        if (y - col == j) picked = v[j];
+                    const float x = pick(v, y - col);
+                    if ((uint32_t)(y - col) < 32u) picked = x;
                 }
                 // The warps that hold parts of the same rows tell one another.  Two turns' worth of room: a warp writes turn i + 2
                 // after all others have arrived at turn i + 1, hence read turn i.
@@ -737,6 +761,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 }
                 const float log_sum = log2f(all), shift = !live ? INFINITY : (P == 2 ? bs : bs + log_sum);
                 const float factor = P == 2 && live ? (float)(1 << kGradExponent) / all : 0.f;
+                const float own = live ? label_gradient(at_label, shift, factor) : 0.f;
                 if (part == 0) {
                     const float loss = live ? kLn2 * (fmaf(-at_label, f, bs) + log_sum) : 0.f;
                     if (live && p.row_loss) p.row_loss[p.row_of[r]] = loss;
@@ -750,8 +775,8 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     const int col = part * kWidth + 32 * c;
                     float v[32];
                     values(c, v);
-                    gradient(v, col, p.classes, y, shift, factor);
-                    write_g(v, r - lane, col, c);
+                    gradient(v, col, p.classes, shift, factor);
+                    write_g(v, r - lane, col, c, y, own);
                 }
                 done();
             } else {
