@@ -475,15 +475,36 @@ __global__ void __launch_bounds__(kNormThreads, 4) __cluster_dims__(kNormCluster
     finish_graph<T, VEC, ACT>(p, chunk, (float)n, at, channel, blockIdx.x == 0);
 }
 
-// One block per graph and group: mean and rstd from the chunks' channels.
-__global__ void __launch_bounds__(kNormThreads) group_norm_join_kernel(const NormArgs p) {
-    wait_for_previous_kernel();
-    let_next_kernel_start();
-    const int b = blockIdx.x / p.groups, g = blockIdx.x % p.groups;
+// Which of the graphs [b0, end), 256 at most, the first kernel has not finished (`empty`: those without rows, too), in their
+// order; every thread looks at one.  Returns how many.
+__device__ __forceinline__ int open_graphs(const NormArgs& p, int b0, int end, bool empty, int* list) {
+    __shared__ int before[kNormThreads / 32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = b0 + threadIdx.x;
+    bool open = false;
+    if (b < end) {
+        const Graph g = graph_of(p, b);
+        open = g.end - g.begin > p.handled || (empty && g.end == g.begin);
+    }
+    const unsigned ballot = __ballot_sync(0xffffffffu, open);
+    __syncthreads();                  // the list and the counts of the last call have been read
+    if (lane == 0) before[warp] = __popc(ballot);
+    __syncthreads();
+    int at = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kNormThreads / 32; w++) {
+        if (w < warp) at += before[w];
+        all += before[w];
+    }
+    if (open) list[at + __popc(ballot & ((1u << lane) - 1))] = b;
+    __syncthreads();
+    return all;
+}
+
+// Mean and rstd of a graph and group from the chunks' channels, by a block.
+__device__ __forceinline__ void join_group(const NormArgs& p, int b, int g) {
     const Graph graph = graph_of(p, b);
     const int64_t n = graph.end - graph.begin;
     const int chunks = chunks_of(p, graph), last = (int)(n - (int64_t)(chunks - 1) * p.chunk);
-    if (chunks > 0 && n <= p.handled) return;       // finished
     // threads along the group's channels, the rest along the chunks; four chunks in flight
     int across = 1;
     while (across < p.per_group && across < kNormThreads) across *= 2;
@@ -529,9 +550,21 @@ __global__ void __launch_bounds__(kNormThreads) group_norm_join_kernel(const Nor
         m2 = lane < kNormThreads / 32 ? room[2][lane] : 0.f;
         join_lanes(4);
         if (lane == 0) {
-            p.mean[blockIdx.x] = mean;
-            p.rstd[blockIdx.x] = rsqrtf((n ? m2 / ((float)n * (float)p.per_group) : 0.f) + p.eps);
+            p.mean[(int64_t)b * p.groups + g] = mean;
+            p.rstd[(int64_t)b * p.groups + g] = rsqrtf((n ? m2 / ((float)n * (float)p.per_group) : 0.f) + p.eps);
         }
+    }
+    __syncthreads();
+}
+// A block per group and `per` graphs.
+__global__ void __launch_bounds__(kNormThreads) group_norm_join_kernel(const NormArgs p, int per) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    __shared__ int list[kNormThreads];
+    const int g = blockIdx.x % p.groups, begin = blockIdx.x / p.groups * per, end = min(begin + per, p.graphs);
+    for (int b0 = begin; b0 < end; b0 += kNormThreads) {
+        const int n = open_graphs(p, b0, end, true, list);
+        for (int i = 0; i < n; i++) join_group(p, list[i], g);
     }
 }
 
@@ -753,18 +786,21 @@ __device__ __forceinline__ float2 sum_of_channel(int n, Value value, float2 (*ro
     for (int i = 0; i < 32; i++) s = add2(s, room[i][c]);
     return s;
 }
-__global__ void __launch_bounds__(kNormThreads) group_norm_grad_join_kernel(const NormArgs p) {
+// The graphs' sums from their chunks': a block per 8 channels and `per` graphs.
+__global__ void __launch_bounds__(kNormThreads) group_norm_grad_join_kernel(const NormArgs p, int per) {
     wait_for_previous_kernel();
     let_next_kernel_start();
     __shared__ float2 room[32][8];
-    const int c = blockIdx.x * 8 + (threadIdx.x & 7);
-    for (int b = blockIdx.y; b < p.graphs; b += gridDim.y) {
-        const Graph graph = graph_of(p, b);
-        const int chunks = chunks_of(p, graph);
-        if (graph.end - graph.begin <= p.handled) continue;      // finished
-        const float2* part = p.part + graph.first * p.channels + c;
-        const float2 s = sum_of_channel(chunks, [&](int j) { return c < p.channels ? part[(int64_t)j * p.channels] : make_float2(0.f, 0.f); }, room);
-        if (threadIdx.x < 8 && c < p.channels) p.sums[(int64_t)b * p.channels + c] = s;
+    __shared__ int list[kNormThreads];
+    const int c = blockIdx.x * 8 + (threadIdx.x & 7), begin = blockIdx.y * per, end = min(begin + per, p.graphs);
+    for (int b0 = begin; b0 < end; b0 += kNormThreads) {
+        const int n = open_graphs(p, b0, end, false, list);
+        for (int i = 0; i < n; i++) {
+            const Graph graph = graph_of(p, list[i]);
+            const float2* part = p.part + graph.first * p.channels + c;
+            const float2 s = sum_of_channel(chunks_of(p, graph), [&](int j) { return c < p.channels ? part[(int64_t)j * p.channels] : make_float2(0.f, 0.f); }, room);
+            if (threadIdx.x < 8 && c < p.channels) p.sums[(int64_t)list[i] * p.channels + c] = s;
+        }
     }
 }
 
@@ -875,6 +911,9 @@ static const char* refuse_norm(const mask_norm* n, bool backward) {
     return nullptr;
 }
 
+// Graphs a block, so that there are at most so many blocks for them (one at least).
+static int share_of(int graphs, int blocks) { return (graphs + std::max(blocks, 1) - 1) / std::max(blocks, 1); }
+
 template <typename T, int VEC, int ACT>
 static int launch_norm(const NormArgs& a, const NormPlan& p, bool backward, cudaStream_t st) {
     const dim3 grid((unsigned)p.chunks, (unsigned)p.slabs);
@@ -884,15 +923,17 @@ static int launch_norm(const NormArgs& a, const NormPlan& p, bool backward, cuda
     if (!backward) {
         if (p.clusters) return launch_overlapped(group_norm_cluster_kernel<T, VEC, ACT>, clusters, kNormThreads, 0, st, a);
         if ((rc = launch_overlapped(group_norm_moments_kernel<T, VEC, ACT>, grid, kNormThreads, 0, st, a)) || (all_handled && !a.offsets)) return rc;
-        if ((rc = launch_overlapped(group_norm_join_kernel, dim3((unsigned)(a.graphs * a.groups)), kNormThreads, 0, st, a))) return rc;
+        const int per = share_of(a.graphs, 4096 / a.groups);
+        if ((rc = launch_overlapped(group_norm_join_kernel, dim3((unsigned)((a.graphs + per - 1) / per * a.groups)), kNormThreads, 0, st, a, per))) return rc;
         return launch_overlapped(group_norm_apply_kernel<T, VEC, ACT>, grid, kNormThreads, 0, st, a);
     }
     if (p.clusters) return launch_overlapped(group_norm_grad_cluster_kernel<T, VEC, ACT>, clusters, kNormThreads, 0, st, a);
     const int32_t parts = (a.channels + 7) / 8;
     if ((rc = launch_overlapped(group_norm_grad_sums_kernel<T, VEC, ACT>, grid, kNormThreads, 0, st, a))) return rc;
-    if (!all_handled && (rc = launch_overlapped(group_norm_grad_join_kernel, dim3((unsigned)parts, (unsigned)std::max(1, std::min(a.graphs, 4 * sm_count() / parts))),
-                                                kNormThreads, 0, st, a)))
-        return rc;
+    if (!all_handled) {
+        const int per = share_of(a.graphs, 4 * sm_count() / parts);
+        if ((rc = launch_overlapped(group_norm_grad_join_kernel, dim3((unsigned)parts, (unsigned)((a.graphs + per - 1) / per)), kNormThreads, 0, st, a, per))) return rc;
+    }
     const unsigned more = a.dweight || a.dbias ? (unsigned)((parts + p.slabs - 1) / p.slabs) : 0;
     return launch_overlapped(group_norm_grad_apply_kernel<T, VEC, ACT>, dim3(grid.x + more, grid.y), kNormThreads, 0, st, a, p.chunks);
 }

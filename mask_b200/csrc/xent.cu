@@ -335,7 +335,7 @@ __device__ __forceinline__ void pack_hidden(const XentPackArgs& p, int64_t w0, i
     auto source = [&](int64_t i) -> const void* {
         return i < count ? static_cast<const char*>(p.hidden) + (int64_t)p.row_of[i] * p.hidden_stride * kBytes : nullptr;
     };
-    if (!kFloat && p.dim % 8 == 0 && p.hidden_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p.hidden) & 15) == 0 && end * (p.dim / 8) < ((int64_t)1 << 31)) {
+    if (!kFloat && p.dim % 8 == 0 && p.hidden_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p.hidden) & 15) == 0 && end * (p.dim / 8) < ((int64_t)1 << 30)) {
         // nothing but a copy, in vectors of 16 bytes, four of a thread's in flight
         const int per_row = p.dim / 8, total = (int)end * per_row, threads = (int)warps * 32;
         for (int i0 = (int)w0 * 32 + lane; i0 < total; i0 += 4 * threads) {

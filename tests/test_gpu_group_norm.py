@@ -205,6 +205,18 @@ def test_many_graphs():
 
 
 @gpu
+@pytest.mark.parametrize("channels,groups", [(64, 64), (96, 3)])
+def test_a_few_long_graphs_among_many_short_ones(channels, groups):
+    """Graphs of several chunks, whose sums are joined, between graphs that are finished at once and graphs without rows."""
+    import torch
+    sizes = torch.randint(0, 6, (400,), generator=torch.Generator().manual_seed(9))
+    for at, n in ((0, 3000), (37, 1500), (38, 2600), (399, 4000)):
+        sizes[at] = n
+    offsets = [0] + torch.cumsum(sizes, 0).tolist()
+    _both(offsets[-1], channels, groups, "f32", offsets, "silu", seed=9)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_far_from_zero_and_outliers(dtype):
     """Means a thousand times the deviation; a first row far from the rest."""
