@@ -259,8 +259,8 @@ class GCN2:
 
     The reference's driver trains such a network from its tensor library's pieces (end2end/gcn/eva_gcn_sparsene.py:316-343,
     599-781).  Here everything between the dense products ``X·W1`` and its gradient is this library's: sparse products with A
-    and A^T, group norm with the activation (per graph of a batch: ``offsets``), and the head with its gradients, which keeps
-    neither the logits nor their gradient in memory.
+    and A^T, group norm with the activation (per graph of a batch: ``offsets``, which cover every node), and the head with its
+    gradients, which does not keep the logits in memory.
 
     ``graph``: square CSR with ``rowptr``, ``colind``, ``values`` (NumPy) and ``M``.  ``ops`` supplies the device's pieces
     (``_TrainOps``), so that the chain of gradients can be checked without one.  ``tf32x3`` as in ``engine.spmm``."""
@@ -268,9 +268,13 @@ class GCN2:
     def __init__(self, graph, device, groups: int, activation: str = "relu", offsets=None, eps: float = 1e-5, tf32x3: bool = False, ops=None):
         if graph.M != graph.K:
             raise RuntimeError("the GCN needs a square adjacency matrix")
+        if offsets is not None:
+            offsets = np.asarray(offsets)
+            if offsets.ndim != 1 or len(offsets) < 2 or offsets[0] != 0 or offsets[-1] != graph.M or (np.diff(offsets) < 0).any():
+                raise RuntimeError("offsets must ascend from 0 to the number of nodes")
         self.groups, self.activation, self.eps = groups, activation, eps
         self.ops = ops if ops is not None else _TrainOps(device, tf32x3)
-        self.offsets = None if offsets is None else torch.as_tensor(np.asarray(offsets), dtype=torch.int32).to(device)
+        self.offsets = None if offsets is None else torch.as_tensor(offsets, dtype=torch.int32).to(device)
         self.A, self.At = self.ops.pack(graph), self.ops.pack(_transposed(graph))
 
     def _forward(self, X, W1, weight, bias):

@@ -114,6 +114,13 @@ def test_a_rectangular_matrix_is_refused():
         GCN2(G.CSR(2, 3, np.array([0, 0, 0], np.int32), np.zeros(0, np.int32), np.zeros(0, np.float32)), "cpu", 1, ops=PlainOps())
 
 
+@pytest.mark.parametrize("offsets", [[0, 100], [5, 256], [0, 300, 256], [0], [0, 100, 50, 256]])
+def test_offsets_that_leave_nodes_out_are_refused(offsets):
+    m = G.rmat_gcn_normalised(scale=8, samples_per_node=4, seed=3)
+    with pytest.raises(RuntimeError, match="offsets"):
+        GCN2(m, "cpu", 4, offsets=offsets, ops=PlainOps())
+
+
 class _Local:
     def __init__(self, t):
         self.local = t
