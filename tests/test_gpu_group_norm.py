@@ -315,12 +315,13 @@ def test_no_rows():
 
 
 @gpu
-def test_another_stream_captured_graphs_and_repeats():
+@pytest.mark.parametrize("rows,batch", [(1200, "ragged"), (1000, None), (60, None), (9000, None)])
+def test_another_stream_captured_graphs_and_repeats(rows, batch):
     import torch
     from mask_b200 import engine
-    x, grad, weight, bias = _inputs(1200, 80, "bf16", 11)
-    other = _inputs(1200, 80, "bf16", 12)[:2]
-    off = torch.tensor(BATCHES["ragged"], dtype=torch.int32, device="cuda")
+    x, grad, weight, bias = _inputs(rows, 80, "bf16", 11)
+    other = _inputs(rows, 80, "bf16", 12)[:2]
+    off = None if batch is None else torch.tensor(BATCHES[batch], dtype=torch.int32, device="cuda")
 
     def step(a, g):
         y, m, r = engine.group_norm(a, 10, weight, bias, off, activation="relu")
@@ -454,3 +455,27 @@ def test_engine_refusals():
                        ((grad, x, m, r.double(), 4), "rstd must be"), ((grad, x, m, r, 8), "mean must be"), ((grad.cpu(), x, m, r, 4), "grad must be a CUDA")):
         with pytest.raises(RuntimeError, match=says):
             engine.group_norm_backward(*args)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """2.5 thousand million values: the last graph's rows lie behind 2^31 elements."""
+    import torch
+    from mask_b200 import engine
+    rows, channels = (1 << 22) + 3, 600
+    g = torch.Generator(device="cuda").manual_seed(31)
+    x = torch.empty(rows, channels, device="cuda", dtype=torch.bfloat16)
+    for part in x.split(1 << 20):
+        part.copy_(torch.randn(part.shape, generator=g, device="cuda"))
+    offsets = [0, rows - 1000, rows]
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    y, m, r = engine.group_norm(x, 30, offsets=off, activation="silu")
+    _check_forward(x[-1000:], 30, None, None, activation="silu", got=(y[-1000:], m[1:], r[1:]))
+    # a mean over 84 million values of unit variance is within 1e-3 of 0, the deviation within 1e-3 of 1
+    assert float(m[0].abs().max()) < 1e-3 and float((r[0] - 1).abs().max()) < 1e-3
+    want = torch.nn.functional.silu((x[-2000:-1000].double().reshape(1000, 30, 20) - m[0].double()[:, None]) * r[0].double()[:, None]).reshape(1000, 600)
+    assert float((y[-2000:-1000].double() - want).abs().max()) < 0.03        # half a step of bfloat16 at 5 or so
+    dx, dw, db = engine.group_norm_backward(y, x, m, r, 30, offsets=off, activation="silu")
+    part = engine.group_norm_backward(y[-1000:].contiguous(), x[-1000:].contiguous(), m[1:].contiguous(), r[1:].contiguous(), 30, activation="silu")
+    assert float((dx[-1000:].double() - part[0].double()).abs().max()) < 0.03
+    assert bool(torch.isfinite(dw).all()) and bool(torch.isfinite(db).all())

@@ -234,13 +234,13 @@ def test_strides(dtype):
 
 
 @gpu
-@pytest.mark.parametrize("classes", [47, 1500])
-def test_another_stream_and_a_captured_graph(classes):
+@pytest.mark.parametrize("classes,dim", [(47, 80), (1500, 80), (1500, 600), (200, 256)])
+def test_another_stream_and_a_captured_graph(classes, dim):
     """Captured, and replayed with other contents in the same buffers while eager calls run beside it."""
     import torch
     from mask_b200 import engine
-    hidden, weight, labels = _inputs(700, 80, classes, "f32", "class", "some", seed=13)
-    other = _inputs(700, 80, classes, "f32", "class", "all", seed=14)
+    hidden, weight, labels = _inputs(700, dim, classes, "f32", "class", "some", seed=13)
+    other = _inputs(700, dim, classes, "f32", "class", "all", seed=14)
     want, want_other = (engine.linear_cross_entropy(*x, grads=True) for x in ((hidden, weight, labels), other))
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -265,6 +265,30 @@ def test_another_stream_and_a_captured_graph(classes):
         for got in (*outs, eager):
             for a, b in zip(got, expected):
                 assert torch.equal(a, b)
+
+
+@gpu
+def test_two_streams_at_once():
+    """Heads of every kind of tile on two streams, none waiting for the other, against the same one after the other."""
+    import torch
+    from mask_b200 import engine
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    problems = [[_inputs(rows, dim, classes, dtype, "class", "some", seed=s + k) for k, (rows, dim, classes, dtype) in
+                 enumerate(((2000, 512, 3000, "bf16"), (5000, 64, 40, "f32"), (1500, 300, 700, "f32"), (9000, 640, 500, "f16"), (100, 16, 7, "f32")))]
+                for s in (41, 51)]
+    wants = [[engine.linear_cross_entropy(*x, grads=True) for x in ps] for ps in problems]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i in range(len(problems[0])):
+            for side, ps, out in zip(sides, problems, got):
+                with torch.cuda.stream(side):
+                    out.append(engine.linear_cross_entropy(*ps[i], grads=True))
+    torch.cuda.synchronize()
+    for out, want in zip(got, wants):
+        for i, result in enumerate(out):
+            for a, b in zip(result, want[i % len(want)]):
+                assert torch.equal(a, b), i
 
 
 @gpu
@@ -399,3 +423,25 @@ def test_engine_refusals():
         with pytest.raises(RuntimeError, match=says):
             call(*args)
     assert torch.isfinite(call(hidden, weight, labels))
+
+
+@gpu
+@pytest.mark.parametrize("classes", [16, 300])
+def test_offsets_beyond_32_bits(classes):
+    """2.2 thousand million features: rows behind 2^31 elements, every other one labelled; rows do not depend on one another."""
+    import torch
+    from mask_b200 import engine
+    rows, dim = (1 << 22) + 5, 520
+    g = torch.Generator(device="cuda").manual_seed(37)
+    hidden = torch.empty(rows, dim, device="cuda", dtype=torch.bfloat16)
+    for part in hidden.split(1 << 20):
+        part.copy_(torch.randn(part.shape, generator=g, device="cuda"))
+    weight = (torch.randn(classes, dim, generator=g, device="cuda") * (2.0 / dim ** 0.5)).bfloat16().t()
+    labels = torch.randint(0, classes, (rows,), generator=g, device="cuda")
+    labels[::2] = -1
+    loss, dhidden, dweight = engine.linear_cross_entropy(hidden, weight, labels, reduction="none", grads=True)
+    tail = slice(rows - 1000, rows)
+    want = _want(hidden[tail], weight, labels[tail], "none")
+    _check(loss[tail], want[0], "loss")
+    _check(dhidden[tail], want[1], "dhidden")
+    assert bool(torch.isfinite(dweight).all()) and bool((loss[::2] == 0).all())
