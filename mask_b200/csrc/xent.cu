@@ -21,10 +21,10 @@
 namespace mask {
 
 constexpr int kXentCountThreads = 1024;
-// Rows and values (of hidden and of a weight that has to be packed) up to which one block prepares them: three launches fewer
-// (2708 x 16 x 7, a twentieth labelled: 33 us in all, 38 with them).
+// Rows and values (of hidden and of a weight that has to be packed) up to which one block prepares them, three launches fewer:
+// 50 x 16 x 64, loss alone, 13.4 us and 17.3 without; 3000 x 20 x 40 58 us and 41.
 constexpr int kXentSmallRows = 4096;
-constexpr int64_t kXentSmallValues = 65536;
+constexpr int64_t kXentSmallValues = 8192;
 // What a piece of G may take.  Few pieces fill the SMs better and add dH up less often: 16384 x 512 x 131072 bf16 takes 7.2 ms
 // with 2 GB, 7.6 with 1, 7.8 with 512 MB (which stays no more in the L2), 9.2 with 128; 200000 x 512 x 1000 float32 2.3, 2.4,
 // 3.0 and 3.3.
@@ -446,10 +446,12 @@ __global__ void __launch_bounds__(kXentCountThreads) xent_prepare_kernel(const X
 }
 
 // ---- tiny heads --------------------------------------------------------------------------------------------
-// The whole head by one block and without tensor cores, for problems that are smaller than their launches (kXentTiny...): a
-// warp per labelled row, its lanes along the classes for the logits and along the features for dH; then dW with the rows of a
-// product dealt to 1024 / (dim classes) threads, whose sums are added in their order.  Labelled rows and G stay in shared
-// memory where they fit.  2708 x 16 x 7, one row in twenty labelled: one launch instead of five.
+// The whole head by one cluster of eight blocks and without tensor cores, in one launch, for problems that are smaller than
+// their launches.  A block takes an eighth of the rows: a warp several labelled rows at a time, its lanes along the classes
+// for the logits and along the features for dH; then its share of dW, with the rows of a product dealt to 1024 / (dim
+// classes) threads.  Labelled rows and G stay in shared memory; the first block adds up the others' dW and losses in their
+// order.  2708 x 16 x 7 with one row in twenty labelled or all of them: 9.2 and 17.6 us, 33 and 36 by the
+// general way; 512 x 32 x 32 18 and 34; where one lane would go through long rows (100 x 1000 x 1) 140 and 54.
 struct XentTinyArgs {
     const void* hidden;
     int64_t hidden_stride;
@@ -460,15 +462,19 @@ struct XentTinyArgs {
     void* dweight;             // or NULL
     int64_t dw_dim_stride, dw_class_stride;
     int32_t dim;
-    float* g;                  // [rows][classes], where shared memory has no room
     float* loss;
     int32_t reduction;
     float scale;
 };
-constexpr int kXentTinyProduct = 1024;                  // dim * classes
-constexpr int kXentTinyKept = 4096;                     // values of labelled rows, and of G, in shared memory
-constexpr int kXentTinyBytes = 4 * (kXentSmallRows + 2 * kXentTinyKept + kXentTinyProduct + kXentCountThreads);
+constexpr int kXentTinyBlocks = 8;
+constexpr int kXentTinyProduct = 1024;                  // dim * classes, at most
+constexpr int kXentTinyDim = 256, kXentTinyClasses = 4; // at most, at least: a lane takes a feature or a class at a time
 constexpr int64_t kXentTinyWork = (int64_t)1 << 19;     // rows * dim * classes
+constexpr int kXentTinyRows = kXentSmallRows / kXentTinyBlocks, kXentTinyFeatures = 32768, kXentTinyGrads = 8192;     // of a block
+constexpr int kXentTinyBytes = 4 * (kXentTinyRows + kXentTinyFeatures + kXentTinyGrads + 2 * kXentTinyProduct + kXentCountThreads);
+
+// Rows (of hidden, of the weight) apart by an odd number of values, so that lanes with different rows use different banks.
+__host__ __device__ constexpr int tiny_pitch(int dim) { return dim | 1; }
 
 template <typename T> __device__ __forceinline__ float load_float(const void* p, int64_t i) {
     if constexpr (std::is_same<T, float>::value) return static_cast<const float*>(p)[i];
@@ -481,18 +487,74 @@ template <typename T> __device__ __forceinline__ void store_float(void* p, int64
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
 
-// Loss, G and gradients of `count` labelled rows (info: row, label << 16); kKept: their features and G are in shared memory.
-template <typename T, bool kKept>
-__device__ __forceinline__ void tiny_rows(const XentNumberArgs& n, const XentTinyArgs& p, int count, const uint32_t* info, const float* h_kept, float* g_all,
-                                          const float* w, float* room) {
+__device__ __forceinline__ float load_of_block(const float* own, uint32_t rank) {
+    float v;
+    asm volatile("{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
+                 : "=f"(v)
+                 : "r"((uint32_t)__cvta_generic_to_shared(own)), "r"(rank)
+                 : "memory");
+    return v;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kXentCountThreads) __cluster_dims__(kXentTinyBlocks, 1, 1) xent_tiny_kernel(const XentNumberArgs n, const XentTinyArgs p) {
+    wait_for_previous_kernel();
+    let_next_kernel_start();
+    extern __shared__ float tiny_smem[];
+    uint32_t* info = reinterpret_cast<uint32_t*>(tiny_smem);          // [labelled row of the block]: row of the block, label << 16
+    float* h = tiny_smem + kXentTinyRows;
+    float* g_all = h + kXentTinyFeatures;
+    float* w = g_all + kXentTinyGrads;                                // [dim][classes]
+    float* room = w + 2 * kXentTinyProduct;
+    __shared__ int sums[32];
+    __shared__ uint32_t have[kXentTinyRows / 32];                     // a bit for each of the block's rows: labelled
     __shared__ double losses_of[32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.dim, V = n.classes;
-    const float scale = xent_scale(p.scale, p.reduction == MASK_REDUCE_MEAN, count);
-    auto feature = [&](int i, int d) {
-        if constexpr (kKept) return h_kept[i * D + d];
-        else return load_float<T>(p.hidden, (int64_t)(info[i] & 0xffff) * p.hidden_stride + d);
-    };
+    __shared__ float result[kXentTinyProduct + 2];                    // the block's dW, then its loss as the sum of two floats
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.dim, V = n.classes, rows = (int)n.rows, pitch = tiny_pitch(D), w_pitch = tiny_pitch(V);
+    const int share = (rows + kXentTinyBlocks - 1) / kXentTinyBlocks, r0 = min(rows, (int)blockIdx.x * share), mine = min(share, rows - r0);
+
+    // labels: how many there are, and the block's own
+    int count_all = 0;
+    for (int r = threadIdx.x; r < (rows + kXentCountThreads - 1) / kXentCountThreads * kXentCountThreads; r += kXentCountThreads)
+        count_all += __syncthreads_count(r < rows && labelled(n.labels[min(r, rows - 1)], V));
+    const int64_t label_of = (int)threadIdx.x < mine ? n.labels[r0 + threadIdx.x] : -1;
+    const bool have_label = labelled(label_of, V);
+    const unsigned ballot = __ballot_sync(0xffffffffu, have_label);
+    if (lane == 0) {
+        sums[warp] = __popc(ballot);
+        if (warp < kXentTinyRows / 32) have[warp] = ballot;
+    }
+    for (int i = threadIdx.x; i < D * V; i += kXentCountThreads) {
+        const int d = i / V, v = i - d * V;
+        w[d * w_pitch + v] = load_float<T>(p.weight, d * p.w_dim_stride + v * p.w_class_stride);
+    }
+    __syncthreads();
+    const int in_warp = sums[lane], count = __reduce_add_sync(0xffffffffu, in_warp);
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? in_warp : 0);
+    if (have_label) info[before + __popc(ballot & ((1u << lane) - 1))] = threadIdx.x | (uint32_t)label_of << 16;
+    else if ((int)threadIdx.x < mine && n.row_loss) n.row_loss[r0 + threadIdx.x] = 0.f;
+    __syncthreads();
+    if (p.dhidden) {
+        // rows without a label, neighbouring threads at neighbouring addresses
+        constexpr int kWide = 16 / (int)sizeof(T);
+        const bool vec = (reinterpret_cast<uintptr_t>(p.dhidden) & 15) == 0 && p.dhidden_stride % kWide == 0 && D % kWide == 0;
+        const int pieces = vec ? D / kWide : D;
+        for (int i = threadIdx.x; i < mine * pieces; i += kXentCountThreads) {
+            const int r = i / pieces, piece = i - r * pieces;
+            if (have[r >> 5] >> (r & 31) & 1) continue;
+            T* to = static_cast<T*>(p.dhidden) + (r0 + r) * p.dhidden_stride;
+            if (vec) reinterpret_cast<uint4*>(to)[piece] = make_uint4(0u, 0u, 0u, 0u);
+            else store_float<T>(to, piece, 0.f);
+        }
+    }
+    for (int i = threadIdx.x; i < count * D; i += kXentCountThreads) {
+        const int at = i / D, d = i - at * D;
+        h[at * pitch + d] = load_float<T>(p.hidden, (int64_t)(r0 + (int)(info[at] & 0xffff)) * p.hidden_stride + d);
+    }
+    __syncthreads();
+
     // a warp takes as many rows at a time as have room for their classes side by side
+    const float scale = xent_scale(p.scale, p.reduction == MASK_REDUCE_MEAN, count_all);
     int width = 1;
     while (width < 32 && width < V) width *= 2;
     const int sub = lane & (width - 1), at_once = 32 / width;
@@ -501,14 +563,14 @@ __device__ __forceinline__ void tiny_rows(const XentNumberArgs& n, const XentTin
         const int i = i0 + lane / width;
         const bool live = i < count;
         const int row = live ? i : 0, label = (int)(info[row] >> 16);
+        const float* x = h + row * pitch;
         float* g = g_all + row * V;
-        float top = -INFINITY, picked = 0.f, first = 0.f;
+        float top = -INFINITY, picked = 0.f;
         for (int v = sub; v < V; v += width) {
             float s = 0.f;
 #pragma unroll 8
-            for (int d = 0; d < D; d++) s = fmaf(feature(row, d), w[d * V + v], s);
-            if (v == sub) first = s;
-            else if (live) g[v] = s;
+            for (int d = 0; d < D; d++) s = fmaf(x[d], w[d * w_pitch + v], s);
+            if (live) g[v] = s;
             top = fmaxf(top, s);
             if (v == label) picked = s;
         }
@@ -516,128 +578,74 @@ __device__ __forceinline__ void tiny_rows(const XentNumberArgs& n, const XentTin
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             picked += __shfl_xor_sync(0xffffffffu, picked, o);
         }
-        float sum = sub < V ? fast_exp2((first - top) * kLog2e) : 0.f;
-        const float e_first = sum;
-        for (int v = sub + width; v < V; v += width) sum += fast_exp2((g[v] - top) * kLog2e);
+        float sum = 0.f;
+        for (int v = sub; v < V; v += width) sum += live ? fast_exp2((g[v] - top) * kLog2e) : 0.f;
         for (int o = width / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const float loss = live ? kLn2 * fmaf(top - picked, kLog2e, log2f(sum)) : 0.f;
-        if (sub == 0) {
+        if (sub == 0 && live) {
             losses += loss;
-            if (live && n.row_loss) n.row_loss[info[row] & 0xffff] = loss;
+            if (n.row_loss) n.row_loss[r0 + (int)(info[row] & 0xffff)] = loss;
         }
         if (!p.dhidden && !p.dweight) continue;
         const float inv = 1.f / sum;
         for (int v = sub; v < V; v += width) {
-            const float e = (v == sub ? e_first : fast_exp2((g[v] - top) * kLog2e)) * inv;
-            if (live) g[v] = v == label ? e - 1.f : e;
+            if (!live) continue;
+            const float e = fast_exp2((g[v] - top) * kLog2e) * inv;
+            g[v] = v == label ? e - 1.f : e;
         }
         __syncwarp();
         if (p.dhidden && live) {
-            const int64_t to = (int64_t)(info[row] & 0xffff) * p.dhidden_stride;
+            const int64_t to = (int64_t)(r0 + (int)(info[row] & 0xffff)) * p.dhidden_stride;
             for (int d = sub; d < D; d += width) {
                 float s = 0.f;
 #pragma unroll 8
-                for (int v = 0; v < V; v++) s = fmaf(g[v], w[d * V + v], s);
+                for (int v = 0; v < V; v++) s = fmaf(g[v], w[d * w_pitch + v], s);
                 store_float<T>(p.dhidden, to + d, scale * s);
             }
         }
+        __syncwarp();
     }
     for (int o = 16; o > 0; o >>= 1) losses += __shfl_xor_sync(0xffffffffu, losses, o);
     if (lane == 0) losses_of[warp] = losses;
     __syncthreads();
-    if (threadIdx.x == 0 && !n.row_loss) {
+    if (threadIdx.x == 0) {
         double s = 0.0;
         for (int i = 0; i < 32; i++) s += losses_of[i];
-        *p.loss = count == 0 ? 0.f : (float)(p.reduction == MASK_REDUCE_MEAN ? s / count : s);
+        result[kXentTinyProduct] = (float)s;
+        result[kXentTinyProduct + 1] = (float)(s - (double)(float)s);
     }
-    if (!p.dweight) return;
-    const int shares = kXentCountThreads / (D * V), share = threadIdx.x / (D * V), pair = threadIdx.x - share * (D * V);
-    const int d = pair / V, v = pair - d * V;
-    float s = 0.f;
-    if (share < shares) {
+    const int shares = kXentCountThreads / (D * V), part = threadIdx.x / (D * V), pair = threadIdx.x - part * (D * V);
+    if (p.dweight) {
+        const int d = pair / V, v = pair - d * V;
+        float s = 0.f;
+        if (part < shares) {
 #pragma unroll 4
-        for (int i = share; i < count; i += shares) s = fmaf(g_all[i * V + v], feature(i, d), s);
-    }
-    room[threadIdx.x] = s;
-    __syncthreads();
-    if (share == 0) {
-        for (int i = 1; i < shares; i++) s += room[i * D * V + pair];
-        store_float<T>(p.dweight, d * p.dw_dim_stride + v * p.dw_class_stride, scale * s);
-    }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kXentCountThreads) xent_tiny_kernel(const XentNumberArgs n, const XentTinyArgs p) {
-    wait_for_previous_kernel();
-    let_next_kernel_start();
-    constexpr int kTurns = kXentSmallRows / kXentCountThreads;
-    extern __shared__ float tiny_smem[];
-    uint32_t* info = reinterpret_cast<uint32_t*>(tiny_smem);         // [labelled row]: row, label << 16
-    float* h_kept = tiny_smem + kXentSmallRows;
-    float* g_kept = h_kept + kXentTinyKept;
-    float* w = g_kept + kXentTinyKept;                                // [dim][classes]
-    float* room = w + kXentTinyProduct;
-    __shared__ int sums[kTurns][32];
-    __shared__ uint32_t have[kXentSmallRows / 32];                    // a bit for each row: labelled
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.dim, V = n.classes, rows = (int)n.rows;
-    // labels, and the rows without one
-    int y[kTurns];
-    unsigned ballot[kTurns];
-#pragma unroll
-    for (int k = 0; k < kTurns; k++) {
-        const int r = k * kXentCountThreads + threadIdx.x;
-        const int64_t label = r < rows ? n.labels[r] : -1;
-        y[k] = labelled(label, V) ? (int)label : -1;
-    }
-    for (int i = threadIdx.x; i < D * V; i += kXentCountThreads) {
-        const int d = i / V, v = i - d * V;
-        w[i] = load_float<T>(p.weight, d * p.w_dim_stride + v * p.w_class_stride);
-    }
-#pragma unroll
-    for (int k = 0; k < kTurns; k++) {
-        ballot[k] = __ballot_sync(0xffffffffu, y[k] >= 0);
-        if (lane == 0) {
-            sums[k][warp] = __popc(ballot[k]);
-            have[k * 32 + warp] = ballot[k];
+            for (int i = part; i < count; i += shares) s = fmaf(g_all[i * V + v], h[i * pitch + d], s);
         }
-    }
-    __syncthreads();
-    int count = 0;
-#pragma unroll
-    for (int k = 0; k < kTurns; k++) {
-        const int r = k * kXentCountThreads + threadIdx.x, in_warp = sums[k][lane];
-        const int before = __reduce_add_sync(0xffffffffu, lane < warp ? in_warp : 0);
-        if (y[k] >= 0) {
-            info[count + before + __popc(ballot[k] & ((1u << lane) - 1))] = (uint32_t)r | (uint32_t)y[k] << 16;
-        } else if (r < rows && n.row_loss) {
-            n.row_loss[r] = 0.f;
-        }
-        count += __reduce_add_sync(0xffffffffu, in_warp);
-    }
-    __syncthreads();
-    if (p.dhidden) {
-        // rows without a label, neighbouring threads at neighbouring addresses
-        constexpr int kWide = 16 / (int)sizeof(T);
-        const bool vec = (reinterpret_cast<uintptr_t>(p.dhidden) & 15) == 0 && p.dhidden_stride % kWide == 0 && D % kWide == 0;
-        const int pieces = vec ? D / kWide : D;
-        for (int i = threadIdx.x; i < rows * pieces; i += kXentCountThreads) {
-            const int r = i / pieces, piece = i - r * pieces;
-            if (have[r >> 5] >> (r & 31) & 1) continue;
-            T* to = static_cast<T*>(p.dhidden) + r * p.dhidden_stride;
-            if (vec) reinterpret_cast<uint4*>(to)[piece] = make_uint4(0u, 0u, 0u, 0u);
-            else store_float<T>(to, piece, 0.f);
-        }
-    }
-    if (count * D <= kXentTinyKept && count * V <= kXentTinyKept) {
-        for (int i = threadIdx.x; i < count * D; i += kXentCountThreads) {
-            const int at = i / D;
-            h_kept[i] = load_float<T>(p.hidden, (int64_t)(info[at] & 0xffff) * p.hidden_stride + (i - at * D));
-        }
+        room[threadIdx.x] = s;
         __syncthreads();
-        tiny_rows<T, true>(n, p, count, info, h_kept, g_kept, w, room);
-    } else {
-        tiny_rows<T, false>(n, p, count, info, nullptr, p.g, w, room);
+        if (part == 0) {
+            for (int i = 1; i < shares; i++) s += room[i * D * V + pair];
+            result[pair] = s;
+        }
     }
+    cluster_sync();
+    if (blockIdx.x == 0) {
+        if (p.dweight && part == 0) {
+            float s = 0.f;
+#pragma unroll
+            for (uint32_t r = 0; r < kXentTinyBlocks; r++) s += load_of_block(result + pair, r);
+            const int d = pair / V, v = pair - d * V;
+            store_float<T>(p.dweight, d * p.dw_dim_stride + v * p.dw_class_stride, scale * s);
+        }
+        if (threadIdx.x == 0 && !n.row_loss) {
+            double s = 0.0;
+            for (uint32_t r = 0; r < kXentTinyBlocks; r++)
+                s += (double)load_of_block(result + kXentTinyProduct, r) + (double)load_of_block(result + kXentTinyProduct + 1, r);
+            *p.loss = count_all == 0 ? 0.f : (float)(p.reduction == MASK_REDUCE_MEAN ? s / count_all : s);
+        }
+    }
+    cluster_sync();                   // the blocks' results have been read
 }
 
 template <typename T>
@@ -645,7 +653,7 @@ static int launch_xent_tiny(const XentNumberArgs& n, const XentTinyArgs& t, cuda
     static std::atomic<uint64_t> done{0};
     const int rc = opt_in_shared_memory(reinterpret_cast<const void*>(xent_tiny_kernel<T>), kXentTinyBytes, done);
     if (rc != MASK_OK) return rc;
-    return launch_overlapped(xent_tiny_kernel<T>, dim3(1), kXentCountThreads, kXentTinyBytes, st, n, t);
+    return launch_overlapped(xent_tiny_kernel<T>, dim3(kXentTinyBlocks), kXentCountThreads, kXentTinyBytes, st, n, t);
 }
 
 // ---- joining -----------------------------------------------------------------------------------------------
@@ -887,7 +895,9 @@ static XentPlan plan_xent(const mask_head& h) {
             p.part_dw_rows = round_up(p.piece, kXentTileM);
         }
     }
-    p.tiny = h.rows <= kXentSmallRows && (int64_t)h.dim * h.classes <= kXentTinyProduct && h.rows * h.dim * h.classes <= kXentTinyWork;
+    const int64_t share = (h.rows + kXentTinyBlocks - 1) / kXentTinyBlocks;
+    p.tiny = h.rows <= kXentSmallRows && h.dim <= kXentTinyDim && h.classes >= kXentTinyClasses && (int64_t)h.dim * h.classes <= kXentTinyProduct && h.rows * h.dim * h.classes <= kXentTinyWork &&
+             share * tiny_pitch(h.dim) <= kXentTinyFeatures && share * h.classes <= kXentTinyGrads;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -904,7 +914,6 @@ static XentPlan plan_xent(const mask_head& h) {
     if (p.tiny) {
         p.chunk = kXentSmallRows;
         p.n_chunks = 1;
-        p.g = take(4 * (size_t)(h.rows * h.classes));
         p.bytes = at;
         return p;
     }
@@ -1021,7 +1030,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
     XentNumberArgs number = {h.d_labels, h.rows, plan.chunk, h.classes, counts, row_of, label, total, total + 1, range, nullptr, 0, row_loss};
     if (plan.tiny) {
         const XentTinyArgs t = {h.d_hidden, h.hidden_stride, h.d_weight, h.weight_dim_stride, h.weight_class_stride, h.d_dhidden, h.dhidden_stride, h.d_dweight,
-                                h.dweight_dim_stride, h.dweight_class_stride, h.dim, reinterpret_cast<float*>(at(plan.g)), h.d_loss, h.reduction, h.grad_scale};
+                                h.dweight_dim_stride, h.dweight_class_stride, h.dim, h.d_loss, h.reduction, h.grad_scale};
         if (h.dtype == MASK_F32) return launch_xent_tiny<float>(number, t, st);
         if (h.dtype == MASK_F16) return launch_xent_tiny<__half>(number, t, st);
         return launch_xent_tiny<__nv_bfloat16>(number, t, st);
