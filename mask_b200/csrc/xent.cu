@@ -165,8 +165,8 @@ __device__ __forceinline__ void scan_rows(int64_t rows, int64_t n, int64_t strid
             row[k] = base(min(i + k * step, rows - 1));
             vec = vec && (reinterpret_cast<uintptr_t>(row[k]) & 15) == 0;
         }
-        int64_t d = 4 * sub;
         if (vec) {
+            int64_t d = 4 * sub;
             for (; d + 4 <= n; d += 4 * lanes) {
                 float4 v[4];
 #pragma unroll
@@ -174,19 +174,29 @@ __device__ __forceinline__ void scan_rows(int64_t rows, int64_t n, int64_t strid
 #pragma unroll
                 for (int k = 0; k < 4; k++) m = max(m, max(max(finite_magnitude(v[k].x), finite_magnitude(v[k].y)), max(finite_magnitude(v[k].z), finite_magnitude(v[k].w))));
             }
-        }
-        for (; d < n; d += 4 * lanes)
-            for (int64_t e = d; e < min(d + 4, n); e++)
+            for (; d < n; d++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) m = max(m, finite_magnitude(__ldg(row[k] + e * stride)));
+                for (int k = 0; k < 4; k++) m = max(m, finite_magnitude(__ldg(row[k] + d)));
+        } else {
+#pragma unroll 2
+            for (int64_t d = sub; d < n; d += lanes)
+#pragma unroll
+                for (int k = 0; k < 4; k++) m = max(m, finite_magnitude(__ldg(row[k] + d * stride)));
+        }
     }
 }
 __device__ __forceinline__ void scan_weight(const XentPackArgs& p, int64_t w0, int64_t warps, uint32_t& m) {
     const float* weight = static_cast<const float*>(p.weight);
-    if (p.w_class_stride == 1)
-        scan_rows(p.dim, p.classes, 1, 32, w0, warps, [&](int64_t d) { return weight + d * p.w_dim_stride; }, m);
-    else
+    if (p.w_class_stride == 1) {
+        // stretches of 4096 of each row, the last one beginning so that it ends with the row
+        const int64_t n = min((int64_t)p.classes, (int64_t)4096), parts = (p.classes + n - 1) / n;
+        scan_rows(p.dim * parts, n, 1, 32, w0, warps, [&](int64_t i) {
+            const int64_t d = i / parts;
+            return weight + d * p.w_dim_stride + min((i - d * parts) * n, p.classes - n);
+        }, m);
+    } else {
         scan_rows(p.classes, p.dim, p.w_dim_stride, lanes_for(p.dim), w0, warps, [&](int64_t v) { return weight + v * p.w_class_stride; }, m);
+    }
 }
 
 // The largest finite magnitudes of both operands (FP32 input) to p.range.  A maximum does not depend on the order.
@@ -401,6 +411,7 @@ __global__ void __launch_bounds__(kXentPackThreads) xent_pack_kernel(const XentP
     const int64_t vt = (p.classes + 31) / 32, dt = (p.dim_pad + 31) / 32;
     for (int64_t i = w0; i < vt * dt; i += warps) {
         const int64_t v0 = i % vt * 32, d0 = i / vt * 32;
+#pragma unroll 8
         for (int j = 0; j < 32; j++) {
             uint32_t x = 0;
             if (d0 + j < p.dim && v0 + lane < p.classes) {
@@ -411,17 +422,21 @@ __global__ void __launch_bounds__(kXentPackThreads) xent_pack_kernel(const XentP
             t[j][lane] = x;
         }
         __syncwarp();
-        for (int j = 0; j < 32; j++) {
-            if (v0 + j < p.classes && d0 + lane < p.dim_pad) {
-                uint16_t* to = p.w_planes + (v0 + j) * p.dim_pad + d0 + lane;
-                const uint32_t x = t[lane][j];
+        // two classes at a time, two features a lane (dim_pad is even)
+        const int d = 2 * (lane & 15);
+#pragma unroll 4
+        for (int j = lane >> 4; j < 32; j += 2) {
+            if (v0 + j < p.classes && d0 + d < p.dim_pad) {
+                uint16_t* to = p.w_planes + (v0 + j) * p.dim_pad + d0 + d;
+                const uint32_t x = t[d][j], y = t[d + 1][j];
                 if constexpr (kFloat) {
-                    uint32_t h, l;
-                    split_half(w_scale * __uint_as_float(x), h, l);
-                    to[0] = (uint16_t)h;
-                    to[p.w_plane] = (uint16_t)l;
+                    uint32_t h[2], l[2];
+                    split_half(w_scale * __uint_as_float(x), h[0], l[0]);
+                    split_half(w_scale * __uint_as_float(y), h[1], l[1]);
+                    *reinterpret_cast<uint32_t*>(to) = h[0] | h[1] << 16;
+                    *reinterpret_cast<uint32_t*>(to + p.w_plane) = l[0] | l[1] << 16;
                 } else {
-                    to[0] = (uint16_t)x;
+                    *reinterpret_cast<uint32_t*>(to) = x | y << 16;
                 }
             }
         }
@@ -853,6 +868,13 @@ static int tile_width(int n) {
     return n <= 128 || round_up(n, 128) < round_up(n, 256) ? 128 : 256;
 }
 
+// Whether rows of a result may be written in vectors of eight values (32 bytes of FP32, 16 of the others).  A product whose
+// rows may not be leaves its tiles in parts, in scratch, which are then written by neighbouring threads: a thread per row
+// costs a request for every value.
+static bool vector_rows(const void* data, int64_t stride, int dtype) {
+    return stride % 8 == 0 && (reinterpret_cast<uintptr_t>(data) & (dtype == MASK_F32 ? 31 : 15)) == 0;
+}
+
 static XentPlan plan_xent(const mask_head& h) {
     XentPlan p = {};
     p.planes = h.dtype == MASK_F32 ? 2 : 1;
@@ -886,12 +908,12 @@ static XentPlan plan_xent(const mask_head& h) {
         p.part_ld = (int)(n_tiles * p.bn_dim);
         if (h.d_dhidden) {
             p.dh_splits = best_splits(p.rows_pad, tile_blocks(p.bn_dim, p.rows_pad), n_tiles, (p.piece + kXentTileK - 1) / kXentTileK, 4);
-            p.dh_parts = p.dh_splits > 1 || p.n_pieces > 1;
+            p.dh_parts = p.dh_splits > 1 || p.n_pieces > 1 || !vector_rows(h.d_dhidden, h.dhidden_stride, h.dtype);
             p.part_dh_rows = p.rows_pad;
         }
         if (h.d_dweight) {
             p.dw_splits = best_splits(p.piece, tile_blocks(p.bn_dim, p.piece), n_tiles, (p.rows_pad + kXentTileK - 1) / kXentTileK, 4);
-            p.dw_parts = p.dw_splits > 1;
+            p.dw_parts = p.dw_splits > 1 || (h.dweight_dim_stride == 1 && h.dweight_class_stride != 1 && !vector_rows(h.d_dweight, h.dweight_class_stride, h.dtype));
             p.part_dw_rows = round_up(p.piece, kXentTileM);
         }
     }
@@ -1116,8 +1138,6 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
         const int64_t n_tiles = plan.part_ld / plan.bn_dim;
         XentReduceArgs r = {};
         r.part_ld = plan.part_ld; r.n = h.dim; r.count = total; r.row_of = row_of; r.out_type = h.dtype; r.scale = a.scale; r.mean = a.mean; r.range = a.range;
-        const int64_t vec = 8;      // elements of a vector: 32 bytes of FP32, 16 of the others
-        const uintptr_t aligned = h.dtype == MASK_F32 ? 31 : 15;
         for (int piece = 0; piece < plan.n_pieces; piece++) {
             a.v0 = piece * plan.piece;
             a.vc = std::min(plan.piece, h.classes - a.v0);
@@ -1131,7 +1151,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
                 b.store = !plan.dh_parts ? kXentFinal : (piece == 0 ? kXentPartial : kXentAccumulate);
                 b.part = reinterpret_cast<float*>(at(plan.part_dh)); b.part_rows = plan.part_dh_rows; b.part_ld = plan.part_ld;
                 b.out = h.d_dhidden; b.out_m = h.dhidden_stride; b.out_n = 1;
-                b.out_vec = h.dhidden_stride % vec == 0 && (reinterpret_cast<uintptr_t>(h.d_dhidden) & aligned) == 0;
+                b.out_vec = vector_rows(h.d_dhidden, h.dhidden_stride, h.dtype);
                 if ((rc = launch_xent_gemm<kXentDHidden>(plan.bn_dim, P, b, rp, n_tiles * b.splits, g_k, w_mn, none, st))) return rc;
             }
             if (h.d_dweight) {
@@ -1140,7 +1160,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
                 b.store = plan.dw_parts ? kXentPartial : kXentFinal;
                 b.part = reinterpret_cast<float*>(at(plan.part_dw)); b.part_rows = plan.part_dw_rows; b.part_ld = plan.part_ld;
                 b.out = h.d_dweight; b.out_m = h.dweight_class_stride; b.out_n = h.dweight_dim_stride;
-                b.out_vec = b.out_n == 1 && b.out_m % vec == 0 && (reinterpret_cast<uintptr_t>(h.d_dweight) & aligned) == 0;
+                b.out_vec = b.out_n == 1 && vector_rows(h.d_dweight, b.out_m, h.dtype);
                 if ((rc = launch_xent_gemm<kXentDWeight>(plan.bn_dim, P, b, a.vc, n_tiles * b.splits, g_mn, h_mn, none, st))) return rc;
                 if (plan.dw_parts) {
                     XentReduceArgs w = r;

@@ -617,35 +617,32 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             }
             const int64_t row = MODE == kXentDHidden ? (int64_t)p.row_of[r] : (int64_t)p.v0 + r;
             const int64_t at = row * p.out_m + (int64_t)col * p.out_n;
-            if (p.out_vec && col + 32 <= n_extent) {
-                if (p.out_type == MASK_F32) {
-                    float* to = static_cast<float*>(p.out) + at;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
+            for (int j = 0; j < 4; j++) {
+                const int left = n_extent - col - 8 * j;      // eight values at a time
+                const int64_t to = at + 8 * j * p.out_n;
+                if (p.out_vec && left >= 8) {
+                    if (p.out_type == MASK_F32) {
                         float x[8];
 #pragma unroll
                         for (int i = 0; i < 8; i++) x[i] = scale(v[8 * j + i]);
-                        st_global_v8(to + 8 * j, x);
-                    }
-                } else {
-                    uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
+                        st_global_v8(static_cast<float*>(p.out) + to, x);
+                    } else {
                         uint32_t h[4];
 #pragma unroll
                         for (int q = 0; q < 4; q++) h[q] = pack_half2(scale(v[8 * j + 2 * q]), scale(v[8 * j + 2 * q + 1]), p.out_type == MASK_F16);
-                        to[j] = make_uint4(h[0], h[1], h[2], h[3]);
+                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to) = make_uint4(h[0], h[1], h[2], h[3]);
                     }
+                    continue;
                 }
-                return;
-            }
 #pragma unroll
-            for (int j = 0; j < 32; j++) {
-                if (col + j >= n_extent) continue;
-                const float x = scale(v[j]);
-                if (p.out_type == MASK_F32) static_cast<float*>(p.out)[at + j * p.out_n] = x;
-                else if (p.out_type == MASK_F16) static_cast<__half*>(p.out)[at + j * p.out_n] = __float2half_rn(x);
-                else static_cast<__nv_bfloat16*>(p.out)[at + j * p.out_n] = __float2bfloat16_rn(x);
+                for (int i = 0; i < 8; i++) {
+                    if (i >= left) continue;
+                    const float x = scale(v[8 * j + i]);
+                    if (p.out_type == MASK_F32) static_cast<float*>(p.out)[to + i * p.out_n] = x;
+                    else if (p.out_type == MASK_F16) static_cast<__half*>(p.out)[to + i * p.out_n] = __float2half_rn(x);
+                    else static_cast<__nv_bfloat16*>(p.out)[to + i * p.out_n] = __float2bfloat16_rn(x);
+                }
             }
         };
         const float f = kLogits ? logit_factor(p.range) : 0.f;
