@@ -418,8 +418,8 @@ int mask_spmm_srbcrs_static_scratch(const mask_plan* plan, const int32_t* d_val_
  * 1024 weight values and 2^19 products are computed in float32 throughout); infinite or NaN logits of a labelled row make its loss and the
  * gradients NaN.  Results do not depend on the order of anything: the same call gives the same bits.
  *
- * Scratch: mask_linear_xent_scratch_bytes(head) bytes, 256-byte aligned, one call at a time (two captured graphs
- * that may run at once need two).  Asynchronous on `stream`.  Should a kernel give up on one of its bounded
+ * Scratch: mask_linear_xent_scratch_bytes(head) bytes for this head's sizes, strides and result addresses (results
+ * off 32 bytes need more), 256-byte aligned, one call at a time (two captured graphs that may run at once need two).  Asynchronous on `stream`.  Should a kernel give up on one of its bounded
  * waits, the losses (of the labelled rows, where they are all that is asked for) are NaN.
  * ------------------------------------------------------------------------------------------ */
 typedef enum mask_dtype { MASK_F32 = 0, MASK_BF16 = 1, MASK_F16 = 2 } mask_dtype;
