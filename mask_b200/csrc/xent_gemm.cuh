@@ -89,9 +89,11 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return y;
 }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// What a product of the planes of hidden and weight is multiplied with to become a logit in units of log 2.
+// What a product of the planes of hidden and weight is multiplied with to become a logit in units of log 2.  Neither infinite
+// (0 stays 0) nor 0 or subnormal (-inf, a row's maximum before its first logit, stays -inf): products that are smaller still
+// vanish beside 1 anyway.
 __device__ __forceinline__ float logit_factor(const uint32_t* range) {
-    return range ? ldexpf(kLog2e, min(plane_exponent(range[0]) + plane_exponent(range[1]) - 28, 126)) : kLog2e;   // finite: 0 stays 0
+    return range ? ldexpf(kLog2e, max(-126, min(plane_exponent(range[0]) + plane_exponent(range[1]) - 28, 126))) : kLog2e;
 }
 
 // CG: blocks that share a tile.  2: a cluster of two takes 256 rows, each block 128 of them and half of the columns' operand,
