@@ -596,6 +596,7 @@ __global__ void __launch_bounds__(kXentCountThreads) __cluster_dims__(kXentTinyB
         float sum = 0.f;
         for (int v = sub; v < V; v += width) sum += live ? fast_exp2((g[v] - top) * kLog2e) : 0.f;
         for (int o = width / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        sum = bounded_sum(sum, top * kLog2e);
         const float loss = live ? kLn2 * fmaf(top - picked, kLog2e, log2f(sum)) : 0.f;
         if (sub == 0 && live) {
             losses += loss;
@@ -679,7 +680,7 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const XentArgs p, int p
     let_next_kernel_start();
     __shared__ float2 room[1024];
     const int count = *p.count, rows = 1024 / shares, share = threadIdx.x / rows, at = threadIdx.x & (rows - 1);
-    const float f = logit_factor(p.range);
+    const float f = logit_factor(p.range), rest = logit_rest(p.range);
     const bool lost = *p.status != 0;
     for (int64_t r0 = rows * (int64_t)blockIdx.x; r0 < count; r0 += rows * (int64_t)gridDim.x) {
         const int64_t r = r0 + at;
@@ -702,10 +703,12 @@ __global__ void __launch_bounds__(1024) xent_join_kernel(const XentArgs p, int p
         for (int i = 1; i < shares; i++) join(room[i * rows + at]);
         float loss = 0.f;
         if (r < count) {
-            const float base = exponent_base(top, f), log_sum = log2f(sum);
-            p.shift[r] = p.range ? base : base + log_sum;
+            const float base = exponent_base(top, f);
+            sum = bounded_sum(sum, base);
+            const float log_sum = log2f(sum);
+            p.shift[r] = p.range ? base : __fadd_ru(base, log_sum);
             p.factor[r] = (float)(1 << kGradExponent) / sum;
-            loss = lost ? NAN : kLn2 * (fmaf(-p.label_logit[r], f, base) + log_sum);
+            loss = lost ? NAN : kLn2 * (fmaf(-p.label_logit[r] * rest, f, base) + log_sum);
             if (p.row_loss) p.row_loss[p.row_of[r]] = loss;
         }
         const bool any = __any_sync(0xffffffffu, r < count);

@@ -47,7 +47,7 @@ struct XentArgs {
     const int32_t* row_of;     // [labelled row] -> row of the caller's arrays
     float2* stats;             // [splits * epilogue parts][rows_pad]: maximum, sum of exp(logit - maximum)
     float* label_logit;        // [labelled row]
-    float* shift;              // [labelled row]: 16-bit input: log2 of the row's sum of exponentials; FP32: what the sum's
+    float* shift;              // [labelled row]: 16-bit input: log2 of the row's sum of exponentials, rounded up (no probability above 1); FP32: what the sum's
     float* factor;             //   exponents were taken less, and 2^15 over the sum (a log sum rounded to 32 bits would put 1e-6 on a whole row)
     float* row_loss;           // caller's, or NULL
     float* warp_loss;          // [rows_pad / 32]: sums of 32 rows' losses
@@ -89,12 +89,18 @@ __device__ __forceinline__ float fast_exp2(float x) {
     return y;
 }
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// What a product of the planes of hidden and weight is multiplied with to become a logit in units of log 2.  Neither infinite
-// (0 stays 0) nor 0 or subnormal (-inf, a row's maximum before its first logit, stays -inf): products that are smaller still
-// vanish beside 1 anyway.
-__device__ __forceinline__ float logit_factor(const uint32_t* range) {
-    return range ? ldexpf(kLog2e, max(-126, min(plane_exponent(range[0]) + plane_exponent(range[1]) - 28, 126))) : kLog2e;
-}
+// Power of two of a product of the planes of hidden and weight.
+__device__ __forceinline__ int logit_exponent(const uint32_t* range) { return plane_exponent(range[0]) + plane_exponent(range[1]) - 28; }
+// What such a product is multiplied with to become a logit in units of log 2.  Neither infinite (0 stays 0) nor 0 or subnormal
+// (-inf, a row's maximum before its first logit, stays -inf): products that are smaller still vanish beside 1 anyway, and larger
+// ones are beyond kLogitBound unless they are 0.
+__device__ __forceinline__ float logit_factor(const uint32_t* range) { return range ? ldexpf(kLog2e, max(-126, min(logit_exponent(range), 126))) : kLog2e; }
+// What the factor leaves out above, for a label's logit, which may be as far below the largest as it likes.
+__device__ __forceinline__ float logit_rest(const uint32_t* range) { return range ? ldexpf(1.f, max(logit_exponent(range) - 126, 0)) : 1.f; }
+// A row's largest logit, in bits, up to which there is a softmax.  Exponents are taken less the rounded number of bits, off by 32
+// here; not much beyond, they pass what an exponential takes, and the sum would be any number.  The row's sum is NaN instead.
+constexpr float kLogitBound = 1073741824.f;
+__device__ __forceinline__ float bounded_sum(float sum, float base) { return fabsf(base) < kLogitBound ? sum : NAN; }
 
 // CG: blocks that share a tile.  2: a cluster of two takes 256 rows, each block 128 of them and half of the columns' operand,
 // and the first issues the MMAs for both.
@@ -759,11 +765,12 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                         at_label += ex[i * 128 * 3 + 2];
                     }
                 }
-                const float log_sum = log2f(all), shift = !live ? INFINITY : (P == 2 ? bs : bs + log_sum);
+                all = bounded_sum(all, bs);
+                const float log_sum = log2f(all), shift = !live ? INFINITY : (P == 2 ? bs : __fadd_ru(bs, log_sum));
                 const float factor = P == 2 && live ? (float)(1 << kGradExponent) / all : 0.f;
                 const float own = live ? label_gradient(at_label, shift, factor) : 0.f;
                 if (part == 0) {
-                    const float loss = live ? kLn2 * (fmaf(-at_label, f, bs) + log_sum) : 0.f;
+                    const float loss = live ? kLn2 * (fmaf(-at_label * logit_rest(p.range), f, bs) + log_sum) : 0.f;
                     if (live && p.row_loss) p.row_loss[p.row_of[r]] = loss;
                     float w = loss;
 #pragma unroll

@@ -20,3 +20,56 @@ def test_logits_that_vanish(scale_h, scale_w, classes):
     loss, dhidden, dweight = _both(hidden * scale_h, weight * scale_w, labels)
     assert abs(float(loss) - math.log(classes)) < 2.0 ** -20 * (1 + math.log(classes))
     assert bool(torch.isfinite(dhidden).all()) and bool(torch.isfinite(dweight).all())
+
+
+def _far_operands(classes):
+    """Logits of row 0: 2^180 for class 0, else 0; of the others: 2^120 for odd classes, else 0."""
+    import torch
+    hidden = torch.zeros(70, 64, device="cuda")
+    weight = torch.zeros(64, classes, device="cuda")
+    hidden[0, 0], hidden[1:, 1] = 2.0 ** 120, 2.0 ** 90
+    weight[0, 0], weight[1, 1::2] = 2.0 ** 60, 2.0 ** 30
+    return hidden, weight, torch.arange(70, device="cuda") % classes
+
+
+@gpu
+@pytest.mark.parametrize("classes", [50, 600])
+def test_logits_beyond_a_float(classes):
+    """Infinite ones are their row's alone; a label's that is far below the largest keeps its size."""
+    import torch
+    from mask_b200 import engine
+    hidden, weight, labels = _far_operands(classes)
+    loss = engine.linear_cross_entropy(hidden, weight, labels, reduction="none")
+    assert bool(loss[0].isnan())
+    # largest logit 0, the label's -2^120 with the same operands' scales
+    hidden[1:, 1] *= -1
+    loss, dhidden, dweight = engine.linear_cross_entropy(hidden, weight, labels, reduction="none", grads=True)
+    assert bool(loss[0].isnan()) and bool(dhidden[0].isnan().any())
+    odd = labels[1:] % 2 == 1
+    even = (classes + 1) // 2
+    assert float((loss[1:][odd] / 2.0 ** 120 - 1).abs().max()) < 2.0 ** -20
+    assert float((loss[1:][~odd] - math.log(even)).abs().max()) < 2.0 ** -20 * 8
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("classes", [12, 50, 600])
+def test_logits_that_no_exponent_tells_apart(classes, dtype):
+    """Beyond 2^29 or so a row's loss and gradients are NaN, not any number; the other rows' are theirs.  Logits of a million
+    are taken."""
+    import torch
+    from mask_b200 import engine
+    hidden, weight, labels = _inputs(90, 64, classes, dtype, seed=12)
+    hidden[40:] *= 2.0 ** 36
+    loss, dhidden, dweight = engine.linear_cross_entropy(hidden, weight, labels, reduction="none", grads=True)
+    far = (hidden.double() @ weight.double()).amax(1).abs() > 2.0 ** 31
+    assert bool(far[40:].any()) and not bool(far[:40].any())
+    assert bool(loss[far].isnan().all()) and bool(dhidden[far].isnan().all()) and bool(torch.isfinite(loss[:40]).all())
+    if dtype == "bf16":         # operands are what they are; float32 ones are exact to 2^-40 of the largest
+        want = _want(hidden[:40], weight, labels[:40], "none")
+        _check(loss[:40], want[0], "loss")
+        _check(dhidden[:40], want[1], "dhidden")
+    hidden, weight, labels = _inputs(90, 64, classes, dtype, seed=12)
+    hidden[:40] *= 2.0 ** 20
+    got = engine.linear_cross_entropy(hidden, weight, labels, reduction="none")
+    _check(got, _want(hidden, weight, labels, "none")[0], "loss")
