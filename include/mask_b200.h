@@ -414,7 +414,7 @@ int mask_spmm_srbcrs_static_scratch(const mask_plan* plan, const int32_t* d_val_
  * float32 operands are multiplied as three products of float16 parts of 22 bits together (relative error of a
  * product at most 2^-20; values below 2^-18 of the largest finite magnitude of their operand, labelled rows
  * only, are exact to 2^-40 of that), 16-bit ones exactly; sums are float32.  The gradient of the logits is
- * held in the same parts, or in the operands' 16-bit type, between its products (heads of up to 4096 rows,
+ * held in the same parts, or in the operands' 16-bit type (float16: times 2^15, since most are small), between its products (heads of up to 4096 rows,
  * 1024 weight values and 2^19 products are computed in float32 throughout).  A labelled row's loss and
  * gradients are NaN if one of its logits is NaN or +inf, or its largest beyond about 7e8 in magnitude (float32
  * logits that large are 64 apart); infinite or NaN logits make dweight NaN.  Results do not depend on the order of anything: the same call gives the same bits.

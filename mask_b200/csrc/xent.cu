@@ -740,7 +740,7 @@ struct XentReduceArgs {
 __device__ __forceinline__ void reduce_parts(const XentReduceArgs& p) {
     const int count = *p.count;
     const int64_t m_end = p.m_is_count ? count : p.m, n_vec = (p.n + 3) / 4;
-    const ProductScale scale = product_scale(p.scale, p.mean, count, p.range, p.operand);
+    const ProductScale scale = product_scale(p.scale, p.mean, count, p.range, p.operand, p.out_type == MASK_F16);
     const bool m_fast = p.out_m == 1 && p.out_n != 1;
     __shared__ float4 room[256];
     const int per_block = 256 / p.shares, share = threadIdx.x / per_block;

@@ -67,7 +67,12 @@ struct XentArgs {
 
 // Power of two of an operand's planes: planes = 2^(14 - e) operand.  Below 2^-100 everything is scaled alike.
 __device__ __forceinline__ int plane_exponent(uint32_t largest) { return max((int)(largest >> 23) - 127, -100); }
-constexpr int kGradExponent = 15;      // planes of G hold 2^15 G for FP32 input
+// fp16 planes of G, one or two, hold 2^15 G: without it the probabilities of a head of 2^14 classes are subnormal, those below
+// 2^-25 are 0 (a column of dW that is nobody's label was off by up to 2 % where most are), and a scaled loss, which comes behind the products,
+// brings none of them back.  bf16 has float32's range.
+constexpr int kGradExponent = 15;
+// A plane of bf16 operands holds G itself, in 8 bits, as the products behind it take them: rounded once, by 2^-9 of each value at most,
+// of the size of the results' own rounding; a second plane would double the two products of it, half of the head's work.
 
 __device__ __forceinline__ float xent_scale(float scale, bool mean, int count) { return mean ? (count > 0 ? scale / (float)count : 0.f) : scale; }
 // The same for a product of G's planes with those of an operand: two factors, since the power of two alone may be too small
@@ -76,9 +81,9 @@ struct ProductScale {
     float a, b;
     __device__ __forceinline__ float operator()(float x) const { return a * x * b; }
 };
-__device__ __forceinline__ ProductScale product_scale(float scale, bool mean, int count, const uint32_t* range, int operand) {
+__device__ __forceinline__ ProductScale product_scale(float scale, bool mean, int count, const uint32_t* range, int operand, bool half_type) {
     scale = xent_scale(scale, mean, count);
-    if (!range) return {scale, 1.f};
+    if (!range) return {half_type ? 1.f / (float)(1 << kGradExponent) : 1.f, scale};
     const int e = plane_exponent(range[operand]) - 14 - kGradExponent;
     return {ldexpf(scale, e / 2), ldexpf(1.f, e - e / 2)};
 }
@@ -654,7 +659,10 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             }
         };
         const float f = kLogits ? logit_factor(p.range) : 0.f;
-        // exp(logit) over the row's sum; 0 outside the classes and, where shift is infinite, the rows.  FP32 input: times 2^15.
+        // exp(logit) over the row's sum, for fp16 planes times 2^15 (one plane: `shift` is less by that, rounded up so that nothing
+        // passes 2^15); 0 outside the classes and, where shift is infinite, the rows
+        const float one = half_type ? (float)(1 << kGradExponent) : 1.f;
+        auto row_shift = [&](float shift) { return P == 1 && half_type ? __fadd_ru(shift, -(float)kGradExponent) : shift; };
         [[maybe_unused]] auto gradient = [&](float (&v)[32], int col, int classes, float shift, float factor) {
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = fast_exp2(fmaf(v[j], f, -shift)) * (P == 2 ? factor : 1.f);
@@ -667,7 +675,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
         // the same less 1 at the row's label, whose logit is `picked`
         [[maybe_unused]] auto label_gradient = [&](float picked, float shift, float factor) {
             const float e = fast_exp2(fmaf(picked, f, -shift));
-            return P == 2 ? e * factor - (float)(1 << kGradExponent) : e - 1.f;
+            return P == 2 ? e * factor - one : e - one;
         };
         for (int64_t i = group; i < items && ok; i += groups) {
             if (L::kGroups > 1 && count_of_items++ % L::kGroups != mine) continue;
@@ -705,7 +713,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             } else if constexpr (MODE == kXentGrad) {
                 const bool live = r < count;
                 const int label = live ? p.label[r] - p.v0 : -1, y = label < p.vc ? label : -1;       // within the piece
-                const float shift = live ? p.shift[r] : INFINITY, factor = P == 2 && live ? p.factor[r] : 0.f;
+                const float shift = live ? row_shift(p.shift[r]) : INFINITY, factor = P == 2 && live ? p.factor[r] : 0.f;
                 const float at_label = y >= 0 ? label_gradient(p.label_logit[r], shift, factor) : 0.f;
                 if (!acquire(t.k0, t.k1)) { ok = false; break; }
 #pragma unroll(kUnroll)
@@ -766,7 +774,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     }
                 }
                 all = bounded_sum(all, bs);
-                const float log_sum = log2f(all), shift = !live ? INFINITY : (P == 2 ? bs : __fadd_ru(bs, log_sum));
+                const float log_sum = log2f(all), shift = !live ? INFINITY : (P == 2 ? bs : row_shift(__fadd_ru(bs, log_sum)));
                 const float factor = P == 2 && live ? (float)(1 << kGradExponent) / all : 0.f;
                 const float own = live ? label_gradient(at_label, shift, factor) : 0.f;
                 if (part == 0) {
@@ -789,7 +797,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             } else {
                 const bool empty = t.k0 >= t.k1;      // nothing to contract: the sum is zero
                 if (!empty && !acquire(t.k0, t.k1)) { ok = false; break; }
-                const ProductScale scale = product_scale(p.scale, p.mean, count, p.range, MODE == kXentDHidden ? 1 : 0);
+                const ProductScale scale = product_scale(p.scale, p.mean, count, p.range, MODE == kXentDHidden ? 1 : 0, half_type);
                 const bool live = r < m_extent;
 #pragma unroll(kUnroll)
                 for (int c = 0; c < kChunks; c++) {

@@ -73,3 +73,21 @@ def test_logits_that_no_exponent_tells_apart(classes, dtype):
     hidden[:40] *= 2.0 ** 20
     got = engine.linear_cross_entropy(hidden, weight, labels, reduction="none")
     _check(got, _want(hidden, weight, labels, "none")[0], "loss")
+
+
+@gpu
+def test_probabilities_below_the_range_of_float16():
+    """Logits of deviation 4 over 60000 classes: most probabilities are below 2^-25.  Columns of dweight that are nobody's label
+    are sums of them; two roundings, of the logits' gradient and of the result, leave at most 2^-11 each of a column that one
+    term makes up and less of one with more, beside 2^-18 of the logits' and the exponential's."""
+    import torch
+    from mask_b200 import engine
+    hidden, weight, labels = _inputs(256, 64, 60000, "f16", seed=18)
+    weight = (2.0 * weight.t().float()).half().t()
+    labels %= 1000
+    _, dhidden, dweight = engine.linear_cross_entropy(hidden, weight, labels, reduction="sum", grads=True, grad_scale=2.0 ** 12)
+    p = torch.softmax(hidden.double() @ weight.double(), 1)
+    want = 2.0 ** 12 * (hidden.double().t() @ p)[:, 1000:]
+    off = (dweight[:, 1000:].double() - want).norm(dim=0)
+    # values of dweight below 2^-14 are rounded to 2^-24
+    assert float((off - 2.0 ** -25 * 8.0).div(want.norm(dim=0)).max()) < 2.0 ** -10 + 2.0 ** -17
