@@ -415,9 +415,11 @@ int mask_spmm_srbcrs_static_scratch(const mask_plan* plan, const int32_t* d_val_
  * product at most 2^-20; values below 2^-18 of the largest finite magnitude of their operand, labelled rows
  * only, are exact to 2^-40 of that), 16-bit ones exactly; sums are float32.  The gradient of the logits is
  * held in the same parts, or in the operands' 16-bit type (float16: times 2^15, since most are small), between its products (heads of up to 4096 rows,
- * 1024 weight values and 2^19 products are computed in float32 throughout).  A labelled row's loss and
- * gradients are NaN if one of its logits is NaN or +inf, or its largest beyond about 7e8 in magnitude (float32
- * logits that large are 64 apart); infinite or NaN logits make dweight NaN.  Results do not depend on the order of anything: the same call gives the same bits.
+ * 1024 weight values and 2^19 products are computed in float32 throughout).  A class whose logit is -inf (a weight of
+ * -inf and a positive feature) has probability 0; an entry of a gradient whose formula multiplies that 0 with the infinite
+ * weight is NaN.  (In float32 a large finite stand-in for -inf costs the other values their bits, as above.)  A
+ * labelled row's loss and gradients are NaN if one of its logits is NaN or +inf, or its largest beyond about 7e8 in
+ * magnitude (float32 logits that large are 64 apart), and so is dweight. Results do not depend on the order of anything: the same call gives the same bits.
  *
  * Scratch: mask_linear_xent_scratch_bytes(head) bytes for this head's sizes, strides and result addresses (results
  * off 32 bytes need more), 256-byte aligned, one call at a time (two captured graphs that may run at once need two).  Asynchronous on `stream`.  Should a kernel give up on one of its bounded

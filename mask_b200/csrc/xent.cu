@@ -285,12 +285,12 @@ __global__ void __launch_bounds__(kXentCountThreads) xent_scan_kernel(const Xent
     }
 }
 
-// hi and lo of a scaled float; an infinite or NaN hi has no lo
+// hi and lo of a scaled float.  An infinity is all lo: of the three products of parts only the one with the other operand's hi
+// is infinite then, none is 0 times infinity.  NaN is all hi.
 __device__ __forceinline__ void split_half(float x, uint32_t& hi, uint32_t& lo) {
-    const __half h = __float2half_rn(x);
-    const float hf = __half2float(h);
+    const __half h = __float2half_rn(isinf(x) ? 0.f : x);
     hi = __half_as_ushort(h);
-    lo = __half_as_ushort(__float2half_rn(isfinite(hf) ? x - hf : 0.f));
+    lo = __half_as_ushort(__float2half_rn(isnan(x) ? 0.f : x - __half2float(h)));
 }
 
 // One row of `dim` elements `stride` apart to the planes, by `lanes` lanes of which this is number `lane`; `src` NULL writes zeros.

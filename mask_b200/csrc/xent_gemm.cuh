@@ -660,12 +660,16 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
         };
         const float f = kLogits ? logit_factor(p.range) : 0.f;
         // exp(logit) over the row's sum, for fp16 planes times 2^15 (one plane: `shift` is less by that, rounded up so that nothing
-        // passes 2^15); 0 outside the classes and, where shift is infinite, the rows
+        // passes 2^15); 0 outside the classes and the rows, whatever the weight made of a row of zeros (infinities: NaN)
         const float one = half_type ? (float)(1 << kGradExponent) : 1.f;
         auto row_shift = [&](float shift) { return P == 1 && half_type ? __fadd_ru(shift, -(float)kGradExponent) : shift; };
-        [[maybe_unused]] auto gradient = [&](float (&v)[32], int col, int classes, float shift, float factor) {
+        [[maybe_unused]] auto gradient = [&](float (&v)[32], int col, int classes, bool live, float shift, float factor) {
 #pragma unroll
             for (int j = 0; j < 32; j++) v[j] = fast_exp2(fmaf(v[j], f, -shift)) * (P == 2 ? factor : 1.f);
+            if (__any_sync(0xffffffffu, !live)) {
+#pragma unroll
+                for (int j = 0; j < 32; j++) v[j] = live ? v[j] : 0.f;
+            }
             if (col + 32 > classes) {
 #pragma unroll
                 for (int j = 0; j < 32; j++)
@@ -713,7 +717,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
             } else if constexpr (MODE == kXentGrad) {
                 const bool live = r < count;
                 const int label = live ? p.label[r] - p.v0 : -1, y = label < p.vc ? label : -1;       // within the piece
-                const float shift = live ? row_shift(p.shift[r]) : INFINITY, factor = P == 2 && live ? p.factor[r] : 0.f;
+                const float shift = live ? row_shift(p.shift[r]) : 0.f, factor = P == 2 && live ? p.factor[r] : 0.f;
                 const float at_label = y >= 0 ? label_gradient(p.label_logit[r], shift, factor) : 0.f;
                 if (!acquire(t.k0, t.k1)) { ok = false; break; }
 #pragma unroll(kUnroll)
@@ -721,7 +725,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     const int col = t.n0 * BN + part * kWidth + 32 * c;     // within the piece
                     float v[32];
                     values(c, v);
-                    gradient(v, col, p.vc, shift, factor);
+                    gradient(v, col, p.vc, live, shift, factor);
                     write_g(v, r - lane, col, c, y, at_label);
                 }
                 done();
@@ -774,7 +778,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     }
                 }
                 all = bounded_sum(all, bs);
-                const float log_sum = log2f(all), shift = !live ? INFINITY : (P == 2 ? bs : row_shift(__fadd_ru(bs, log_sum)));
+                const float log_sum = log2f(all), shift = P == 2 ? bs : row_shift(__fadd_ru(bs, log_sum));
                 const float factor = P == 2 && live ? (float)(1 << kGradExponent) / all : 0.f;
                 const float own = live ? label_gradient(at_label, shift, factor) : 0.f;
                 if (part == 0) {
@@ -790,7 +794,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                     const int col = part * kWidth + 32 * c;
                     float v[32];
                     values(c, v);
-                    gradient(v, col, p.classes, shift, factor);
+                    gradient(v, col, p.classes, live, shift, factor);
                     write_g(v, r - lane, col, c, y, own);
                 }
                 done();

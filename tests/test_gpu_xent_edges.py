@@ -75,6 +75,75 @@ def test_logits_that_no_exponent_tells_apart(classes, dtype):
     _check(got, _want(hidden, weight, labels, "none")[0], "loss")
 
 
+MASKED = [(100, 16, 20), (150, 64, 50), (300, 64, 600), (129, 200, 300)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("rows,dim,classes", MASKED)
+@pytest.mark.parametrize("layout", ["dim", "class"])
+def test_classes_masked_by_minus_infinity(rows, dim, classes, dtype, layout):
+    """A feature that is 1 and whose weight is -inf takes classes out: probability 0, whatever way the sizes take.  What is
+    multiplied with that weight, the feature's own gradient, is 0 times infinity."""
+    import torch
+    from mask_b200 import engine
+    hidden, weight, labels = _inputs(rows, dim, classes, dtype, "dim", "some", seed=15)
+    hidden[:, dim - 1] = 1.0
+    masked = torch.arange(classes, device="cuda") % 3 == 1
+    labels[(labels >= 0) & (labels < classes) & (labels % 3 == 1)] = 0
+    out = weight.clone()
+    out[dim - 1, masked] = -math.inf
+    out = out.t().contiguous().t() if layout == "dim" else out.contiguous()
+    kept = torch.nonzero(~masked).squeeze(1)
+    place = torch.full((classes,), -1, dtype=torch.int64, device="cuda")
+    place[kept] = torch.arange(len(kept), device="cuda")
+    real = (labels >= 0) & (labels < classes)
+    fewer = torch.where(real, place[labels.clamp(0, classes - 1)], -1)
+    want = _want(hidden, weight[:, kept], fewer, "sum")
+    for got in (engine.linear_cross_entropy(hidden, out, labels, reduction="sum"),
+                engine.linear_cross_entropy(hidden, out, labels, reduction="sum", grads=True)[0]):
+        _check(got, want[0], "loss")
+    _, dhidden, dweight = engine.linear_cross_entropy(hidden, out, labels, reduction="sum", grads=True)
+    _check(dweight[:, kept], want[2], "dweight")
+    assert bool((dweight[:, masked] == 0).all())
+    _check(dhidden[:, :dim - 1], tuple(t[:, :dim - 1] for t in want[1]), "dhidden")
+    assert bool(dhidden[real, dim - 1].isnan().all()) and bool((dhidden[~real] == 0).all())
+    # a label that is masked: the loss is infinite
+    at = int(torch.nonzero(real)[0])
+    labels[at] = 1
+    loss = engine.linear_cross_entropy(hidden, out, labels, reduction="none")
+    assert float(loss[at]) == math.inf
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("rows,dim,classes", MASKED)
+def test_classes_masked_by_the_lowest_value(rows, dim, classes, dtype):
+    """In 16 bits the lowest value is as good: products with it are exact."""
+    import torch
+    hidden, weight, labels = _inputs(rows, dim, classes, dtype, "dim", "some", seed=16)
+    hidden[:, dim - 1] = 1.0
+    masked = torch.arange(classes, device="cuda") % 3 == 1
+    labels[(labels >= 0) & (labels < classes) & (labels % 3 == 1)] = 0
+    weight = weight.clone()
+    weight[dim - 1, masked] = torch.finfo(weight.dtype).min
+    from mask_b200 import engine
+    loss, dhidden, dweight = engine.linear_cross_entropy(hidden, weight, labels, grads=True)
+    kept = torch.nonzero(~masked).squeeze(1)
+    real = (labels >= 0) & (labels < classes)
+    logits = hidden[real].double() @ weight.double()
+    want = torch.nn.functional.cross_entropy(logits, labels[real])
+    assert abs(float(loss) - float(want)) < 2.0 ** -16 * (1 + float(want))
+    assert bool(torch.isfinite(dhidden).all()) and bool((dweight[:, masked] == 0).all())
+    g = torch.softmax(logits, 1)
+    g[torch.arange(len(g)), labels[real]] -= 1.0
+    dw = hidden[real].double().t() @ g / len(g)
+    # two roundings to 8 or 11 bits: of the logits' gradient and of the result
+    step = torch.finfo(weight.dtype).eps / 2
+    bound = (hidden[real].double().abs().t() @ g.abs() / len(g) + dw.abs()) * (step + 2.0 ** -16) + 2.0 ** -24
+    assert bool(((dweight.double() - dw).abs()[:, kept] <= bound[:, kept]).all())
+
+
 @gpu
 def test_probabilities_below_the_range_of_float16():
     """Logits of deviation 4 over 60000 classes: most probabilities are below 2^-25.  Columns of dweight that are nobody's label
