@@ -839,6 +839,7 @@ struct XentPlan {
     int piece, n_pieces;                 // classes of a piece (a multiple of 256 unless one tile holds all), pieces
     int g_ld;
     int dh_splits, dw_splits;
+    int segment;                         // blocks of their contraction that an accumulator takes (16-bit operands)
     bool dh_parts, dw_parts;
     int64_t part_dh_rows, part_dw_rows;
     int part_ld;
@@ -909,14 +910,20 @@ static XentPlan plan_xent(const mask_head& h) {
         p.n_pieces = (int)((h.classes + (int64_t)p.piece - 1) / p.piece);
         const int64_t n_tiles = (h.dim + p.bn_dim - 1) / p.bn_dim;
         p.part_ld = (int)(n_tiles * p.bn_dim);
+        p.segment = h.dtype == MASK_F16 ? kXentLongSegmentF16 : kXentLongSegmentBf16;
+        // contractions of several segments are added up in the parts
+        auto segmented = [&](int64_t contracted, int splits) {
+            const int64_t units = (contracted + kXentTileK - 1) / kXentTileK;
+            return p.planes == 1 && (units + splits - 1) / splits > p.segment;
+        };
         if (h.d_dhidden) {
             p.dh_splits = best_splits(p.rows_pad, tile_blocks(p.bn_dim, p.rows_pad), n_tiles, (p.piece + kXentTileK - 1) / kXentTileK, 4);
-            p.dh_parts = p.dh_splits > 1 || p.n_pieces > 1 || !vector_rows(h.d_dhidden, h.dhidden_stride, h.dtype);
+            p.dh_parts = p.dh_splits > 1 || p.n_pieces > 1 || segmented(p.piece, p.dh_splits) || !vector_rows(h.d_dhidden, h.dhidden_stride, h.dtype);
             p.part_dh_rows = p.rows_pad;
         }
         if (h.d_dweight) {
             p.dw_splits = best_splits(p.piece, tile_blocks(p.bn_dim, p.piece), n_tiles, (p.rows_pad + kXentTileK - 1) / kXentTileK, 4);
-            p.dw_parts = p.dw_splits > 1 || (h.dweight_dim_stride == 1 && h.dweight_class_stride != 1 && !vector_rows(h.d_dweight, h.dweight_class_stride, h.dtype));
+            p.dw_parts = p.dw_splits > 1 || segmented(p.rows_pad, p.dw_splits) || (h.dweight_dim_stride == 1 && h.dweight_class_stride != 1 && !vector_rows(h.d_dweight, h.dweight_class_stride, h.dtype));
             p.part_dw_rows = round_up(p.piece, kXentTileM);
         }
     }
@@ -1117,7 +1124,7 @@ static int run_xent(const mask_head& h, const XentPlan& plan, char* scratch, cud
     a.shift = reinterpret_cast<float*>(at(plan.shift));
     a.factor = reinterpret_cast<float*>(at(plan.factor));
     a.warp_loss = reinterpret_cast<float*>(at(plan.warp_loss));
-    a.scale = h.grad_scale; a.mean = h.reduction == MASK_REDUCE_MEAN;
+    a.segment = plan.segment; a.scale = h.grad_scale; a.mean = h.reduction == MASK_REDUCE_MEAN;
     a.out_type = h.dtype;
 
     if (!plan.one_pass) {

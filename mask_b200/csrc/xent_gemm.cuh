@@ -6,9 +6,11 @@
 // Operands are 16-bit "planes": one for bf16 and fp16 input.  FP32 input is scaled by a power of two that brings the
 // operand's largest magnitude to 2^14..2^15 and split into two fp16 planes, x = hi + lo + e with |e| <= 2^-22 |x|, or 2^-40
 // of the largest where that is more; a product is hi hi + hi lo + lo hi (the dropped lo lo is 2^-22 of it at most).
-// The MMA cuts its sum off to 32 bits toward zero after every 16 products (2730 such steps in a row left 2e-5 of the
-// result); for FP32 input an accumulator therefore takes kXentSegment blocks of the contraction, and the segments are added
-// in registers, rounded to nearest.  For 16-bit input what is cut off is far below the result's own rounding.
+// The MMA cuts its sum off toward zero after every 16 products: 2e-7 of it at most, which adds up where the terms have one sign
+// (16384 steps in a row left 1.7e-3 of dW; 2730 with terms of both signs 2e-5).  For FP32 input an accumulator therefore
+// takes kXentSegment blocks of the contraction, and the segments are added in registers, rounded to nearest.  For 16-bit input the
+// products with G, whose contraction has no bound, leave an accumulator after kXentLongSegment blocks and are added up in the parts
+// (1e-7 times 512 steps in fp16, 4096 in bf16: a tenth or a fifth of the results' own rounding); logits take all of theirs.
 // All three products have the layouts TMA and the MMA take as they are, whichever axis is contracted:
 //     logits[r,v] = sum_d H[r,d] W[v,d]     both operands K-major
 //     dH[r,d]     = sum_v G[r,v] W[v,d]     G K-major, W MN-major
@@ -26,6 +28,7 @@ namespace mask {
 
 constexpr int kXentTileM = 128, kXentTileK = 64;
 constexpr int kXentSegment = 2;                     // blocks of the contraction that an accumulator takes (FP32 input)
+constexpr int kXentLongSegmentF16 = 128, kXentLongSegmentBf16 = 1024;      // the same for products with G of 16-bit input
 enum XentMode {
     kXentStats,      // logits -> running maximum and sum of each row over a range of classes
     kXentGrad,       // logits -> G of a piece of the classes, with the rows' log sums known
@@ -54,7 +57,8 @@ struct XentArgs {
     float* part;               // [splits][m_pad][n_pad]
     int64_t part_rows;         // m_pad
     int32_t part_ld;           // n_pad
-    int32_t store;             // XentStore
+    int32_t store;             // XentStore of a tile's first segment; the others are added to it
+    int32_t segment;           // 16-bit input, products with G: blocks of the contraction that an accumulator takes
     void* out;                 // final store: element (m, n) at m * out_m + n * out_n
     int64_t out_m, out_n;
     int32_t out_type;          // MASK_F32 / MASK_BF16 / MASK_F16
@@ -455,7 +459,7 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                             if (!open) {
                                 buf = 2 * g + (acc_it & 1);
                                 acc = tmem_base + buf * BN;
-                                left = P == 2 ? min(kXentSegment, t.k1 - k) : t.k1 - k;
+                                left = P == 2 ? min(kXentSegment, t.k1 - k) : (kLogits ? t.k1 - k : min(p.segment, t.k1 - k));
                                 if (acc_it >= 2 && !wait_all_lanes(acce_bar(buf), ((acc_it >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
                             }
                             if (!wait_all_lanes(full_bar(s), round & 1, abort_flag)) { ok = false; break; }
@@ -610,10 +614,10 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
 
         [[maybe_unused]] uint32_t turn = 0, count_of_items = 0;
         // 32 values of row r of a product, from column col, to the parts or to the caller
-        [[maybe_unused]] auto write_out = [&](const float (&v)[32], const ProductScale& scale, int split, int r, int col) {
-            if (p.store != kXentFinal) {
+        [[maybe_unused]] auto write_out = [&](const float (&v)[32], const ProductScale& scale, int store, int split, int r, int col) {
+            if (store != kXentFinal) {
                 float* to = p.part + ((int64_t)split * p.part_rows + r) * p.part_ld + col;
-                if (p.store == kXentAccumulate) {
+                if (store == kXentAccumulate) {
                     float sum[32];
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
@@ -800,24 +804,29 @@ xent_gemm_kernel(const XentArgs p, const __grid_constant__ CUtensorMap map_a, co
                 done();
             } else {
                 const bool empty = t.k0 >= t.k1;      // nothing to contract: the sum is zero
-                if (!empty && !acquire(t.k0, t.k1)) { ok = false; break; }
                 const ProductScale scale = product_scale(p.scale, p.mean, count, p.range, MODE == kXentDHidden ? 1 : 0, half_type);
                 const bool live = r < m_extent;
+                int store = p.store, k = t.k0;
+                do {                                  // segment by segment
+                    if (!empty && !acquire(t.k0, t.k1)) { ok = false; break; }
 #pragma unroll(kUnroll)
-                for (int c = 0; c < kChunks; c++) {
-                    const int col = t.n0 * BN + part * kWidth + 32 * c;
-                    if (col >= n_extent) break;
-                    float v[32];
-                    if (!empty) {
-                        __syncwarp();
-                        values(c, v);
-                    } else {
+                    for (int c = 0; c < kChunks; c++) {
+                        const int col = t.n0 * BN + part * kWidth + 32 * c;
+                        if (col >= n_extent) break;
+                        float v[32];
+                        if (!empty) {
+                            __syncwarp();
+                            values(c, v);
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < 32; j++) v[j] = 0.f;
+                            for (int j = 0; j < 32; j++) v[j] = 0.f;
+                        }
+                        if (live) write_out(v, scale, store, t.split, r, col);
                     }
-                    if (live) write_out(v, scale, t.split, r, col);
-                }
-                if (!empty) done();
+                    if (!empty) done();
+                    store = kXentAccumulate;
+                    k += p.segment;
+                } while (P == 1 && k < t.k1);
             }
         }
         if constexpr (L::kWritesG) {

@@ -160,3 +160,29 @@ def test_probabilities_below_the_range_of_float16():
     off = (dweight[:, 1000:].double() - want).norm(dim=0)
     # values of dweight below 2^-14 are rounded to 2^-24
     assert float((off - 2.0 ** -25 * 8.0).div(want.norm(dim=0)).max()) < 2.0 ** -10 + 2.0 ** -17
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_sums_over_many_rows_are_not_cut_short(dtype):
+    """The tensor core cuts its sum off toward zero after every 16 products; where all terms have one sign that adds up, 16384
+    times for 2^18 rows of positive features (1.7e-3).  A quarter of the result's own rounding is granted."""
+    import torch
+    from mask_b200 import engine
+    rows, dim, classes = 1 << 18, 1024, 4096
+    hidden, weight, labels = _inputs(rows, dim, classes, dtype, seed=20)
+    hidden.abs_()
+    labels %= 16
+    dweight = engine.linear_cross_entropy(hidden, weight, labels, reduction="sum", grads=True, grad_scale=1.0)[2][:, 16:]
+    want = torch.zeros(dim, classes, dtype=torch.float64, device="cuda")
+    for part in hidden.split(1 << 15):
+        want += part.double().t() @ torch.softmax(part.double() @ weight.double(), 1)
+    want = want[:, 16:]
+    slope = float((dweight.double() * want).sum() / want.square().sum()) - 1
+    assert abs(slope) < torch.finfo(hidden.dtype).eps / 8, slope
+
+
+@gpu
+def test_segments_and_pieces():
+    """Contractions over the classes of a piece and over the rows that leave the tensor core more than once, with more than one piece."""
+    _both(*_inputs(40000, 64, 60001, "f16", "dim", "some", seed=22), scale=2.0 ** 12)
