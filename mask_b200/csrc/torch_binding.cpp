@@ -110,6 +110,10 @@ const at::Tensor* device_tensor(PyObject* o, const char* name, int dims, int* de
         PyErr_Format(PyExc_RuntimeError, "%s must be a dense %d-D tensor", name, dims);
         return nullptr;
     }
+    if (t.is_neg()) {       // a view whose values have another sign than its memory
+        PyErr_Format(PyExc_RuntimeError, "%s is a negative view: pass resolve_neg() of it", name);
+        return nullptr;
+    }
     if (*device < 0) *device = at::cuda::current_device();
     if (t.get_device() != *device) {
         PyErr_Format(PyExc_RuntimeError, "%s is on cuda:%d, the current device is cuda:%d", name, (int)t.get_device(), *device);

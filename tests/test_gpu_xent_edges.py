@@ -186,3 +186,16 @@ def test_sums_over_many_rows_are_not_cut_short(dtype):
 def test_segments_and_pieces():
     """Contractions over the classes of a piece and over the rows that leave the tensor core more than once, with more than one piece."""
     _both(*_inputs(40000, 64, 60001, "f16", "dim", "some", seed=22), scale=2.0 ** 12)
+
+
+@gpu
+def test_lazily_negated_operands_are_refused():
+    """The imaginary part of a conjugate is a view whose sign has yet to be applied."""
+    import torch
+    from mask_b200 import engine
+    hidden, weight, labels = _inputs(20, 8, 5, "f32", "class")
+    z = torch.complex(weight, weight).conj().imag
+    assert z.is_neg()
+    with pytest.raises(RuntimeError, match="weight"):
+        engine.linear_cross_entropy(hidden, z, labels)
+    assert bool(torch.isfinite(engine.linear_cross_entropy(hidden, z.resolve_neg(), labels)))
