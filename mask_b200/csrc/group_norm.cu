@@ -862,7 +862,9 @@ static NormPlan plan_norm(const mask_norm& n, bool backward) {
     int64_t least_cost = INT64_MAX;
     for (int tx = unit; tx <= 32; tx += unit) {
         const int64_t slabs = (vectors + tx - 1) / tx, cost = slabs * 256 / (kNormThreads / tx);     // threads' time for a row
-        const bool wide = tx * (p.vec == 1 ? bytes / kNormVec : bytes) >= 128 || tx + unit > 32;          // 128 bytes of a row, or what there is
+        // 128 bytes of a row, or what there is: threads behind the row's end would have nothing to do (2^20 x 16 bf16: 25 us
+        // forward and 38 backward, 61 and 97 with 16 threads for the row's four vectors)
+        const bool wide = tx * (p.vec == 1 ? bytes / kNormVec : bytes) >= 128 || tx >= vectors || tx + unit > 32;
         if (wide && cost <= least_cost) { least_cost = cost; p.tx = tx; }
     }
     p.slabs = (vectors + p.tx - 1) / p.tx;
