@@ -35,3 +35,45 @@ def test_few_channels(rows, channels, groups, dtype):
     for activation in ("relu", "silu"):
         _both(rows, channels, groups, dtype, activation=activation, seed=rows)
     _both(rows, channels, groups, dtype, [0, 0, rows // 3, rows // 3 + 1, rows], "none", seed=rows)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_rows(dtype):
+    """The hidden layer of a full graph, as it is trained."""
+    _both(1 << 18, 512, 32, dtype, activation="relu", seed=41)
+
+
+@gpu
+def test_gradients_of_features_beyond_32_bits():
+    """2.5 thousand million values; the sums in 64 bits by pieces of rows."""
+    import torch
+    from mask_b200 import engine
+    rows, channels, groups = (1 << 22) + 3, 600, 30
+    g = torch.Generator(device="cuda").manual_seed(32)
+    x = torch.empty(rows, channels, device="cuda", dtype=torch.bfloat16)
+    for part in x.split(1 << 20):
+        part.copy_(torch.randn(part.shape, generator=g, device="cuda"))
+    offsets = [0, rows - 1000, rows]
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    y, m, r = engine.group_norm(x, groups, offsets=off, activation="silu")
+    dx, dw, db = engine.group_norm_backward(y, x, m, r, groups, offsets=off, activation="silu")
+    want, size = torch.zeros(2, channels, dtype=torch.float64, device="cuda"), torch.zeros(2, channels, dtype=torch.float64, device="cuda")
+    for lo in range(0, rows, 1 << 17):
+        hi = min(lo + (1 << 17), rows)
+        graph = (torch.arange(lo, hi, device="cuda") >= offsets[1]).long()
+        per = lambda t: t.double()[graph].repeat_interleave(channels // groups, 1)   # noqa: E731
+        u = (x[lo:hi].double() - per(m)) * per(r)
+        s = torch.sigmoid(u)
+        du = y[lo:hi].double() * s * (1 + u * (1 - s))
+        for i, t in enumerate((du * u, du)):
+            want[i] += t.sum(0)
+            size[i] += t.abs().sum(0)
+    # 585 additions of 2^-24; the activation's derivative is good to 2^-18 of (1 + |u|)
+    for got, w, a in zip((dw, db), want, size):
+        assert bool(((got.double() - w).abs() <= a * (585 * 2.0 ** -24 + 2.0 ** -16)).all())
+        assert float(w.abs().min()) > 0.1 * float(a.min())         # no cancellation that would hide rows from another place
+    # the last graph, behind 2^31 values, against the definition; its own sums from a call of it alone
+    tail = slice(rows - 1000, rows)
+    alone = engine.group_norm_backward(y[tail], x[tail], m[1:], r[1:], groups, activation="silu")
+    _check_backward(y[tail], x[tail], m[1:], r[1:], groups, None, None, activation="silu", got=(dx[tail], alone[1], alone[2]))

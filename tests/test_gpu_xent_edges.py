@@ -199,3 +199,51 @@ def test_lazily_negated_operands_are_refused():
     with pytest.raises(RuntimeError, match="weight"):
         engine.linear_cross_entropy(hidden, z, labels)
     assert bool(torch.isfinite(engine.linear_cross_entropy(hidden, z.resolve_neg(), labels)))
+
+
+@gpu
+@pytest.mark.parametrize("classes", [16, 300])
+def test_gradient_of_the_weight_over_features_beyond_32_bits(classes):
+    """2.2 thousand million features, every other row labelled, half of them behind 2^31 elements.  dweight in 64 bits by pieces: two
+    roundings to bfloat16 leave at most 2^-9 each of a sum whose terms are independent; rows taken from another place, most of it."""
+    import torch
+    from mask_b200 import engine
+    rows, dim = (1 << 22) + 5, 520
+    g = torch.Generator(device="cuda").manual_seed(38)
+    hidden = torch.empty(rows, dim, device="cuda", dtype=torch.bfloat16)
+    for part in hidden.split(1 << 20):
+        part.copy_(torch.randn(part.shape, generator=g, device="cuda"))
+    weight = (torch.randn(classes, dim, generator=g, device="cuda") * (2.0 / dim ** 0.5)).bfloat16().t()
+    labels = torch.randint(0, classes, (rows,), generator=g, device="cuda")
+    labels[::2] = -1
+    loss, dhidden, dweight = engine.linear_cross_entropy(hidden, weight, labels, reduction="sum", grads=True)
+    want, total = torch.zeros(dim, classes, dtype=torch.float64, device="cuda"), 0.0
+    for part, y in zip(hidden.split(1 << 18), labels.split(1 << 18)):
+        keep = y >= 0
+        h, y = part[keep].double(), y[keep, None]
+        logits = h @ weight.double()
+        total += float((torch.logsumexp(logits, 1, keepdim=True) - logits.gather(1, y)).sum())
+        want += h.t() @ (torch.softmax(logits, 1).scatter_add_(1, y, -torch.ones_like(y, dtype=torch.float64)))
+    assert float((dweight.double() - want).norm() / want.norm()) < 2.0 ** -8
+    # half of the rows alone: as far off as if the other half had been taken for it
+    assert abs(float(loss) - total) < 2.0 ** -16 * total
+    for part in dhidden[::2].split(1 << 19):
+        assert bool((part == 0).all())
+    assert all(bool(part.any(1).all()) for part in dhidden[1::2].split(1 << 19))
+
+
+@gpu
+def test_same_call_same_bits_whatever_memory_held():
+    """Pieces of the classes, pairs of blocks, one pass and tiny heads, in scratch that held NaN."""
+    import torch
+    from mask_b200 import engine
+    for rows, dim, classes, dtype in ((16384, 512, 70001, "bf16"), (5000, 640, 3000, "f16"), (3000, 130, 700, "f32"), (20000, 64, 40, "f32"), (500, 16, 7, "f32")):
+        x = _inputs(rows, dim, classes, dtype, labelled="some", seed=19)
+        first = [t.clone() for t in engine.linear_cross_entropy(*x, grads=True)]
+        for value in (float("nan"), 1.0):
+            torch.cuda.empty_cache()
+            free = torch.cuda.mem_get_info()[0]
+            dirty = [torch.full((min(free // 8, 1 << 30),), value, device="cuda") for _ in range(3)]
+            del dirty
+            for a, b in zip(engine.linear_cross_entropy(*x, grads=True), first):
+                assert torch.equal(a, b)
