@@ -10,7 +10,8 @@
 // (16384 steps in a row left 1.7e-3 of dW; 2730 with terms of both signs 2e-5).  For FP32 input an accumulator therefore
 // takes kXentSegment blocks of the contraction, and the segments are added in registers, rounded to nearest.  For 16-bit input the
 // products with G, whose contraction has no bound, leave an accumulator after kXentLongSegment blocks and are added up in the parts
-// (1e-7 times 512 steps in fp16, 4096 in bf16: a tenth or a fifth of the results' own rounding); logits take all of theirs.
+// (1e-7 times 1024 steps in fp16, 4096 in bf16: a fifth or a tenth of the results' own rounding; half as long cost the two products
+// of 16384 x 512 x 16384 fp16 202 us each instead of 192); logits take all of theirs.
 // All three products have the layouts TMA and the MMA take as they are, whichever axis is contracted:
 //     logits[r,v] = sum_d H[r,d] W[v,d]     both operands K-major
 //     dH[r,d]     = sum_v G[r,v] W[v,d]     G K-major, W MN-major
@@ -28,7 +29,7 @@ namespace mask {
 
 constexpr int kXentTileM = 128, kXentTileK = 64;
 constexpr int kXentSegment = 2;                     // blocks of the contraction that an accumulator takes (FP32 input)
-constexpr int kXentLongSegmentF16 = 128, kXentLongSegmentBf16 = 1024;      // the same for products with G of 16-bit input
+constexpr int kXentLongSegmentF16 = 256, kXentLongSegmentBf16 = 1024;      // the same for products with G of 16-bit input
 enum XentMode {
     kXentStats,      // logits -> running maximum and sum of each row over a range of classes
     kXentGrad,       // logits -> G of a piece of the classes, with the rows' log sums known
