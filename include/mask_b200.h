@@ -417,7 +417,8 @@ int mask_spmm_srbcrs_static_scratch(const mask_plan* plan, const int32_t* d_val_
  * held in the same parts, or in the operands' 16-bit type (float16: times 2^15, since most are small), between its products (heads of up to 4096 rows,
  * 1024 weight values and 2^19 products are computed in float32 throughout).  A class whose logit is -inf (a weight of
  * -inf and a positive feature) has probability 0; an entry of a gradient whose formula multiplies that 0 with the infinite
- * weight is NaN.  (In float32 a large finite stand-in for -inf costs the other values their bits, as above.)  A
+ * weight is NaN.  float32 values of 2^110 and more count as infinite too (but for the small heads above); a smaller stand-in
+ * for -inf is the largest magnitude by which the other values are measured: mask with -inf or the lowest value.  A
  * labelled row's loss and gradients are NaN if one of its logits is NaN or +inf, or its largest beyond about 7e8 in
  * magnitude (float32 logits that large are 64 apart), and so is dweight. Results do not depend on the order of anything: the same call gives the same bits.
  *

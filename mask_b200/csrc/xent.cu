@@ -140,9 +140,11 @@ struct XentPackArgs {
     uint32_t* range;           // FP32: bits of the largest finite magnitude of the labelled rows of hidden, and of weight
 };
 
+// Bits of |x|; 0 for infinities, NaN and what counts as infinite: from 2^110 on a factor of 2^-80 is enough for a logit beyond
+// kLogitBound, and the one use of such a weight is to take a class out.  It must not set the scale of all others.
 __device__ __forceinline__ uint32_t finite_magnitude(float x) {
     const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-    return b < 0x7f800000u ? b : 0u;
+    return b < ((110u + 127u) << 23) ? b : 0u;
 }
 
 // Lanes for a row of n values, four to a lane: a power of two, so that a warp takes several short rows at a time.
@@ -285,12 +287,14 @@ __global__ void __launch_bounds__(kXentCountThreads) xent_scan_kernel(const Xent
     }
 }
 
-// hi and lo of a scaled float.  An infinity is all lo: of the three products of parts only the one with the other operand's hi
-// is infinite then, none is 0 times infinity.  NaN is all hi.
+// hi and lo of a scaled float.  What is beyond the scale (2^15 and more: all that finite_magnitude leaves out) is infinite, and
+// an infinity is all lo: of the three products of parts only the one with the other operand's hi is infinite then, none is 0 times
+// infinity.  NaN is all hi.
 __device__ __forceinline__ void split_half(float x, uint32_t& hi, uint32_t& lo) {
-    const __half h = __float2half_rn(isinf(x) ? 0.f : x);
+    const bool beyond = fabsf(x) >= 32768.f;
+    const __half h = __float2half_rn(beyond ? 0.f : x);
     hi = __half_as_ushort(h);
-    lo = __half_as_ushort(__float2half_rn(isnan(x) ? 0.f : x - __half2float(h)));
+    lo = __half_as_ushort(__float2half_rn(beyond ? copysignf(INFINITY, x) : (isnan(x) ? 0.f : x - __half2float(h))));
 }
 
 // One row of `dim` elements `stride` apart to the planes, by `lanes` lanes of which this is number `lane`; `src` NULL writes zeros.

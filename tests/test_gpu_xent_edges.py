@@ -247,3 +247,46 @@ def test_same_call_same_bits_whatever_memory_held():
             del dirty
             for a, b in zip(engine.linear_cross_entropy(*x, grads=True), first):
                 assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("value", [-3.4028234663852886e38, -1e36])
+@pytest.mark.parametrize("rows,dim,classes", MASKED)
+def test_float32_classes_masked_by_the_lowest_value(rows, dim, classes, value):
+    """A weight that no float32 logit survives counts as infinite: it takes its class out and no bits from the others."""
+    import torch
+    from mask_b200 import engine
+    hidden, weight, labels = _inputs(rows, dim, classes, "f32", "dim", "some", seed=26)
+    hidden[:, dim - 1] = 1.0
+    masked = torch.arange(classes, device="cuda") % 3 == 1
+    labels[(labels >= 0) & (labels < classes) & (labels % 3 == 1)] = 0
+    out = weight.clone()
+    out[dim - 1, masked] = value
+    kept = torch.nonzero(~masked).squeeze(1)
+    place = torch.full((classes,), -1, dtype=torch.int64, device="cuda")
+    place[kept] = torch.arange(len(kept), device="cuda")
+    real = (labels >= 0) & (labels < classes)
+    want = _want(hidden, weight[:, kept], torch.where(real, place[labels.clamp(0, classes - 1)], -1), "sum")
+    loss, dhidden, dweight = engine.linear_cross_entropy(hidden, out, labels, reduction="sum", grads=True)
+    _check(loss, want[0], "loss")
+    _check(dweight[:, kept], want[2], "dweight")
+    assert bool((dweight[:, masked] == 0).all())
+    _check(dhidden[:, :dim - 1], tuple(t[:, :dim - 1] for t in want[1]), "dhidden")
+
+
+@gpu
+@pytest.mark.parametrize("classes", [50, 600])
+def test_powers_of_two_beyond_what_a_factor_holds(classes):
+    """Operands up to 2^108 and 2^60, whose other values make logits of 2^120 and 0: the label's keeps its size."""
+    import torch
+    from mask_b200 import engine
+    hidden = torch.zeros(70, 64, device="cuda")
+    weight = torch.zeros(64, classes, device="cuda")
+    hidden[0, 0], hidden[1:, 1] = 2.0 ** 108, -2.0 ** 85
+    weight[0, 0], weight[1, 1::2] = 2.0 ** 60, 2.0 ** 35
+    labels = torch.arange(70, device="cuda") % classes
+    loss = engine.linear_cross_entropy(hidden, weight, labels, reduction="none")
+    odd = labels[1:] % 2 == 1
+    assert bool(loss[0].isnan())
+    assert float((loss[1:][odd] / 2.0 ** 120 - 1).abs().max()) < 2.0 ** -20
+    assert float((loss[1:][~odd] - math.log((classes + 1) // 2)).abs().max()) < 2.0 ** -20 * 8
