@@ -402,8 +402,9 @@ int mask_spmm_srbcrs_static_scratch(const mask_plan* plan, const int32_t* d_val_
 
 /* ------------------------------------------------------------------------------------------
  * Classifier head: softmax cross entropy of hidden * weight over the labelled rows, with its
- * gradients, without the logits in memory.  What follows the last sparse product of a graph network
- * in training and evaluation (the reference's GCN driver takes it from its tensor library,
+ * gradients.  The logits are never in memory; of their gradient there is a piece of the classes at a
+ * time, 2 GB at most (or 256 classes, where those take more).  What follows the last sparse product of a
+ * graph network in training and evaluation (the reference's GCN driver takes it from its tensor library,
  * end2end/gcn/eva_gcn_sparsene.py:599-781).
  *
  * A row is labelled if 0 <= label < classes; every other label leaves the row out: its loss and its
@@ -411,20 +412,26 @@ int mask_spmm_srbcrs_static_scratch(const mask_plan* plan, const int32_t* d_val_
  *   logit[r,v] = sum_d hidden[r,d] weight[d,v],  loss[r] = log sum_v exp logit[r,v] - logit[r,label[r]]
  *   mean: loss[0] = their mean over the labelled rows, sum: their sum (both 0 if no row is labelled);
  *   none: loss[r] for every row, gradients those of the sum.  Gradients are multiplied by grad_scale.
- * float32 operands are multiplied as three products of float16 parts of 22 bits together (relative error of a
- * product at most 2^-20; values below 2^-18 of the largest finite magnitude of their operand, labelled rows
- * only, are exact to 2^-40 of that), 16-bit ones exactly; sums are float32.  The gradient of the logits is
- * held in the same parts, or in the operands' 16-bit type (float16: times 2^15, since most are small), between its products (heads of up to 4096 rows,
- * 1024 weight values and 2^19 products are computed in float32 throughout).  A class whose logit is -inf (a weight of
- * -inf and a positive feature) has probability 0; an entry of a gradient whose formula multiplies that 0 with the infinite
- * weight is NaN.  float32 values of 2^110 and more count as infinite too (but for the small heads above); a smaller stand-in
- * for -inf is the largest magnitude by which the other values are measured: mask with -inf or the lowest value.  A
- * labelled row's loss and gradients are NaN if one of its logits is NaN or +inf, or its largest beyond about 7e8 in
- * magnitude (float32 logits that large are 64 apart), and so is dweight. Results do not depend on the order of anything: the same call gives the same bits.
  *
- * Scratch: mask_linear_xent_scratch_bytes(head) bytes for this head's sizes, strides and result addresses (results
- * off 32 bytes need more), 256-byte aligned, one call at a time (two captured graphs that may run at once need two).  Asynchronous on `stream`.  Should a kernel give up on one of its bounded
- * waits, the losses (of the labelled rows, where they are all that is asked for) are NaN.
+ * Numerics.  float32 operands are multiplied as three products of float16 parts of 22 bits together
+ * (relative error of a product at most 2^-20; values below 2^-18 of the largest finite magnitude of their
+ * operand, labelled rows only, are exact to 2^-40 of that), 16-bit ones exactly; sums are float32.  The
+ * gradient of the logits is held in the same parts, or in the operands' 16-bit type (float16: times 2^15,
+ * since most of it is small), between its products: one rounding of the size of the results' own.  Heads
+ * of up to 4096 rows, 1024 weight values and 2^19 products are computed in float32 throughout.
+ * Results do not depend on the order of anything: the same call gives the same bits.
+ *
+ * Infinities.  A class whose logit is -inf (a weight of -inf and a positive feature) has probability 0; an
+ * entry of a gradient whose formula multiplies that 0 with the infinite weight is NaN.  float32 values of
+ * 2^110 and more count as infinite (not in the small heads); a smaller stand-in for -inf is the largest
+ * magnitude by which the other values are measured: mask with -inf or the lowest value.  A labelled row's
+ * loss and gradients are NaN, and so is dweight, if one of its logits is NaN or +inf, or if its largest is
+ * beyond about 7e8 in magnitude (float32 numbers of that size are 64 apart).
+ *
+ * Scratch: mask_linear_xent_scratch_bytes(head) bytes for this head's sizes, strides and result addresses
+ * (results off 32 bytes need more), 256-byte aligned, one call at a time (two captured graphs that may run at
+ * once need two).  Asynchronous on `stream`.  Should a kernel give up on one of its bounded waits, the losses
+ * (of the labelled rows, where they are all that is asked for) are NaN.
  * ------------------------------------------------------------------------------------------ */
 typedef enum mask_dtype { MASK_F32 = 0, MASK_BF16 = 1, MASK_F16 = 2 } mask_dtype;
 typedef enum mask_reduction { MASK_REDUCE_NONE = 0, MASK_REDUCE_MEAN = 1, MASK_REDUCE_SUM = 2 } mask_reduction;

@@ -869,7 +869,9 @@ static NormPlan plan_norm(const mask_norm& n, bool backward) {
     }
     p.slabs = (vectors + p.tx - 1) / p.tx;
     // Four blocks an SM are resident: as many chunks as that, in whole batches of rows.  (300007 x 256 bf16 backward: 159 us;
-    // twice as many 164, four times 199, since every chunk leaves sums to join and blocks have a start and an end.)
+    // twice as many 164, four times 199, since every chunk leaves sums to join and blocks have a start and an end.)  Four blocks
+    // leave 64 registers a thread, of which the float32 backward kernels of four channels spill 56 to 120 bytes, the 16-bit ones
+    // 4 to 16 (2^18 x 512 float32, ReLU, backward: 501 us, five passes over the features 410).
     const int64_t want = 4 * (int64_t)sm_count(), batch = 8 * (kNormThreads / p.tx), most = std::max<int64_t>(4096 / batch, 1) * batch;
     p.chunk = (int)std::min(std::max((n.rows * p.slabs + want * batch - 1) / (want * batch) * batch, std::min<int64_t>(batch, 256)), most);
     // Graphs of a chunk are finished by its block, one that is not much longer by clusters.

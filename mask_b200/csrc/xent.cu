@@ -1,5 +1,5 @@
 // Classifier head: softmax cross entropy of hidden * weight over the labelled rows and its gradients, without the
-// logits in memory (mask_linear_xent).
+// logits in memory and with at most 2 GB (or 256 classes) of their gradient at a time (mask_linear_xent).
 //
 // With L the labelled rows, l = H W, s_r = log sum_v exp l_rv and G_rv = exp(l_rv - s_r) - [v = y_r]:
 //     loss_r = s_r - l_{r,y_r},   dH = scale G W^T,   dW = scale H^T G.

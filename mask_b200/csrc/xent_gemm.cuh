@@ -2,7 +2,8 @@
 // softmax or its gradient as epilogue, and the two products of that gradient G with W and with H.
 //
 // One persistent block per SM: a producer thread feeds a ring of stages by TMA, one thread issues the MMAs into two
-// accumulators of tensor memory, eight warps take the finished accumulator apart while the next one is computed.
+// accumulators of tensor memory (of each group of epilogue warps), eight warps, or sixteen where every logit costs an exponential
+// or tiles are narrow, take the finished accumulator apart while the next one is computed.
 // Operands are 16-bit "planes": one for bf16 and fp16 input.  FP32 input is scaled by a power of two that brings the
 // operand's largest magnitude to 2^14..2^15 and split into two fp16 planes, x = hi + lo + e with |e| <= 2^-22 |x|, or 2^-40
 // of the largest where that is more; a product is hi hi + hi lo + lo hi (the dropped lo lo is 2^-22 of it at most).

@@ -334,13 +334,15 @@ def _product(packed, dense, out, policy, relu, plan, tf32x3, whole_vectors):
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, reduction: str = "mean", grads: bool = False,
                          grad_scale: float = 1.0):
     """Softmax cross entropy of ``hidden[rows, dim] @ weight[dim, classes]`` against int64 ``labels[rows]`` on the current
-    stream, without the logits in memory; float32, bfloat16 or float16.  Rows whose label is not one of the classes (-1, say)
-    are left out: no loss, no gradient, whatever they hold.  ``reduction``: "mean" over the labelled rows or "sum" (0 without
-    any), "none" for a loss per row.  The loss is float32.
+    stream; float32, bfloat16 or float16.  The logits are never in memory, their gradient in pieces of at most 2 GB (or 256
+    classes).  Rows whose label is not one of the classes (-1, say) are left out: no loss, no gradient, whatever they hold.
+    A weight of -inf times a positive feature takes a class out (probability 0).  ``reduction``: "mean" over the labelled rows
+    or "sum" (0 without any), "none" for a loss per row.  The loss is float32.
 
     With ``grads`` returns (loss, dhidden, dweight): the gradients of the loss (of its sum for "none") times ``grad_scale``,
-    in the operands' dtype, dweight contiguous along the axis along which ``weight`` is.  ``weight`` may have any strides
-    (pass a table of one embedding per class as ``table.t()``), ``hidden`` any distance between its rows."""
+    in the operands' dtype, dweight contiguous along the axis along which ``weight`` is.  Nothing is recorded for autograd,
+    whether or not the operands require gradients.  ``weight`` may have any strides (pass a table of one embedding per class as
+    ``table.t()``), ``hidden`` any distance between its rows."""
     if reduction not in _lib.REDUCTION:
         raise RuntimeError(f"reduction must be one of {', '.join(_lib.REDUCTION)}")
     got = (_lib._binding or _lib.binding()).linear_xent(hidden, weight, labels, _lib.REDUCTION[reduction], grad_scale, grads)
@@ -361,7 +363,8 @@ def group_norm(x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
     "silu") on the current stream: returns (y, mean, rstd), the statistics float32 ``[graphs, groups]`` over a graph's rows
     and a group's neighbouring channels.  ``offsets`` (int32, graphs + 1) are the batch's first rows, ascending; without them
     all rows are one graph.  Rows outside every graph are not written.  ``weight`` and ``bias`` are float32 ``[channels]``.
-    ``x`` may have any distance between its rows; ``out`` may be ``x``."""
+    ``x`` may have any distance between its rows; ``out`` may be ``x``.  Nothing is recorded for autograd:
+    ``group_norm_backward`` has the gradients."""
     got = (_lib._binding or _lib.binding()).group_norm(x, groups, weight, bias, offsets, eps, _activation(activation), out)
     if type(got) is int:
         check(got, "mask_group_norm")

@@ -1,5 +1,5 @@
 """2-layer GCNs: the row-sharded forward ``out = A·(ReLU(A·(X·W1))·W2)`` over P ranks, and training on one device
-(``GCN2``: loss and gradients, with group norm between the layers and the classifier head without its logits in memory).
+(``GCN2``: loss and gradients, with group norm between the layers and the classifier head behind them).
 
 The reference project is single-GPU (its GCN driver, end2end/gcn/eva_gcn_sparsene.py:316-343,
 calls one SpMM per layer on one device); this module is the multi-GPU harness the benchmark
@@ -260,7 +260,8 @@ class GCN2:
     The reference's driver trains such a network from its tensor library's pieces (end2end/gcn/eva_gcn_sparsene.py:316-343,
     599-781).  Here everything between the dense products ``X·W1`` and its gradient is this library's: sparse products with A
     and A^T, group norm with the activation (per graph of a batch: ``offsets``, which cover every node), and the head with its
-    gradients, which does not keep the logits in memory.
+    gradients, which keeps no logits and a piece of their gradient in memory.  Gradients are returned, nothing is recorded for
+    autograd.
 
     ``graph``: square CSR with ``rowptr``, ``colind``, ``values`` (NumPy) and ``M``.  ``ops`` supplies the device's pieces
     (``_TrainOps``), so that the chain of gradients can be checked without one.  ``tf32x3`` as in ``engine.spmm``."""
