@@ -425,8 +425,8 @@ int mask_spmm_srbcrs_static_scratch(const mask_plan* plan, const int32_t* d_val_
  * entry of a gradient whose formula multiplies that 0 with the infinite weight is NaN.  float32 values of
  * 2^110 and more count as infinite (not in the small heads); a smaller stand-in for -inf is the largest
  * magnitude by which the other values are measured: mask with -inf or the lowest value.  A labelled row's
- * loss and gradients are NaN, and so is dweight, if one of its logits is NaN or +inf, or if its largest is
- * beyond about 7e8 in magnitude (float32 numbers of that size are 64 apart).
+ * loss and gradients are NaN, and so is dweight, if one of its logits is NaN or +inf, or (not in the small
+ * heads) if its largest is beyond about 1.4e9 in magnitude, where float32 numbers are 128 apart.
  *
  * Scratch: mask_linear_xent_scratch_bytes(head) bytes for this head's sizes, strides and result addresses
  * (results off 32 bytes need more), 256-byte aligned, one call at a time (two captured graphs that may run at

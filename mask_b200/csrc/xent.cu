@@ -600,7 +600,6 @@ __global__ void __launch_bounds__(kXentCountThreads) __cluster_dims__(kXentTinyB
         float sum = 0.f;
         for (int v = sub; v < V; v += width) sum += live ? fast_exp2((g[v] - top) * kLog2e) : 0.f;
         for (int o = width / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        sum = bounded_sum(sum, top * kLog2e);
         const float loss = live ? kLn2 * fmaf(top - picked, kLog2e, log2f(sum)) : 0.f;
         if (sub == 0 && live) {
             losses += loss;

@@ -108,9 +108,10 @@ __device__ __forceinline__ int logit_exponent(const uint32_t* range) { return pl
 __device__ __forceinline__ float logit_factor(const uint32_t* range) { return range ? ldexpf(kLog2e, max(-126, min(logit_exponent(range), 126))) : kLog2e; }
 // What the factor leaves out above, for a label's logit, which may be as far below the largest as it likes.
 __device__ __forceinline__ float logit_rest(const uint32_t* range) { return range ? ldexpf(1.f, max(logit_exponent(range) - 126, 0)) : 1.f; }
-// A row's largest logit, in bits, up to which there is a softmax.  Exponents are taken less the rounded number of bits, off by 32
-// here; not much beyond, they pass what an exponential takes, and the sum would be any number.  The row's sum is NaN instead.
-constexpr float kLogitBound = 1073741824.f;
+// A row's largest logit, in bits, up to which there is a softmax.  Exponents are taken less the rounded number of bits, off by 64
+// at most here; from twice that on they pass what an exponential takes, and the sum would be any number.  The row's sum is NaN
+// instead.  (Tiny heads subtract the logits themselves.)
+constexpr float kLogitBound = 2147483648.f;
 __device__ __forceinline__ float bounded_sum(float sum, float base) { return fabsf(base) < kLogitBound ? sum : NAN; }
 
 // CG: blocks that share a tile.  2: a cluster of two takes 256 rows, each block 128 of them and half of the columns' operand,
